@@ -406,6 +406,100 @@ int vqa_class_stats_dev(int device, void* stream, const int64_t* d_counts, const
                         int want_variances, double* d_out_sums, double* d_out_grad_data);
 
 /*
+ * Softmax read-out.  A row of `width` scores z (expectation values of as many observables, scaled) stands for the
+ * distribution p = softmax(scale * z) over its outcomes: the read-out of softmax classifiers and policies, where
+ * vqa_class_stats_dev reads class frequencies.  No counterpart in the reference.
+ *
+ * dtype is the scores' type; log probabilities, entropies and their weights are double for VQA_DTYPE_F64 and float for
+ * the others, sums are held in that type.  Rows lie row_stride elements apart.  scale > 0, finite.
+ *   log_prob[r]  log p of outcome targets[r]; 0 for targets[r] < 0 (no outcome given)
+ *   entropy[r]   -sum p log p
+ *   top_index / top_log_prob [r, top_k]   the outcomes with the largest stored scores, largest first, equal ones by
+ *                lower index, and their log p (top_k in [0, min(64, width)])
+ * A score of -inf masks its outcome (p = 0, never among the top ones; places that find no outcome hold -1 and -inf).
+ * A row with every outcome masked: log_prob -inf, entropy 0.  A row that holds a NaN or +inf, or a targets[r] >= width:
+ * NaN in the row's outputs, -1 in its top_index.  log_prob (with targets) and entropy may each be NULL.
+ * Deterministic; columns behind `width` are not read.
+ * _dev: device pointers, queued on `stream`, not waited for, nothing allocated: workspace is
+ * vqa_log_probs_workspace(...) bytes of the caller's device memory (0: may be NULL), not shared with work that may run
+ * at the same time.  The calling thread's current device is kept.
+ */
+#define VQA_DTYPE_F64  0
+#define VQA_DTYPE_F32  1
+#define VQA_DTYPE_BF16 2
+#define VQA_DTYPE_F16  3
+int64_t vqa_log_probs_workspace(int dtype, int64_t rows, int64_t width, int top_k);
+int vqa_log_probs_dev(int device, void* stream, int dtype, const void* d_scores, int64_t rows, int64_t width,
+                      int64_t row_stride, double scale, const int32_t* d_targets, int top_k, void* d_workspace,
+                      void* d_log_prob, void* d_entropy, void* d_top_log_prob, int32_t* d_top_index);
+/* The same with host pointers; synchronous. */
+int vqa_log_probs(int device, int dtype, const void* scores, int64_t rows, int64_t width, int64_t row_stride, double scale,
+                  const int32_t* targets, int top_k, void* log_prob, void* entropy, void* top_log_prob, int32_t* top_index);
+
+/*
+ * The gradient of a loss of these outputs, with the outputs themselves (a training step needs both):
+ * given d_dlog_prob[r] = d loss / d log_prob[r] and d_dentropy[r] = d loss / d entropy[r] (NULL: 0),
+ *   d_dscores[r, c] = scale * (dlog_prob (delta_{c, target} - p_c) - dentropy p_c (log p_c + entropy))
+ * in the scores' type, rows dscores_row_stride elements apart, columns behind `width` left as they were.  A row without
+ * a target takes dlog_prob as 0; a row with every outcome masked has gradient 0, a row with NaN outputs has NaN.
+ * d_targets is needed for d_dlog_prob.  d_dscores must not overlap the scores.  Workspace: vqa_log_probs_workspace with
+ * top_k 0.  The chain into circuit parameters is vqa_psr_chain_dev.
+ */
+int vqa_log_probs_grad_dev(int device, void* stream, int dtype, const void* d_scores, int64_t rows, int64_t width,
+                           int64_t row_stride, double scale, const int32_t* d_targets, const void* d_dlog_prob,
+                           const void* d_dentropy, void* d_workspace, void* d_log_prob, void* d_entropy, void* d_dscores,
+                           int64_t dscores_row_stride);
+int vqa_log_probs_grad(int device, int dtype, const void* scores, int64_t rows, int64_t width, int64_t row_stride,
+                       double scale, const int32_t* targets, const void* dlog_prob, const void* dentropy, void* log_prob,
+                       void* entropy, void* dscores, int64_t dscores_row_stride);
+
+/*
+ * The chain rule through a parameter-shift sweep: from d_expect[n_samples, 2 n_params + 1, n_obs] (out_expect of
+ * vqa_psr_full_dev) and d_dexpect[n_samples, n_obs] = d loss / d (unshifted expectation value),
+ *   out[i] = factor * sum_b sum_o dexpect[b, o] (expect[b, 2 i + 1, o] - expect[b, 2 i + 2, o]);
+ * factor 1/2 for the shift pi/2 gives d loss / d theta_i (the difference of vqa/QNN/myQNNs_base.py:1388-1394).  Sums:
+ * the ranks of a split batch add them.  Fixed summation order; n_samples up to 2^22.  Workspace:
+ * vqa_psr_chain_workspace bytes.
+ */
+int64_t vqa_psr_chain_workspace(int64_t n_samples, int n_params);
+int vqa_psr_chain_dev(int device, void* stream, const double* d_expect, int64_t n_samples, int n_params, int n_obs,
+                      double factor, const double* d_dexpect, double* d_workspace, double* d_out);
+
+/*
+ * Orthogonalised update of a [batch, rows, cols] array by Newton-Schulz products, for parameters that form matrices
+ * (layers x angles of a layered ansatz).  Per matrix, X = G / (|G|_F + eps) and `steps` times
+ *   A = X X^T,  X <- coefs[0] X + (coefs[1] A + coefs[2] A A) X
+ * (on the transpose when rows > cols), which keeps G's singular vectors and carries its singular values towards 1.
+ * No counterpart in the reference.  dtype as above; state and sums are double for VQA_DTYPE_F64, else 32 bits or
+ * pairs of 16-bit floats that hold as much.  Matrix b's element (i, j) is d_g[b * batch_stride + i * row_stride + j];
+ * d_out is contiguous and may be d_g where that is contiguous too, but not overlap it otherwise.
+ * rows, cols in [1, 65536], batch in [0, 65535], steps in [1, 100], eps > 0.  coefs that let a singular value
+ * exceed 4 within `steps` steps, or the polynomial of A 32, are refused (VQA_EUNSUPPORTED).
+ * A zero matrix gives zero; NaN or inf in a matrix gives NaN in that matrix.  Workspace as for vqa_log_probs_dev.
+ */
+int64_t vqa_orthogonalize_workspace(int dtype, int batch, int rows, int cols);
+int vqa_orthogonalize_dev(int device, void* stream, int dtype, const void* d_g, int batch, int rows, int cols,
+                          int64_t row_stride, int64_t batch_stride, int steps, const double* coefs, double eps,
+                          void* d_workspace, void* d_out);
+int vqa_orthogonalize(int device, int dtype, const void* g, int batch, int rows, int cols, int64_t row_stride,
+                      int64_t batch_stride, int steps, const double* coefs, double eps, void* out);
+
+/*
+ * One optimizer step with an orthogonalised momentum, in place, beside the step rules the host layer offers (SGDM:
+ * vqa/VQA_optimizers/qml_optimizers.py:981-1027):
+ *   momentum <- mu * momentum + g;   u = g + mu * momentum (nesterov) or momentum;
+ *   weight <- (1 - lr * weight_decay) * weight - lr * sqrt(max(1, rows / cols)) * orthogonalize(u)
+ * weight and momentum are contiguous, double for VQA_DTYPE_F64 gradients and float for the others; the three arrays must
+ * not overlap.  Limits and workspace as for vqa_orthogonalize_dev.
+ */
+int vqa_muon_step_dev(int device, void* stream, int dtype, void* d_weight, const void* d_g, void* d_momentum, int batch,
+                      int rows, int cols, int64_t row_stride, int64_t batch_stride, double lr, double mu,
+                      double weight_decay, int nesterov, int steps, const double* coefs, double eps, void* d_workspace);
+int vqa_muon_step(int device, int dtype, void* weight, const void* g, void* momentum, int batch, int rows, int cols,
+                  int64_t row_stride, int64_t batch_stride, double lr, double mu, double weight_decay, int nesterov,
+                  int steps, const double* coefs, double eps);
+
+/*
  * Final state of ONE instance, interleaved (re, im) doubles, 2 * 2^n values,
  * host pointer.  For plumbing tests of the per-sample circuit.run(x) shim
  * (vqa/QNN/myQNNs_base.py:913); not a hot-path call.

@@ -1,0 +1,282 @@
+"""Newton-Schulz products and the optimizer step on the GPU against the definition on singular values, in 64 bits.
+
+Tolerances.  With u = 2^-53 or 2^-24, a product over K terms is off by about u sqrt(K) of its factors' sizes (independent
+roundings), a step of the iteration by that times |a| + |b| + |c| = 10.3 (X in norm at most 1.3), and what a step adds in the
+direction of a small singular value grows by at most |a| = 3.4445 a step after it: in Frobenius norm, with r rows of norm
+about 1,  u sqrt(K) 10.3 (3.4445^steps - 1) / 2.4445 sqrt(r).  That bound is loose where many roundings cancel, so matrices of
+32 bits are also held to four times what a plain 32-bit run of the same formulas is off: values in 16-bit pairs and their
+left-out product round at 2^-22 to 2^-23, a quarter of a 32-bit step.  A result of 16 bits adds half a step of each value."""
+import math
+
+import numpy as np
+import pytest
+
+import vqa_amd
+from vqa_amd.orthogonal import COEFS
+
+pytestmark = pytest.mark.gpu
+
+UNIT = {"float64": 2.0 ** -53, "float32": 2.0 ** -24, "bfloat16": 2.0 ** -24, "float16": 2.0 ** -24}
+
+
+def defined(g, steps=5, coefs=COEFS, eps=1e-7):
+    """U p(S) V^T in numpy, 64 bits"""
+    u, s, vt = np.linalg.svd(g, full_matrices=False)
+    s = s / (np.sqrt((g ** 2).sum(axis=(-2, -1)))[..., None] + eps)
+    for _ in range(steps):
+        s = s * (coefs[0] + s * s * (coefs[1] + coefs[2] * s * s))
+    return (u * s[..., None, :]) @ vt
+
+
+def plain(g, dtype, steps=5, coefs=COEFS, eps=1e-7):
+    """the products in `dtype` on the GPU"""
+    import torch
+
+    x = (g.double() / (torch.linalg.vector_norm(g.double(), dim=(1, 2), keepdim=True) + eps)).to(dtype)
+    turned = x.shape[1] > x.shape[2]
+    if turned:
+        x = x.transpose(1, 2).contiguous()
+    for _ in range(steps):
+        a = torch.matmul(x, x.transpose(1, 2).contiguous())
+        x = coefs[0] * x + torch.matmul(coefs[1] * a + coefs[2] * torch.matmul(a, a), x)
+    return x.transpose(1, 2).contiguous() if turned else x
+
+
+def bound(t, r, c, steps=5):
+    return UNIT[t] * math.sqrt(c + 2 * r) * 10.3 * (3.4445 ** steps - 1) / 2.4445 * math.sqrt(r)
+
+
+def matrices(rng, batch, rows, cols, t, noise=0.5):
+    import torch
+
+    k = max(1, min(rows, cols) // 8)
+    g = rng.standard_normal((batch, rows, k)) @ rng.standard_normal((batch, k, cols)) / math.sqrt(k) + noise * rng.standard_normal((batch, rows, cols))
+    return torch.from_numpy(g * 1e-2).to(getattr(torch, t)).cuda()
+
+
+def check(got, g, t, steps=5, coefs=COEFS, eps=1e-7):
+    import torch
+
+    rows, cols = g.shape[-2:]
+    r, c = min(rows, cols), max(rows, cols)
+    g64 = g.double().reshape(-1, rows, cols)
+    want = defined(g64.cpu().numpy(), steps, coefs, eps)
+    o = got.double().cpu().numpy().reshape(want.shape)
+    assert np.isfinite(o).all()
+    off = np.sqrt(((o - want) ** 2).sum(axis=(1, 2)))
+    half = 0.0 if t in ("float64", "float32") else torch.finfo(getattr(torch, t)).eps / 2
+    stored = half * np.sqrt((want ** 2).sum(axis=(1, 2))) + (2.0 ** -25 * math.sqrt(r * c) if t == "float16" else 0.0)
+    assert (off <= bound(t, r, c, steps) + stored).all(), (off.max(), bound(t, r, c, steps))
+    wide = torch.float64 if t == "float64" else torch.float32
+    p = plain(g64, wide, steps, coefs, eps).double().cpu().numpy()
+    poff = np.sqrt(((p - want) ** 2).sum(axis=(1, 2)))
+    # (a few elements' roundings say little: at least those of a single product of K terms)
+    floor = UNIT[t] * math.sqrt(c + 2 * r) * np.sqrt((want ** 2).sum(axis=(1, 2))) * 4
+    assert (off <= 4 * poff + floor + stored).all(), (off.max(), poff.max())
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (3, 5), (11, 36), (36, 11), (9, 60), (16, 16), (17, 33), (64, 64), (64, 200), (200, 64),
+          (65, 65), (64, 513), (63, 130), (1, 700), (2, 5000), (100, 100), (128, 128), (129, 257), (300, 100), (257, 640)]
+
+
+@pytest.mark.parametrize("t", list(UNIT))
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_orthogonalize_matches_the_definition(t, rows, cols):
+    rng = np.random.default_rng(rows * 1000 + cols)
+    g = matrices(rng, 2, rows, cols, t)
+    check(vqa_amd.orthogonalize(g), g, t)
+
+
+@pytest.mark.parametrize("t", ["float32", "bfloat16", "float64"])
+def test_larger_matrices(t):
+    rng = np.random.default_rng(1)
+    for rows, cols in [(777, 1000), (1000, 520)]:
+        g = matrices(rng, 1, rows, cols, t)[0]
+        o = vqa_amd.orthogonalize(g)
+        assert o.shape == g.shape and o.dtype == g.dtype
+        check(o, g, t)
+
+
+@pytest.mark.parametrize("t", ["float64", "float32"])
+@pytest.mark.parametrize("rows,cols", [(11, 36), (150, 70)])
+@pytest.mark.parametrize("steps,coefs", [(1, COEFS), (2, COEFS), (3, (15 / 8, -10 / 8, 3 / 8)), (12, (1.5, -0.5, 0.0)), (5, (3.0, -3.2, 1.2))])
+def test_steps_and_coefficients(t, rows, cols, steps, coefs):
+    g = matrices(np.random.default_rng(2), 1, rows, cols, t)[0]
+    import torch
+
+    o = vqa_amd.orthogonalize(g, steps=steps, coefs=coefs)
+    want = defined(g.double().cpu().numpy(), steps, coefs)
+    r, c = min(rows, cols), max(rows, cols)
+    # |a| a step in the direction of small singular values, the sum of the coefficients' sizes in a step
+    a, all3 = max(abs(coefs[0]), 1.01), sum(abs(v) for v in coefs)
+    tol = UNIT[t] * math.sqrt(c + 2 * r) * (all3 + 1) * (a ** steps - 1) / (a - 1) * math.sqrt(r)
+    assert np.sqrt(((o.double().cpu().numpy() - want) ** 2).sum()) <= tol
+    assert isinstance(o, torch.Tensor)
+
+
+@pytest.mark.parametrize("t", list(UNIT))
+@pytest.mark.parametrize("rows,cols", [(5, 9), (70, 90)])
+def test_matrices_that_are_special(t, rows, cols):
+    import torch
+
+    g = matrices(np.random.default_rng(3), 6, rows, cols, t)
+    g[1] = 0
+    g[2, 0, 0] = float("nan")
+    g[3, rows - 1, cols - 1] = float("inf")
+    g[4] = 0
+    g[4, 1, 2] = 3.0                                     # rank one
+    o = vqa_amd.orthogonalize(g)
+    assert (o[1] == 0).all() and torch.isnan(o[2]).all() and torch.isnan(o[3]).all()
+    keep = torch.stack([g[0], g[4], g[5]])
+    check(torch.stack([o[0], o[4], o[5]]), keep, t)
+    # one matrix of a batch does not touch another
+    assert torch.equal(vqa_amd.orthogonalize(g[5]), o[5])
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_sizes_of_entries(size):
+    """the norm is taken in 64 bits: squares of 1e30 do not overflow; entries far below eps give a result near 0"""
+    import torch
+
+    for rows, cols in [(6, 10), (80, 70)]:
+        g = (matrices(np.random.default_rng(4), 1, rows, cols, "float64")[0] * size).float()
+        o = vqa_amd.orthogonalize(g)
+        if size > 1:
+            check(o, g, "float32")
+        else:
+            assert o.abs().max() < 1e-18
+
+
+@pytest.mark.parametrize("t", ["float64", "bfloat16"])
+def test_strides_out_and_in_place(t):
+    import torch
+
+    for rows, cols in [(11, 36), (90, 100)]:
+        big = matrices(np.random.default_rng(5), 3, rows + 2, cols + 5, t)
+        g = big[:, 1:rows + 1, 3:cols + 3]
+        want = vqa_amd.orthogonalize(g.contiguous())
+        assert torch.equal(vqa_amd.orthogonalize(g), want)
+        tr = g.transpose(1, 2)                                  # columns apart: taken through a copy
+        assert torch.equal(vqa_amd.orthogonalize(tr), vqa_amd.orthogonalize(tr.contiguous()))
+        h = g.contiguous()
+        assert vqa_amd.orthogonalize(h, out=h).data_ptr() == h.data_ptr() and torch.equal(h, want)
+        e = g[:1].expand(3, rows, cols)
+        assert torch.equal(vqa_amd.orthogonalize(e)[2], want[0])
+        with pytest.raises(ValueError):
+            vqa_amd.orthogonalize(h, out=big[:, 1:rows + 1, 3:cols + 3])
+    assert vqa_amd.orthogonalize(torch.zeros(0, 3, 4, dtype=torch.float64).cuda()).shape == (0, 3, 4)
+
+
+@pytest.mark.parametrize("t", list(UNIT))
+@pytest.mark.parametrize("rows,cols", [(11, 36), (36, 11), (1, 1), (130, 70), (70, 300)])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_step_matches_the_formulas(t, rows, cols, nesterov):
+    import torch
+
+    rng = np.random.default_rng(6)
+    wide = torch.float64 if t == "float64" else torch.float32
+    g = matrices(rng, 2, rows, cols, t)
+    w = torch.from_numpy(rng.standard_normal((2, rows, cols))).to(wide).cuda()
+    m = torch.from_numpy(1e-2 * rng.standard_normal((2, rows, cols))).to(wide).cuda()
+    lr, mu, wd = 0.03, 0.9, 0.1
+    w64, m64, g64 = (x.double().cpu().numpy() for x in (w, m, g))
+    m64 = mu * m64 + g64
+    u64 = g64 + mu * m64 if nesterov else m64
+    rate = lr * math.sqrt(max(1.0, rows / cols))
+    w64 = (1 - lr * wd) * w64 - rate * defined(u64)
+    assert vqa_amd.muon_step(w, g, m, lr, mu, wd, nesterov) is w
+    u = UNIT[t]
+    # mu is rounded to the type, then a product and a sum
+    assert (np.abs(m.double().cpu().numpy() - m64) <= u * (3 * np.abs(m64) + 3 * np.abs(g64) + 3 * np.abs(m64 - g64))).all()
+    off = np.sqrt(((w.double().cpu().numpy() - w64) ** 2).sum(axis=(1, 2)))
+    r, c = min(rows, cols), max(rows, cols)
+    # the entering matrix is off by a few u of its norm: the same bound again, K = 1
+    tol = rate * bound(t, r, c) * 2 + 4 * u * np.sqrt((w64 ** 2).sum(axis=(1, 2)))
+    assert (off <= tol).all(), (off, tol)
+
+
+@pytest.mark.parametrize("dt", [np.float64, np.float32])
+def test_host_pointer_paths(dt):
+    import torch
+
+    rng = np.random.default_rng(7)
+    for shape in ((11, 36), (2, 70, 66)):
+        g = rng.standard_normal(shape).astype(dt)
+        dev = torch.from_numpy(g).cuda()
+        assert np.array_equal(vqa_amd.orthogonalize(g), vqa_amd.orthogonalize(dev).cpu().numpy())
+        w, m = rng.standard_normal(shape).astype(dt), np.zeros(shape, dt)
+        wt, mt = torch.from_numpy(w.copy()).cuda(), torch.from_numpy(m.copy()).cuda()
+        vqa_amd.muon_step(w, g, m, 0.1)
+        vqa_amd.muon_step(wt, dev, mt, 0.1)
+        assert np.array_equal(w, wt.cpu().numpy()) and np.array_equal(m, mt.cpu().numpy())
+
+
+@pytest.mark.parametrize("rows,cols", [(11, 36), (200, 300)])
+def test_streams_and_captured_steps(rows, cols):
+    """a captured optimizer step is replayed; eager steps on copies run beside it and agree bit for bit"""
+    import torch
+
+    rng = np.random.default_rng(9)
+    grads = [matrices(rng, 1, rows, cols, "float32") for _ in range(3)]
+    w = torch.from_numpy(rng.standard_normal((1, rows, cols))).float().cuda()
+    m, g = torch.zeros_like(w), grads[0].clone()
+    ew, em = w.clone(), m.clone()
+    a = vqa_amd.orthogonalize(g)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        b = vqa_amd.orthogonalize(g)
+        vqa_amd.muon_step(w.clone(), g, m.clone(), 0.01)       # loads the kernels before the capture
+    s.synchronize()
+    assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        vqa_amd.muon_step(w, g, m, 0.01)
+    for n in range(5):
+        g.copy_(grads[n % 3])
+        graph.replay()
+        vqa_amd.muon_step(ew, grads[n % 3], em, 0.01)
+        torch.cuda.synchronize()
+        assert torch.equal(w, ew) and torch.equal(m, em), n
+
+
+def test_refusals_on_the_gpu():
+    import torch
+
+    w = torch.zeros(4, 6).cuda()
+    g = torch.zeros(4, 6, dtype=torch.bfloat16).cuda()
+    m = torch.zeros(4, 6).cuda()
+    with pytest.raises(ValueError):
+        vqa_amd.muon_step(w.double(), g, m, 0.1)
+    with pytest.raises(ValueError):
+        vqa_amd.muon_step(w.t().contiguous().t(), g, m, 0.1)
+    with pytest.raises(ValueError):
+        vqa_amd.muon_step(w, g, torch.zeros(4, 6), 0.1)
+    from vqa_amd import _lib
+    with pytest.raises(_lib.VqaError):
+        vqa_amd.muon_step(w, g, w, 0.1)
+    with pytest.raises(_lib.VqaError):
+        vqa_amd.orthogonalize(w, coefs=(9.0, 0.0, 0.0))
+    with pytest.raises(ValueError):
+        vqa_amd.orthogonalize(w.to(torch.int32))
+
+
+def test_muon_optimizer_trains_the_regressor():
+    """compile / fit with optimizer="Muon": the matrix part takes the orthogonalised step, the scale parameter SGDM's"""
+    from vqa_amd.qml_utils import create_ibm_HEA_ansatz
+    from vqa_amd.qnn_base import myQNN_base
+
+    rng = np.random.default_rng(0)
+    x = rng.uniform(0, 1, (16, 4))
+    q = myQNN_base(4, create_ibm_HEA_ansatz(4, 1, seed=2), x, np.sin(x.sum(1)), x, np.sin(x.sum(1)), min_approx_shots=-10)
+    p = np.concatenate([rng.uniform(-3, 3, q.n_c_params), [0.9]])
+    q.compile(optimizer="Muon", hpara=dict(LR_rule=0.02, batch_size_rule=16, s_list_rule=100), init_params=p, min_approx_shots=-10)
+    res = q.fit(options=dict(max_iter=2), auto_save=False)
+    path = np.array(res["para_evol"])
+    g = q.MSE_grad_eval(p, np.full(len(p), 100), mini_batch_size=16, option_min_approx=-10)
+    o = defined((g + 0.95 * g)[:24].reshape(2, 12))
+    from vqa_amd.optimizers import map_to_pi_range
+
+    want = p - 0.02 * np.concatenate([o.reshape(-1), g[24:]])
+    want = map_to_pi_range(want, q.optimizer.periodic_para_inds)
+    assert np.max(np.abs(path[1] - want)) < 1e-9

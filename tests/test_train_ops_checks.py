@@ -1,0 +1,168 @@
+"""Refusals of the softmax read-out and of the orthogonalised updates (C ABI and Python): no GPU is needed, every check comes
+before the device is touched.  The pointers are host memory that no call reads."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import vqa_amd
+from vqa_amd import _lib
+
+MEM = np.zeros(1 << 16, np.float64)
+P = MEM.ctypes.data
+
+
+def refused(rc, code, *words):
+    assert rc == code
+    msg = _lib.lib().vqa_last_error().decode()
+    for w in words:
+        assert w in msg, msg
+
+
+def score(dtype=0, z=P, rows=4, width=8, stride=8, scale=1.0, t=P + 4096, k=2, ws=None, lp=P + 8192, ent=P + 12288, tl=P + 16384,
+          ti=P + 20480):
+    return _lib.lib().vqa_log_probs_dev(0, None, dtype, z, rows, width, stride, scale, t, k, ws, lp, ent, tl, ti)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dtype=4), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "rows"), (dict(width=0), "width"),
+    (dict(width=2 ** 31, stride=2 ** 31), "width"), (dict(stride=7), "row stride"), (dict(stride=2 ** 41), "row stride"),
+    (dict(z=None), "NULL"), (dict(z=P + 4), "aligned"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(k=-1), "top_k"), (dict(k=9), "top_k"),
+    (dict(width=100, stride=100, k=65), "top_k"), (dict(tl=None), "top_log_prob"), (dict(ti=None), "top_log_prob"),
+    (dict(t=None), "targets"), (dict(width=5000, stride=5000, rows=1), "workspace"),
+    (dict(rows=2 ** 40, width=2 ** 30, stride=2 ** 30), "too large"),
+])
+def test_score_refusals(kw, word):
+    refused(score(**kw), _lib.EINVAL, word)
+
+
+def test_score_of_nothing():
+    assert score(rows=0, z=None, t=None, lp=None, ent=None, tl=None, ti=None) == 0
+
+
+def loss(dtype=0, z=P, rows=4, width=8, stride=8, scale=1.0, t=P + 4096, g=P + 4096, h=None, ws=None, lp=P + 8192, ent=None,
+         dz=P + 16384, dz_stride=8):
+    return _lib.lib().vqa_log_probs_grad_dev(0, None, dtype, z, rows, width, stride, scale, t, g, h, ws, lp, ent, dz, dz_stride)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dz=None), "dscores"), (dict(dz_stride=7), "dscores"), (dict(dz=P), "overlap"), (dict(dz=P + 8 * 31), "overlap"),
+    (dict(z=P + 8 * 31, dz=P), "overlap"), (dict(t=None), "targets"), (dict(t=None, lp=None), "targets"), (dict(scale=-2.0), "scale"),
+    (dict(dtype=9), "dtype"), (dict(width=3000, stride=3000, dz_stride=3000, rows=1, dz=P + 32768), "workspace"),
+])
+def test_loss_refusals(kw, word):
+    refused(loss(**kw), _lib.EINVAL, word)
+
+
+K = (C.c_double * 3)(*vqa_amd.orthogonal.COEFS)
+
+
+def ortho(dtype=0, g=P, batch=2, rows=4, cols=8, sr=8, sb=32, steps=5, k=K, eps=1e-7, ws=None, out=P + 8192):
+    return _lib.lib().vqa_orthogonalize_dev(0, None, dtype, g, batch, rows, cols, sr, sb, steps, k, eps, ws, out)
+
+
+def k3(*v):
+    return (C.c_double * 3)(*v)
+
+
+@pytest.mark.parametrize("kw,code,word", [
+    (dict(dtype=7), _lib.EINVAL, "dtype"), (dict(batch=-1), _lib.EINVAL, "batch"), (dict(batch=65536), _lib.EINVAL, "batch"),
+    (dict(rows=0), _lib.EINVAL, "rows"), (dict(cols=65537, sr=65537), _lib.EINVAL, "rows"), (dict(sr=7), _lib.EINVAL, "row_stride"),
+    (dict(sb=31), _lib.EINVAL, "batch_stride"), (dict(steps=0), _lib.EINVAL, "steps"), (dict(steps=101), _lib.EINVAL, "steps"),
+    (dict(k=None), _lib.EINVAL, "coefs"), (dict(k=k3(1, float("nan"), 0)), _lib.EINVAL, "finite"),
+    (dict(k=k3(5.0, 0, 0)), _lib.EUNSUPPORTED, "singular value"), (dict(k=k3(1.5, 0, 0)), _lib.EUNSUPPORTED, "singular value"),
+    (dict(k=k3(0.0, 0.0, 40.0)), _lib.EUNSUPPORTED, "polynomial"), (dict(eps=0.0), _lib.EINVAL, "eps"),
+    (dict(eps=float("inf")), _lib.EINVAL, "eps"), (dict(g=None), _lib.EINVAL, "g is NULL"), (dict(g=P + 2), _lib.EINVAL, "aligned"),
+    (dict(out=None), _lib.EINVAL, "out"), (dict(out=P + 8), _lib.EINVAL, "overlap"), (dict(out=P, sr=9, sb=36), _lib.EINVAL, "overlap"),
+    (dict(rows=100, cols=100, sr=100, sb=10000, batch=1, out=P + 80000), _lib.EINVAL, "workspace"),
+])
+def test_orthogonalize_refusals(kw, code, word):
+    refused(ortho(**kw), code, word)
+
+
+def test_ordinary_coefficients_pass_the_range_check():
+    # (3, -3.2, 1.2) and (15/8, -10/8, 3/8) stay within range for many steps; the check is the last before the batch of 0 returns
+    for k in (vqa_amd.orthogonal.COEFS, (3.0, -3.2, 1.2), (15 / 8, -10 / 8, 3 / 8), (1.5, -0.5, 0.0)):
+        assert ortho(batch=0, g=None, out=None, k=k3(*k), steps=100) == 0
+
+
+def step(dtype=0, w=P, g=P + 8192, m=P + 16384, batch=2, rows=4, cols=8, sr=8, sb=32, lr=0.1, mu=0.9, wd=0.0):
+    return _lib.lib().vqa_muon_step_dev(0, None, dtype, w, g, m, batch, rows, cols, sr, sb, lr, mu, wd, 1, 5, K, 1e-7, None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(w=None), "weight"), (dict(m=None), "weight"), (dict(m=P + 8), "overlap"), (dict(g=P + 8), "overlap"),
+    (dict(g=P + 16384), "overlap"), (dict(lr=float("nan")), "finite"), (dict(mu=float("inf")), "finite"), (dict(wd=float("nan")), "finite"),
+])
+def test_step_refusals(kw, word):
+    refused(step(**kw), _lib.EINVAL, word)
+
+
+def test_chain_refusals():
+    L = _lib.lib()
+    call = lambda e=P, B=2, n=3, o=1, d=P, ws=P, out=P: L.vqa_psr_chain_dev(0, None, e, B, n, o, 0.5, d, ws, out)
+    refused(call(B=-1), _lib.EINVAL, "n_samples")
+    refused(call(B=2 ** 22 + 1), _lib.EINVAL, "n_samples")
+    refused(call(o=0), _lib.EINVAL, "n_obs")
+    refused(call(out=None), _lib.EINVAL, "out")
+    refused(call(e=None), _lib.EINVAL, "NULL")
+    assert call(n=0) == 0
+
+
+def test_workspace_of_bad_arguments_is_zero():
+    L = _lib.lib()
+    assert L.vqa_log_probs_workspace(9, 1, 1, 0) == 0 and L.vqa_log_probs_workspace(0, -1, 1, 0) == 0
+    assert L.vqa_orthogonalize_workspace(0, 1, 0, 5) == 0
+    assert L.vqa_log_probs_workspace(0, 5, 3, 3) == 0
+    assert L.vqa_log_probs_workspace(0, 5, 10 ** 6, 3) > 0 and L.vqa_orthogonalize_workspace(2, 3, 500, 600) > 0
+
+
+def test_python_refusals():
+    z = np.zeros((3, 4))
+    for bad in (np.zeros(4), np.zeros((2, 3, 4))):
+        with pytest.raises(ValueError):
+            vqa_amd.log_probs(bad)
+    with pytest.raises(ValueError):
+        vqa_amd.log_probs(z, top_k=5)
+    with pytest.raises(ValueError):
+        vqa_amd.log_probs(z, targets=np.zeros(4, int))
+    with pytest.raises(ValueError):
+        vqa_amd.log_probs(z, targets=np.zeros(3))
+    with pytest.raises(ValueError):
+        vqa_amd.log_probs_grad(z, None, d_log_prob=1.0)
+    with pytest.raises(ValueError):
+        vqa_amd.log_probs_grad(z, np.zeros(3, int), 1.0, out=np.zeros((3, 5)))
+    with pytest.raises(ValueError):
+        vqa_amd.orthogonalize(np.zeros(4))
+    with pytest.raises(ValueError):
+        vqa_amd.orthogonalize(z, coefs=(1.0, 2.0))
+    with pytest.raises(ValueError):
+        vqa_amd.orthogonalize(z, out=np.zeros((4, 3)))
+    w = np.zeros((3, 4))
+    with pytest.raises(ValueError):
+        vqa_amd.muon_step(w.T, w.T, w.T, 0.1)          # not C-contiguous: an in-place step would go to a copy
+    with pytest.raises(ValueError):
+        vqa_amd.muon_step(w, w, np.zeros((4, 3)), 0.1)
+    import torch
+    with pytest.raises(ValueError):
+        vqa_amd.log_probs(torch.zeros(3, 4))           # a tensor on the host: numpy is the host path
+    with pytest.raises(ValueError):
+        vqa_amd.orthogonalize(torch.zeros(3, 4))
+
+
+def test_muon_needs_a_matrix():
+    class Target:
+        n_c_params, n_qubits = 14, 4
+        shots_counter = call_counter = circuit_counter = epoch_counter = [0]
+        methods_for_optimization = {}
+
+    with pytest.raises(ValueError, match="matrix_shape"):
+        vqa_amd.optimizers.Muon({}, dict(target_obj=Target(), init_params=np.zeros(14)))
+    with pytest.raises(ValueError, match="matrix_shape"):
+        vqa_amd.optimizers.Muon(dict(matrix_shape=(4, 4)), dict(target_obj=Target(), init_params=np.zeros(14)))
+    o = vqa_amd.optimizers.Muon(dict(matrix_shape=(2, 7)), dict(target_obj=Target(), init_params=np.zeros(14)))
+    assert o._shape() == (2, 7)
+    Target.n_c_params = 24
+    o = vqa_amd.optimizers.get_optimizer_class("Muon")({}, dict(target_obj=Target(), init_params=np.zeros(25)))
+    assert o._shape() == (2, 12)

@@ -15,5 +15,7 @@ from .qnn_classifier import myQNN_classifier  # noqa: F401
 from .vqe_target import PauliSumVQE  # noqa: F401
 from . import optimizers  # noqa: F401
 from .sampling import sample_counts, sample_z_means  # noqa: F401
+from .softmax import log_probs, log_probs_grad, psr_chain  # noqa: F401
+from .orthogonal import muon_step, orthogonalize  # noqa: F401
 
 __version__ = "0.1.0"

@@ -23,6 +23,9 @@ EXPORTS = (
     "vqa_statevector", "vqa_sample_counts", "vqa_sample_counts_dev", "vqa_dead_parameters", "vqa_psr_params_dev",
     "vqa_psr_full_noalloc_dev", "vqa_mse_stats_workspace", "vqa_mse_stats_dev", "vqa_mse_stats_shard_dev", "vqa_irandom_stats_dev", "vqa_class_grad_dev", "vqa_class_stats_dev", "vqa_sample_counts_shard_dev",
     "vqa_state_pass_counters", "vqa_light_cone_groups",
+    "vqa_log_probs_workspace", "vqa_log_probs_dev", "vqa_log_probs", "vqa_log_probs_grad_dev", "vqa_log_probs_grad",
+    "vqa_psr_chain_workspace", "vqa_psr_chain_dev",
+    "vqa_orthogonalize_workspace", "vqa_orthogonalize_dev", "vqa_orthogonalize", "vqa_muon_step_dev", "vqa_muon_step",
 )
 
 
@@ -84,11 +87,23 @@ def lib():
     L.vqa_sample_counts_shard_dev.argtypes = L.vqa_sample_counts_dev.argtypes + [C.c_int64]
     L.vqa_state_pass_counters.argtypes = [C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.c_int]
     L.vqa_light_cone_groups.argtypes = [vp, vp, C.c_int, C.c_int, C.c_int, C.c_int64, vp, C.c_int]
+    i32, i64, f64 = C.c_int, C.c_int64, C.c_double
+    L.vqa_log_probs_workspace.argtypes = [i32, i64, i64, i32]
+    L.vqa_log_probs_dev.argtypes = [i32, vp, i32, vp, i64, i64, i64, f64, ip, i32, vp, vp, vp, vp, ip]
+    L.vqa_log_probs.argtypes = [i32, i32, vp, i64, i64, i64, f64, ip, i32, vp, vp, vp, ip]
+    L.vqa_log_probs_grad_dev.argtypes = [i32, vp, i32, vp, i64, i64, i64, f64, ip, vp, vp, vp, vp, vp, vp, i64]
+    L.vqa_log_probs_grad.argtypes = [i32, i32, vp, i64, i64, i64, f64, ip, vp, vp, vp, vp, vp, i64]
+    L.vqa_psr_chain_workspace.argtypes = [i64, i32]
+    L.vqa_psr_chain_dev.argtypes = [i32, vp, dp, i64, i32, i32, f64, dp, dp, dp]
+    L.vqa_orthogonalize_workspace.argtypes = [i32, i32, i32, i32]
+    L.vqa_orthogonalize_dev.argtypes = [i32, vp, i32, vp, i32, i32, i32, i64, i64, i32, dp, f64, vp, vp]
+    L.vqa_orthogonalize.argtypes = [i32, i32, vp, i32, i32, i32, i64, i64, i32, dp, f64, vp]
+    L.vqa_muon_step_dev.argtypes = [i32, vp, i32, vp, vp, vp, i32, i32, i32, i64, i64, f64, f64, f64, i32, i32, dp, f64, vp]
+    L.vqa_muon_step.argtypes = [i32, i32, vp, vp, vp, i32, i32, i32, i64, i64, f64, f64, f64, i32, i32, dp, f64]
     for name in EXPORTS:
         fn = getattr(L, name)
-        if name not in ("vqa_last_error", "vqa_mse_stats_workspace"):
-            fn.restype = C.c_int
-    L.vqa_mse_stats_workspace.restype = C.c_int64
+        if name != "vqa_last_error":
+            fn.restype = C.c_int64 if name.endswith("_workspace") else C.c_int
     _lib = L
     return L
 

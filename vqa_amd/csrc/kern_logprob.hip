@@ -1,0 +1,599 @@
+// Softmax read-out of rows of scores: log probabilities of given outcomes, the rows' entropies and most probable
+// outcomes, and the gradient of a loss that weighs them.
+//
+// With x = scale * z and the row's maximum m:  s = sum over the row of exp(x - m), WITHOUT the one term 1 of the first
+// element that attains m, and t = sum exp(x - m) (x - m).  Then log p_c = (x_c - m) - log1p(s) and the entropy is
+// log1p(s) - t / (1 + s); both keep their relative accuracy for a row whose probability sits in one outcome, where
+// log(1 + s) would lose s.  (m, s, t) of two parts of a row join exactly like running maximum and sum of a softmax,
+// so a row is read once, by lanes, waves and workgroups that each take a part (Part, join).
+// m is kept as the stored score z: (z - m) * scale rounds the small difference and not the large product.
+#include <algorithm>
+
+#include "vqa_core.h"
+
+namespace vqa {
+
+namespace {
+
+constexpr int kT = 256;
+constexpr int kWaves = kT / 64;
+
+// ---- stored types: A is the type of the sums (64 bits for double, else 32) --------------------------------------
+struct F64 { using S = double; using A = double; static constexpr bool kFast = false;
+    static __device__ A up(S v) { return v; } static __device__ S down(A v) { return v; } };
+struct F32 { using S = float; using A = float; static constexpr bool kFast = false;
+    static __device__ A up(S v) { return v; } static __device__ S down(A v) { return v; } };
+struct F16 { using S = _Float16; using A = float; static constexpr bool kFast = true;
+    static __device__ A up(S v) { return (float)v; } static __device__ S down(A v) { return (_Float16)v; } };
+struct BF16 { using S = uint16_t; using A = float; static constexpr bool kFast = true;
+    static __device__ A up(S v) { return __uint_as_float((uint32_t)v << 16); }
+    static __device__ S down(A v) {   // round to nearest even; NaN stays NaN
+        const uint32_t u = __float_as_uint(v);
+        if (v != v) return (uint16_t)((u >> 16) | 0x40);
+        return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+    } };
+
+__device__ __forceinline__ double neg_inf(double) { return -__builtin_inf(); }
+__device__ __forceinline__ float neg_inf(float) { return -__builtin_inff(); }
+__device__ __forceinline__ double nan_of(double) { return __builtin_nan(""); }
+__device__ __forceinline__ float nan_of(float) { return __builtin_nanf(""); }
+__device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double exp_of(double d) { return exp(d); }
+__device__ __forceinline__ float exp_of(float d) { return expf(d); }
+__device__ __forceinline__ double log1p_of(double d) { return log1p(d); }
+__device__ __forceinline__ float log1p_of(float d) { return log1pf(d); }
+
+// exp(d) for d <= 0.  Scores of 16 bits: the hardware's exp2 of the rounded product, off by |d| 2^-24 of a term exp(d),
+// which adds at most 2^-25 to a sum and is far below a 16-bit gradient's own rounding.
+template <class Ty>
+__device__ __forceinline__ typename Ty::A exp_neg(typename Ty::A d) {
+    if constexpr (Ty::kFast) return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+    else return exp_of(d);
+}
+
+// below this difference a term is 0 in every type; sums take it in place of -inf, whose product with 0 is NaN
+template <class A>
+__device__ __forceinline__ A floor_of(A d) { return max_of(d, A(-16000)); }
+
+template <class A>
+struct Part {
+    A m, s, t;   // m = -inf: nothing seen but masked places (s is then 0, or NaN once a NaN was seen)
+};
+
+template <class A>
+__device__ __forceinline__ Part<A> join(const Part<A>& a, const Part<A>& b, A scale) {
+    const A ni = neg_inf(A(0));
+    const bool a_first = a.m >= b.m;
+    const Part<A>&hi = a_first ? a : b, &lo = a_first ? b : a;
+    if (lo.m == ni) return Part<A>{ hi.m, hi.s + lo.s, hi.t };   // lo.s: 0, or NaN
+    const A d = floor_of((lo.m - hi.m) * scale), f = exp_of(d), all = lo.s + A(1);
+    return Part<A>{ hi.m, hi.s + f * all, hi.t + f * (lo.t + d * all) };
+}
+
+// the finished row; a NaN or +inf among the scores makes everything NaN
+template <class A>
+struct Row {
+    A m, ls, entropy;   // log p = (z - m) * scale - ls
+    bool bad, empty;
+};
+template <class A>
+__device__ __forceinline__ Row<A> finish(const Part<A>& p) {
+    Row<A> r;
+    r.m = p.m;
+    r.bad = p.s != p.s || p.m == -neg_inf(A(0));
+    r.empty = !r.bad && p.m == neg_inf(A(0));
+    r.ls = log1p_of(p.s);
+    r.entropy = r.bad ? nan_of(A(0)) : (r.empty ? A(0) : r.ls - p.t / (A(1) + p.s));
+    return r;
+}
+template <class A>
+__device__ __forceinline__ A log_p(const Row<A>& r, A z, A scale) {
+    if (r.bad) return nan_of(A(0));
+    if (r.empty || z == neg_inf(A(0))) return neg_inf(A(0));
+    return (z - r.m) * scale - r.ls;
+}
+// a target of a row: < 0 none, >= width does not exist (the row's outputs become NaN)
+template <class A>
+__device__ __forceinline__ void given(Row<A>& r, int target, int64_t width) {
+    if (target >= 0 && (int64_t)target >= width) {
+        r.bad = true;
+        r.empty = false;
+        r.entropy = nan_of(A(0));
+    }
+}
+
+template <class A>
+__device__ __forceinline__ bool before(A v, int i, A w, int j) { return v > w || (v == w && i < j); }
+
+template <class A>
+struct Grad {   // weights of a row's log probability and entropy in the loss
+    A g, h;
+};
+// d loss / d z_c = scale (g (delta - p) - h p (log p + H))
+template <class Ty>
+__device__ __forceinline__ typename Ty::A slope(const Row<typename Ty::A>& r, typename Ty::A z, typename Ty::A scale, bool hit,
+                                                const Grad<typename Ty::A>& w) {
+    using A = typename Ty::A;
+    if (r.bad) return nan_of(A(0));
+    if (r.empty) return A(0);
+    A v = hit ? w.g : A(0);
+    const A lp = (z - r.m) * scale - r.ls;
+    const A p = exp_neg<Ty>(lp);
+    if (p > A(0)) v -= p * (w.g + w.h * (lp + r.entropy));
+    return v * scale;
+}
+
+// ---- short rows: G lanes of a wave hold a row, E elements each ----------------------------------------------------
+// Everything stays in registers; the best outcomes are taken one by one (an argmax over the lanes' own best).
+template <class Ty, int G, int E, bool kGrad>
+__global__ __launch_bounds__(kT) void k_lp_short(const typename Ty::S* __restrict__ z, int64_t rows, int width, int64_t ld,
+                                                 typename Ty::A scale, const int32_t* __restrict__ target, int top_k,
+                                                 const typename Ty::A* __restrict__ dg, const typename Ty::A* __restrict__ dh,
+                                                 typename Ty::A* lp_out, typename Ty::A* ent_out, typename Ty::A* top_lp,
+                                                 int32_t* top_ix, typename Ty::S* dz, int64_t ld_dz) {
+    using A = typename Ty::A;
+    constexpr int kRows = kT / G;
+    const int lane = threadIdx.x % G;
+    for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * kRows) {
+        const typename Ty::S* zr = z + row * ld;
+        A v[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int c = lane + G * i;
+            v[i] = c < width ? Ty::up(zr[c]) : neg_inf(A(0));
+        }
+        A m = v[0];
+        bool nan = v[0] != v[0];
+#pragma unroll
+        for (int i = 1; i < E; ++i) {
+            m = max_of(m, v[i]);
+            nan |= v[i] != v[i];
+        }
+        if (nan) m = neg_inf(A(0));
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) m = max_of(m, __shfl_xor(m, o, G));
+        const A base = m == neg_inf(A(0)) ? A(0) : m;
+        // which element is the one whose term is left out: the first at the maximum
+        int first = 0x7fffffff;
+#pragma unroll
+        for (int i = E - 1; i >= 0; --i)
+            if (v[i] == m) first = lane + G * i;
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) first = min(first, __shfl_xor(first, o, G));
+        A s = nan ? nan_of(A(0)) : A(0), t = A(0);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const A d = (v[i] - base) * scale;
+            const bool skip = v[i] == neg_inf(A(0)) || lane + G * i == first;
+            const A e = skip ? A(0) : exp_neg<Ty>(d);
+            s += e;
+            t += skip ? A(0) : e * floor_of(d);
+        }
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) {
+            s += __shfl_xor(s, o, G);
+            t += __shfl_xor(t, o, G);
+        }
+        Row<A> r = finish(Part<A>{ m, s, t });
+        const int tg = target ? target[row] : -1;
+        given(r, tg, width);
+        if (lane == 0) {
+            if (ent_out) ent_out[row] = r.entropy;
+            if (lp_out) lp_out[row] = r.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(r, Ty::up(zr[tg]), scale));
+        }
+        if constexpr (kGrad) {
+            const Grad<A> w = { tg < 0 ? A(0) : (dg ? dg[row] : A(0)), dh ? dh[row] : A(0) };
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int c = lane + G * i;
+                if (c < width) dz[row * ld_dz + c] = Ty::down(slope<Ty>(r, v[i], scale, c == tg, w));
+            }
+        } else {
+            uint32_t used = 0;
+            for (int k = 0; k < top_k; ++k) {
+                A bv = neg_inf(A(0));
+                int bi = 0x7fffffff, at = -1;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (!(used >> i & 1) && v[i] > bv) { bv = v[i]; bi = lane + G * i; at = i; }
+                const int mine = bi;
+#pragma unroll
+                for (int o = 1; o < G; o <<= 1) {
+                    const A ov = __shfl_xor(bv, o, G);
+                    const int oi = __shfl_xor(bi, o, G);
+                    if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+                }
+                if (at >= 0 && mine == bi) used |= 1u << at;
+                if (lane == 0) {
+                    const bool none = r.bad || bi == 0x7fffffff;
+                    top_lp[row * top_k + k] = r.bad ? nan_of(A(0)) : (none ? neg_inf(A(0)) : log_p(r, bv, scale));
+                    top_ix[row * top_k + k] = none ? -1 : bi;
+                }
+            }
+        }
+    }
+}
+
+// ---- long rows ----------------------------------------------------------------------------------------------------
+// A workgroup reads one of `splits` equal parts of a row, in 16-byte pieces; part boundaries and the first piece are
+// aligned in memory, elements outside the row count as masked (-inf).
+template <class Ty>
+struct Piece {
+    static constexpr int N = 16 / sizeof(typename Ty::S);
+    int64_t off, pieces;            // elements before the row in its first piece; pieces of the whole row
+    __device__ Piece(const typename Ty::S* row, int64_t width) {
+        off = (int64_t)(((uintptr_t)row & 15) / sizeof(typename Ty::S));
+        pieces = (off + width + N - 1) / N;
+    }
+};
+
+template <class Ty>
+__device__ __forceinline__ void load_piece(const typename Ty::S* zr, int64_t e0, int64_t width, typename Ty::A* v) {
+    constexpr int N = Piece<Ty>::N;
+    if (e0 >= 0 && e0 + N <= width) {
+        alignas(16) typename Ty::S raw[N];
+        *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(zr + e0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = Ty::up(raw[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = e0 + j >= 0 && e0 + j < width ? Ty::up(zr[e0 + j]) : neg_inf(typename Ty::A(0));
+    }
+}
+
+// a wave's list of its best outcomes, one a lane, best first (value, then lower index)
+template <class A>
+struct Best {
+    A v;
+    int i;
+};
+template <class A>
+__device__ __forceinline__ void insert(Best<A>& b, A v, int i, int lane) {
+    const int pos = __popcll(__ballot(before(b.v, b.i, v, i)));
+    const A uv = __shfl_up(b.v, 1);
+    const int ui = __shfl_up(b.i, 1);
+    if (lane == pos) { b.v = v; b.i = i; }
+    else if (lane > pos) { b.v = uv; b.i = ui; }
+}
+
+template <class Ty, int B, bool kTop>
+__device__ __forceinline__ void take(const typename Ty::A* v, const int64_t* at, Part<typename Ty::A>& p, Best<typename Ty::A>& best,
+                                     int top_k, typename Ty::A scale, int lane) {
+    using A = typename Ty::A;
+    constexpr int N = Piece<Ty>::N;
+    A mx = v[0];
+#pragma unroll
+    for (int j = 1; j < B; ++j) mx = max_of(mx, v[j]);
+    if constexpr (kTop) {
+        A kv = __shfl(best.v, top_k - 1);
+        if (__any(mx >= kv && mx > neg_inf(A(0)))) {
+            int ki = __shfl(best.i, top_k - 1);
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const int ix = (int)(at[j / N] + j % N);
+                uint64_t want = __ballot(v[j] > neg_inf(A(0)) && before(v[j], ix, kv, ki));
+                while (want) {
+                    const int src = __builtin_ctzll(want);
+                    insert(best, __shfl(v[j], src), __shfl(ix, src), lane);
+                    kv = __shfl(best.v, top_k - 1);
+                    ki = __shfl(best.i, top_k - 1);
+                    want &= want - 1;
+                    want &= __ballot(before(v[j], ix, kv, ki));
+                }
+            }
+        }
+    }
+    const A m = max_of(p.m, mx);                 // (a NaN is not taken as the maximum, it shows in s)
+    const A base = m == neg_inf(A(0)) ? A(0) : m;
+    bool left_out = !(mx > p.m);                 // the maximum stays where it was: its term is out already
+    if (!left_out && p.m > neg_inf(A(0))) {      // the old maximum's term comes in
+        const A d = floor_of((p.m - m) * scale), f = exp_neg<Ty>(d), all = p.s + A(1);
+        p.s = f * all;
+        p.t = f * (p.t + d * all);
+    }
+    p.m = m;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+        const A d = (v[j] - base) * scale;
+        const bool out = !left_out && v[j] == m;
+        left_out |= out;
+        const A e = out ? A(0) : exp_neg<Ty>(d);
+        p.s += e;
+        p.t += e * floor_of(d);
+    }
+}
+
+// the same row part by one workgroup; the result is complete in wave 0 (all lanes)
+template <class Ty, bool kTop>
+__device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* zr, int64_t width, int64_t split, int64_t splits,
+                                                          typename Ty::A scale, int top_k, Best<typename Ty::A>& best) {
+    using A = typename Ty::A;
+    constexpr int N = Piece<Ty>::N, U = 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Piece<Ty> pc(zr, width);
+    const int64_t per = (pc.pieces + splits - 1) / splits;
+    const int64_t p0 = split * per, p1 = min(pc.pieces, p0 + per);
+    Part<A> p = { neg_inf(A(0)), A(0), A(0) };
+    best = Best<A>{ neg_inf(A(0)), 0x7fffffff };
+    for (int64_t q = p0 + wave * 64; q < p1; q += kT * U) {    // the same count for a wave's lanes
+        A v[U * N];
+        int64_t at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t piece = q + u * kT + lane;
+            at[u] = piece * N - pc.off;
+            load_piece<Ty>(zr, piece < p1 ? at[u] : width, width, v + u * N);
+        }
+        take<Ty, U * N, kTop>(v, at, p, best, top_k, scale, lane);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
+    __shared__ Part<A> sp[kWaves];
+    __shared__ Best<A> sb[kWaves][64];
+    if (lane == 0) sp[wave] = p;
+    if constexpr (kTop) sb[wave][lane] = best;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) p = join(p, sp[w], scale);
+        if constexpr (kTop) {
+            for (int w = 1; w < kWaves; ++w)
+                for (int k = 0; k < top_k; ++k) {
+                    const Best<A> c = sb[w][k];
+                    if (!(c.v > neg_inf(A(0))) || !before(c.v, c.i, __shfl(best.v, top_k - 1), __shfl(best.i, top_k - 1))) break;
+                    insert(best, c.v, c.i, lane);
+                }
+        }
+    }
+    return p;
+}
+
+template <class A>
+struct Ws {   // the parts of the rows, and the parts' best outcomes
+    Part<A>* part;
+    Best<A>* best;
+};
+
+template <class Ty, bool kTop>
+__global__ __launch_bounds__(kT) void k_lp_parts(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                 typename Ty::A scale, int top_k, int splits, Ws<typename Ty::A> ws) {
+    using A = typename Ty::A;
+    for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
+        const int64_t row = it / splits, split = it - row * splits;
+        Best<A> best;
+        const Part<A> p = read_part<Ty, kTop>(z + row * ld, width, split, splits, scale, top_k, best);
+        if (threadIdx.x == 0) ws.part[it] = p;
+        if constexpr (kTop)
+            if ((int)threadIdx.x < top_k) ws.best[it * top_k + threadIdx.x] = best;
+        __syncthreads();   // the shared arrays are written again
+    }
+}
+
+// one wave a row: joins its parts (at most 64, one a lane, in a fixed tree) and merges their lists of best outcomes
+template <class Ty>
+__global__ __launch_bounds__(64) void k_lp_join(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                typename Ty::A scale, const int32_t* __restrict__ target, int top_k, int splits,
+                                                Ws<typename Ty::A> ws, typename Ty::A* lp_out, typename Ty::A* ent_out,
+                                                typename Ty::A* top_lp, int32_t* top_ix) {
+    using A = typename Ty::A;
+    const int lane = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        Part<A> p = { neg_inf(A(0)), A(0), A(0) };
+        if (lane < splits) p = ws.part[row * splits + lane];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
+        Row<A> r = finish(p);
+        const int tg = target ? target[row] : -1;
+        given(r, tg, width);
+        if (lane == 0) {
+            if (ent_out) ent_out[row] = r.entropy;
+            if (lp_out) lp_out[row] = r.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(r, Ty::up(z[row * ld + tg]), scale));
+        }
+        int head = 0;
+        Best<A> c = { neg_inf(A(0)), 0x7fffffff };
+        if (lane < splits && top_k > 0) c = ws.best[(row * splits + lane) * top_k];
+        for (int k = 0; k < top_k; ++k) {
+            A bv = c.v;
+            int bi = c.i;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const A ov = __shfl_xor(bv, o);
+                const int oi = __shfl_xor(bi, o);
+                if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+            }
+            const bool none = r.bad || bi == 0x7fffffff;
+            if (lane == 0) {
+                top_lp[row * top_k + k] = r.bad ? nan_of(A(0)) : (none ? neg_inf(A(0)) : log_p(r, bv, scale));
+                top_ix[row * top_k + k] = none ? -1 : bi;
+            }
+            if (c.i == bi && bi != 0x7fffffff) {
+                ++head;
+                c = head < top_k ? ws.best[(row * splits + lane) * top_k + head] : Best<A>{ neg_inf(A(0)), 0x7fffffff };
+            }
+        }
+    }
+}
+
+// the gradient of one part of a row, from the joined parts
+template <class Ty>
+__global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                 typename Ty::A scale, const int32_t* __restrict__ target,
+                                                 const typename Ty::A* __restrict__ dg, const typename Ty::A* __restrict__ dh,
+                                                 int splits, Ws<typename Ty::A> ws, typename Ty::A* lp_out, typename Ty::A* ent_out,
+                                                 typename Ty::S* dz, int64_t ld_dz) {
+    using A = typename Ty::A;
+    const int lane = threadIdx.x & 63;
+    for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
+        const int64_t row = it / splits, split = it - row * splits;
+        const typename Ty::S* zr = z + row * ld;
+        typename Ty::S* dr = dz + row * ld_dz;
+        Part<A> p = { neg_inf(A(0)), A(0), A(0) };
+        if (lane < splits) p = ws.part[row * splits + lane];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
+        Row<A> r = finish(p);
+        const int tg = target ? target[row] : -1;
+        given(r, tg, width);
+        if (split == 0 && threadIdx.x == 0) {
+            if (ent_out) ent_out[row] = r.entropy;
+            if (lp_out) lp_out[row] = r.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(r, Ty::up(zr[tg]), scale));
+        }
+        const Grad<A> w = { tg < 0 ? A(0) : (dg ? dg[row] : A(0)), dh ? dh[row] : A(0) };
+        const int64_t per = (width + splits - 1) / splits;
+        const int64_t c1 = min(width, (split + 1) * per);
+        for (int64_t c = split * per + threadIdx.x; c < c1; c += kT)
+            dr[c] = Ty::down(slope<Ty>(r, Ty::up(zr[c]), scale, c == tg, w));
+    }
+}
+
+// ---- the chain into circuit parameters ------------------------------------------------------------------------------
+// part[chunk][i] = sum over the chunk's samples b and observables o of d[b][o] (E[b][1 + 2 i][o] - E[b][2 + 2 i][o]):
+// a lane a parameter (neighbouring lanes read neighbouring rows of the sweep), a wave a quarter of the chunk.
+constexpr int kChainRows = 64;
+
+__global__ __launch_bounds__(kT) void k_psr_chain(const double* __restrict__ e, int64_t B, int P, int n_obs,
+                                                  const double* __restrict__ d, double* __restrict__ part) {
+    __shared__ double sh[kWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = (int64_t)blockIdx.y * 64 + lane, K = 2 * (int64_t)P + 1;
+    const int64_t b0 = (int64_t)blockIdx.x * kChainRows, b1 = min(B, b0 + kChainRows);
+    double s = 0.0;
+    if (i < P)
+        for (int64_t b = b0 + wave; b < b1; b += kWaves) {
+            const double* up = e + (b * K + 1 + 2 * i) * n_obs;
+            const double* db = d + b * n_obs;
+            for (int o = 0; o < n_obs; ++o) s += db[o] * (up[o] - up[n_obs + o]);
+        }
+    sh[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && i < P) part[blockIdx.x * (int64_t)P + i] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+}
+__global__ __launch_bounds__(kT) void k_psr_chain_sum(const double* __restrict__ part, int64_t chunks, int P, double factor,
+                                                      double* __restrict__ out) {
+    const int i = blockIdx.x * kT + threadIdx.x;
+    if (i >= P) return;
+    double s = 0.0;
+    for (int64_t c = 0; c < chunks; ++c) s += part[c * P + i];
+    out[i] = factor * s;
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+constexpr int kShortWidth = 1024;
+constexpr int64_t kMaxGrid = 1 << 20;
+
+// Parts of a row: enough workgroups for the chip (about 4 a CU) while a part keeps 4096 elements, at most one a lane of
+// the joining wave.
+int splits_of(int64_t rows, int64_t width) {
+    int64_t s = (1024 + rows - 1) / rows;
+    const int64_t most = width / 4096;
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+}
+
+template <class Ty, bool kGrad>
+void launch_short(hipStream_t st, const typename Ty::S* z, int64_t rows, int width, int64_t ld, double scale, const int32_t* target,
+                  int top_k, const typename Ty::A* dg, const typename Ty::A* dh, typename Ty::A* lp, typename Ty::A* ent,
+                  typename Ty::A* top_lp, int32_t* top_ix, typename Ty::S* dz, int64_t ld_dz) {
+#define VQA_SHORT(G, E)                                                                                                      \
+    hipLaunchKernelGGL((k_lp_short<Ty, G, E, kGrad>), dim3((unsigned)std::min<int64_t>(kMaxGrid, (rows + kT / G - 1) / (kT / G))), \
+                       dim3(kT), 0, st, z, rows, width, ld, (typename Ty::A)scale, target, top_k, dg, dh, lp, ent, top_lp,   \
+                       top_ix, dz, ld_dz)
+    if (width <= 4) VQA_SHORT(4, 1);
+    else if (width <= 16) VQA_SHORT(4, 4);
+    else if (width <= 64) VQA_SHORT(16, 4);
+    else if (width <= 256) VQA_SHORT(64, 4);
+    else VQA_SHORT(64, 16);
+#undef VQA_SHORT
+}
+
+template <class A>
+Ws<A> ws_of(void* p, int64_t parts) {
+    return Ws<A>{ (Part<A>*)p, (Best<A>*)((char*)p + (parts * sizeof(Part<A>) + 15) / 16 * 16) };
+}
+
+template <class Ty>
+int score(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld, double scale, const int32_t* target, int top_k,
+          void* ws, void* lp, void* ent, void* top_lp, int32_t* top_ix) {
+    using A = typename Ty::A;
+    const auto* zz = (const typename Ty::S*)z;
+    if (width <= kShortWidth) {
+        launch_short<Ty, false>(st, zz, rows, (int)width, ld, scale, target, top_k, nullptr, nullptr, (A*)lp, (A*)ent, (A*)top_lp,
+                                top_ix, nullptr, 0);
+    } else {
+        const int splits = splits_of(rows, width);
+        const Ws<A> w = ws_of<A>(ws, rows * splits);
+        const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows * splits)), grid2((unsigned)std::min<int64_t>(kMaxGrid, rows));
+        if (top_k > 0) hipLaunchKernelGGL((k_lp_parts<Ty, true>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w);
+        else hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w);
+        hipLaunchKernelGGL((k_lp_join<Ty>), grid2, dim3(64), 0, st, zz, rows, width, ld, (A)scale, target, top_k, splits, w, (A*)lp,
+                           (A*)ent, (A*)top_lp, top_ix);
+    }
+    VQA_HIP(hipGetLastError());
+    return VQA_OK;
+}
+
+template <class Ty>
+int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld, double scale, const int32_t* target, const void* dg,
+         const void* dh, void* ws, void* lp, void* ent, void* dz, int64_t ld_dz) {
+    using A = typename Ty::A;
+    const auto* zz = (const typename Ty::S*)z;
+    if (width <= kShortWidth) {
+        launch_short<Ty, true>(st, zz, rows, (int)width, ld, scale, target, 0, (const A*)dg, (const A*)dh, (A*)lp, (A*)ent, nullptr,
+                               nullptr, (typename Ty::S*)dz, ld_dz);
+    } else {
+        const int splits = splits_of(rows, width);
+        const Ws<A> w = ws_of<A>(ws, rows * splits);
+        const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows * splits));
+        hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, 0, splits, w);
+        hipLaunchKernelGGL((k_lp_slope<Ty>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, target, (const A*)dg, (const A*)dh,
+                           splits, w, (A*)lp, (A*)ent, (typename Ty::S*)dz, ld_dz);
+    }
+    VQA_HIP(hipGetLastError());
+    return VQA_OK;
+}
+
+}  // namespace
+
+size_t log_probs_workspace_bytes(int dtype, int64_t rows, int64_t width, int top_k) {
+    if (width <= kShortWidth || rows <= 0) return 0;
+    const size_t parts = (size_t)rows * splits_of(rows, width);
+    const bool wide = dtype == VQA_DTYPE_F64;
+    return (parts * (wide ? sizeof(Part<double>) : sizeof(Part<float>)) + 15) / 16 * 16 +
+           parts * top_k * (wide ? sizeof(Best<double>) : sizeof(Best<float>));
+}
+
+int log_probs_launch(hipStream_t st, int dtype, const void* z, int64_t rows, int64_t width, int64_t ld, double scale,
+                     const int32_t* target, int top_k, void* ws, void* lp, void* ent, void* top_lp, int32_t* top_ix) {
+    switch (dtype) {
+        case VQA_DTYPE_F64: return score<F64>(st, z, rows, width, ld, scale, target, top_k, ws, lp, ent, top_lp, top_ix);
+        case VQA_DTYPE_F32: return score<F32>(st, z, rows, width, ld, scale, target, top_k, ws, lp, ent, top_lp, top_ix);
+        case VQA_DTYPE_BF16: return score<BF16>(st, z, rows, width, ld, scale, target, top_k, ws, lp, ent, top_lp, top_ix);
+        default: return score<F16>(st, z, rows, width, ld, scale, target, top_k, ws, lp, ent, top_lp, top_ix);
+    }
+}
+
+int log_probs_grad_launch(hipStream_t st, int dtype, const void* z, int64_t rows, int64_t width, int64_t ld, double scale,
+                          const int32_t* target, const void* dg, const void* dh, void* ws, void* lp, void* ent, void* dz,
+                          int64_t ld_dz) {
+    switch (dtype) {
+        case VQA_DTYPE_F64: return loss<F64>(st, z, rows, width, ld, scale, target, dg, dh, ws, lp, ent, dz, ld_dz);
+        case VQA_DTYPE_F32: return loss<F32>(st, z, rows, width, ld, scale, target, dg, dh, ws, lp, ent, dz, ld_dz);
+        case VQA_DTYPE_BF16: return loss<BF16>(st, z, rows, width, ld, scale, target, dg, dh, ws, lp, ent, dz, ld_dz);
+        default: return loss<F16>(st, z, rows, width, ld, scale, target, dg, dh, ws, lp, ent, dz, ld_dz);
+    }
+}
+
+size_t psr_chain_workspace_bytes(int64_t B, int P) { return (size_t)((B + kChainRows - 1) / kChainRows) * P * 8; }
+
+int psr_chain_launch(hipStream_t st, const double* e, int64_t B, int P, int n_obs, double factor, const double* d, double* ws,
+                     double* out) {
+    const int64_t chunks = (B + kChainRows - 1) / kChainRows;
+    if (chunks > 0)
+        hipLaunchKernelGGL(k_psr_chain, dim3((unsigned)chunks, (unsigned)((P + 63) / 64)), dim3(kT), 0, st, e, B, P, n_obs, d, ws);
+    hipLaunchKernelGGL(k_psr_chain_sum, dim3((unsigned)((P + kT - 1) / kT)), dim3(kT), 0, st, ws, chunks, P, factor, out);
+    VQA_HIP(hipGetLastError());
+    return VQA_OK;
+}
+
+}  // namespace vqa

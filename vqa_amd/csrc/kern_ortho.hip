@@ -1,0 +1,561 @@
+// Orthogonalised updates: Newton-Schulz products that carry the singular values of a matrix towards 1, and the
+// optimizer step around them (momentum, orthogonalisation, weight update).
+//
+// X0 = G / (|G|_F + eps), then `steps` times  A = X X^T,  X <- a X + (b A + c A A) X.  A singular value s of X goes to
+// a s + b s^3 + c s^5 and the singular vectors stay, so the result is U p(S) V^T of G = U S V^T without an SVD.
+// r = min(rows, cols), c = max: X is taken r x c (the transpose of a matrix with more rows than columns).
+//
+// Two forms:
+// * r <= 64 and X fits the LDS of a CU: one workgroup carries a matrix through all steps (k_ns_small), in 64-bit or
+//   32-bit matrix instructions.
+// * else: three tiled products a step (k_ns_product), X, X^T, A and b A + c A A in device memory, all row-major with the
+//   summed index contiguous, padded with zeros to whole tiles.  64-bit matrices use 64-bit matrix instructions; the
+//   others hold every value as a sum of two 16-bit floats hi + lo (22 bits and a sign, scaled so that neither part
+//   leaves its normal range) and take the three products hi hi + hi lo + lo hi with 32-bit sums: the left-out lo lo is
+//   2^-22 of a product, the size of the roundings that 32-bit products make along a sum, at 5 times their rate.
+#include <math.h>
+
+#include <algorithm>
+
+#include "vqa_core.h"
+
+namespace vqa {
+
+namespace {
+
+constexpr int kT = 256;
+constexpr int kWaves = kT / 64;
+
+typedef double double4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+
+// ---- stored types; C: the type of the state and of the products' sums --------------------------------------------
+struct F64 { using S = double; using C = double;
+    static __device__ C up(S v) { return v; } static __device__ S down(C v) { return v; } };
+struct F32 { using S = float; using C = float;
+    static __device__ C up(S v) { return v; } static __device__ S down(C v) { return v; } };
+struct F16 { using S = _Float16; using C = float;
+    static __device__ C up(S v) { return (float)v; } static __device__ S down(C v) { return (_Float16)v; } };
+struct BF16 { using S = uint16_t; using C = float;
+    static __device__ C up(S v) { return __uint_as_float((uint32_t)v << 16); }
+    static __device__ S down(C v) {   // round to nearest even; NaN stays NaN
+        const uint32_t u = __float_as_uint(v);
+        if (v != v) return (uint16_t)((u >> 16) | 0x40);
+        return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+    } };
+
+// what a call does, by value to every kernel
+template <class Ty>
+struct Job {
+    using S = typename Ty::S;
+    using C = typename Ty::C;
+    const S* g;
+    int64_t g_row, g_batch;    // strides in elements
+    S* out;                    // [batch, rows, cols], contiguous (null: an optimizer step)
+    C* w;                      // optimizer step: weights and momentum, contiguous
+    C* m;
+    C mu, decay, rate;         // w <- decay w - rate O
+    int nesterov;
+    int batch, rows, cols, r, c, turned, steps;
+    C ka, kb, kc;
+    double eps;
+
+    // element e of a matrix in row-major order as it enters the products; first: the momentum is brought up to date
+    template <bool kFirst>
+    __device__ __forceinline__ C enter(int b, int64_t row, int64_t col) const {
+        const C v = Ty::up(g[b * g_batch + row * g_row + col]);
+        if (!m) return v;
+        const int64_t at = ((int64_t)b * rows + row) * cols + col;
+        C mm = m[at];
+        if (kFirst) m[at] = mm = mu * mm + v;
+        return nesterov ? v + mu * mm : mm;
+    }
+    __device__ __forceinline__ void leave(int b, int64_t row, int64_t col, C o) const {
+        const int64_t at = ((int64_t)b * rows + row) * cols + col;
+        if (m) w[at] = decay * w[at] - rate * o;
+        else out[at] = Ty::down(o);
+    }
+};
+
+__device__ __forceinline__ double block_sum(double v, double* sh) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) s += sh[w];
+    return s;
+}
+
+// ---- 16 x 16 x 4 matrix instruction: lane l holds A[l % 16][l / 16], B[l / 16][l % 16]; D[row(l, reg)][l % 16] ------
+template <class C> struct Mma;
+template <> struct Mma<double> {
+    using Acc = double4v;
+    static __device__ Acc go(double a, double b, Acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+    static __device__ int row(int l, int reg) { return (l >> 4) + 4 * reg; }
+};
+template <> struct Mma<float> {
+    using Acc = float4v;
+    static __device__ Acc go(float a, float b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+    static __device__ int row(int l, int reg) { return 4 * (l >> 4) + reg; }
+};
+
+// ---- one workgroup a matrix ---------------------------------------------------------------------------------------
+constexpr int kSmallRows = 64;
+
+int pad16(int v) { return (v + 15) / 16 * 16; }
+size_t small_lds(int r, int c, size_t size) {
+    const size_t rp = pad16(r), cp = pad16(c);
+    return (rp * (cp + 4) + 2 * rp * (rp + 4) + 4 * 256) * size + 64;
+}
+
+template <class Ty>
+__global__ __launch_bounds__(kT) void k_ns_small(Job<Ty> j) {
+    using C = typename Ty::C;
+    using Acc = typename Mma<C>::Acc;
+    extern __shared__ char lds[];
+    const int rp = (j.r + 15) / 16 * 16, cp = (j.c + 15) / 16 * 16, nt = rp / 16;
+    const int ldx = cp + 4, lda = rp + 4;
+    double* sh = (double*)lds;
+    C* X = (C*)(lds + 64);
+    C* A = X + rp * ldx;
+    C* B = A + rp * lda;
+    C* part = B + rp * lda;              // [4][256]: a single tile's product, its summed index in four parts
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lk = lane >> 4;
+
+    for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
+        for (int i = threadIdx.x; i < rp * ldx; i += kT) X[i] = C(0);
+        __syncthreads();
+        double ss = 0;
+        const int n = j.rows * j.cols;
+        for (int e = threadIdx.x; e < n; e += kT) {
+            const int row = e / j.cols, col = e - row * j.cols;
+            const C v = j.template enter<true>(b, row, col);
+            X[j.turned ? col * ldx + row : row * ldx + col] = v;
+            ss += (double)v * (double)v;
+        }
+        const double norm = sqrt(block_sum(ss, sh)) + j.eps;
+        for (int i = threadIdx.x; i < rp * ldx; i += kT) X[i] = (C)((double)X[i] / norm);
+        __syncthreads();
+
+        const int tiles = nt * (nt + 1) / 2, parts = nt == 1 ? kWaves : 1;
+        for (int s = 0; s < j.steps; ++s) {
+            // A = X X^T, its lower tiles
+            for (int it = wave; it < tiles * parts; it += kWaves) {
+                const int t = it / parts, p = it - t * parts;
+                int ti = 0;
+                while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+                const int tj = t - ti * (ti + 1) / 2, len = cp / parts;
+                const C* xa = X + (ti * 16 + lr) * ldx + p * len + lk;
+                const C* xb = X + (tj * 16 + lr) * ldx + p * len + lk;
+                Acc acc = { 0, 0, 0, 0 };
+                for (int k = 0; k < len; k += 4) acc = Mma<C>::go(xa[k], xb[k], acc);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = Mma<C>::row(lane, q);
+                    if (parts > 1) part[p * 256 + row * 16 + lr] = acc[q];
+                    else {
+                        A[(ti * 16 + row) * lda + tj * 16 + lr] = acc[q];
+                        A[(tj * 16 + lr) * lda + ti * 16 + row] = acc[q];
+                    }
+                }
+            }
+            __syncthreads();
+            if (parts > 1) {
+                const int e = threadIdx.x;
+                A[(e >> 4) * lda + (e & 15)] = (part[e] + part[256 + e]) + (part[512 + e] + part[768 + e]);
+                __syncthreads();
+            }
+            // B = b A + c A A
+            for (int t = wave; t < tiles; t += kWaves) {
+                int ti = 0;
+                while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+                const int tj = t - ti * (ti + 1) / 2;
+                const C* xa = A + (ti * 16 + lr) * lda + lk;
+                const C* xb = A + (tj * 16 + lr) * lda + lk;
+                Acc acc = { 0, 0, 0, 0 };
+                for (int k = 0; k < rp; k += 4) acc = Mma<C>::go(xa[k], xb[k], acc);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = Mma<C>::row(lane, q);
+                    const C v = j.kb * A[(ti * 16 + row) * lda + tj * 16 + lr] + j.kc * acc[q];
+                    B[(ti * 16 + row) * lda + tj * 16 + lr] = v;
+                    B[(tj * 16 + lr) * lda + ti * 16 + row] = v;
+                }
+            }
+            __syncthreads();
+            // X <- a X + B X, a strip of 16 columns by one wave: it reads all of the strip before it writes any
+            for (int n0 = wave * 16; n0 < cp; n0 += kWaves * 16) {
+                Acc acc[kSmallRows / 16];
+#pragma unroll
+                for (int i = 0; i < kSmallRows / 16; ++i) acc[i] = Acc{ 0, 0, 0, 0 };
+                for (int k = 0; k < rp; k += 4) {
+                    const C xb = X[(k + lk) * ldx + n0 + lr];
+#pragma unroll
+                    for (int i = 0; i < kSmallRows / 16; ++i)
+                        if (i < nt) acc[i] = Mma<C>::go(B[(i * 16 + lr) * lda + k + lk], xb, acc[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < kSmallRows / 16; ++i)
+                    if (i < nt)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            C* x = X + (i * 16 + Mma<C>::row(lane, q)) * ldx + n0 + lr;
+                            *x = j.ka * *x + acc[i][q];
+                        }
+            }
+            __syncthreads();
+        }
+        for (int e = threadIdx.x; e < n; e += kT) {
+            const int row = e / j.cols, col = e - row * j.cols;
+            j.leave(b, row, col, X[j.turned ? col * ldx + row : row * ldx + col]);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- tiled products -------------------------------------------------------------------------------------------------
+constexpr int kTile = 64;
+constexpr int kNormParts = 256;
+
+// Scales of the 16-bit pairs (powers of two).  Entries of X are at most the largest singular value, below 4 by the
+// caller's check, and 1 / sqrt(r c) at the start; of A below 16; of b A + c A A below 32.
+constexpr float kSX = 4096.f, kSA = 1024.f, kSB = 1024.f;
+
+// values of a padded matrix: 64-bit, or a 16-bit pair in two arrays
+struct Pair {
+    _Float16 *hi, *lo;
+    __device__ __forceinline__ float get(size_t i, float scale) const { return ((float)hi[i] + (float)lo[i]) * (1.f / scale); }
+    __device__ __forceinline__ void put(size_t i, float v, float scale) const {
+        v *= scale;
+        const _Float16 h = (_Float16)v;
+        hi[i] = h;
+        lo[i] = (_Float16)(v - (float)h);
+    }
+    __device__ __forceinline__ Pair at(size_t bytes) const { return Pair{ (_Float16*)((char*)hi + bytes), (_Float16*)((char*)lo + bytes) }; }
+};
+struct Wide {
+    double* v;
+    __device__ __forceinline__ double get(size_t i, float) const { return v[i]; }
+    __device__ __forceinline__ void put(size_t i, double x, float) const { v[i] = x; }
+    __device__ __forceinline__ Wide at(size_t bytes) const { return Wide{ (double*)((char*)v + bytes) }; }
+};
+template <class C> struct StoreOf { using T = Pair; };
+template <> struct StoreOf<double> { using T = Wide; };
+
+// a matrix's working memory: X and X^T twice (a step reads one and writes the other), A, b A + c A A, partial sums
+template <class M>
+struct Mats {
+    M x[2], xt[2], a, b;
+    double* part;
+    size_t stride;    // bytes to the next matrix of the batch
+    int rp, cp;
+};
+
+template <class Ty>
+__global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t stride) {
+    __shared__ double sh[kWaves];
+    const int b = blockIdx.y;
+    const int64_t n = (int64_t)j.rows * j.cols;
+    double ss = 0;
+    for (int64_t e = (int64_t)blockIdx.x * kT + threadIdx.x; e < n; e += (int64_t)gridDim.x * kT) {
+        const int64_t row = e / j.cols, col = e - row * j.cols;
+        const double v = (double)j.template enter<true>(b, row, col);
+        ss += v * v;
+    }
+    ss = block_sum(ss, sh);
+    if (threadIdx.x == 0) ((double*)((char*)part + b * stride))[blockIdx.x] = ss;
+}
+
+// X0 and its transpose, a tile a workgroup
+template <class Ty>
+__global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int norm_parts) {
+    using C = typename Ty::C;
+    __shared__ double sh[kWaves];
+    __shared__ C tile[kTile][kTile + 1];
+    const int b = blockIdx.z;
+    const size_t off = b * w.stride;
+    const double* part = (const double*)((char*)w.part + off);
+    const double norm = sqrt(block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh)) + j.eps;
+    // rows and columns of the caller's matrix
+    const int64_t r0 = (int64_t)(j.turned ? blockIdx.x : blockIdx.y) * kTile, c0 = (int64_t)(j.turned ? blockIdx.y : blockIdx.x) * kTile;
+    for (int e = threadIdx.x; e < kTile * kTile; e += kT) {
+        const int y = e / kTile, x = e % kTile;
+        tile[y][x] = r0 + y < j.rows && c0 + x < j.cols ? (C)((double)j.template enter<false>(b, r0 + y, c0 + x) / norm) : C(0);
+    }
+    __syncthreads();
+    const auto xm = w.x[0].at(off), xt = w.xt[0].at(off);
+    const size_t x0 = (size_t)blockIdx.y * kTile, y0 = (size_t)blockIdx.x * kTile;   // row and column of X
+    for (int e = threadIdx.x; e < kTile * kTile; e += kT) {
+        const int y = e / kTile, x = e % kTile;
+        xm.put((x0 + y) * w.cp + y0 + x, j.turned ? tile[x][y] : tile[y][x], kSX);
+        xt.put((y0 + y) * w.rp + x0 + x, j.turned ? tile[y][x] : tile[x][y], kSX);
+    }
+}
+
+enum Kind { kGram, kPoly, kUpdate, kLast };
+
+// D[i][j] = sum_k P[i][k] Q[j][k] of one 64 x 64 tile, 4 waves of 32 x 32
+template <class C> struct Tile;
+template <> struct Tile<float> {
+    static constexpr int BK = 32;
+    float16v acc;
+    __device__ __forceinline__ void run(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int K) {
+        __shared__ __attribute__((aligned(16))) _Float16 sp[2][kTile][BK + 8], sq[2][kTile][BK + 8];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+        const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 8;
+        acc = 0.f;
+        for (int k = 0; k < K; k += BK) {
+            const size_t ap = (i0 + y) * ld + k + x, aq = (j0 + y) * ld + k + x;
+            const half8v a = *(const half8v*)(p.hi + ap), b = *(const half8v*)(p.lo + ap);
+            const half8v c = *(const half8v*)(q.hi + aq), d = *(const half8v*)(q.lo + aq);
+            __syncthreads();
+            *(half8v*)&sp[0][y][x] = a;
+            *(half8v*)&sp[1][y][x] = b;
+            *(half8v*)&sq[0][y][x] = c;
+            *(half8v*)&sq[1][y][x] = d;
+            __syncthreads();
+#pragma unroll
+            for (int kk = 0; kk < BK; kk += 16) {
+                const int ko = kk + (lane >> 5) * 8;
+                const half8v ph = *(const half8v*)&sp[0][wi + (lane & 31)][ko], pl = *(const half8v*)&sp[1][wi + (lane & 31)][ko];
+                const half8v qh = *(const half8v*)&sq[0][wj + (lane & 31)][ko], ql = *(const half8v*)&sq[1][wj + (lane & 31)][ko];
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+            }
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32 + (lane & 31);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) f(wi + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3), wj, acc[q]);
+    }
+};
+template <> struct Tile<double> {
+    static constexpr int BK = 16;
+    double4v acc[2][2];
+    __device__ __forceinline__ void run(const Wide& p, const Wide& q, size_t i0, size_t j0, int ld, int K) {
+        __shared__ __attribute__((aligned(16))) double sp[kTile][BK + 2], sq[kTile][BK + 2];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
+        const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) acc[i][jj] = double4v{ 0, 0, 0, 0 };
+        for (int k = 0; k < K; k += BK) {
+            const double2* ap = (const double2*)(p.v + (i0 + y) * ld + k + x);
+            const double2* aq = (const double2*)(q.v + (j0 + y) * ld + k + x);
+            const double2 a = ap[0], b = ap[1], c = aq[0], d = aq[1];
+            __syncthreads();
+            *(double2*)&sp[y][x] = a;
+            *(double2*)&sp[y][x + 2] = b;
+            *(double2*)&sq[y][x] = c;
+            *(double2*)&sq[y][x + 2] = d;
+            __syncthreads();
+#pragma unroll
+            for (int kk = 0; kk < BK; kk += 4) {
+                double pv[2], qv[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    pv[i] = sp[wi + 16 * i + (lane & 15)][kk + (lane >> 4)];
+                    qv[i] = sq[wj + 16 * i + (lane & 15)][kk + (lane >> 4)];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj) acc[i][jj] = Mma<double>::go(pv[i], qv[jj], acc[i][jj]);
+            }
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32 + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) f(wi + 16 * i + Mma<double>::row(lane, q), wj + 16 * jj, acc[i][jj][q]);
+    }
+};
+
+// One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
+// diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
+template <class Ty, Kind kind>
+__global__ __launch_bounds__(kT) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
+    using C = typename Ty::C;
+    constexpr bool kSym = kind == kGram || kind == kPoly;
+    const size_t off = blockIdx.z * w.stride;
+    size_t ti = blockIdx.y, tj = blockIdx.x;
+    if (kSym) {
+        ti = (size_t)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
+        while (ti * (ti + 1) / 2 > blockIdx.x) --ti;
+        while ((ti + 1) * (ti + 2) / 2 <= blockIdx.x) ++ti;
+        tj = blockIdx.x - ti * (ti + 1) / 2;
+    }
+    const size_t i0 = ti * kTile, j0 = tj * kTile;
+    const auto a = w.a.at(off), bm = w.b.at(off);
+    Tile<C> t;
+    if (kind == kGram) {
+        const auto x = w.x[from].at(off);
+        t.run(x, x, i0, j0, w.cp, w.cp);
+        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSX));
+        t.each([&](int y, int x, C v) {
+            a.put((j0 + x) * w.rp + i0 + y, v * f, kSA);
+            if (ti != tj) a.put((i0 + y) * w.rp + j0 + x, v * f, kSA);
+        });
+    } else if (kind == kPoly) {
+        t.run(a, a, i0, j0, w.rp, w.rp);
+        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSA * kSA));
+        t.each([&](int y, int x, C v) {
+            const C o = j.kb * a.get((j0 + x) * w.rp + i0 + y, kSA) + j.kc * (v * f);
+            bm.put((j0 + x) * w.rp + i0 + y, o, kSB);
+            if (ti != tj) bm.put((i0 + y) * w.rp + j0 + x, o, kSB);
+        });
+    } else {
+        const auto xt = w.xt[from].at(off), x = w.x[from].at(off), nx = w.x[from ^ 1].at(off), nt = w.xt[from ^ 1].at(off);
+        t.run(xt, bm, i0, j0, w.rp, w.rp);   // rows: columns of X; columns: rows of X
+        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB));
+        t.each([&](int yy, int xx, C v) {
+            const size_t col = i0 + yy, row = j0 + xx;
+            const C o = j.ka * x.get(row * w.cp + col, kSX) + v * f;
+            if (kind == kUpdate) {
+                nx.put(row * w.cp + col, o, kSX);
+                nt.put(col * w.rp + row, o, kSX);
+            } else if ((int)row < j.r && (int)col < j.c) {
+                if (j.turned) j.leave(blockIdx.z, col, row, o);
+                else j.leave(blockIdx.z, row, col, o);
+            }
+        });
+    }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------
+constexpr size_t kLds = 160 * 1024;
+
+bool is_small(int dtype, int r, int c) {
+    return r <= kSmallRows && c <= 32768 && small_lds(r, c, dtype == VQA_DTYPE_F64 ? 8 : 4) <= kLds;
+}
+int pad_tile(int v) { return (v + kTile - 1) / kTile * kTile; }
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+template <class M>
+size_t lay_out(char* base, int r, int c, Mats<M>* w);
+template <>
+size_t lay_out<Pair>(char* base, int r, int c, Mats<Pair>* w) {
+    w->rp = pad_tile(r);
+    w->cp = pad_tile(c);
+    const size_t x = up256((size_t)w->rp * w->cp * 2), a = up256((size_t)w->rp * w->rp * 2);
+    char* p = base;
+    auto next = [&](size_t n) { char* q = p; p += n; return (_Float16*)q; };
+    for (int i = 0; i < 2; ++i) {
+        w->x[i].hi = next(x); w->x[i].lo = next(x);
+        w->xt[i].hi = next(x); w->xt[i].lo = next(x);
+    }
+    w->a.hi = next(a); w->a.lo = next(a);
+    w->b.hi = next(a); w->b.lo = next(a);
+    w->part = (double*)p;
+    p += kNormParts * 8;
+    return w->stride = (size_t)(p - base);
+}
+template <>
+size_t lay_out<Wide>(char* base, int r, int c, Mats<Wide>* w) {
+    w->rp = pad_tile(r);
+    w->cp = pad_tile(c);
+    const size_t x = up256((size_t)w->rp * w->cp * 8), a = up256((size_t)w->rp * w->rp * 8);
+    char* p = base;
+    auto next = [&](size_t n) { char* q = p; p += n; return (double*)q; };
+    for (int i = 0; i < 2; ++i) {
+        w->x[i].v = next(x);
+        w->xt[i].v = next(x);
+    }
+    w->a.v = next(a);
+    w->b.v = next(a);
+    w->part = (double*)p;
+    p += kNormParts * 8;
+    return w->stride = (size_t)(p - base);
+}
+
+template <class Ty>
+int run(hipStream_t st, const OrthoCall& q) {
+    using C = typename Ty::C;
+    Job<Ty> j;
+    j.g = (const typename Ty::S*)q.g;
+    j.g_row = q.g_row_stride;
+    j.g_batch = q.g_batch_stride;
+    j.out = (typename Ty::S*)q.out;
+    j.w = (C*)q.weight;
+    j.m = (C*)q.momentum;
+    j.mu = (C)q.mu;
+    j.decay = (C)(1.0 - q.lr * q.weight_decay);
+    j.rate = (C)(q.lr * sqrt(std::max(1.0, (double)q.rows / (double)q.cols)));
+    j.nesterov = q.nesterov;
+    j.batch = q.batch;
+    j.rows = q.rows;
+    j.cols = q.cols;
+    j.r = std::min(q.rows, q.cols);
+    j.c = std::max(q.rows, q.cols);
+    j.turned = q.rows > q.cols;
+    j.steps = q.steps;
+    j.ka = (C)q.coefs[0];
+    j.kb = (C)q.coefs[1];
+    j.kc = (C)q.coefs[2];
+    j.eps = q.eps;
+    if (is_small(q.dtype, j.r, j.c)) {
+        const size_t lds = small_lds(j.r, j.c, sizeof(C));
+        VQA_HIP(hipFuncSetAttribute((const void*)k_ns_small<Ty>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
+        hipLaunchKernelGGL((k_ns_small<Ty>), dim3((unsigned)q.batch), dim3(kT), lds, st, j);
+        VQA_HIP(hipGetLastError());
+        return VQA_OK;
+    }
+    Mats<typename StoreOf<C>::T> w;
+    lay_out((char*)q.workspace, j.r, j.c, &w);
+    const int64_t n = (int64_t)j.rows * j.cols;
+    const int parts = (int)std::min<int64_t>(kNormParts, (n + 4 * kT - 1) / (4 * kT));
+    const unsigned tr = w.rp / kTile, tc = w.cp / kTile, sym = tr * (tr + 1) / 2, nb = (unsigned)q.batch;
+    hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride);
+    hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(tc, tr, nb), dim3(kT), 0, st, j, w, parts);
+    for (int s = 0; s < j.steps; ++s) {
+        const int from = s & 1;
+        hipLaunchKernelGGL((k_ns_product<Ty, kGram>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
+        hipLaunchKernelGGL((k_ns_product<Ty, kPoly>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
+        if (s + 1 < j.steps) hipLaunchKernelGGL((k_ns_product<Ty, kUpdate>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
+        else hipLaunchKernelGGL((k_ns_product<Ty, kLast>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
+    }
+    VQA_HIP(hipGetLastError());
+    return VQA_OK;
+}
+
+}  // namespace
+
+size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
+    const int r = std::min(rows, cols), c = std::max(rows, cols);
+    if (is_small(dtype, r, c)) return 0;
+    if (dtype == VQA_DTYPE_F64) {
+        Mats<Wide> w;
+        return lay_out<Wide>(nullptr, r, c, &w) * (size_t)batch;
+    }
+    Mats<Pair> w;
+    return lay_out<Pair>(nullptr, r, c, &w) * (size_t)batch;
+}
+
+int ortho_launch(hipStream_t stream, const OrthoCall& q) {
+    switch (q.dtype) {
+        case VQA_DTYPE_F64: return run<F64>(stream, q);
+        case VQA_DTYPE_F32: return run<F32>(stream, q);
+        case VQA_DTYPE_BF16: return run<BF16>(stream, q);
+        default: return run<F16>(stream, q);
+    }
+}
+
+}  // namespace vqa

@@ -85,6 +85,14 @@ static int device_state(int device, DeviceState** out) {
     return VQA_OK;
 }
 
+int library_stream(int device, hipStream_t* stream) {
+    DeviceState* ds;
+    int rc = device_state(device, &ds);
+    if (rc) return rc;
+    *stream = ds->stream;
+    return VQA_OK;
+}
+
 // Locks a device for one call; on the way out, when the call took the workspace, records the event
 // the next user on another stream waits for.
 struct DeviceGuard {

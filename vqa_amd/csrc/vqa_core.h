@@ -245,6 +245,41 @@ int irandom_stats_launch(hipStream_t stream, const double* d_expect, int n_obs, 
                          const int64_t* d_shots, const int32_t* d_seg, const double* d_n_list, int C, int kind,
                          int has_scale, double w, double M_tot, uint64_t seed, double* d_out);
 
+// softmax read-out of rows of scores (kern_logprob.hip)
+size_t log_probs_workspace_bytes(int dtype, int64_t rows, int64_t width, int top_k);
+int log_probs_launch(hipStream_t stream, int dtype, const void* d_logits, int64_t rows, int64_t width, int64_t row_stride,
+                     double scale, const int32_t* d_target, int top_k, void* d_workspace, void* d_log_prob, void* d_entropy,
+                     void* d_top_log_prob, int32_t* d_top_index);
+int log_probs_grad_launch(hipStream_t stream, int dtype, const void* d_logits, int64_t rows, int64_t width, int64_t row_stride,
+                          double scale, const int32_t* d_target, const void* d_dlog_prob, const void* d_dentropy,
+                          void* d_workspace, void* d_log_prob, void* d_entropy, void* d_dlogits, int64_t dlogits_row_stride);
+
+size_t psr_chain_workspace_bytes(int64_t B, int P);
+int psr_chain_launch(hipStream_t stream, const double* d_expect, int64_t B, int P, int n_obs, double factor, const double* d_dexpect,
+                     double* d_workspace, double* d_out);
+
+// orthogonalised updates (kern_ortho.hip)
+struct OrthoCall {
+    int dtype;
+    const void* g;
+    int64_t g_row_stride, g_batch_stride;
+    int batch, rows, cols;
+    int steps;
+    double coefs[3];
+    double eps;
+    void* workspace;
+    void* out;        // orthogonalise alone
+    void* weight;     // an optimizer step: out is null
+    void* momentum;
+    double lr, mu, weight_decay;
+    int nesterov;
+};
+size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols);
+int ortho_launch(hipStream_t stream, const OrthoCall& call);
+
+// the library's own stream of a device (host-pointer entry points)
+int library_stream(int device, hipStream_t* stream);
+
 // Working memory of a call: the per-device workspace owned by the library (grown on demand, never
 // shrunk; users on different streams are ordered by an event) or, for a call with a fixed region,
 // the next `bytes` of that region (VQA_EUNSUPPORTED when it does not hold them).

@@ -6,7 +6,8 @@ unchanged on the target objects of this package.  This module is the compact
 counterpart shipped with the package so that ``compile`` / ``fit`` run where the
 reference is not installed: the same target-object protocol
 (``methods_for_optimization``, shared one-element counters; base.py:390-415),
-the same step rules and bookkeeping for Adam, SGD and SGDM.  ``LR_rule`` /
+the same step rules and bookkeeping for Adam, SGD and SGDM (and Muon, which the
+reference does not have).  ``LR_rule`` /
 ``s_list_rule`` / ``batch_size_rule`` are callables (or plain constants); as in
 the reference (base.py:595-615) a rule is called with the shots spent so far
 unless ``<name>_annealing_by_shots`` is False, in which case it is called with
@@ -237,12 +238,57 @@ class SGDM(MiniBatchOptimizer):
         return params - self.LR_t * self.m_t
 
 
-_BUILTIN = {"Adam": Adam, "SGD": SGD, "SGDM": SGDM}
+class Muon(MiniBatchOptimizer):
+    """SGDM whose update is orthogonalised (vqa_amd.orthogonal.muon_step, on the GPU): the circuit parameters are taken as a
+    matrix, one row a layer, and the momentum's singular values are carried towards 1 before it is applied.  Parameters
+    behind the matrix (the regressor's scale) take SGDM's step.  Rules evaluated as in SGDM.
+
+    hpara: mu, nesterov, weight_decay, ns_steps, and matrix_shape = (layers, angles of a layer); by default the layers of
+    the shipped ansatz builders, three angles a qubit (vqa/QNN/QML_utils.py:76-98, 143-163).  Not in the reference."""
+
+    optimizer_name = "Muon"
+    default_hpara = dict(mu=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, matrix_shape=None)
+
+    def _shape(self):
+        if self.matrix_shape is not None:
+            rows, cols = (int(v) for v in self.matrix_shape)
+            if rows < 1 or cols < 1 or rows * cols > self.n_params:
+                raise ValueError(f"matrix_shape {self.matrix_shape} does not fit {self.n_params} parameters")
+            return rows, cols
+        n_c, n_q = getattr(self.target_obj, "n_c_params", self.n_params), getattr(self.target_obj, "n_qubits", None)
+        if not n_q or n_c < 1 or n_c % (3 * n_q):
+            raise ValueError("the circuit parameters do not form layers of three angles a qubit: give matrix_shape")
+        return n_c // (3 * n_q), 3 * n_q
+
+    def _reset_state(self):
+        self.m_t = np.zeros(self.n_params)
+        self._shape()
+
+    def optimizer_step(self, params, **kwargs):
+        from .orthogonal import muon_step
+
+        t = self.iteration_num
+        self.LR_t = self._rule("LR_rule", t + 1)
+        self.s_list = self._rule("s_list_rule", t + 1, floor=True)
+        self.batch_size = self._rule("batch_size_rule", t, floor=True)
+        g = np.asarray(self.grad(params=params, n_shots_list=self.s_list, mini_batch_size=self.batch_size, **kwargs), dtype=float)
+        rows, cols = self._shape()
+        n = rows * cols
+        new = np.array(params, dtype=float)
+        w, m = new[:n].reshape(rows, cols), self.m_t[:n].reshape(rows, cols)
+        muon_step(w, g[:n].reshape(rows, cols), m, lr=self.LR_t, mu=self.mu, weight_decay=self.weight_decay, nesterov=self.nesterov,
+                  steps=self.ns_steps, device=getattr(getattr(self.target_obj, "circuit", None), "device", None) or 0)
+        self.m_t[n:] = self.mu * self.m_t[n:] + g[n:]
+        new[n:] -= self.LR_t * self.m_t[n:]
+        return new
+
+
+_BUILTIN = {"Adam": Adam, "SGD": SGD, "SGDM": SGDM, "Muon": Muon}
 
 
 def get_optimizer_class(name, prefer_reference: bool = False):
     """Optimizer class by name (a class is passed through).  Built-in: Adam, SGD,
-    SGDM.  Any other name, or every name with ``prefer_reference``, is looked
+    SGDM, Muon.  Any other name, or every name with ``prefer_reference``, is looked
     up in the reference's ``vqa.VQA_optimizers.qml_optimizers`` when that
     package is importable (SantaQlaus, gCANS, SPSA, Adam_ASS live only there)."""
     if not isinstance(name, str):

@@ -88,11 +88,23 @@ class myQNN_classifier(myQNN_base):
             "func_to_track": "exact_error_both_to_track", "loss": "CE_loss_eval", "grad": "CE_grad_eval",
             "iEvaluate": "CE_iEval", "iEvaluate_iRandom": "CE_iEval_iRandom",
         },
+        # softmax of the exact class values (not in the reference; see softmax_CE_grad_eval)
+        "softmax_cross_entropy": {
+            "func_to_track": "exact_softmax_CE_to_track", "loss": "softmax_CE_loss_eval", "grad": "softmax_CE_grad_eval",
+        },
     }
 
-    def compile(self, *args, partial_MSE=False, eps=0.0, **kwargs):
+    # softmax read-out: p = softmax(softmax_scale * class values); weight of the entropy bonus in its loss
+    softmax_scale = 1.0
+    entropy_weight = 0.0
+
+    def compile(self, *args, partial_MSE=False, eps=0.0, softmax_scale=None, entropy_weight=None, **kwargs):
         self.partial_MSE = partial_MSE
         self._eps = eps
+        if softmax_scale is not None:
+            self.softmax_scale = float(softmax_scale)
+        if entropy_weight is not None:
+            self.entropy_weight = float(entropy_weight)
         super().compile(*args, **kwargs)
 
     # the inherited Z0 estimators (MSE_loss_eval) evaluate this class's default observable
@@ -604,6 +616,65 @@ class myQNN_classifier(myQNN_base):
 
     def CE_loss_eval(self):
         """Empty in the reference (myQNNs_classifier.py:1275-1276)."""
+
+    # ---- softmax read-out of the exact class values (vqa_amd.softmax; not in the reference) --------------------
+    def softmax_log_probs(self, x_list, params=None, labels=None, top_k=0):
+        """Log probabilities of the softmax read-out p = softmax(softmax_scale * class values) for each sample: of the given
+        labels, the entropy, and the top_k most probable classes (vqa_amd.softmax.LogProbs, numpy)."""
+        from .softmax import log_probs
+
+        if params is None:
+            params = self.model_params
+        return log_probs(self._exact_probs(params, x_list=x_list), labels, top_k=top_k, scale=self.softmax_scale,
+                         device=getattr(self.circuit, "device", None) or 0)
+
+    def _softmax_CE(self, params, which, idx=None):
+        from .softmax import log_probs
+
+        y = self.y_train if which == "train" else self.y_test
+        if idx is not None:
+            y = y[idx]
+        r = log_probs(self._exact_probs(params, which=which, idx=idx), np.asarray(y).astype(np.int64), scale=self.softmax_scale,
+                      device=getattr(self.circuit, "device", None) or 0)
+        return float(-np.mean(r.log_prob) - self.entropy_weight * np.mean(r.entropy))
+
+    def exact_softmax_CE_to_track(self, params):
+        """{"test": .., "train": ..}: mean negative log probability of the labels under the softmax read-out, less
+        entropy_weight times the mean entropy."""
+        return {"test": self._softmax_CE(params, "test"), "train": self._softmax_CE(params, "train")}
+
+    def softmax_CE_loss_eval(self, params, n_shots=None, mini_batch_size=None, option_weight=None, **unused):
+        _, eval_ind, _, _ = self._setup(mini_batch_size, option_weight)
+        self.circuit_counter[0] += len(eval_ind)
+        self.call_counter[0] += len(eval_ind)
+        return self._softmax_CE(params, "train", idx=eval_ind)
+
+    def softmax_CE_grad_eval(self, params, n_shots_list=None, mini_batch_size=None, option_weight=None, **unused):
+        """Gradient of the mini-batch loss  mean(-log p_label) - entropy_weight * mean(entropy)  of the softmax read-out, from
+        exact class values (no shots are drawn or counted): the parameter-shift sweep of the class observables, the loss's
+        gradient by the unshifted values, and their chain, all on the GPU.  With a process group the batch is split over the
+        ranks and the sums are added with one all-reduce, as in the other oracles."""
+        import torch
+
+        from .softmax import log_probs_grad, psr_chain
+
+        _, eval_ind, y_eval, _ = self._setup(mini_batch_size, option_weight)
+        theta = np.asarray(params[:self.n_c_params], dtype=np.float64)
+        B = len(eval_ind)
+        sh = self._shard(B)
+        rows = slice(None) if sh is None else slice(sh.lo, sh.hi)
+        E, _ = self.circuit.psr_full(theta, self._handle("train"), sel=np.asarray(eval_ind[rows], np.int32),
+                                     obs_list=self.class_observables(), n_marg_bits=0)
+        if not hasattr(E, "is_cuda"):
+            E = torch.from_numpy(np.ascontiguousarray(E)).cuda()
+        r = log_probs_grad(E[:, 0], np.asarray(y_eval)[rows].astype(np.int32), -1.0 / B, -self.entropy_weight / B if self.entropy_weight else None,
+                           scale=self.softmax_scale)
+        sums = psr_chain(E, r.d_logits)
+        self.circuit_counter[0] += B * E.shape[1]
+        self.call_counter[0] += B * E.shape[1]
+        out = np.zeros_like(params, dtype=float)
+        out[:self.n_c_params] = sums.cpu().numpy() if sh is None else sh.reduce(sums)[0]
+        return out
 
     # MSE_loss_eval: inherited from the regressor as in the reference (myQNNs_base.py:1397-1419 through
     # myQNNs_classifier.py:48): a Z-readout estimator scaled by params[-1], which is a CIRCUIT parameter
