@@ -299,51 +299,96 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
 
 enum Kind { kGram, kPoly, kUpdate, kLast };
 
-// D[i][j] = sum_k P[i][k] Q[j][k] of one 64 x 64 tile, 4 waves of 32 x 32
-template <class C> struct Tile;
-template <> struct Tile<float> {
-    static constexpr int BK = 32;
-    float16v acc;
-    __device__ __forceinline__ void run(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int K) {
-        __shared__ __attribute__((aligned(16))) _Float16 sp[2][kTile][BK + 8], sq[2][kTile][BK + 8];
+// 16 bytes of global memory straight to LDS, lane l's to base + 16 l (base: the same for the wave)
+__device__ __forceinline__ void copy_to_lds(const void* from, void* base) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+}
+
+// D[i][j] = sum_k P[i][k] Q[j][k] of one T x T tile, 4 waves of T/2 x T/2
+template <class C, int T> struct Tile;
+template <int T> struct Tile<float, T> {
+    static constexpr int BK = 32, W = T / 2, NT = W / 32;
+    float16v acc[NT][NT];
+    // A stage holds BK values of T rows of the four arrays; a row is 4 pieces of 16 bytes, whose order in the row is
+    // turned by swz(row), so that the 16 rows a quarter of a wave reads at once lie in different banks.
+    static __device__ __forceinline__ int swz(int row) { return (((row >> 1) ^ (row >> 3)) & 1) | ((row >> 2) & 1) << 1; }
+    static constexpr int kArray = T * BK;                 // values of one array in a stage
+    static constexpr int kStage = 4 * kArray;
+
+    __device__ __forceinline__ void fetch(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int k, _Float16* st) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-        const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 8;
-        acc = 0.f;
-        for (int k = 0; k < K; k += BK) {
-            const size_t ap = (i0 + y) * ld + k + x, aq = (j0 + y) * ld + k + x;
-            const half8v a = *(const half8v*)(p.hi + ap), b = *(const half8v*)(p.lo + ap);
-            const half8v c = *(const half8v*)(q.hi + aq), d = *(const half8v*)(q.lo + aq);
-            __syncthreads();
-            *(half8v*)&sp[0][y][x] = a;
-            *(half8v*)&sp[1][y][x] = b;
-            *(half8v*)&sq[0][y][x] = c;
-            *(half8v*)&sq[1][y][x] = d;
-            __syncthreads();
 #pragma unroll
-            for (int kk = 0; kk < BK; kk += 16) {
-                const int ko = kk + (lane >> 5) * 8;
-                const half8v ph = *(const half8v*)&sp[0][wi + (lane & 31)][ko], pl = *(const half8v*)&sp[1][wi + (lane & 31)][ko];
-                const half8v qh = *(const half8v*)&sq[0][wj + (lane & 31)][ko], ql = *(const half8v*)&sq[1][wj + (lane & 31)][ko];
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+        for (int n = 0; n < T / 64; ++n) {
+            const int r0 = (n * kWaves + wave) * 16, row = r0 + (lane >> 2);
+            const size_t x = k + ((lane & 3) ^ swz(row)) * 8;
+            const size_t ap = (i0 + row) * ld + x, aq = (j0 + row) * ld + x;
+            copy_to_lds(p.hi + ap, st + r0 * BK);
+            copy_to_lds(p.lo + ap, st + kArray + r0 * BK);
+            copy_to_lds(q.hi + aq, st + 2 * kArray + r0 * BK);
+            copy_to_lds(q.lo + aq, st + 3 * kArray + r0 * BK);
+        }
+    }
+    __device__ __forceinline__ void run(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int K) {
+        __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kStage];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave >> 1) * W + (lane & 31), wj = (wave & 1) * W + (lane & 31), half = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = 0.f;
+        fetch(p, q, i0, j0, ld, 0, lds);
+        int at = 0;
+        for (int k = 0; k < K; k += BK) {
+            // this stage has arrived (each wave waits for its own copies, the barrier for the waves), the other one was read
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (k + BK < K) fetch(p, q, i0, j0, ld, k + BK, lds + (at ^ 1) * kStage);
+            const _Float16* st = lds + at * kStage;
+            at ^= 1;
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk) {
+                half8v ph[NT], pl[NT], qh[NT], ql[NT];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const int ri = wi + 32 * i, rj = wj + 32 * i;
+                    const int xi = ri * BK + ((2 * kk + half) ^ swz(ri)) * 8, xj = rj * BK + ((2 * kk + half) ^ swz(rj)) * 8;
+                    ph[i] = *(const half8v*)(st + xi);
+                    pl[i] = *(const half8v*)(st + kArray + xi);
+                    qh[i] = *(const half8v*)(st + 2 * kArray + xj);
+                    ql[i] = *(const half8v*)(st + 3 * kArray + xj);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
             }
         }
     }
     template <class F>
     __device__ __forceinline__ void each(F f) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32 + (lane & 31);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) f(wi + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3), wj, acc[q]);
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q)
+                    f((wave >> 1) * W + 32 * i + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3), (wave & 1) * W + 32 * j + (lane & 31), acc[i][j][q]);
     }
 };
-template <> struct Tile<double> {
+template <> struct Tile<double, 64> {
     static constexpr int BK = 16;
     double4v acc[2][2];
     __device__ __forceinline__ void run(const Wide& p, const Wide& q, size_t i0, size_t j0, int ld, int K) {
-        __shared__ __attribute__((aligned(16))) double sp[kTile][BK + 2], sq[kTile][BK + 2];
+        __shared__ __attribute__((aligned(16))) double sp[64][BK + 2], sq[64][BK + 2];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
         const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 4;
@@ -391,7 +436,7 @@ template <> struct Tile<double> {
 
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
-template <class Ty, Kind kind>
+template <class Ty, Kind kind, int T>
 __global__ __launch_bounds__(kT) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
     using C = typename Ty::C;
     constexpr bool kSym = kind == kGram || kind == kPoly;
@@ -403,9 +448,9 @@ __global__ __launch_bounds__(kT) void k_ns_product(Job<Ty> j, Mats<typename Stor
         while ((ti + 1) * (ti + 2) / 2 <= blockIdx.x) ++ti;
         tj = blockIdx.x - ti * (ti + 1) / 2;
     }
-    const size_t i0 = ti * kTile, j0 = tj * kTile;
+    const size_t i0 = ti * T, j0 = tj * T;
     const auto a = w.a.at(off), bm = w.b.at(off);
-    Tile<C> t;
+    Tile<C, T> t;
     if (kind == kGram) {
         const auto x = w.x[from].at(off);
         t.run(x, x, i0, j0, w.cp, w.cp);
@@ -446,15 +491,20 @@ constexpr size_t kLds = 160 * 1024;
 bool is_small(int dtype, int r, int c) {
     return r <= kSmallRows && c <= 32768 && small_lds(r, c, dtype == VQA_DTYPE_F64 ? 8 : 4) <= kLds;
 }
-int pad_tile(int v) { return (v + kTile - 1) / kTile * kTile; }
+// Side of a product's tile.  128 where the update has at least as many tiles as half the chip's CUs
+int tile_of(int dtype, int batch, int r, int c) {
+    const int64_t n = (int64_t)((r + 127) / 128) * ((c + 127) / 128) * batch;
+    return dtype != VQA_DTYPE_F64 && n >= 128 ? 128 : 64;
+}
+int pad_to(int v, int t) { return (v + t - 1) / t * t; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 template <class M>
-size_t lay_out(char* base, int r, int c, Mats<M>* w);
+size_t lay_out(char* base, int r, int c, int tile, Mats<M>* w);
 template <>
-size_t lay_out<Pair>(char* base, int r, int c, Mats<Pair>* w) {
-    w->rp = pad_tile(r);
-    w->cp = pad_tile(c);
+size_t lay_out<Pair>(char* base, int r, int c, int tile, Mats<Pair>* w) {
+    w->rp = pad_to(r, tile);
+    w->cp = pad_to(c, tile);
     const size_t x = up256((size_t)w->rp * w->cp * 2), a = up256((size_t)w->rp * w->rp * 2);
     char* p = base;
     auto next = [&](size_t n) { char* q = p; p += n; return (_Float16*)q; };
@@ -469,9 +519,9 @@ size_t lay_out<Pair>(char* base, int r, int c, Mats<Pair>* w) {
     return w->stride = (size_t)(p - base);
 }
 template <>
-size_t lay_out<Wide>(char* base, int r, int c, Mats<Wide>* w) {
-    w->rp = pad_tile(r);
-    w->cp = pad_tile(c);
+size_t lay_out<Wide>(char* base, int r, int c, int tile, Mats<Wide>* w) {
+    w->rp = pad_to(r, tile);
+    w->cp = pad_to(c, tile);
     const size_t x = up256((size_t)w->rp * w->cp * 8), a = up256((size_t)w->rp * w->rp * 8);
     char* p = base;
     auto next = [&](size_t n) { char* q = p; p += n; return (double*)q; };
@@ -484,6 +534,18 @@ size_t lay_out<Wide>(char* base, int r, int c, Mats<Wide>* w) {
     w->part = (double*)p;
     p += kNormParts * 8;
     return w->stride = (size_t)(p - base);
+}
+
+template <class Ty, int T>
+void steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w) {
+    const unsigned tr = w.rp / T, tc = w.cp / T, sym = tr * (tr + 1) / 2, nb = (unsigned)j.batch;
+    for (int s = 0; s < j.steps; ++s) {
+        const int from = s & 1;
+        hipLaunchKernelGGL((k_ns_product<Ty, kGram, T>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
+        hipLaunchKernelGGL((k_ns_product<Ty, kPoly, T>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
+        if (s + 1 < j.steps) hipLaunchKernelGGL((k_ns_product<Ty, kUpdate, T>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
+        else hipLaunchKernelGGL((k_ns_product<Ty, kLast, T>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
+    }
 }
 
 template <class Ty>
@@ -519,19 +581,17 @@ int run(hipStream_t st, const OrthoCall& q) {
         return VQA_OK;
     }
     Mats<typename StoreOf<C>::T> w;
-    lay_out((char*)q.workspace, j.r, j.c, &w);
+    const int tile = tile_of(q.dtype, q.batch, j.r, j.c);
+    lay_out((char*)q.workspace, j.r, j.c, tile, &w);
     const int64_t n = (int64_t)j.rows * j.cols;
     const int parts = (int)std::min<int64_t>(kNormParts, (n + 4 * kT - 1) / (4 * kT));
-    const unsigned tr = w.rp / kTile, tc = w.cp / kTile, sym = tr * (tr + 1) / 2, nb = (unsigned)q.batch;
+    const unsigned nb = (unsigned)q.batch;
     hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride);
-    hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(tc, tr, nb), dim3(kT), 0, st, j, w, parts);
-    for (int s = 0; s < j.steps; ++s) {
-        const int from = s & 1;
-        hipLaunchKernelGGL((k_ns_product<Ty, kGram>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
-        hipLaunchKernelGGL((k_ns_product<Ty, kPoly>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
-        if (s + 1 < j.steps) hipLaunchKernelGGL((k_ns_product<Ty, kUpdate>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
-        else hipLaunchKernelGGL((k_ns_product<Ty, kLast>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
-    }
+    hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(w.cp / kTile, w.rp / kTile, nb), dim3(kT), 0, st, j, w, parts);
+    if constexpr (sizeof(C) == 4) {
+        if (tile == 128) steps<Ty, 128>(st, j, w);
+        else steps<Ty, 64>(st, j, w);
+    } else steps<Ty, 64>(st, j, w);
     VQA_HIP(hipGetLastError());
     return VQA_OK;
 }
@@ -543,10 +603,10 @@ size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
     if (is_small(dtype, r, c)) return 0;
     if (dtype == VQA_DTYPE_F64) {
         Mats<Wide> w;
-        return lay_out<Wide>(nullptr, r, c, &w) * (size_t)batch;
+        return lay_out<Wide>(nullptr, r, c, tile_of(dtype, batch, r, c), &w) * (size_t)batch;
     }
     Mats<Pair> w;
-    return lay_out<Pair>(nullptr, r, c, &w) * (size_t)batch;
+    return lay_out<Pair>(nullptr, r, c, tile_of(dtype, batch, r, c), &w) * (size_t)batch;
 }
 
 int ortho_launch(hipStream_t stream, const OrthoCall& q) {
