@@ -14,6 +14,7 @@
 //   leaves its normal range) and take the three products hi hi + hi lo + lo hi with 32-bit sums: the left-out lo lo is
 //   2^-22 of a product, the size of the roundings that 32-bit products make along a sum, at 5 times their rate.
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -236,12 +237,47 @@ struct Pair {
         hi[i] = h;
         lo[i] = (_Float16)(v - (float)h);
     }
+    // 16 neighbours, the first at a multiple of 16
+    __device__ __forceinline__ void get16(size_t i, float scale, float* v) const {
+        const half8v h0 = *(const half8v*)(hi + i), h1 = *(const half8v*)(hi + i + 8);
+        const half8v l0 = *(const half8v*)(lo + i), l1 = *(const half8v*)(lo + i + 8);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            v[n] = ((float)h0[n] + (float)l0[n]) * (1.f / scale);
+            v[8 + n] = ((float)h1[n] + (float)l1[n]) * (1.f / scale);
+        }
+    }
+    __device__ __forceinline__ void put16(size_t i, const float* v, float scale) const {
+        half8v h[2], l[2];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+            const float x = v[n] * scale;
+            h[n >> 3][n & 7] = (_Float16)x;
+            l[n >> 3][n & 7] = (_Float16)(x - (float)h[n >> 3][n & 7]);
+        }
+        *(half8v*)(hi + i) = h[0];
+        *(half8v*)(hi + i + 8) = h[1];
+        *(half8v*)(lo + i) = l[0];
+        *(half8v*)(lo + i + 8) = l[1];
+    }
     __device__ __forceinline__ Pair at(size_t bytes) const { return Pair{ (_Float16*)((char*)hi + bytes), (_Float16*)((char*)lo + bytes) }; }
 };
 struct Wide {
     double* v;
     __device__ __forceinline__ double get(size_t i, float) const { return v[i]; }
     __device__ __forceinline__ void put(size_t i, double x, float) const { v[i] = x; }
+    __device__ __forceinline__ void get16(size_t i, float, double* x) const {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const double2 d = *(const double2*)(v + i + 2 * n);
+            x[2 * n] = d.x;
+            x[2 * n + 1] = d.y;
+        }
+    }
+    __device__ __forceinline__ void put16(size_t i, const double* x, float) const {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) *(double2*)(v + i + 2 * n) = make_double2(x[2 * n], x[2 * n + 1]);
+    }
     __device__ __forceinline__ Wide at(size_t bytes) const { return Wide{ (double*)((char*)v + bytes) }; }
 };
 template <class C> struct StoreOf { using T = Pair; };
@@ -304,22 +340,31 @@ __device__ __forceinline__ void copy_to_lds(const void* from, void* base) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
 }
 
-// D[i][j] = sum_k P[i][k] Q[j][k] of one T x T tile, 4 waves of T/2 x T/2
+// D[i][j] = sum_k P[i][k] Q[j][k] of one T x T tile
 template <class C, int T> struct Tile;
 template <int T> struct Tile<float, T> {
-    static constexpr int BK = 32, W = T / 2, NT = W / 32;
-    float16v acc[NT][NT];
+    // T = 256: 8 waves of 128 x 64;  128 and 64: 4 waves of T/2 x T/2
+    static constexpr int kThreads = T == 256 ? 512 : 256, kWv = kThreads / 64;
+    static constexpr int WJ = T == 256 ? 4 : 2;                     // waves side by side
+    static constexpr int NI = T == 256 ? 4 : T / 64, NJ = T == 256 ? 2 : T / 64;   // 32 x 32 blocks of a wave
+    static constexpr int BK = 32;
+    float16v acc[NI][NJ];
     // A stage holds BK values of T rows of the four arrays; a row is 4 pieces of 16 bytes, whose order in the row is
     // turned by swz(row), so that the 16 rows a quarter of a wave reads at once lie in different banks.
     static __device__ __forceinline__ int swz(int row) { return (((row >> 1) ^ (row >> 3)) & 1) | ((row >> 2) & 1) << 1; }
     static constexpr int kArray = T * BK;                 // values of one array in a stage
     static constexpr int kStage = 4 * kArray;
+    static constexpr size_t kBytes = 2 * kStage * sizeof(_Float16);
+    static_assert(kBytes >= kWv * 32 * 33 * sizeof(float));
+
+    static __device__ __forceinline__ int wave_i() { return (threadIdx.x >> 6) / WJ * (NI * 32); }
+    static __device__ __forceinline__ int wave_j() { return (threadIdx.x >> 6) % WJ * (NJ * 32); }
 
     __device__ __forceinline__ void fetch(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int k, _Float16* st) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int n = 0; n < T / 64; ++n) {
-            const int r0 = (n * kWaves + wave) * 16, row = r0 + (lane >> 2);
+        for (int n = 0; n < T / (16 * kWv); ++n) {
+            const int r0 = (n * kWv + wave) * 16, row = r0 + (lane >> 2);
             const size_t x = k + ((lane & 3) ^ swz(row)) * 8;
             const size_t ap = (i0 + row) * ld + x, aq = (j0 + row) * ld + x;
             copy_to_lds(p.hi + ap, st + r0 * BK);
@@ -328,14 +373,14 @@ template <int T> struct Tile<float, T> {
             copy_to_lds(q.lo + aq, st + 3 * kArray + r0 * BK);
         }
     }
-    __device__ __forceinline__ void run(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int K) {
-        __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kStage];
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wi = (wave >> 1) * W + (lane & 31), wj = (wave & 1) * W + (lane & 31), half = lane >> 5;
+    __device__ __forceinline__ void run(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int K, char* shared) {
+        _Float16* lds = (_Float16*)shared;
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        const int wi = wave_i() + (lane & 31), wj = wave_j() + (lane & 31);
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = 0.f;
+            for (int j = 0; j < NJ; ++j) acc[i][j] = 0.f;
         fetch(p, q, i0, j0, ld, 0, lds);
         int at = 0;
         for (int k = 0; k < K; k += BK) {
@@ -347,48 +392,56 @@ template <int T> struct Tile<float, T> {
             at ^= 1;
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-                half8v ph[NT], pl[NT], qh[NT], ql[NT];
+                half8v ph[NI], pl[NI], qh[NJ], ql[NJ];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const int ri = wi + 32 * i, rj = wj + 32 * i;
-                    const int xi = ri * BK + ((2 * kk + half) ^ swz(ri)) * 8, xj = rj * BK + ((2 * kk + half) ^ swz(rj)) * 8;
-                    ph[i] = *(const half8v*)(st + xi);
-                    pl[i] = *(const half8v*)(st + kArray + xi);
-                    qh[i] = *(const half8v*)(st + 2 * kArray + xj);
-                    ql[i] = *(const half8v*)(st + 3 * kArray + xj);
+                for (int j = 0; j < NJ; ++j) {
+                    const int r = wj + 32 * j, x = r * BK + ((2 * kk + half) ^ swz(r)) * 8;
+                    qh[j] = *(const half8v*)(st + 2 * kArray + x);
+                    ql[j] = *(const half8v*)(st + 3 * kArray + x);
                 }
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < NI; ++i) {
+                    const int r = wi + 32 * i, x = r * BK + ((2 * kk + half) ^ swz(r)) * 8;
+                    ph[i] = *(const half8v*)(st + x);
+                    pl[i] = *(const half8v*)(st + kArray + x);
+                }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+                for (int i = 0; i < NI; ++i) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+                }
             }
         }
     }
+    // The result block by block: a wave lays its 32 x 32 blocks one after another into its own part of the shared memory
+    // (after the barrier: the stages are read) and hands each to f(row, column of the block, block).
     template <class F>
-    __device__ __forceinline__ void each(F f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __device__ __forceinline__ void blocks(char* shared, F f) {
+        const int lane = threadIdx.x & 63;
+        auto blk = (float(*)[33])shared + (threadIdx.x >> 6) * 32;
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-                for (int q = 0; q < 16; ++q)
-                    f((wave >> 1) * W + 32 * i + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3), (wave & 1) * W + 32 * j + (lane & 31), acc[i][j][q]);
+                for (int q = 0; q < 16; ++q) blk[8 * (q >> 2) + 4 * (lane >> 5) + (q & 3)][lane & 31] = acc[i][j][q];
+                f(wave_i() + 32 * i, wave_j() + 32 * j, blk);
+            }
     }
 };
 template <> struct Tile<double, 64> {
+    static constexpr int kThreads = 256;
     static constexpr int BK = 16;
+    static constexpr size_t kBytes = kWaves * 32 * 33 * sizeof(double);   // of the result's blocks; the stages take less
+    static_assert(kBytes >= 2 * 64 * (BK + 2) * sizeof(double));
     double4v acc[2][2];
-    __device__ __forceinline__ void run(const Wide& p, const Wide& q, size_t i0, size_t j0, int ld, int K) {
-        __shared__ __attribute__((aligned(16))) double sp[64][BK + 2], sq[64][BK + 2];
+    __device__ __forceinline__ void run(const Wide& p, const Wide& q, size_t i0, size_t j0, int ld, int K, char* shared) {
+        double(*sp)[BK + 2] = (double(*)[BK + 2])shared, (*sq)[BK + 2] = sp + 64;
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
         const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 4;
@@ -422,24 +475,27 @@ template <> struct Tile<double, 64> {
         }
     }
     template <class F>
-    __device__ __forceinline__ void each(F f) {
+    __device__ __forceinline__ void blocks(char* shared, F f) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32 + (lane & 15);
+        auto blk = (double(*)[33])shared + wave * 32;
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) f(wi + 16 * i + Mma<double>::row(lane, q), wj + 16 * jj, acc[i][jj][q]);
+                for (int q = 0; q < 4; ++q) blk[16 * i + Mma<double>::row(lane, q)][16 * jj + (lane & 15)] = acc[i][jj][q];
+        f((wave >> 1) * 32, (wave & 1) * 32, blk);
     }
 };
 
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
 template <class Ty, Kind kind, int T>
-__global__ __launch_bounds__(kT) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
+__global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
     using C = typename Ty::C;
     constexpr bool kSym = kind == kGram || kind == kPoly;
+    extern __shared__ __attribute__((aligned(16))) char product_lds[];
     const size_t off = blockIdx.z * w.stride;
     size_t ti = blockIdx.y, tj = blockIdx.x;
     if (kSym) {
@@ -451,35 +507,56 @@ __global__ __launch_bounds__(kT) void k_ns_product(Job<Ty> j, Mats<typename Stor
     const size_t i0 = ti * T, j0 = tj * T;
     const auto a = w.a.at(off), bm = w.b.at(off);
     Tile<C, T> t;
-    if (kind == kGram) {
-        const auto x = w.x[from].at(off);
-        t.run(x, x, i0, j0, w.cp, w.cp);
-        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSX));
-        t.each([&](int y, int x, C v) {
-            a.put((j0 + x) * w.rp + i0 + y, v * f, kSA);
-            if (ti != tj) a.put((i0 + y) * w.rp + j0 + x, v * f, kSA);
-        });
-    } else if (kind == kPoly) {
-        t.run(a, a, i0, j0, w.rp, w.rp);
-        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSA * kSA));
-        t.each([&](int y, int x, C v) {
-            const C o = j.kb * a.get((j0 + x) * w.rp + i0 + y, kSA) + j.kc * (v * f);
-            bm.put((j0 + x) * w.rp + i0 + y, o, kSB);
-            if (ti != tj) bm.put((i0 + y) * w.rp + j0 + x, o, kSB);
+    // a lane's 16 neighbours of a block: half a row, or half a column
+    const int lane = threadIdx.x & 63, line = lane >> 1, half = (lane & 1) * 16;
+    if (kind == kGram || kind == kPoly) {
+        const auto& src = kind == kGram ? w.x[from] : w.a;
+        const auto m = src.at(off), out = kind == kGram ? a : bm;
+        const int ld = kind == kGram ? w.cp : w.rp;
+        t.run(m, m, i0, j0, ld, ld, product_lds);
+        const float so = kind == kGram ? kSA : kSB;
+        const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA));
+        t.blocks(product_lds, [&](int bi, int bj, C(*blk)[33]) {
+            const size_t y = i0 + bi + line, x = j0 + bj + half;
+            C v[16];
+            if (kind == kPoly) {
+                a.get16(y * w.rp + x, kSA, v);
+#pragma unroll
+                for (int n = 0; n < 16; ++n) blk[line][half + n] = v[n] = j.kb * v[n] + j.kc * (f * blk[line][half + n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 16; ++n) blk[line][half + n] = v[n] = f * blk[line][half + n];
+            }
+            out.put16(y * w.rp + x, v, so);
+            if (ti == tj) return;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) v[n] = blk[half + n][line];
+            out.put16((j0 + bj + line) * w.rp + i0 + bi + half, v, so);
         });
     } else {
-        const auto xt = w.xt[from].at(off), x = w.x[from].at(off), nx = w.x[from ^ 1].at(off), nt = w.xt[from ^ 1].at(off);
-        t.run(xt, bm, i0, j0, w.rp, w.rp);   // rows: columns of X; columns: rows of X
+        const auto xt = w.xt[from].at(off), nx = w.x[from ^ 1].at(off), nt = w.xt[from ^ 1].at(off);
+        t.run(xt, bm, i0, j0, w.rp, w.rp, product_lds);   // rows: columns of X; columns: rows of X
         const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB));
-        t.each([&](int yy, int xx, C v) {
-            const size_t col = i0 + yy, row = j0 + xx;
-            const C o = j.ka * x.get(row * w.cp + col, kSX) + v * f;
+        t.blocks(product_lds, [&](int bi, int bj, C(*blk)[33]) {
+            const size_t y = i0 + bi + line, x = j0 + bj + half;
+            C v[16];
+            xt.get16(y * w.rp + x, kSX, v);
+#pragma unroll
+            for (int n = 0; n < 16; ++n) blk[line][half + n] = v[n] = j.ka * v[n] + f * blk[line][half + n];
             if (kind == kUpdate) {
-                nx.put(row * w.cp + col, o, kSX);
-                nt.put(col * w.rp + row, o, kSX);
-            } else if ((int)row < j.r && (int)col < j.c) {
-                if (j.turned) j.leave(blockIdx.z, col, row, o);
-                else j.leave(blockIdx.z, row, col, o);
+                nt.put16(y * w.rp + x, v, kSX);
+#pragma unroll
+                for (int n = 0; n < 16; ++n) v[n] = blk[half + n][line];
+                nx.put16((j0 + bj + line) * w.cp + i0 + bi + half, v, kSX);
+            } else {
+                // the caller's rows are the block's rows (turned) or its columns: 32 neighbours of a row by half a wave
+                const int64_t r0 = (j.turned ? i0 + bi : j0 + bj) + (lane >> 5), col = (j.turned ? j0 + bj : i0 + bi) + (lane & 31);
+#pragma unroll
+                for (int n = 0; n < 16; ++n) {
+                    const int d = 2 * n + (lane >> 5);
+                    const C o = j.turned ? blk[d][lane & 31] : blk[lane & 31][d];
+                    if (r0 + 2 * n < j.rows && col < j.cols) j.leave(blockIdx.z, r0 + 2 * n, col, o);
+                }
             }
         });
     }
@@ -493,8 +570,11 @@ bool is_small(int dtype, int r, int c) {
 }
 // Side of a product's tile.  128 where the update has at least as many tiles as half the chip's CUs
 int tile_of(int dtype, int batch, int r, int c) {
+    if (dtype == VQA_DTYPE_F64) return 64;
     const int64_t n = (int64_t)((r + 127) / 128) * ((c + 127) / 128) * batch;
-    return dtype != VQA_DTYPE_F64 && n >= 128 ? 128 : 64;
+    static const int forced = getenv("NS_TILE") ? atoi(getenv("NS_TILE")) : 0;
+    if (forced) return forced;
+    return n >= 1024 ? 256 : n >= 128 ? 128 : 64;
 }
 int pad_to(int v, int t) { return (v + t - 1) / t * t; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -536,16 +616,38 @@ size_t lay_out<Wide>(char* base, int r, int c, int tile, Mats<Wide>* w) {
     return w->stride = (size_t)(p - base);
 }
 
-template <class Ty, int T>
-void steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w) {
-    const unsigned tr = w.rp / T, tc = w.cp / T, sym = tr * (tr + 1) / 2, nb = (unsigned)j.batch;
-    for (int s = 0; s < j.steps; ++s) {
-        const int from = s & 1;
-        hipLaunchKernelGGL((k_ns_product<Ty, kGram, T>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
-        hipLaunchKernelGGL((k_ns_product<Ty, kPoly, T>), dim3(sym, 1, nb), dim3(kT), 0, st, j, w, from);
-        if (s + 1 < j.steps) hipLaunchKernelGGL((k_ns_product<Ty, kUpdate, T>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
-        else hipLaunchKernelGGL((k_ns_product<Ty, kLast, T>), dim3(tr, tc, nb), dim3(kT), 0, st, j, w, from);
+// Dynamic shared memory beyond 64 KB is asked for once for each kernel and device
+template <class F>
+int allow_lds(F* fn, size_t bytes) {
+    static uint64_t done = 0;   // a bit a device; asking twice does no harm
+    int dev = 0;
+    VQA_HIP(hipGetDevice(&dev));
+    if (bytes > 65536 && !(done >> (dev & 63) & 1)) {
+        VQA_HIP(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
+        done |= (uint64_t)1 << (dev & 63);
     }
+    return VQA_OK;
+}
+
+template <class Ty, Kind kind, int T>
+int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
+    using Tl = Tile<typename Ty::C, T>;
+    if (int rc = allow_lds(k_ns_product<Ty, kind, T>, Tl::kBytes)) return rc;
+    hipLaunchKernelGGL((k_ns_product<Ty, kind, T>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
+    return VQA_OK;
+}
+
+template <class Ty, int T>
+int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w) {
+    const unsigned tr = w.rp / T, tc = w.cp / T, sym = tr * (tr + 1) / 2, nb = (unsigned)j.batch;
+    int rc = VQA_OK;
+    for (int s = 0; s < j.steps && !rc; ++s) {
+        const int from = s & 1;
+        rc = product<Ty, kGram, T>(st, dim3(sym, 1, nb), j, w, from);
+        if (!rc) rc = product<Ty, kPoly, T>(st, dim3(sym, 1, nb), j, w, from);
+        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate, T>(st, dim3(tr, tc, nb), j, w, from) : product<Ty, kLast, T>(st, dim3(tr, tc, nb), j, w, from);
+    }
+    return rc;
 }
 
 template <class Ty>
@@ -575,7 +677,7 @@ int run(hipStream_t st, const OrthoCall& q) {
     j.eps = q.eps;
     if (is_small(q.dtype, j.r, j.c)) {
         const size_t lds = small_lds(j.r, j.c, sizeof(C));
-        VQA_HIP(hipFuncSetAttribute((const void*)k_ns_small<Ty>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
+        if (int rc = allow_lds(k_ns_small<Ty>, lds)) return rc;
         hipLaunchKernelGGL((k_ns_small<Ty>), dim3((unsigned)q.batch), dim3(kT), lds, st, j);
         VQA_HIP(hipGetLastError());
         return VQA_OK;
@@ -588,10 +690,11 @@ int run(hipStream_t st, const OrthoCall& q) {
     const unsigned nb = (unsigned)q.batch;
     hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride);
     hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(w.cp / kTile, w.rp / kTile, nb), dim3(kT), 0, st, j, w, parts);
+    int rc;
     if constexpr (sizeof(C) == 4) {
-        if (tile == 128) steps<Ty, 128>(st, j, w);
-        else steps<Ty, 64>(st, j, w);
-    } else steps<Ty, 64>(st, j, w);
+        rc = tile == 256 ? steps<Ty, 256>(st, j, w) : tile == 128 ? steps<Ty, 128>(st, j, w) : steps<Ty, 64>(st, j, w);
+    } else rc = steps<Ty, 64>(st, j, w);
+    if (rc) return rc;
     VQA_HIP(hipGetLastError());
     return VQA_OK;
 }
