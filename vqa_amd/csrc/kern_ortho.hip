@@ -237,28 +237,34 @@ struct Pair {
         hi[i] = h;
         lo[i] = (_Float16)(v - (float)h);
     }
-    // 16 neighbours, the first at a multiple of 16
-    __device__ __forceinline__ void get16(size_t i, float scale, float* v) const {
-        const half8v h0 = *(const half8v*)(hi + i), h1 = *(const half8v*)(hi + i + 8);
-        const half8v l0 = *(const half8v*)(lo + i), l1 = *(const half8v*)(lo + i + 8);
+    // N neighbours, the first at a multiple of N
+    template <int N>
+    __device__ __forceinline__ void get(size_t i, float scale, float* v) const {
+        constexpr int V = N < 8 ? N : 8;
+        typedef _Float16 halves __attribute__((ext_vector_type(V)));
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            v[n] = ((float)h0[n] + (float)l0[n]) * (1.f / scale);
-            v[8 + n] = ((float)h1[n] + (float)l1[n]) * (1.f / scale);
+        for (int m = 0; m < N / V; ++m) {
+            const halves h = *(const halves*)(hi + i + m * V), l = *(const halves*)(lo + i + m * V);
+#pragma unroll
+            for (int n = 0; n < V; ++n) v[m * V + n] = ((float)h[n] + (float)l[n]) * (1.f / scale);
         }
     }
-    __device__ __forceinline__ void put16(size_t i, const float* v, float scale) const {
-        half8v h[2], l[2];
+    template <int N>
+    __device__ __forceinline__ void put(size_t i, const float* v, float scale) const {
+        constexpr int V = N < 8 ? N : 8;
+        typedef _Float16 halves __attribute__((ext_vector_type(V)));
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-            const float x = v[n] * scale;
-            h[n >> 3][n & 7] = (_Float16)x;
-            l[n >> 3][n & 7] = (_Float16)(x - (float)h[n >> 3][n & 7]);
+        for (int m = 0; m < N / V; ++m) {
+            halves h, l;
+#pragma unroll
+            for (int n = 0; n < V; ++n) {
+                const float x = v[m * V + n] * scale;
+                h[n] = (_Float16)x;
+                l[n] = (_Float16)(x - (float)h[n]);
+            }
+            *(halves*)(hi + i + m * V) = h;
+            *(halves*)(lo + i + m * V) = l;
         }
-        *(half8v*)(hi + i) = h[0];
-        *(half8v*)(hi + i + 8) = h[1];
-        *(half8v*)(lo + i) = l[0];
-        *(half8v*)(lo + i + 8) = l[1];
     }
     __device__ __forceinline__ Pair at(size_t bytes) const { return Pair{ (_Float16*)((char*)hi + bytes), (_Float16*)((char*)lo + bytes) }; }
 };
@@ -266,17 +272,19 @@ struct Wide {
     double* v;
     __device__ __forceinline__ double get(size_t i, float) const { return v[i]; }
     __device__ __forceinline__ void put(size_t i, double x, float) const { v[i] = x; }
-    __device__ __forceinline__ void get16(size_t i, float, double* x) const {
+    template <int N>
+    __device__ __forceinline__ void get(size_t i, float, double* x) const {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        for (int n = 0; n < N / 2; ++n) {
             const double2 d = *(const double2*)(v + i + 2 * n);
             x[2 * n] = d.x;
             x[2 * n + 1] = d.y;
         }
     }
-    __device__ __forceinline__ void put16(size_t i, const double* x, float) const {
+    template <int N>
+    __device__ __forceinline__ void put(size_t i, const double* x, float) const {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) *(double2*)(v + i + 2 * n) = make_double2(x[2 * n], x[2 * n + 1]);
+        for (int n = 0; n < N / 2; ++n) *(double2*)(v + i + 2 * n) = make_double2(x[2 * n], x[2 * n + 1]);
     }
     __device__ __forceinline__ Wide at(size_t bytes) const { return Wide{ (double*)((char*)v + bytes) }; }
 };
@@ -340,152 +348,223 @@ __device__ __forceinline__ void copy_to_lds(const void* from, void* base) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
 }
 
-// D[i][j] = sum_k P[i][k] Q[j][k] of one T x T tile
-template <class C, int T> struct Tile;
-template <int T> struct Tile<float, T> {
-    // T = 256: 8 waves of 128 x 64;  128 and 64: 4 waves of T/2 x T/2
-    static constexpr int kThreads = T == 256 ? 512 : 256, kWv = kThreads / 64;
-    static constexpr int WJ = T == 256 ? 4 : 2;                     // waves side by side
-    static constexpr int NI = T == 256 ? 4 : T / 64, NJ = T == 256 ? 2 : T / 64;   // 32 x 32 blocks of a wave
-    static constexpr int BK = 32;
-    float16v acc[NI][NJ];
-    // A stage holds BK values of T rows of the four arrays; a row is 4 pieces of 16 bytes, whose order in the row is
-    // turned by swz(row), so that the 16 rows a quarter of a wave reads at once lie in different banks.
-    static __device__ __forceinline__ int swz(int row) { return (((row >> 1) ^ (row >> 3)) & 1) | ((row >> 2) & 1) << 1; }
-    static constexpr int kArray = T * BK;                 // values of one array in a stage
-    static constexpr int kStage = 4 * kArray;
-    static constexpr size_t kBytes = 2 * kStage * sizeof(_Float16);
-    static_assert(kBytes >= kWv * 32 * 33 * sizeof(float));
+// waits until at most N of the wave's copies are under way and its reads of shared memory are done, then for the other waves
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+    static_assert(N < 64);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
-    static __device__ __forceinline__ int wave_i() { return (threadIdx.x >> 6) / WJ * (NI * 32); }
-    static __device__ __forceinline__ int wave_j() { return (threadIdx.x >> 6) % WJ * (NJ * 32); }
+// D[i][j] = sum_k P[i][k] Q[j][k] of one T x T tile.  WI x WJ waves lie over the tile, KG times: group g of the waves takes
+// every KG-th piece of the summed index of a stage, so that small tiles still have two or more waves a SIMD to hide the
+// way from shared memory; the groups' sums are added at the end.
+// A stage holds BK values of T rows of each array; a row is Q pieces of 16 bytes, whose order in the row is turned by
+// swz(row), so that the 8 or 16 rows that a part of a wave reads at once lie in different banks.
+template <class C, int T> struct Shape;
+// Stages in flight: a stage's way from memory takes about 0.5 us, longer than small tiles compute on it, so two or three
+// are under way while one is read; 256 x 256 tiles compute longer than that on one stage, and have room for two.
+template <> struct Shape<float, 64> { static constexpr int WI = 2, WJ = 2, KG = 4, BK = 64, S = 4; };
+template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 32, S = 4; };
+template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG = 1, BK = 32, S = 2; };
+template <> struct Shape<double, 64> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 16, S = 4; };
 
-    __device__ __forceinline__ void fetch(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int k, _Float16* st) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <class C> struct Frag;   // what a wave reads of one 32-row (16 for 64 bits) block at once, and its products
+template <> struct Frag<float> {
+    using M = Pair;
+    using Acc = float16v;
+    static constexpr int kArrays = 4, kSide = 32, kRegs = 16;
+    static __device__ __forceinline__ int row(int lane, int q) { return 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3); }
+};
+template <> struct Frag<double> {
+    using M = Wide;
+    using Acc = double4v;
+    static constexpr int kArrays = 2, kSide = 16, kRegs = 4;
+    static __device__ __forceinline__ int row(int lane, int q) { return Mma<double>::row(lane, q); }
+};
+
+template <class C, int T>
+struct Tile : Shape<C, T> {
+    using Sh = Shape<C, T>;
+    using Fr = Frag<C>;
+    using M = typename Fr::M;
+    static constexpr int WI = Sh::WI, WJ = Sh::WJ, KG = Sh::KG, BK = Sh::BK, S = Sh::S;
+    static constexpr int kWv = WI * WJ * KG, kThreads = 64 * kWv;
+    static constexpr int kSize = sizeof(C) == 8 ? 8 : 2;              // of a stored value
+    static constexpr int Q = BK * kSize / 16;                         // pieces of a row
+    static constexpr int kArray = T * Q * 16, kStage = Fr::kArrays * kArray;   // bytes
+    static constexpr int kCopies = kStage / 1024 / kWv;               // a wave's copies (1 KB each) of a stage
+    static constexpr int NI = T / WI / Fr::kSide, NJ = T / WJ / Fr::kSide;     // blocks of a wave
+    static constexpr int BI = T / WI / 32, BJ = T / WJ / 32;          // its 32 x 32 blocks as they leave
+    static constexpr int kBlock = 32 * 33;
+    static constexpr size_t kOut = (size_t)kWv * BJ * kBlock * sizeof(C);
+    static constexpr size_t kBytes = (size_t)S * kStage > kOut ? (size_t)S * kStage : kOut;
+    static constexpr int N = 16 / KG;                                 // neighbours of a block's row that a lane takes
+    static_assert(kStage % (1024 * kWv) == 0 && (Q == 4 || Q == 8) && kBytes <= 160 * 1024);
+
+    typename Fr::Acc acc[NI][NJ];
+
+    static __device__ __forceinline__ int swz(int row) {
+        return Q == 4 ? (((row >> 1) ^ (row >> 3)) & 1) | ((row >> 2) & 1) << 1 : ((row ^ (row >> 3)) & 1) | (row & 6);
+    }
+    static __device__ __forceinline__ int wave() { return threadIdx.x >> 6; }
+    static __device__ __forceinline__ int group() { return wave() / (WI * WJ); }
+    static __device__ __forceinline__ int wave_i() { return wave() % (WI * WJ) / WJ * (T / WI); }
+    static __device__ __forceinline__ int wave_j() { return wave() % WJ * (T / WJ); }
+
+    static __device__ __forceinline__ const char* base(const Pair& p, const Pair& q, int arr) {
+        return (const char*)(arr < 2 ? arr == 0 ? p.hi : p.lo : arr == 2 ? q.hi : q.lo);
+    }
+    static __device__ __forceinline__ const char* base(const Wide& p, const Wide& q, int arr) { return (const char*)(arr ? q.v : p.v); }
+
+    // where the wave's copies of a stage come from (a lane's 16 bytes, at the first stage) and go to
+    struct Copies {
+        const char* from[kCopies];
+        int to[kCopies];
+    };
+    __device__ __forceinline__ void aim(const M& p, const M& q, size_t i0, size_t j0, int ld, Copies& c) {
+        const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(wave());
+        constexpr int kRows = 64 / Q, kChunks = T / kRows;            // rows of a copy, copies of an array
 #pragma unroll
-        for (int n = 0; n < T / (16 * kWv); ++n) {
-            const int r0 = (n * kWv + wave) * 16, row = r0 + (lane >> 2);
-            const size_t x = k + ((lane & 3) ^ swz(row)) * 8;
-            const size_t ap = (i0 + row) * ld + x, aq = (j0 + row) * ld + x;
-            copy_to_lds(p.hi + ap, st + r0 * BK);
-            copy_to_lds(p.lo + ap, st + kArray + r0 * BK);
-            copy_to_lds(q.hi + aq, st + 2 * kArray + r0 * BK);
-            copy_to_lds(q.lo + aq, st + 3 * kArray + r0 * BK);
+        for (int n = 0; n < kCopies; ++n) {
+            const int id = n * kWv + w, arr = id / kChunks, r0 = id % kChunks * kRows, row = r0 + lane / Q;
+            c.from[n] = base(p, q, arr) + ((arr >= Fr::kArrays / 2 ? j0 : i0) + row) * (size_t)ld * kSize + ((lane % Q) ^ swz(row)) * 16;
+            c.to[n] = arr * kArray + r0 * Q * 16;
         }
     }
-    __device__ __forceinline__ void run(const Pair& p, const Pair& q, size_t i0, size_t j0, int ld, int K, char* shared) {
-        _Float16* lds = (_Float16*)shared;
-        const int lane = threadIdx.x & 63, half = lane >> 5;
-        const int wi = wave_i() + (lane & 31), wj = wave_j() + (lane & 31);
+    __device__ __forceinline__ void fetch(const Copies& c, int t, char* st) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[i][j] = 0.f;
-        fetch(p, q, i0, j0, ld, 0, lds);
-        int at = 0;
-        for (int k = 0; k < K; k += BK) {
-            // this stage has arrived (each wave waits for its own copies, the barrier for the waves), the other one was read
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (k + BK < K) fetch(p, q, i0, j0, ld, k + BK, lds + (at ^ 1) * kStage);
-            const _Float16* st = lds + at * kStage;
-            at ^= 1;
-#pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-                half8v ph[NI], pl[NI], qh[NJ], ql[NJ];
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const int r = wj + 32 * j, x = r * BK + ((2 * kk + half) ^ swz(r)) * 8;
-                    qh[j] = *(const half8v*)(st + 2 * kArray + x);
-                    ql[j] = *(const half8v*)(st + 3 * kArray + x);
-                }
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int r = wi + 32 * i, x = r * BK + ((2 * kk + half) ^ swz(r)) * 8;
-                    ph[i] = *(const half8v*)(st + x);
-                    pl[i] = *(const half8v*)(st + kArray + x);
-                }
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
-                }
-            }
-        }
+        for (int n = 0; n < kCopies; ++n) copy_to_lds(c.from[n] + (size_t)t * (BK * kSize), st + c.to[n]);
     }
-    // The result block by block: a wave lays its 32 x 32 blocks one after another into its own part of the shared memory
-    // (after the barrier: the stages are read) and hands each to f(row, column of the block, block).
-    template <class F>
-    __device__ __forceinline__ void blocks(char* shared, F f) {
+
+    // the products of one piece pair of the summed index
+    __device__ __forceinline__ void multiply(const char* st, int kk) {
         const int lane = threadIdx.x & 63;
-        auto blk = (float(*)[33])shared + (threadIdx.x >> 6) * 32;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
+        if constexpr (sizeof(C) == 4) {
+            const int piece = 2 * kk + (lane >> 5);
+            half8v ph[NI], pl[NI], qh[NJ], ql[NJ];
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-#pragma unroll
-                for (int q = 0; q < 16; ++q) blk[8 * (q >> 2) + 4 * (lane >> 5) + (q & 3)][lane & 31] = acc[i][j][q];
-                f(wave_i() + 32 * i, wave_j() + 32 * j, blk);
+                const int r = wave_j() + 32 * j + (lane & 31);
+                const char* at = st + (r * Q + (piece ^ swz(r))) * 16;
+                qh[j] = *(const half8v*)(at + 2 * kArray);
+                ql[j] = *(const half8v*)(at + 3 * kArray);
             }
-    }
-};
-template <> struct Tile<double, 64> {
-    static constexpr int kThreads = 256;
-    static constexpr int BK = 16;
-    static constexpr size_t kBytes = kWaves * 32 * 33 * sizeof(double);   // of the result's blocks; the stages take less
-    static_assert(kBytes >= 2 * 64 * (BK + 2) * sizeof(double));
-    double4v acc[2][2];
-    __device__ __forceinline__ void run(const Wide& p, const Wide& q, size_t i0, size_t j0, int ld, int K, char* shared) {
-        double(*sp)[BK + 2] = (double(*)[BK + 2])shared, (*sq)[BK + 2] = sp + 64;
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-        const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 4;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int jj = 0; jj < 2; ++jj) acc[i][jj] = double4v{ 0, 0, 0, 0 };
-        for (int k = 0; k < K; k += BK) {
-            const double2* ap = (const double2*)(p.v + (i0 + y) * ld + k + x);
-            const double2* aq = (const double2*)(q.v + (j0 + y) * ld + k + x);
-            const double2 a = ap[0], b = ap[1], c = aq[0], d = aq[1];
-            __syncthreads();
-            *(double2*)&sp[y][x] = a;
-            *(double2*)&sp[y][x + 2] = b;
-            *(double2*)&sq[y][x] = c;
-            *(double2*)&sq[y][x + 2] = d;
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < BK; kk += 4) {
-                double pv[2], qv[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    pv[i] = sp[wi + 16 * i + (lane & 15)][kk + (lane >> 4)];
-                    qv[i] = sq[wj + 16 * i + (lane & 15)][kk + (lane >> 4)];
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int jj = 0; jj < 2; ++jj) acc[i][jj] = Mma<double>::go(pv[i], qv[jj], acc[i][jj]);
+            for (int i = 0; i < NI; ++i) {
+                const int r = wave_i() + 32 * i + (lane & 31);
+                const char* at = st + (r * Q + (piece ^ swz(r))) * 16;
+                ph[i] = *(const half8v*)at;
+                pl[i] = *(const half8v*)(at + kArray);
             }
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+            }
+        } else {
+            // a lane's piece holds two neighbours of the summed index; the first ones of the four pieces make one matrix
+            // instruction, the second ones another (the order of a sum's terms is free, as long as P's and Q's agree)
+            const int piece = 4 * kk + (lane >> 4);
+            double2 pv[NI], qv[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int r = wave_j() + 16 * j + (lane & 15);
+                qv[j] = *(const double2*)(st + kArray + (r * Q + (piece ^ swz(r))) * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r = wave_i() + 16 * i + (lane & 15);
+                pv[i] = *(const double2*)(st + (r * Q + (piece ^ swz(r))) * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = Mma<double>::go(pv[i].x, qv[j].x, acc[i][j]);
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = Mma<double>::go(pv[i].y, qv[j].y, acc[i][j]);
         }
     }
-    template <class F>
-    __device__ __forceinline__ void blocks(char* shared, F f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        auto blk = (double(*)[33])shared + wave * 32;
-        __syncthreads();
+
+    // K: a multiple of BK
+    __device__ __forceinline__ void run(const M& p, const M& q, size_t i0, size_t j0, int ld, int K, char* lds) {
+        constexpr int kSteps = Q / (sizeof(C) == 4 ? 2 : 4);
+        static_assert(kSteps % KG == 0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int jj = 0; jj < 2; ++jj)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) blk[16 * i + Mma<double>::row(lane, q)][16 * jj + (lane & 15)] = acc[i][jj][q];
-        f((wave >> 1) * 32, (wave & 1) * 32, blk);
+                for (int r = 0; r < Fr::kRegs; ++r) acc[i][j][r] = 0;
+        const int n = K / BK;
+        Copies c;
+        aim(p, q, i0, j0, ld, c);
+#pragma unroll
+        for (int t = 0; t < S - 1; ++t)
+            if (t < n) fetch(c, t, lds + t * kStage);
+        for (int t = 0; t < n; ++t) {
+            // Stage t has arrived: each wave waits for its own copies (those of the later stages may be under way), the
+            // barrier for the waves'.  The wave has also read what it needs of stage t - 1, which the next copies replace.
+            if (t + S - 1 <= n) wait_and_meet<kCopies * (S - 2)>();
+            else wait_and_meet<0>();
+            if (t + S - 1 < n) fetch(c, t + S - 1, lds + (t + S - 1) % S * kStage);
+            const char* st = lds + t % S * kStage;
+#pragma unroll
+            for (int kk = 0; kk < kSteps / KG; ++kk) multiply(st, kk * KG + group());
+        }
+        __syncthreads();   // the stages are read: the shared memory takes the result
+    }
+
+    // The result, a row of 32 x 32 blocks of each wave at a time, through shared memory:  first(y, x, v) gets N neighbours
+    // D[y][x ..] and may change them, second(y, x, v) then N neighbours D[y ..][x] of the changed result.
+    template <class F, class G>
+    __device__ __forceinline__ void leave(char* lds, F first, G second) {
+        const int lane = threadIdx.x & 63, w = wave() % (WI * WJ), at = group() * 64 + lane, line = at / (2 * KG), seg = at % (2 * KG) * N;
+        auto blk = [&](int g, int j) { return (C(*)[33])lds + ((g * WI * WJ + w) * BJ + j) * 32; };
+        auto meet = [] { if (KG > 1) __syncthreads(); };
+        constexpr int kPer = 32 / Fr::kSide;
+#pragma unroll
+        for (int i = 0; i < BI; ++i) {
+#pragma unroll
+            for (int j = 0; j < BJ; ++j) {
+                auto mine = blk(group(), j);
+#pragma unroll
+                for (int a = 0; a < kPer; ++a)
+#pragma unroll
+                    for (int b = 0; b < kPer; ++b)
+#pragma unroll
+                        for (int q = 0; q < Fr::kRegs; ++q)
+                            mine[a * Fr::kSide + Fr::row(lane, q)][b * Fr::kSide + lane % Fr::kSide] = acc[i * kPer + a][j * kPer + b][q];
+            }
+            meet();
+#pragma unroll
+            for (int j = 0; j < BJ; ++j) {
+                C v[N];
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    v[n] = blk(0, j)[line][seg + n];
+#pragma unroll
+                    for (int g = 1; g < KG; ++g) v[n] += blk(g, j)[line][seg + n];
+                }
+                first(wave_i() + 32 * i + line, wave_j() + 32 * j + seg, v);
+#pragma unroll
+                for (int n = 0; n < N; ++n) blk(0, j)[line][seg + n] = v[n];
+            }
+            meet();
+#pragma unroll
+            for (int j = 0; j < BJ; ++j) {
+                C v[N];
+#pragma unroll
+                for (int n = 0; n < N; ++n) v[n] = blk(0, j)[seg + n][line];
+                second(wave_i() + 32 * i + seg, wave_j() + 32 * j + line, v);
+            }
+            meet();
+        }
     }
 };
 
@@ -507,58 +586,56 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
     const size_t i0 = ti * T, j0 = tj * T;
     const auto a = w.a.at(off), bm = w.b.at(off);
     Tile<C, T> t;
-    // a lane's 16 neighbours of a block: half a row, or half a column
-    const int lane = threadIdx.x & 63, line = lane >> 1, half = (lane & 1) * 16;
+    constexpr int N = Tile<C, T>::N;
     if (kind == kGram || kind == kPoly) {
-        const auto& src = kind == kGram ? w.x[from] : w.a;
-        const auto m = src.at(off), out = kind == kGram ? a : bm;
+        const auto m = (kind == kGram ? w.x[from] : w.a).at(off), out = kind == kGram ? a : bm;
         const int ld = kind == kGram ? w.cp : w.rp;
         t.run(m, m, i0, j0, ld, ld, product_lds);
         const float so = kind == kGram ? kSA : kSB;
         const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA));
-        t.blocks(product_lds, [&](int bi, int bj, C(*blk)[33]) {
-            const size_t y = i0 + bi + line, x = j0 + bj + half;
-            C v[16];
-            if (kind == kPoly) {
-                a.get16(y * w.rp + x, kSA, v);
+        t.leave(product_lds,
+            [&](int y, int x, C* v) {
+                const size_t at = (i0 + y) * w.rp + j0 + x;
+                if (kind == kPoly) {
+                    C av[N];
+                    a.template get<N>(at, kSA, av);
 #pragma unroll
-                for (int n = 0; n < 16; ++n) blk[line][half + n] = v[n] = j.kb * v[n] + j.kc * (f * blk[line][half + n]);
-            } else {
+                    for (int n = 0; n < N; ++n) v[n] = j.kb * av[n] + j.kc * (f * v[n]);
+                } else {
 #pragma unroll
-                for (int n = 0; n < 16; ++n) blk[line][half + n] = v[n] = f * blk[line][half + n];
-            }
-            out.put16(y * w.rp + x, v, so);
-            if (ti == tj) return;
-#pragma unroll
-            for (int n = 0; n < 16; ++n) v[n] = blk[half + n][line];
-            out.put16((j0 + bj + line) * w.rp + i0 + bi + half, v, so);
-        });
+                    for (int n = 0; n < N; ++n) v[n] *= f;
+                }
+                out.template put<N>(at, v, so);
+            },
+            [&](int y, int x, const C* v) {
+                if (ti != tj) out.template put<N>((j0 + x) * w.rp + i0 + y, v, so);
+            });
     } else {
         const auto xt = w.xt[from].at(off), nx = w.x[from ^ 1].at(off), nt = w.xt[from ^ 1].at(off);
         t.run(xt, bm, i0, j0, w.rp, w.rp, product_lds);   // rows: columns of X; columns: rows of X
         const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB));
-        t.blocks(product_lds, [&](int bi, int bj, C(*blk)[33]) {
-            const size_t y = i0 + bi + line, x = j0 + bj + half;
-            C v[16];
-            xt.get16(y * w.rp + x, kSX, v);
+        t.leave(product_lds,
+            [&](int y, int x, C* v) {
+                const size_t at = (i0 + y) * w.rp + j0 + x;
+                C xv[N];
+                xt.template get<N>(at, kSX, xv);
 #pragma unroll
-            for (int n = 0; n < 16; ++n) blk[line][half + n] = v[n] = j.ka * v[n] + f * blk[line][half + n];
-            if (kind == kUpdate) {
-                nt.put16(y * w.rp + x, v, kSX);
+                for (int n = 0; n < N; ++n) v[n] = j.ka * xv[n] + f * v[n];
+                if (kind == kUpdate) nt.template put<N>(at, v, kSX);
+                else if (j.turned) {
 #pragma unroll
-                for (int n = 0; n < 16; ++n) v[n] = blk[half + n][line];
-                nx.put16((j0 + bj + line) * w.cp + i0 + bi + half, v, kSX);
-            } else {
-                // the caller's rows are the block's rows (turned) or its columns: 32 neighbours of a row by half a wave
-                const int64_t r0 = (j.turned ? i0 + bi : j0 + bj) + (lane >> 5), col = (j.turned ? j0 + bj : i0 + bi) + (lane & 31);
-#pragma unroll
-                for (int n = 0; n < 16; ++n) {
-                    const int d = 2 * n + (lane >> 5);
-                    const C o = j.turned ? blk[d][lane & 31] : blk[lane & 31][d];
-                    if (r0 + 2 * n < j.rows && col < j.cols) j.leave(blockIdx.z, r0 + 2 * n, col, o);
+                    for (int n = 0; n < N; ++n)
+                        if ((int)i0 + y < j.rows && (int)j0 + x + n < j.cols) j.leave(blockIdx.z, i0 + y, j0 + x + n, v[n]);
                 }
-            }
-        });
+            },
+            [&](int y, int x, const C* v) {
+                if (kind == kUpdate) nx.template put<N>((j0 + x) * w.cp + i0 + y, v, kSX);
+                else if (!j.turned) {
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+                        if ((int)j0 + x < j.rows && (int)i0 + y + n < j.cols) j.leave(blockIdx.z, j0 + x, i0 + y + n, v[n]);
+                }
+            });
     }
 }
 
