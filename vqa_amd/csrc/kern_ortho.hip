@@ -14,7 +14,6 @@
 //   leaves its normal range) and take the three products hi hi + hi lo + lo hi with 32-bit sums: the left-out lo lo is
 //   2^-22 of a product, the size of the roundings that 32-bit products make along a sum, at 5 times their rate.
 #include <math.h>
-#include <stdlib.h>
 
 #include <algorithm>
 
@@ -64,20 +63,78 @@ struct Job {
     C ka, kb, kc;
     double eps;
 
-    // element e of a matrix in row-major order as it enters the products; first: the momentum is brought up to date
-    template <bool kFirst>
-    __device__ __forceinline__ C enter(int b, int64_t row, int64_t col) const {
-        const C v = Ty::up(g[b * g_batch + row * g_row + col]);
-        if (!m) return v;
-        const int64_t at = ((int64_t)b * rows + row) * cols + col;
-        C mm = m[at];
-        if (kFirst) m[at] = mm = mu * mm + v;
-        return nesterov ? v + mu * mm : mm;
+    // A thread's U elements as they enter the products, all loads under way before the first is used.  at(u, row, col) names
+    // element u (false: there is none, 0).  kFirst: the momentum is brought up to date.
+    template <bool kFirst, int U, class F>
+    __device__ __forceinline__ void enter(int b, C* v, F at) const {
+        const S* gb = g + b * g_batch;
+        C* mb = m + (int64_t)b * rows * cols;
+        S raw[U];
+        C mm[U];
+        bool ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int row = 0, col = 0;
+            ok[u] = at(u, row, col);
+            raw[u] = gb[ok[u] ? row * g_row + col : 0];
+        }
+        if (m) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                int row = 0, col = 0;
+                mm[u] = at(u, row, col) ? mb[(int64_t)row * cols + col] : C(0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] = ok[u] ? Ty::up(raw[u]) : C(0);
+            if (m) {
+                int row = 0, col = 0;
+                at(u, row, col);
+                if (kFirst) {
+                    mm[u] = mu * mm[u] + v[u];
+                    if (ok[u]) mb[(int64_t)row * cols + col] = mm[u];
+                }
+                v[u] = nesterov ? v[u] + mu * mm[u] : mm[u];
+            }
+        }
     }
-    __device__ __forceinline__ void leave(int b, int64_t row, int64_t col, C o) const {
-        const int64_t at = ((int64_t)b * rows + row) * cols + col;
-        if (m) w[at] = decay * w[at] - rate * o;
-        else out[at] = Ty::down(o);
+    // U elements of the result, in the same way
+    template <int U, class F>
+    __device__ __forceinline__ void leave(int b, const C* o, F at) const {
+        const int64_t base = (int64_t)b * rows * cols;
+        int64_t to[U];
+        bool ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int row = 0, col = 0;
+            ok[u] = at(u, row, col);
+            to[u] = base + (ok[u] ? (int64_t)row * cols + col : 0);
+        }
+        if (m) {
+            C ww[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) ww[u] = w[to[u]];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (ok[u]) w[to[u]] = decay * ww[u] - rate * o[u];
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (ok[u]) out[to[u]] = Ty::down(o[u]);
+        }
+    }
+};
+
+// the elements of a rows x cols matrix in row-major order, T threads apart, U at a time: next(row, col) steps T elements on
+template <int T>
+struct Walk {
+    int row, col, dr, dc, cols;
+    __device__ __forceinline__ Walk(int first, int cols_) : row(first / cols_), col(first % cols_), dr(T / cols_), dc(T % cols_), cols(cols_) {}
+    __device__ __forceinline__ void step() {
+        row += dr;
+        col += dc;
+        if (col >= cols) { col -= cols; ++row; }
     }
 };
 
@@ -90,6 +147,14 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
     double s = 0;
     for (int w = 0; w < (int)(blockDim.x >> 6); ++w) s += sh[w];
     return s;
+}
+
+// What a wave's lanes wrote to shared memory before this is what its lanes read after it (and the other way round).  The
+// hardware runs a wave's shared memory accesses in order; this keeps the compiler from moving one lane's accesses past each
+// other that do not meet in that lane.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // ---- 16 x 16 x 4 matrix instruction: lane l holds A[l % 16][l / 16], B[l / 16][l % 16]; D[row(l, reg)][l % 16] ------
@@ -105,117 +170,267 @@ template <> struct Mma<float> {
     static __device__ int row(int l, int reg) { return 4 * (l >> 4) + reg; }
 };
 
-// ---- one workgroup a matrix ---------------------------------------------------------------------------------------
-constexpr int kSmallRows = 64;
-
-int pad16(int v) { return (v + 15) / 16 * 16; }
-size_t small_lds(int r, int c, size_t size) {
-    const size_t rp = pad16(r), cp = pad16(c);
-    return (rp * (cp + 4) + 2 * rp * (rp + 4) + 4 * 256) * size + 64;
-}
-
-template <class Ty>
-__global__ __launch_bounds__(kT) void k_ns_small(Job<Ty> j) {
+// ---- one workgroup a matrix, r <= 16: X in registers -----------------------------------------------------------------
+// A wave holds strips of 16 columns: lane l has X[row(l, q)][l % 16] of a strip in register q, which is at once
+// * the second operand of a product B X (summed index row(l, q)), and its result's layout: X never leaves its registers;
+// * for a symmetric matrix the first operand as well, so A A and B X take A and B as the products before left them.
+// Only X X^T needs X with the columns as summed index: each wave turns its own strip through shared memory and sums over its
+// own columns; the waves' parts of A are added in a fixed order (one barrier a step, two with 16 waves).
+// Bound by the chain of 12 dependent matrix instructions a step (64 cycles each in 64 bits).
+template <class Ty, int NW, int S>
+__global__ __launch_bounds__(NW * 64) void k_ns_strip(Job<Ty> j) {
     using C = typename Ty::C;
     using Acc = typename Mma<C>::Acc;
-    extern __shared__ char lds[];
-    const int rp = (j.r + 15) / 16 * 16, cp = (j.c + 15) / 16 * 16, nt = rp / 16;
-    const int ldx = cp + 4, lda = rp + 4;
-    double* sh = (double*)lds;
-    C* X = (C*)(lds + 64);
+    __shared__ double sh[NW];
+    __shared__ C turn[NW][16][17];
+    __shared__ C part[2][NW][256];
+    __shared__ C total[NW > 4 ? 256 : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15;
+    const int active = min(NW, (j.c + 15) / 16);          // waves with a strip
+
+    const int b = blockIdx.x;
+    C x[S][4];
+    constexpr int SU = S < 4 ? S : 4;                  // strips whose loads are under way at once
+    // (of: the thread's number, as one value for the way in and another for the way out, so that the places of 4 S
+    // elements are worked out twice and not kept in registers through the steps)
+    int of = threadIdx.x;
+    auto at = [&](int s0, int u, int& row, int& col) {
+        const int r = Mma<C>::row(of & 63, u & 3), c = ((s0 + (u >> 2)) * NW + (of >> 6)) * 16 + (of & 15);
+        row = j.turned ? c : r;
+        col = j.turned ? r : c;
+        return r < j.r && c < j.c;
+    };
+#pragma unroll
+    for (int s = 0; s < S; s += SU)
+        j.template enter<true, 4 * SU>(b, x[s], [&](int u, int& row, int& col) { return at(s, u, row, col); });
+    double ss = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ss += (double)x[s][q] * (double)x[s][q];
+    const double norm = sqrt(block_sum(ss, sh)) + j.eps;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[s][q] = (C)((double)x[s][q] / norm);
+
+    for (int step = 0; step < j.steps; ++step) {
+        Acc acc = { 0, 0, 0, 0 };
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if ((s * NW + wave) * 16 < j.c) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) turn[wave][Mma<C>::row(lane, q)][lr] = x[s][q];
+                wave_fence();
+                C a[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) a[q] = turn[wave][lr][Mma<C>::row(lane, q)];
+                wave_fence();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc = Mma<C>::go(a[q], a[q], acc);
+            }
+        auto& pt = part[step & 1];                     // (the other one may still be read)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pt[wave][q * 64 + lane] = acc[q];
+        __syncthreads();
+        C A[4];
+        if constexpr (NW > 4) {
+            if (threadIdx.x < 256) {
+                C v = pt[0][threadIdx.x];
+                for (int w = 1; w < active; ++w) v += pt[w][threadIdx.x];
+                total[threadIdx.x] = v;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) A[q] = total[q * 64 + lane];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                A[q] = pt[0][q * 64 + lane];
+#pragma unroll
+                for (int w = 1; w < NW; ++w) A[q] += pt[w][q * 64 + lane];
+            }
+        }
+        Acc aa = { 0, 0, 0, 0 };
+#pragma unroll
+        for (int q = 0; q < 4; ++q) aa = Mma<C>::go(A[q], A[q], aa);
+        C B[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) B[q] = j.kb * A[q] + j.kc * aa[q];
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if ((s * NW + wave) * 16 < j.c) {
+                Acc up = { 0, 0, 0, 0 };
+#pragma unroll
+                for (int q = 0; q < 4; ++q) up = Mma<C>::go(B[q], x[s][q], up);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[s][q] = j.ka * x[s][q] + up[q];
+            }
+    }
+    asm volatile("" : "+v"(of));
+#pragma unroll
+    for (int s = 0; s < S; s += SU)
+        j.template leave<4 * SU>(b, x[s], [&](int u, int& row, int& col) { return at(s, u, row, col); });
+}
+
+// ---- one workgroup a matrix, 16 < r <= 64: X, A and b A + c A A in shared memory --------------------------------------
+// NT = r / 16 tile rows.  X X^T is dealt as (lower tile, part of the columns) over the 16 waves, the parts added in a fixed
+// order; X <- a X + B X by strips of 16 columns, each read whole by its wave before it is written.
+constexpr int kBlockWaves = 16, kBlockThreads = 64 * kBlockWaves;
+template <int NT>
+struct Block {
+    static constexpr int kRows = 16 * NT, kTiles = NT * (NT + 1) / 2, kParts = kBlockWaves / kTiles, LDA = kRows + 4;
+    static size_t bytes(int c, size_t size) {
+        const size_t cp = (c + 15) / 16 * 16;
+        return (kRows * (cp + 4) + 2 * kRows * LDA + (kParts > 1 ? kTiles * kParts * 256 : 0)) * size + 128;
+    }
+};
+
+// the tile row and column of lower tile t
+__device__ __forceinline__ void lower(int t, int& ti, int& tj) {
+    ti = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0;
+    tj = t - ti * (ti + 1) / 2;
+}
+
+// sum over n4 groups of 4 of xa[4 k] xb[4 k]: operands of four instructions are read before the first is issued
+template <class C>
+__device__ __forceinline__ typename Mma<C>::Acc dot16(const C* xa, const C* xb, int n4) {
+    typename Mma<C>::Acc a0 = { 0, 0, 0, 0 }, a1 = { 0, 0, 0, 0 };
+    int k = 0;
+    for (; k + 4 <= n4; k += 4) {
+        C p[4], q[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) { p[u] = xa[4 * (k + u)]; q[u] = xb[4 * (k + u)]; }
+        a0 = Mma<C>::go(p[0], q[0], a0);
+        a1 = Mma<C>::go(p[1], q[1], a1);
+        a0 = Mma<C>::go(p[2], q[2], a0);
+        a1 = Mma<C>::go(p[3], q[3], a1);
+    }
+    for (; k < n4; ++k) a0 = Mma<C>::go(xa[4 * k], xb[4 * k], a0);
+    return a0 + a1;
+}
+
+template <class Ty, int NT>
+__global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
+    using C = typename Ty::C;
+    using Acc = typename Mma<C>::Acc;
+    using Bl = Block<NT>;
+    constexpr int rp = Bl::kRows, lda = Bl::LDA, tiles = Bl::kTiles, parts = Bl::kParts;
+    extern __shared__ __attribute__((aligned(16))) char block_lds[];
+    const int cp = (j.c + 15) / 16 * 16, ldx = cp + 4;
+    double* sh = (double*)block_lds;
+    C* X = (C*)(block_lds + 128);
     C* A = X + rp * ldx;
     C* B = A + rp * lda;
-    C* part = B + rp * lda;              // [4][256]: a single tile's product, its summed index in four parts
+    C* part = B + rp * lda;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lk = lane >> 4;
+    // this wave's share of X X^T and of A A
+    const int g_part = wave / tiles, g_tile = wave - g_part * tiles;
+    int gi, gj, pi, pj;
+    lower(g_tile, gi, gj);
+    lower(wave < tiles ? wave : 0, pi, pj);
+    const int n4 = cp / 4, per = (n4 + parts - 1) / parts, k0 = g_part * per, kn = min(per, n4 - k0);
 
-    for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
-        for (int i = threadIdx.x; i < rp * ldx; i += kT) X[i] = C(0);
-        __syncthreads();
-        double ss = 0;
-        const int n = j.rows * j.cols;
-        for (int e = threadIdx.x; e < n; e += kT) {
-            const int row = e / j.cols, col = e - row * j.cols;
-            const C v = j.template enter<true>(b, row, col);
-            X[j.turned ? col * ldx + row : row * ldx + col] = v;
-            ss += (double)v * (double)v;
+    const int b = blockIdx.x;
+    for (int i = threadIdx.x; i < rp * ldx; i += kBlockThreads) X[i] = C(0);
+    __syncthreads();
+    double ss = 0;
+    for (Walk<kBlockThreads> w(threadIdx.x, j.cols); w.row < j.rows;) {
+        int row[8], col[8];
+        C v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { row[u] = w.row; col[u] = w.col; w.step(); }
+        j.template enter<true, 8>(b, v, [&](int u, int& r, int& c) { r = row[u]; c = col[u]; return row[u] < j.rows; });
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (row[u] < j.rows) X[j.turned ? col[u] * ldx + row[u] : row[u] * ldx + col[u]] = v[u];
+            ss += (double)v[u] * (double)v[u];
         }
-        const double norm = sqrt(block_sum(ss, sh)) + j.eps;
-        for (int i = threadIdx.x; i < rp * ldx; i += kT) X[i] = (C)((double)X[i] / norm);
-        __syncthreads();
+    }
+    const double norm = sqrt(block_sum(ss, sh)) + j.eps;
+    for (int i = threadIdx.x; i < rp * ldx; i += kBlockThreads) X[i] = (C)((double)X[i] / norm);
+    __syncthreads();
 
-        const int tiles = nt * (nt + 1) / 2, parts = nt == 1 ? kWaves : 1;
-        for (int s = 0; s < j.steps; ++s) {
-            // A = X X^T, its lower tiles
-            for (int it = wave; it < tiles * parts; it += kWaves) {
-                const int t = it / parts, p = it - t * parts;
-                int ti = 0;
-                while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-                const int tj = t - ti * (ti + 1) / 2, len = cp / parts;
-                const C* xa = X + (ti * 16 + lr) * ldx + p * len + lk;
-                const C* xb = X + (tj * 16 + lr) * ldx + p * len + lk;
-                Acc acc = { 0, 0, 0, 0 };
-                for (int k = 0; k < len; k += 4) acc = Mma<C>::go(xa[k], xb[k], acc);
+    for (int s = 0; s < j.steps; ++s) {
+        // A = X X^T, its lower tiles
+        if (g_part < parts) {
+            const Acc acc = dot16<C>(X + (gi * 16 + lr) * ldx + 4 * k0 + lk, X + (gj * 16 + lr) * ldx + 4 * k0 + lk, kn);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = Mma<C>::row(lane, q);
+                if constexpr (parts > 1) part[(g_part * tiles + g_tile) * 256 + row * 16 + lr] = acc[q];
+                else {
+                    A[(gi * 16 + row) * lda + gj * 16 + lr] = acc[q];
+                    A[(gj * 16 + lr) * lda + gi * 16 + row] = acc[q];
+                }
+            }
+        }
+        __syncthreads();
+        if constexpr (parts > 1) {
+            for (int e = threadIdx.x; e < tiles * 256; e += kBlockThreads) {
+                C v = part[e];
+#pragma unroll
+                for (int p = 1; p < parts; ++p) v += part[p * tiles * 256 + e];
+                int ti, tj;
+                lower(e >> 8, ti, tj);
+                const int row = e >> 4 & 15, col = e & 15;
+                A[(ti * 16 + row) * lda + tj * 16 + col] = v;
+                A[(tj * 16 + col) * lda + ti * 16 + row] = v;
+            }
+            __syncthreads();
+        }
+        // B = b A + c A A
+        if (wave < tiles) {
+            const Acc acc = dot16<C>(A + (pi * 16 + lr) * lda + lk, A + (pj * 16 + lr) * lda + lk, rp / 4);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = Mma<C>::row(lane, q);
+                const C v = j.kb * A[(pi * 16 + row) * lda + pj * 16 + lr] + j.kc * acc[q];
+                B[(pi * 16 + row) * lda + pj * 16 + lr] = v;
+                B[(pj * 16 + lr) * lda + pi * 16 + row] = v;
+            }
+        }
+        __syncthreads();
+        // X <- a X + B X
+        for (int n0 = wave * 16; n0 < cp; n0 += kBlockWaves * 16) {
+            Acc acc[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i] = Acc{ 0, 0, 0, 0 };
+#pragma unroll
+            for (int k = 0; k < rp; k += 16) {
+                C xb[4], bv[NT][4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    xb[u] = X[(k + 4 * u + lk) * ldx + n0 + lr];
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) bv[i][u] = B[(i * 16 + lr) * lda + k + 4 * u + lk];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) acc[i] = Mma<C>::go(bv[i][u], xb[u], acc[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int row = Mma<C>::row(lane, q);
-                    if (parts > 1) part[p * 256 + row * 16 + lr] = acc[q];
-                    else {
-                        A[(ti * 16 + row) * lda + tj * 16 + lr] = acc[q];
-                        A[(tj * 16 + lr) * lda + ti * 16 + row] = acc[q];
-                    }
+                    C* x = X + (i * 16 + Mma<C>::row(lane, q)) * ldx + n0 + lr;
+                    *x = j.ka * *x + acc[i][q];
                 }
-            }
-            __syncthreads();
-            if (parts > 1) {
-                const int e = threadIdx.x;
-                A[(e >> 4) * lda + (e & 15)] = (part[e] + part[256 + e]) + (part[512 + e] + part[768 + e]);
-                __syncthreads();
-            }
-            // B = b A + c A A
-            for (int t = wave; t < tiles; t += kWaves) {
-                int ti = 0;
-                while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-                const int tj = t - ti * (ti + 1) / 2;
-                const C* xa = A + (ti * 16 + lr) * lda + lk;
-                const C* xb = A + (tj * 16 + lr) * lda + lk;
-                Acc acc = { 0, 0, 0, 0 };
-                for (int k = 0; k < rp; k += 4) acc = Mma<C>::go(xa[k], xb[k], acc);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int row = Mma<C>::row(lane, q);
-                    const C v = j.kb * A[(ti * 16 + row) * lda + tj * 16 + lr] + j.kc * acc[q];
-                    B[(ti * 16 + row) * lda + tj * 16 + lr] = v;
-                    B[(tj * 16 + lr) * lda + ti * 16 + row] = v;
-                }
-            }
-            __syncthreads();
-            // X <- a X + B X, a strip of 16 columns by one wave: it reads all of the strip before it writes any
-            for (int n0 = wave * 16; n0 < cp; n0 += kWaves * 16) {
-                Acc acc[kSmallRows / 16];
-#pragma unroll
-                for (int i = 0; i < kSmallRows / 16; ++i) acc[i] = Acc{ 0, 0, 0, 0 };
-                for (int k = 0; k < rp; k += 4) {
-                    const C xb = X[(k + lk) * ldx + n0 + lr];
-#pragma unroll
-                    for (int i = 0; i < kSmallRows / 16; ++i)
-                        if (i < nt) acc[i] = Mma<C>::go(B[(i * 16 + lr) * lda + k + lk], xb, acc[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < kSmallRows / 16; ++i)
-                    if (i < nt)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            C* x = X + (i * 16 + Mma<C>::row(lane, q)) * ldx + n0 + lr;
-                            *x = j.ka * *x + acc[i][q];
-                        }
-            }
-            __syncthreads();
-        }
-        for (int e = threadIdx.x; e < n; e += kT) {
-            const int row = e / j.cols, col = e - row * j.cols;
-            j.leave(b, row, col, X[j.turned ? col * ldx + row : row * ldx + col]);
         }
         __syncthreads();
+    }
+    for (Walk<kBlockThreads> w(threadIdx.x, j.cols); w.row < j.rows;) {
+        int row[8], col[8];
+        C v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            row[u] = w.row;
+            col[u] = w.col;
+            v[u] = row[u] < j.rows ? X[j.turned ? col[u] * ldx + row[u] : row[u] * ldx + col[u]] : C(0);
+            w.step();
+        }
+        j.template leave<8>(b, v, [&](int u, int& r, int& c) { r = row[u]; c = col[u]; return row[u] < j.rows; });
     }
 }
 
@@ -300,16 +515,23 @@ struct Mats {
     int rp, cp;
 };
 
+// Parts of the sum of squares (and the momentum): a workgroup takes whole rows in turn, or, of few long rows, pieces of them.
+// 16 loads of a thread are under way at once.
 template <class Ty>
-__global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t stride) {
+__global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t stride, int pieces) {
+    using C = typename Ty::C;
+    constexpr int U = 16;
     __shared__ double sh[kWaves];
     const int b = blockIdx.y;
-    const int64_t n = (int64_t)j.rows * j.cols;
     double ss = 0;
-    for (int64_t e = (int64_t)blockIdx.x * kT + threadIdx.x; e < n; e += (int64_t)gridDim.x * kT) {
-        const int64_t row = e / j.cols, col = e - row * j.cols;
-        const double v = (double)j.template enter<true>(b, row, col);
-        ss += v * v;
+    for (int it = blockIdx.x; it < j.rows * pieces; it += gridDim.x) {
+        const int row = it / pieces, per = (j.cols + pieces - 1) / pieces, c0 = (it - row * pieces) * per, c1 = min(j.cols, c0 + per);
+        for (int c = c0 + threadIdx.x; c < c1; c += kT * U) {
+            C v[U];
+            j.template enter<true, U>(b, v, [&](int u, int& r, int& cc) { r = row; cc = c + u * kT; return c + u * kT < c1; });
+#pragma unroll
+            for (int u = 0; u < U; ++u) ss += (double)v[u] * (double)v[u];
+        }
     }
     ss = block_sum(ss, sh);
     if (threadIdx.x == 0) ((double*)((char*)part + b * stride))[blockIdx.x] = ss;
@@ -327,18 +549,29 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
     const double norm = sqrt(block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh)) + j.eps;
     // rows and columns of the caller's matrix
     const int64_t r0 = (int64_t)(j.turned ? blockIdx.x : blockIdx.y) * kTile, c0 = (int64_t)(j.turned ? blockIdx.y : blockIdx.x) * kTile;
-    for (int e = threadIdx.x; e < kTile * kTile; e += kT) {
-        const int y = e / kTile, x = e % kTile;
-        tile[y][x] = r0 + y < j.rows && c0 + x < j.cols ? (C)((double)j.template enter<false>(b, r0 + y, c0 + x) / norm) : C(0);
-    }
+    constexpr int U = kTile * kTile / kT;
+    C v[U];
+    j.template enter<false, U>(b, v, [&](int u, int& row, int& col) {
+        const int e = threadIdx.x + u * kT;
+        row = (int)r0 + e / kTile;
+        col = (int)c0 + e % kTile;
+        return row < j.rows && col < j.cols;
+    });
+#pragma unroll
+    for (int u = 0; u < U; ++u) tile[(threadIdx.x + u * kT) / kTile][threadIdx.x % kTile] = (C)((double)v[u] / norm);
     __syncthreads();
     const auto xm = w.x[0].at(off), xt = w.xt[0].at(off);
     const size_t x0 = (size_t)blockIdx.y * kTile, y0 = (size_t)blockIdx.x * kTile;   // row and column of X
-    for (int e = threadIdx.x; e < kTile * kTile; e += kT) {
-        const int y = e / kTile, x = e % kTile;
-        xm.put((x0 + y) * w.cp + y0 + x, j.turned ? tile[x][y] : tile[y][x], kSX);
-        xt.put((y0 + y) * w.rp + x0 + x, j.turned ? tile[y][x] : tile[x][y], kSX);
+    // a lane's 16 neighbours of a row of X, and of X^T
+    const int y = threadIdx.x >> 2, x = (threadIdx.x & 3) * 16;
+    C p[16], q[16];
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        p[n] = j.turned ? tile[x + n][y] : tile[y][x + n];
+        q[n] = j.turned ? tile[y][x + n] : tile[x + n][y];
     }
+    xm.template put<16>((x0 + y) * w.cp + y0 + x, p, kSX);
+    xt.template put<16>((y0 + y) * w.rp + x0 + x, q, kSX);
 }
 
 enum Kind { kGram, kPoly, kUpdate, kLast };
@@ -526,7 +759,7 @@ struct Tile : Shape<C, T> {
     __device__ __forceinline__ void leave(char* lds, F first, G second) {
         const int lane = threadIdx.x & 63, w = wave() % (WI * WJ), at = group() * 64 + lane, line = at / (2 * KG), seg = at % (2 * KG) * N;
         auto blk = [&](int g, int j) { return (C(*)[33])lds + ((g * WI * WJ + w) * BJ + j) * 32; };
-        auto meet = [] { if (KG > 1) __syncthreads(); };
+        auto meet = [] { if (KG > 1) __syncthreads(); else wave_fence(); };
         constexpr int kPer = 32 / Fr::kSide;
 #pragma unroll
         for (int i = 0; i < BI; ++i) {
@@ -622,19 +855,21 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
 #pragma unroll
                 for (int n = 0; n < N; ++n) v[n] = j.ka * xv[n] + f * v[n];
                 if (kind == kUpdate) nt.template put<N>(at, v, kSX);
-                else if (j.turned) {
-#pragma unroll
-                    for (int n = 0; n < N; ++n)
-                        if ((int)i0 + y < j.rows && (int)j0 + x + n < j.cols) j.leave(blockIdx.z, i0 + y, j0 + x + n, v[n]);
-                }
+                else if (j.turned)
+                    j.template leave<N>(blockIdx.z, v, [&](int n, int& row, int& col) {
+                        row = (int)i0 + y;
+                        col = (int)j0 + x + n;
+                        return row < j.rows && col < j.cols;
+                    });
             },
             [&](int y, int x, const C* v) {
                 if (kind == kUpdate) nx.template put<N>((j0 + x) * w.cp + i0 + y, v, kSX);
-                else if (!j.turned) {
-#pragma unroll
-                    for (int n = 0; n < N; ++n)
-                        if ((int)j0 + x < j.rows && (int)i0 + y + n < j.cols) j.leave(blockIdx.z, j0 + x, i0 + y + n, v[n]);
-                }
+                else if (!j.turned)
+                    j.template leave<N>(blockIdx.z, v, [&](int n, int& row, int& col) {
+                        row = (int)j0 + x;
+                        col = (int)i0 + y + n;
+                        return row < j.rows && col < j.cols;
+                    });
             });
     }
 }
@@ -642,16 +877,23 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
 // ---- launches -------------------------------------------------------------------------------------------------------
 constexpr size_t kLds = 160 * 1024;
 
-bool is_small(int dtype, int r, int c) {
-    return r <= kSmallRows && c <= 32768 && small_lds(r, c, dtype == VQA_DTYPE_F64 ? 8 : 4) <= kLds;
+// Which form carries a matrix: 0 tiled products, 1 strips in registers, 2 blocks in shared memory
+int form_of(int dtype, int r, int c) {
+    const size_t size = dtype == VQA_DTYPE_F64 ? 8 : 4;
+    if (r <= 16) return c <= (size == 8 ? 2048 : 4096) ? 1 : 0;   // (the registers of 16 waves)
+    if (r > 64 || c > 8192) return 0;
+    return (r <= 32 ? Block<2>::bytes(c, size) : r <= 48 ? Block<3>::bytes(c, size) : Block<4>::bytes(c, size)) <= kLds ? 2 : 0;
 }
-// Side of a product's tile.  128 where the update has at least as many tiles as half the chip's CUs
-int tile_of(int dtype, int batch, int r, int c) {
+// Side of a product's tile: the largest whose symmetric products still have a tile for half of the 256 CUs; below that the
+// chip stands still, above it larger tiles read less.  All five steps, 32 bits, us: 4096 x 4096  6443 (64), 5295 (128),
+// 4892 (256);  2048 x 2048  956, 823, 2265;  1024 x 1024  199, 424, 1236.
+int tile_of(int dtype, int batch, int r) {
     if (dtype == VQA_DTYPE_F64) return 64;
-    const int64_t n = (int64_t)((r + 127) / 128) * ((c + 127) / 128) * batch;
-    static const int forced = getenv("NS_TILE") ? atoi(getenv("NS_TILE")) : 0;
-    if (forced) return forced;
-    return n >= 1024 ? 256 : n >= 128 ? 128 : 64;
+    for (int t = 256; t > 64; t /= 2) {
+        const int64_t n = (r + t - 1) / t;
+        if (n * (n + 1) / 2 * batch >= 128) return t;
+    }
+    return 64;
 }
 int pad_to(int v, int t) { return (v + t - 1) / t * t; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -706,6 +948,14 @@ int allow_lds(F* fn, size_t bytes) {
     return VQA_OK;
 }
 
+template <class Ty, int NT>
+int block(hipStream_t st, const Job<Ty>& j) {
+    const size_t lds = Block<NT>::bytes(j.c, sizeof(typename Ty::C));
+    if (int rc = allow_lds(k_ns_block<Ty, NT>, lds)) return rc;
+    hipLaunchKernelGGL((k_ns_block<Ty, NT>), dim3((unsigned)j.batch), dim3(kBlockThreads), lds, st, j);
+    return VQA_OK;
+}
+
 template <class Ty, Kind kind, int T>
 int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
     using Tl = Tile<typename Ty::C, T>;
@@ -752,20 +1002,31 @@ int run(hipStream_t st, const OrthoCall& q) {
     j.kb = (C)q.coefs[1];
     j.kc = (C)q.coefs[2];
     j.eps = q.eps;
-    if (is_small(q.dtype, j.r, j.c)) {
-        const size_t lds = small_lds(j.r, j.c, sizeof(C));
-        if (int rc = allow_lds(k_ns_small<Ty>, lds)) return rc;
-        hipLaunchKernelGGL((k_ns_small<Ty>), dim3((unsigned)q.batch), dim3(kT), lds, st, j);
+    const int form = form_of(q.dtype, j.r, j.c);
+    if (form == 1) {
+        const int strips = (j.c + 15) / 16;
+        const dim3 grid((unsigned)q.batch);
+        if (strips <= 4) hipLaunchKernelGGL((k_ns_strip<Ty, 4, 1>), grid, dim3(256), 0, st, j);
+        else if (strips <= 16) hipLaunchKernelGGL((k_ns_strip<Ty, 4, 4>), grid, dim3(256), 0, st, j);
+        else if (strips <= 64) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 4>), grid, dim3(1024), 0, st, j);
+        else if (strips <= 128) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 8>), grid, dim3(1024), 0, st, j);
+        else if constexpr (sizeof(C) == 4) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 16>), grid, dim3(1024), 0, st, j);
+        VQA_HIP(hipGetLastError());
+        return VQA_OK;
+    }
+    if (form == 2) {
+        const int rc = j.r <= 32 ? block<Ty, 2>(st, j) : j.r <= 48 ? block<Ty, 3>(st, j) : block<Ty, 4>(st, j);
+        if (rc) return rc;
         VQA_HIP(hipGetLastError());
         return VQA_OK;
     }
     Mats<typename StoreOf<C>::T> w;
-    const int tile = tile_of(q.dtype, q.batch, j.r, j.c);
+    const int tile = tile_of(q.dtype, q.batch, j.r);
     lay_out((char*)q.workspace, j.r, j.c, tile, &w);
-    const int64_t n = (int64_t)j.rows * j.cols;
-    const int parts = (int)std::min<int64_t>(kNormParts, (n + 4 * kT - 1) / (4 * kT));
     const unsigned nb = (unsigned)q.batch;
-    hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride);
+    const int pieces = std::max(1, std::min((j.cols + 4 * kT - 1) / (4 * kT), (2 * kNormParts + j.rows - 1) / j.rows));
+    const int parts = std::min(kNormParts, j.rows * pieces);
+    hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride, pieces);
     hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(w.cp / kTile, w.rp / kTile, nb), dim3(kT), 0, st, j, w, parts);
     int rc;
     if constexpr (sizeof(C) == 4) {
@@ -780,13 +1041,13 @@ int run(hipStream_t st, const OrthoCall& q) {
 
 size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
     const int r = std::min(rows, cols), c = std::max(rows, cols);
-    if (is_small(dtype, r, c)) return 0;
+    if (form_of(dtype, r, c)) return 0;
     if (dtype == VQA_DTYPE_F64) {
         Mats<Wide> w;
-        return lay_out<Wide>(nullptr, r, c, tile_of(dtype, batch, r, c), &w) * (size_t)batch;
+        return lay_out<Wide>(nullptr, r, c, tile_of(dtype, batch, r), &w) * (size_t)batch;
     }
     Mats<Pair> w;
-    return lay_out<Pair>(nullptr, r, c, tile_of(dtype, batch, r, c), &w) * (size_t)batch;
+    return lay_out<Pair>(nullptr, r, c, tile_of(dtype, batch, r), &w) * (size_t)batch;
 }
 
 int ortho_launch(hipStream_t stream, const OrthoCall& q) {
