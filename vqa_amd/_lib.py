@@ -117,3 +117,17 @@ def check(rc: int) -> int:
 def nptr(a):
     """void* of a C-contiguous numpy array (or None)."""
     return None if a is None else C.c_void_p(a.ctypes.data)
+
+
+_raw_stream = None
+
+
+def current_stream(index: int) -> int:
+    """The current torch stream of a device as the C ABI takes it.  torch's own accessor of the handle where it has one: an
+    optimizer step or a read-out of a few rows takes less time than making a Stream object around it."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)

@@ -27,11 +27,8 @@ struct F16 { using S = _Float16; using A = float; static constexpr bool kFast = 
     static __device__ A up(S v) { return (float)v; } static __device__ S down(A v) { return (_Float16)v; } };
 struct BF16 { using S = uint16_t; using A = float; static constexpr bool kFast = true;
     static __device__ A up(S v) { return __uint_as_float((uint32_t)v << 16); }
-    static __device__ S down(A v) {   // round to nearest even; NaN stays NaN
-        const uint32_t u = __float_as_uint(v);
-        if (v != v) return (uint16_t)((u >> 16) | 0x40);
-        return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
-    } };
+    static __device__ S down(A v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest even
+    };
 
 __device__ __forceinline__ double neg_inf(double) { return -__builtin_inf(); }
 __device__ __forceinline__ float neg_inf(float) { return -__builtin_inff(); }
@@ -242,6 +239,34 @@ __device__ __forceinline__ void load_piece(const typename Ty::S* zr, int64_t e0,
     }
 }
 
+// ---- lanes ---------------------------------------------------------------------------------------------------------
+// a value of one lane (the lane's number is the same for the whole wave) for all, and a value of the lane before
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(lane_of(__float_as_int(v), lane)); }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    return __hiloint2double(lane_of(__double2hiint(v), lane), lane_of(__double2loint(v), lane));
+}
+template <int kCtrl>
+__device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, kCtrl, 0xf, 0xf, false); }
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float old, float v) { return __int_as_float(dpp<kCtrl>(__float_as_int(old), __float_as_int(v))); }
+template <int kCtrl>
+__device__ __forceinline__ double dpp(double old, double v) {
+    return __hiloint2double(dpp<kCtrl>(__double2hiint(old), __double2hiint(v)), dpp<kCtrl>(__double2loint(old), __double2loint(v)));
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143, kWaveShr1 = 0x138;
+// the largest of a wave's values, for all lanes
+template <class A>
+__device__ __forceinline__ A wave_max(A v) {
+    v = max_of(v, dpp<kShr1>(v, v));
+    v = max_of(v, dpp<kShr2>(v, v));
+    v = max_of(v, dpp<kShr4>(v, v));
+    v = max_of(v, dpp<kShr8>(v, v));
+    v = max_of(v, dpp<kBcast15>(v, v));
+    v = max_of(v, dpp<kBcast31>(v, v));
+    return lane_of(v, 63);
+}
+
 // a wave's list of its best outcomes, one a lane, best first (value, then lower index)
 template <class A>
 struct Best {
@@ -249,16 +274,31 @@ struct Best {
     int i;
 };
 template <class A>
+__device__ __forceinline__ Best<A> nobody() { return Best<A>{ neg_inf(A(0)), 0x7fffffff }; }
+// v and i: the same for the whole wave
+template <class A>
 __device__ __forceinline__ void insert(Best<A>& b, A v, int i, int lane) {
     const int pos = __popcll(__ballot(before(b.v, b.i, v, i)));
-    const A uv = __shfl_up(b.v, 1);
-    const int ui = __shfl_up(b.i, 1);
-    if (lane == pos) { b.v = v; b.i = i; }
-    else if (lane > pos) { b.v = uv; b.i = ui; }
+    const A uv = dpp<kWaveShr1>(b.v, b.v);
+    const int ui = dpp<kWaveShr1>(b.i, b.i);
+    b.v = lane < pos ? b.v : lane == pos ? v : uv;
+    b.i = lane < pos ? b.i : lane == pos ? i : ui;
 }
 
+// another list (best first, one a lane) into a wave's
+template <class A>
+__device__ __forceinline__ void merge(Best<A>& b, const Best<A>& c, int top_k, int lane) {
+    for (int k = 0; k < top_k; ++k) {
+        const A v = lane_of(c.v, k);
+        const int i = lane_of(c.i, k);
+        if (!(v > neg_inf(A(0))) || !before(v, i, lane_of(b.v, top_k - 1), lane_of(b.i, top_k - 1))) break;
+        insert(b, v, i, lane);
+    }
+}
+
+// B elements a lane into the wave's running state.  m is the wave's (the same in all lanes), s and t are the lane's.
 template <class Ty, int B, bool kTop>
-__device__ __forceinline__ void take(const typename Ty::A* v, const int64_t* at, Part<typename Ty::A>& p, Best<typename Ty::A>& best,
+__device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Part<typename Ty::A>& p, Best<typename Ty::A>& best,
                                      int top_k, typename Ty::A scale, int lane) {
     using A = typename Ty::A;
     constexpr int N = Piece<Ty>::N;
@@ -266,47 +306,61 @@ __device__ __forceinline__ void take(const typename Ty::A* v, const int64_t* at,
 #pragma unroll
     for (int j = 1; j < B; ++j) mx = max_of(mx, v[j]);
     if constexpr (kTop) {
-        A kv = __shfl(best.v, top_k - 1);
-        if (__any(mx >= kv && mx > neg_inf(A(0)))) {
-            int ki = __shfl(best.i, top_k - 1);
+        A kv = lane_of(best.v, top_k - 1);
+        if (__ballot(mx >= kv && mx > neg_inf(A(0)))) {
+            int ki = lane_of(best.i, top_k - 1);
 #pragma unroll
             for (int j = 0; j < B; ++j) {
-                const int ix = (int)(at[j / N] + j % N);
-                uint64_t want = __ballot(v[j] > neg_inf(A(0)) && before(v[j], ix, kv, ki));
+                uint64_t want = __ballot(v[j] >= kv && v[j] > neg_inf(A(0)));
                 while (want) {
                     const int src = __builtin_ctzll(want);
-                    insert(best, __shfl(v[j], src), __shfl(ix, src), lane);
-                    kv = __shfl(best.v, top_k - 1);
-                    ki = __shfl(best.i, top_k - 1);
+                    const A cv = lane_of(v[j], src);
+                    const int ci = lane_of(at[j / N], src) + j % N;
                     want &= want - 1;
-                    want &= __ballot(before(v[j], ix, kv, ki));
+                    if (before(cv, ci, kv, ki)) {
+                        insert(best, cv, ci, lane);
+                        kv = lane_of(best.v, top_k - 1);
+                        ki = lane_of(best.i, top_k - 1);
+                        want &= __ballot(v[j] >= kv);
+                    }
                 }
             }
         }
     }
-    const A m = max_of(p.m, mx);                 // (a NaN is not taken as the maximum, it shows in s)
-    const A base = m == neg_inf(A(0)) ? A(0) : m;
-    bool left_out = !(mx > p.m);                 // the maximum stays where it was: its term is out already
-    if (!left_out && p.m > neg_inf(A(0))) {      // the old maximum's term comes in
-        const A d = floor_of((p.m - m) * scale), f = exp_neg<Ty>(d), all = p.s + A(1);
-        p.s = f * all;
-        p.t = f * (p.t + d * all);
-    }
-    p.m = m;
+    if (__ballot(mx > p.m)) {                     // a new maximum (a NaN is not taken as one, it shows in s)
+        const A m = wave_max(max_of(mx, p.m));
+        const uint64_t holders = __ballot(mx == m);
+        if (p.m > neg_inf(A(0))) {                // the old one's term comes in, in lane 0's sums
+            const A d = floor_of((p.m - m) * scale), f = exp_neg<Ty>(d), all = p.s + (lane == 0 ? A(1) : A(0));
+            p.s = f * all;
+            p.t = f * (p.t + d * all);
+        }
+        p.m = m;
+        bool left_out = lane != __builtin_ctzll(holders);     // one of the lanes that have it leaves its first one out
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-        const A d = (v[j] - base) * scale;
-        const bool out = !left_out && v[j] == m;
-        left_out |= out;
-        const A e = out ? A(0) : exp_neg<Ty>(d);
-        p.s += e;
-        p.t += e * floor_of(d);
+        for (int j = 0; j < B; ++j) {
+            const A d = (v[j] - m) * scale;
+            const bool out = !left_out && v[j] == m;
+            left_out |= out;
+            const A e = out ? A(0) : exp_neg<Ty>(d);
+            p.s += e;
+            p.t += e * floor_of(d);
+        }
+    } else {
+        const A m = p.m == neg_inf(A(0)) ? A(0) : p.m;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const A d = (v[j] - m) * scale;
+            const A e = exp_neg<Ty>(d);
+            p.s += e;
+            p.t += e * floor_of(d);
+        }
     }
 }
 
-// the same row part by one workgroup; the result is complete in wave 0 (all lanes)
+// a part of a row by one workgroup; the result is complete in wave 0 (all lanes)
 template <class Ty, bool kTop>
-__device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* zr, int64_t width, int64_t split, int64_t splits,
+__device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* zr, int64_t width, int split, int splits,
                                                           typename Ty::A scale, int top_k, Best<typename Ty::A>& best) {
     using A = typename Ty::A;
     constexpr int N = Piece<Ty>::N, U = 4;
@@ -315,20 +369,23 @@ __device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* 
     const int64_t per = (pc.pieces + splits - 1) / splits;
     const int64_t p0 = split * per, p1 = min(pc.pieces, p0 + per);
     Part<A> p = { neg_inf(A(0)), A(0), A(0) };
-    best = Best<A>{ neg_inf(A(0)), 0x7fffffff };
+    best = nobody<A>();
     for (int64_t q = p0 + wave * 64; q < p1; q += kT * U) {    // the same count for a wave's lanes
         A v[U * N];
-        int64_t at[U];
+        int at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t piece = q + u * kT + lane;
-            at[u] = piece * N - pc.off;
-            load_piece<Ty>(zr, piece < p1 ? at[u] : width, width, v + u * N);
+            const int64_t piece = q + u * kT + lane, e0 = piece < p1 ? piece * N - pc.off : width;
+            at[u] = (int)e0;
+            load_piece<Ty>(zr, e0, width, v + u * N);
         }
         take<Ty, U * N, kTop>(v, at, p, best, top_k, scale, lane);
     }
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
+    for (int o = 1; o < 64; o <<= 1) {
+        p.s += __shfl_xor(p.s, o);
+        p.t += __shfl_xor(p.t, o);
+    }
     __shared__ Part<A> sp[kWaves];
     __shared__ Best<A> sb[kWaves][64];
     if (lane == 0) sp[wave] = p;
@@ -338,12 +395,7 @@ __device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* 
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) p = join(p, sp[w], scale);
         if constexpr (kTop) {
-            for (int w = 1; w < kWaves; ++w)
-                for (int k = 0; k < top_k; ++k) {
-                    const Best<A> c = sb[w][k];
-                    if (!(c.v > neg_inf(A(0))) || !before(c.v, c.i, __shfl(best.v, top_k - 1), __shfl(best.i, top_k - 1))) break;
-                    insert(best, c.v, c.i, lane);
-                }
+            for (int w = 1; w < kWaves; ++w) merge(best, sb[w][lane], top_k, lane);
         }
     }
     return p;
@@ -355,95 +407,251 @@ struct Ws {   // the parts of the rows, and the parts' best outcomes
     Best<A>* best;
 };
 
-template <class Ty, bool kTop>
-__global__ __launch_bounds__(kT) void k_lp_parts(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
-                                                 typename Ty::A scale, int top_k, int splits, Ws<typename Ty::A> ws) {
-    using A = typename Ty::A;
-    for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
-        const int64_t row = it / splits, split = it - row * splits;
-        Best<A> best;
-        const Part<A> p = read_part<Ty, kTop>(z + row * ld, width, split, splits, scale, top_k, best);
-        if (threadIdx.x == 0) ws.part[it] = p;
-        if constexpr (kTop)
-            if ((int)threadIdx.x < top_k) ws.best[it * top_k + threadIdx.x] = best;
-        __syncthreads();   // the shared arrays are written again
-    }
-}
-
-// one wave a row: joins its parts (at most 64, one a lane, in a fixed tree) and merges their lists of best outcomes
+// what a row's call returns, by the lanes of one wave that all hold the row's state
 template <class Ty>
-__global__ __launch_bounds__(64) void k_lp_join(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
-                                                typename Ty::A scale, const int32_t* __restrict__ target, int top_k, int splits,
-                                                Ws<typename Ty::A> ws, typename Ty::A* lp_out, typename Ty::A* ent_out,
-                                                typename Ty::A* top_lp, int32_t* top_ix) {
+struct Out {
     using A = typename Ty::A;
-    const int lane = threadIdx.x;
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        Part<A> p = { neg_inf(A(0)), A(0), A(0) };
-        if (lane < splits) p = ws.part[row * splits + lane];
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
+    const int32_t* target;
+    A *lp, *ent, *top_lp;
+    int32_t* top_ix;
+    int top_k;
+    __device__ __forceinline__ void write(int64_t row, const typename Ty::S* zr, int64_t width, const Part<A>& p, const Best<A>& best,
+                                          A scale, int lane) const {
         Row<A> r = finish(p);
         const int tg = target ? target[row] : -1;
         given(r, tg, width);
         if (lane == 0) {
-            if (ent_out) ent_out[row] = r.entropy;
-            if (lp_out) lp_out[row] = r.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(r, Ty::up(z[row * ld + tg]), scale));
+            if (ent) ent[row] = r.entropy;
+            if (lp) lp[row] = r.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(r, Ty::up(zr[tg]), scale));
         }
-        int head = 0;
-        Best<A> c = { neg_inf(A(0)), 0x7fffffff };
-        if (lane < splits && top_k > 0) c = ws.best[(row * splits + lane) * top_k];
-        for (int k = 0; k < top_k; ++k) {
-            A bv = c.v;
-            int bi = c.i;
+        if (lane < top_k) {
+            const bool none = r.bad || best.i == 0x7fffffff;
+            top_lp[row * top_k + lane] = r.bad ? nan_of(A(0)) : (none ? neg_inf(A(0)) : log_p(r, best.v, scale));
+            top_ix[row * top_k + lane] = none ? -1 : best.i;
+        }
+    }
+};
+
+// splits = 1: the workgroup writes the row's results, else its part of them
+template <class Ty, bool kTop>
+__global__ __launch_bounds__(kT) void k_lp_parts(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                 typename Ty::A scale, int top_k, int splits, Ws<typename Ty::A> ws, Out<Ty> out) {
+    using A = typename Ty::A;
+    for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
+        const int64_t row = it / splits;
+        const int split = (int)(it - row * splits);
+        Best<A> best;
+        const Part<A> p = read_part<Ty, kTop>(z + row * ld, width, split, splits, scale, top_k, best);
+        if (threadIdx.x < 64) {
+            if (splits == 1 && !ws.part) {
+                out.write(row, z + row * ld, width, p, best, scale, threadIdx.x);
+            } else {
+                if (threadIdx.x == 0) ws.part[it] = p;
+                if constexpr (kTop)
+                    if ((int)threadIdx.x < top_k) ws.best[it * top_k + threadIdx.x] = best;
+            }
+        }
+        __syncthreads();   // the shared arrays are written again
+    }
+}
+
+// a row's parts (at most 64), joined in a fixed tree by a wave
+template <class A>
+__device__ __forceinline__ Part<A> join_parts(const Part<A>* part, int splits, A scale, int lane) {
+    Part<A> p = { neg_inf(A(0)), A(0), A(0) };
+    if (lane < splits) p = part[lane];
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const A ov = __shfl_xor(bv, o);
-                const int oi = __shfl_xor(bi, o);
-                if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+    for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
+    return p;
+}
+
+// one wave a row: joins its parts and their lists of best outcomes
+template <class Ty>
+__global__ __launch_bounds__(64) void k_lp_join(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                typename Ty::A scale, int top_k, int splits, Ws<typename Ty::A> ws, Out<Ty> out) {
+    using A = typename Ty::A;
+    const int lane = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        Best<A> best = nobody<A>();
+        if (top_k > 0) {
+            constexpr int U = 8;
+            for (int s0 = 0; s0 < splits; s0 += U) {
+                Best<A> c[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) c[u] = s0 + u < splits && lane < top_k ? ws.best[(row * splits + s0 + u) * top_k + lane] : nobody<A>();
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (s0 + u == 0) best = c[u];
+                    else merge(best, c[u], top_k, lane);
+                }
             }
-            const bool none = r.bad || bi == 0x7fffffff;
-            if (lane == 0) {
-                top_lp[row * top_k + k] = r.bad ? nan_of(A(0)) : (none ? neg_inf(A(0)) : log_p(r, bv, scale));
-                top_ix[row * top_k + k] = none ? -1 : bi;
-            }
-            if (c.i == bi && bi != 0x7fffffff) {
-                ++head;
-                c = head < top_k ? ws.best[(row * splits + lane) * top_k + head] : Best<A>{ neg_inf(A(0)), 0x7fffffff };
-            }
+        }
+        out.write(row, z + row * ld, width, join_parts(ws.part + row * splits, splits, scale, lane), best, scale, lane);
+    }
+}
+
+// one piece of the gradient: 16 bytes at once where both rows allow it
+template <class Ty>
+__device__ __forceinline__ void store_piece(typename Ty::S* dr, int64_t e0, int64_t width, bool whole, const typename Ty::A* v) {
+    constexpr int N = Piece<Ty>::N;
+    if (whole && e0 >= 0 && e0 + N <= width) {
+        alignas(16) typename Ty::S raw[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) raw[j] = Ty::down(v[j]);
+        *reinterpret_cast<uint4*>(dr + e0) = *reinterpret_cast<const uint4*>(raw);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (e0 + j >= 0 && e0 + j < width) dr[e0 + j] = Ty::down(v[j]);
+    }
+}
+
+// the row's log probability and entropy beside its gradient, by one thread; returns the state for the gradient
+template <class Ty>
+struct LossOut {
+    using A = typename Ty::A;
+    const int32_t* target;
+    const A *dg, *dh;
+    A *lp, *ent;
+    typename Ty::S* dz;
+    int64_t ld_dz;
+    __device__ __forceinline__ Row<A> row(int64_t r, const typename Ty::S* zr, int64_t width, const Part<A>& p, A scale, bool write,
+                                          int& tg, Grad<A>& w) const {
+        Row<A> s = finish(p);
+        tg = target ? target[r] : -1;
+        given(s, tg, width);
+        if (write) {
+            if (ent) ent[r] = s.entropy;
+            if (lp) lp[r] = s.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(s, Ty::up(zr[tg]), scale));
+        }
+        w = Grad<A>{ tg < 0 ? A(0) : (dg ? dg[r] : A(0)), dh ? dh[r] : A(0) };
+        return s;
+    }
+};
+
+// the gradient of one part of a row, from the joined parts (few rows: the row is read again)
+template <class Ty>
+__global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                 typename Ty::A scale, int splits, Ws<typename Ty::A> ws, LossOut<Ty> out) {
+    using A = typename Ty::A;
+    constexpr int N = Piece<Ty>::N;
+    for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
+        const int64_t row = it / splits;
+        const int split = (int)(it - row * splits);
+        const typename Ty::S* zr = z + row * ld;
+        typename Ty::S* dr = out.dz + row * out.ld_dz;
+        int tg;
+        Grad<A> w;
+        const Row<A> r = out.row(row, zr, width, join_parts(ws.part + row * splits, splits, scale, threadIdx.x & 63), scale,
+                                 split == 0 && threadIdx.x == 0, tg, w);
+        const Piece<Ty> pc(zr, width);
+        const bool whole = (((uintptr_t)zr ^ (uintptr_t)dr) & 15) == 0;
+        const int64_t per = (pc.pieces + splits - 1) / splits, p1 = min(pc.pieces, (split + 1) * per);
+        for (int64_t q = split * per + threadIdx.x; q < p1; q += kT) {
+            A v[N];
+            const int64_t e0 = q * N - pc.off;
+            load_piece<Ty>(zr, e0, width, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = slope<Ty>(r, v[j], scale, e0 + j == tg, w);
+            store_piece<Ty>(dr, e0, width, whole, v);
         }
     }
 }
 
-// the gradient of one part of a row, from the joined parts
-template <class Ty>
-__global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
-                                                 typename Ty::A scale, const int32_t* __restrict__ target,
-                                                 const typename Ty::A* __restrict__ dg, const typename Ty::A* __restrict__ dh,
-                                                 int splits, Ws<typename Ty::A> ws, typename Ty::A* lp_out, typename Ty::A* ent_out,
-                                                 typename Ty::S* dz, int64_t ld_dz) {
+// A row's loss with the row in the registers of one workgroup (NP pieces of 16 bytes a thread): read once, written once.
+template <class Ty, int T, int NP>
+__global__ __launch_bounds__(T) void k_lp_loss(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                               typename Ty::A scale, LossOut<Ty> out) {
     using A = typename Ty::A;
-    const int lane = threadIdx.x & 63;
-    for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
-        const int64_t row = it / splits, split = it - row * splits;
-        const typename Ty::S* zr = z + row * ld;
-        typename Ty::S* dr = dz + row * ld_dz;
-        Part<A> p = { neg_inf(A(0)), A(0), A(0) };
-        if (lane < splits) p = ws.part[row * splits + lane];
+    using S = typename Ty::S;
+    constexpr int N = Piece<Ty>::N, W = T / 64;
+    __shared__ A sm[W], ss[W], st[W];
+    __shared__ int sc[W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const S* zr = z + row * ld;
+        const int off = (int)Piece<Ty>(zr, width).off;
+        uint4 raw[NP];
+        A m = neg_inf(A(0));
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
-        Row<A> r = finish(p);
-        const int tg = target ? target[row] : -1;
-        given(r, tg, width);
-        if (split == 0 && threadIdx.x == 0) {
-            if (ent_out) ent_out[row] = r.entropy;
-            if (lp_out) lp_out[row] = r.bad ? nan_of(A(0)) : (tg < 0 ? A(0) : log_p(r, Ty::up(zr[tg]), scale));
+        for (int n = 0; n < NP; ++n) {
+            const int e0 = (n * T + (int)threadIdx.x) * N - off;
+            alignas(16) S v[N];
+            if (e0 >= 0 && e0 + N <= width) {
+                raw[n] = *reinterpret_cast<const uint4*>(zr + e0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = e0 + j >= 0 && e0 + j < width ? zr[e0 + j] : Ty::down(neg_inf(A(0)));
+                raw[n] = *reinterpret_cast<const uint4*>(v);
+            }
         }
-        const Grad<A> w = { tg < 0 ? A(0) : (dg ? dg[row] : A(0)), dh ? dh[row] : A(0) };
-        const int64_t per = (width + splits - 1) / splits;
-        const int64_t c1 = min(width, (split + 1) * per);
-        for (int64_t c = split * per + threadIdx.x; c < c1; c += kT)
-            dr[c] = Ty::down(slope<Ty>(r, Ty::up(zr[c]), scale, c == tg, w));
+        // the stored 16 bits are unpacked anew in each pass (twice the registers would not do), so the compiler may not
+        // know that they are the same
+        auto piece = [&](int n, A* v) {
+            alignas(16) S x[N];
+            asm volatile("" : "+v"(raw[n].x), "+v"(raw[n].y), "+v"(raw[n].z), "+v"(raw[n].w));
+            *reinterpret_cast<uint4*>(x) = raw[n];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = Ty::up(x[j]);
+        };
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            A v[N];
+            piece(n, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) m = max_of(m, v[j]);
+        }
+        m = wave_max(m);
+        if (lane == 0) sm[wave] = m;
+        __syncthreads();
+        m = sm[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = max_of(m, sm[w]);
+        const A base = m == neg_inf(A(0)) ? A(0) : m;
+        // s: the terms below the maximum; the elements at the maximum are counted, and one of them is left out
+        A s = A(0), t = A(0);
+        int top = 0;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            A v[N];
+            piece(n, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const A d = (v[j] - base) * scale, e = exp_neg<Ty>(d);
+                const bool at = v[j] == m && m > neg_inf(A(0));
+                top += at;
+                s += at ? A(0) : e;
+                t += e * floor_of(d);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            s += __shfl_xor(s, o);
+            t += __shfl_xor(t, o);
+            top += __shfl_xor(top, o);
+        }
+        if (lane == 0) { ss[wave] = s; st[wave] = t; sc[wave] = top; }
+        __syncthreads();
+        s = A(0);
+        t = A(0);
+        top = -1;
+        for (int w = 0; w < W; ++w) { s += ss[w]; t += st[w]; top += sc[w]; }
+        if (top > 0) s += (A)top;
+        int tg;
+        Grad<A> w;
+        const Row<A> r = out.row(row, zr, width, Part<A>{ m, s, t }, scale, threadIdx.x == 0, tg, w);
+        S* dr = out.dz + row * out.ld_dz;
+        const bool whole = (((uintptr_t)zr ^ (uintptr_t)dr) & 15) == 0;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int e0 = (n * T + (int)threadIdx.x) * N - off;
+            A v[N];
+            piece(n, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = slope<Ty>(r, v[j], scale, e0 + j == tg, w);
+            store_piece<Ty>(dr, e0, width, whole, v);
+        }
+        __syncthreads();   // the shared arrays are written again
     }
 }
 
@@ -522,12 +730,12 @@ int score(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld
                                 top_ix, nullptr, 0);
     } else {
         const int splits = splits_of(rows, width);
-        const Ws<A> w = ws_of<A>(ws, rows * splits);
+        const Ws<A> w = splits > 1 ? ws_of<A>(ws, rows * splits) : Ws<A>{ nullptr, nullptr };
+        const Out<Ty> out = { target, (A*)lp, (A*)ent, (A*)top_lp, top_ix, top_k };
         const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows * splits)), grid2((unsigned)std::min<int64_t>(kMaxGrid, rows));
-        if (top_k > 0) hipLaunchKernelGGL((k_lp_parts<Ty, true>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w);
-        else hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w);
-        hipLaunchKernelGGL((k_lp_join<Ty>), grid2, dim3(64), 0, st, zz, rows, width, ld, (A)scale, target, top_k, splits, w, (A*)lp,
-                           (A*)ent, (A*)top_lp, top_ix);
+        if (top_k > 0) hipLaunchKernelGGL((k_lp_parts<Ty, true>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
+        else hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
+        if (splits > 1) hipLaunchKernelGGL((k_lp_join<Ty>), grid2, dim3(64), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
     }
     VQA_HIP(hipGetLastError());
     return VQA_OK;
@@ -537,17 +745,29 @@ template <class Ty>
 int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld, double scale, const int32_t* target, const void* dg,
          const void* dh, void* ws, void* lp, void* ent, void* dz, int64_t ld_dz) {
     using A = typename Ty::A;
-    const auto* zz = (const typename Ty::S*)z;
+    using S = typename Ty::S;
+    const auto* zz = (const S*)z;
     if (width <= kShortWidth) {
         launch_short<Ty, true>(st, zz, rows, (int)width, ld, scale, target, 0, (const A*)dg, (const A*)dh, (A*)lp, (A*)ent, nullptr,
-                               nullptr, (typename Ty::S*)dz, ld_dz);
+                               nullptr, (S*)dz, ld_dz);
+        VQA_HIP(hipGetLastError());
+        return VQA_OK;
+    }
+    const LossOut<Ty> out = { target, (const A*)dg, (const A*)dh, (A*)lp, (A*)ent, (S*)dz, ld_dz };
+    const int64_t pieces = (width + 2 * Piece<Ty>::N - 2) / Piece<Ty>::N;    // of a row that begins anywhere
+    const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows));
+    // One workgroup a row needs rows enough for half of the CUs; fewer rows are split, and read a second time.
+    if (rows >= 128 && pieces <= 16 * 1024) {
+        if (pieces <= 4 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 4>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
+        else if (pieces <= 4 * 1024) hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 4>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
+        else if (pieces <= 8 * 1024) hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 8>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
+        else hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 16>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
     } else {
         const int splits = splits_of(rows, width);
         const Ws<A> w = ws_of<A>(ws, rows * splits);
-        const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows * splits));
-        hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, 0, splits, w);
-        hipLaunchKernelGGL((k_lp_slope<Ty>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, target, (const A*)dg, (const A*)dh,
-                           splits, w, (A*)lp, (A*)ent, (typename Ty::S*)dz, ld_dz);
+        const dim3 all((unsigned)std::min<int64_t>(kMaxGrid, rows * splits));
+        hipLaunchKernelGGL((k_lp_parts<Ty, false>), all, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, 0, splits, w, Out<Ty>{});
+        hipLaunchKernelGGL((k_lp_slope<Ty>), all, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, splits, w, out);
     }
     VQA_HIP(hipGetLastError());
     return VQA_OK;

@@ -143,14 +143,20 @@ int check_coefs(int steps, const double* k) {
     for (int s = 0; s < steps; ++s) {
         const double y = most * most, poly = fabs(k[1]) * y + fabs(k[2]) * y * y;
         if (poly > 32.0) VQA_FAIL(VQA_EUNSUPPORTED, "coefs (%g, %g, %g): the polynomial of X X^T reaches %g (at most 32)", k[0], k[1], k[2], poly);
-        // the largest |p| on [0, most]: sampled, and between two samples no further off than the slope allows
-        const int n = 1000;
-        double next = 0.0;
-        for (int i = 0; i <= n; ++i) {
-            const double x = most * i / n, q = x * x;
-            next = std::max(next, fabs(x * (k[0] + q * (k[1] + q * k[2]))));
+        // the largest |p| on [0, most]: at its end, or where k0 + 3 k1 y + 5 k2 y^2 = 0 (y = the square)
+        auto size = [&](double q) { return sqrt(q) * fabs(k[0] + q * (k[1] + q * k[2])); };
+        double next = size(y);
+        const double disc = 9 * k[1] * k[1] - 20 * k[0] * k[2];
+        if (k[2] != 0.0 && disc >= 0.0) {
+            for (double sign : { -1.0, 1.0 }) {
+                const double q = (-3 * k[1] + sign * sqrt(disc)) / (10 * k[2]);
+                if (q > 0.0 && q < y) next = std::max(next, size(q));
+            }
+        } else if (k[2] == 0.0 && k[1] != 0.0) {
+            const double q = -k[0] / (3 * k[1]);
+            if (q > 0.0 && q < y) next = std::max(next, size(q));
         }
-        next += most / (2 * n) * (fabs(k[0]) + 3 * fabs(k[1]) * y + 5 * fabs(k[2]) * y * y);
+        next = next * (1 + 1e-6) + 1e-6;      // (what roundings add)
         if (next > 4.0) VQA_FAIL(VQA_EUNSUPPORTED, "coefs (%g, %g, %g) carry a singular value to %g (at most 4)", k[0], k[1], k[2], next);
         most = next;
     }

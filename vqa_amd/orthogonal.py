@@ -92,7 +92,7 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
         raise ValueError("out must be contiguous, of G's shape, type and device")
     n = L.vqa_orthogonalize_workspace(code, batch, rows, cols)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _lib.check(L.vqa_orthogonalize_dev(dev.index, torch.cuda.current_stream(dev).cuda_stream, code, g.data_ptr(), batch, rows, cols,
+    _lib.check(L.vqa_orthogonalize_dev(dev.index, _lib.current_stream(dev.index), code, g.data_ptr(), batch, rows, cols,
                                        sr, sb, int(steps), k, float(eps), None if ws is None else ws.data_ptr(), out.data_ptr()))
     return out
 
@@ -131,7 +131,7 @@ def muon_step(weight, grad, momentum, lr: float, mu: float = 0.95, weight_decay:
             raise ValueError(f"{what} must be a contiguous {wide} tensor of grad's shape on its device")
     n = L.vqa_orthogonalize_workspace(code, batch, rows, cols)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _lib.check(L.vqa_muon_step_dev(dev.index, torch.cuda.current_stream(dev).cuda_stream, code, weight.data_ptr(), g.data_ptr(),
+    _lib.check(L.vqa_muon_step_dev(dev.index, _lib.current_stream(dev.index), code, weight.data_ptr(), g.data_ptr(),
                                    momentum.data_ptr(), batch, rows, cols, sr, sb, float(lr), float(mu), float(weight_decay),
                                    int(bool(nesterov)), int(steps), k, float(eps), None if ws is None else ws.data_ptr()))
     return weight

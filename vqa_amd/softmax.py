@@ -159,7 +159,7 @@ def log_probs(logits, targets=None, top_k: int = 0, scale: float = 1.0, device: 
     ix = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
     n = L.vqa_log_probs_workspace(code, rows, width, top_k)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _lib.check(L.vqa_log_probs_dev(dev.index, torch.cuda.current_stream(dev).cuda_stream, code, z.data_ptr(), rows, width, stride,
+    _lib.check(L.vqa_log_probs_dev(dev.index, _lib.current_stream(dev.index), code, z.data_ptr(), rows, width, stride,
                                    scale, _ptr(t), top_k, _ptr(ws), _ptr(lp), ent.data_ptr(), _ptr(top), _ptr(ix)))
     return LogProbs(lp, ent, top, ix)
 
@@ -209,7 +209,7 @@ def log_probs_grad(logits, targets, d_log_prob=None, d_entropy=None, scale: floa
     ent = torch.empty(rows, dtype=wide, device=dev)
     n = L.vqa_log_probs_workspace(code, rows, width, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _lib.check(L.vqa_log_probs_grad_dev(dev.index, torch.cuda.current_stream(dev).cuda_stream, code, z.data_ptr(), rows, width,
+    _lib.check(L.vqa_log_probs_grad_dev(dev.index, _lib.current_stream(dev.index), code, z.data_ptr(), rows, width,
                                         stride, scale, _ptr(t), _ptr(g), _ptr(h), _ptr(ws), _ptr(lp), ent.data_ptr(),
                                         out.data_ptr(), out.stride(0) if rows > 1 else width))
     return LogProbsGrad(lp, ent, out)
@@ -233,6 +233,6 @@ def psr_chain(E, d_expect, factor: float = 0.5):
     out = torch.empty(P, dtype=torch.float64, device=E.device)
     L = _lib.lib()
     ws = torch.empty(max(int(L.vqa_psr_chain_workspace(B, max(P, 1))) // 8, 1), dtype=torch.float64, device=E.device)
-    _lib.check(L.vqa_psr_chain_dev(E.device.index, torch.cuda.current_stream(E.device).cuda_stream, E.data_ptr(), B, P, n_obs,
+    _lib.check(L.vqa_psr_chain_dev(E.device.index, _lib.current_stream(E.device.index), E.data_ptr(), B, P, n_obs,
                                    float(factor), d.data_ptr(), ws.data_ptr(), out.data_ptr()))
     return out
