@@ -147,6 +147,66 @@ def test_gradient_matches_the_formula(t, V):
     assert r.d_logits.dtype == z.dtype
 
 
+def special_rows(z, V):
+    z[0] = -np.inf
+    z[1] = -np.inf
+    z[1, V - 1] = 2.0
+    z[2, V // 2] = float("nan")
+    z[3, 0] = float("inf")
+    z[4] = 1.5
+    z[5, V - 1] = float("nan")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("R,V", [(600, 1031), (513, 4100), (520, 8192), (512, 8193), (130, 2047), (129, 16001), (140, 33333), (130, 70001),
+                                 (128, 131075), (1100, 20011)])
+def test_many_rows(t, R, V):
+    """the forms that take a row a wave and a row a workgroup, on every eighth row and the special ones"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(R + V)
+    z = torch.randn(R, V, device="cuda", generator=gen, dtype=torch.float64) * 2.5
+    z[torch.rand(R, V, device="cuda", generator=gen) < 0.1] = -np.inf
+    z = z.to(getattr(torch, t))
+    special_rows(z, V)
+    tg = torch.randint(-1, V, (R,), device="cuda", generator=gen)
+    rows = torch.cat([torch.arange(6), torch.arange(6, R, max(8, R // 12))]).tolist()
+    k = 17
+    scale = 0.9
+    g, h = 0.7, -0.4
+    r = vqa_amd.log_probs(z, tg, top_k=k, scale=scale)
+    d = vqa_amd.log_probs_grad(z, tg, g, h, scale=scale)
+    tgn = tg.cpu().numpy()[rows]
+    lp, ent, top, ix, logs = reference(z[rows], tgn, scale, k)
+    a, b = tolerances(t, V, lp)
+    for o in (r, d):
+        near(o.log_prob.cpu()[rows], lp, a)
+        near(o.entropy.cpu()[rows], ent, b)
+    assert np.array_equal(r.top_index.cpu().numpy()[rows], ix)
+    near(r.top_log_prob.cpu()[rows], top, tolerances(t, V, top)[0])
+    p = np.exp(logs)
+    u, L = unit(t), V / 256 + 64
+    f = torch.finfo(z.dtype)
+    gw, hw = (float(torch.tensor(x, dtype=r.entropy.dtype)) for x in (g, h))
+    for n, i in enumerate(rows):
+        got = d.d_logits[i].double().cpu().numpy()
+        if np.isnan(ent[n]):
+            assert np.isnan(got).all()
+            continue
+        live = logs[n] > -np.inf
+        gi = gw if tgn[n] >= 0 else 0.0
+        want, size = np.zeros(V), np.zeros(V)
+        want[live] = -gi * p[n, live] - hw * p[n, live] * (logs[n, live] + ent[n])
+        size[live] = (abs(gi) * p[n, live] + abs(hw) * p[n, live] * (np.abs(logs[n, live]) + ent[n] + 1)) * (4 * np.abs(logs[n, live]) + L + 128)
+        size *= 2 + math.log(V)
+        if tgn[n] >= 0 and live.any():
+            want[tgn[n]] += gi
+            size[tgn[n]] += 4 * abs(gi)
+        tol = u * scale * size
+        tol += half_step(t) * (np.abs(scale * want) + tol) + f.smallest_normal * f.eps + 1e-38
+        near(got, scale * want, tol)
+
+
 @pytest.mark.parametrize("V", [5, 700, 6000])
 def test_gradient_matches_differences(V):
     """central differences of the loss, float64: the third derivative is below 4 scale^3, so a step of 1e-4 leaves 1e-8, and

@@ -8,6 +8,7 @@
 // so a row is read once, by lanes, waves and workgroups that each take a part (Part, join).
 // m is kept as the stored score z: (z - m) * scale rounds the small difference and not the large product.
 #include <algorithm>
+#include <type_traits>
 
 #include "vqa_core.h"
 
@@ -53,10 +54,29 @@ __device__ __forceinline__ typename Ty::A exp_neg(typename Ty::A d) {
 template <class A>
 __device__ __forceinline__ A floor_of(A d) { return max_of(d, A(-16000)); }
 
+// In a row's inner loop differences are multiplied by scale * unit and raised by raise(): the fast types work in powers of
+// two, so that the multiplication by log2 e is the scale's, and their t is brought back at the end.
+template <class Ty>
+__device__ __forceinline__ typename Ty::A unit() { return Ty::kFast ? typename Ty::A(1.4426950408889634) : typename Ty::A(1); }
+template <class Ty>
+__device__ __forceinline__ typename Ty::A raise(typename Ty::A d) {
+    if constexpr (Ty::kFast) return __builtin_amdgcn_exp2f(d);
+    else return exp_of(d);
+}
+
 template <class A>
 struct Part {
     A m, s, t;   // m = -inf: nothing seen but masked places (s is then 0, or NaN once a NaN was seen)
 };
+
+// Nothing read yet.  m goes through a register that the compiler cannot see into: where it knew this m to be the same for a
+// wave and -infinity in 64 bits, it moved it with one scalar instruction whose constant holds 32 bits, and it became 0.
+template <class A>
+__device__ __forceinline__ Part<A> nothing() {
+    A m = neg_inf(A(0));
+    asm volatile("" : "+v"(m));
+    return Part<A>{ m, A(0), A(0) };
+}
 
 template <class A>
 __device__ __forceinline__ Part<A> join(const Part<A>& a, const Part<A>& b, A scale) {
@@ -121,6 +141,52 @@ __device__ __forceinline__ typename Ty::A slope(const Row<typename Ty::A>& r, ty
     return v * scale;
 }
 
+// ---- lanes ---------------------------------------------------------------------------------------------------------
+// a value of one lane (the lane's number is the same for the whole wave) for all, and a value of the lane before
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(lane_of(__float_as_int(v), lane)); }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    return __hiloint2double(lane_of(__double2hiint(v), lane), lane_of(__double2loint(v), lane));
+}
+template <int kCtrl>
+__device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, kCtrl, 0xf, 0xf, false); }
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float old, float v) { return __int_as_float(dpp<kCtrl>(__float_as_int(old), __float_as_int(v))); }
+template <int kCtrl>
+__device__ __forceinline__ double dpp(double old, double v) {
+    return __hiloint2double(dpp<kCtrl>(__double2hiint(old), __double2hiint(v)), dpp<kCtrl>(__double2loint(old), __double2loint(v)));
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143, kWaveShr1 = 0x138;
+// the largest of a wave's values, for all lanes
+template <class A>
+__device__ __forceinline__ A wave_max(A v) {
+    v = max_of(v, dpp<kShr1>(v, v));
+    v = max_of(v, dpp<kShr2>(v, v));
+    v = max_of(v, dpp<kShr4>(v, v));
+    v = max_of(v, dpp<kShr8>(v, v));
+    v = max_of(v, dpp<kBcast15>(v, v));
+    v = max_of(v, dpp<kBcast31>(v, v));
+    return lane_of(v, 63);
+}
+// an exchange with the lane 2^o away, without shared memory up to 16 lanes (within groups that are uniform already, which
+// is what a reduction over all smaller distances leaves)
+template <int o, class A>
+__device__ __forceinline__ A across(A v) {
+    if constexpr (o == 1) return dpp<0xB1>(v, v);        // pairs
+    else if constexpr (o == 2) return dpp<0x4E>(v, v);   // halves of four
+    else if constexpr (o == 4) return dpp<0x141>(v, v);  // eight, mirrored
+    else if constexpr (o == 8) return dpp<0x140>(v, v);  // sixteen, mirrored
+    else return __shfl_xor(v, o);
+}
+// f(value of the other half) for distances 1, 2 .. G / 2
+template <int G, int o = 1, class F>
+__device__ __forceinline__ void reduce(F f) {
+    if constexpr (o < G) {
+        f(std::integral_constant<int, o>());
+        reduce<G, 2 * o>(f);
+    }
+}
+
 // ---- short rows: G lanes of a wave hold a row, E elements each ----------------------------------------------------
 // Everything stays in registers; the best outcomes are taken one by one (an argmax over the lanes' own best).
 template <class Ty, int G, int E, bool kGrad>
@@ -148,16 +214,14 @@ __global__ __launch_bounds__(kT) void k_lp_short(const typename Ty::S* __restric
             nan |= v[i] != v[i];
         }
         if (nan) m = neg_inf(A(0));
-#pragma unroll
-        for (int o = 1; o < G; o <<= 1) m = max_of(m, __shfl_xor(m, o, G));
+        reduce<G>([&](auto o) { m = max_of(m, across<o.value>(m)); });
         const A base = m == neg_inf(A(0)) ? A(0) : m;
         // which element is the one whose term is left out: the first at the maximum
         int first = 0x7fffffff;
 #pragma unroll
         for (int i = E - 1; i >= 0; --i)
             if (v[i] == m) first = lane + G * i;
-#pragma unroll
-        for (int o = 1; o < G; o <<= 1) first = min(first, __shfl_xor(first, o, G));
+        reduce<G>([&](auto o) { first = min(first, across<o.value>(first)); });
         A s = nan ? nan_of(A(0)) : A(0), t = A(0);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -167,11 +231,10 @@ __global__ __launch_bounds__(kT) void k_lp_short(const typename Ty::S* __restric
             s += e;
             t += skip ? A(0) : e * floor_of(d);
         }
-#pragma unroll
-        for (int o = 1; o < G; o <<= 1) {
-            s += __shfl_xor(s, o, G);
-            t += __shfl_xor(t, o, G);
-        }
+        reduce<G>([&](auto o) {
+            s += across<o.value>(s);
+            t += across<o.value>(t);
+        });
         Row<A> r = finish(Part<A>{ m, s, t });
         const int tg = target ? target[row] : -1;
         given(r, tg, width);
@@ -195,12 +258,11 @@ __global__ __launch_bounds__(kT) void k_lp_short(const typename Ty::S* __restric
                 for (int i = 0; i < E; ++i)
                     if (!(used >> i & 1) && v[i] > bv) { bv = v[i]; bi = lane + G * i; at = i; }
                 const int mine = bi;
-#pragma unroll
-                for (int o = 1; o < G; o <<= 1) {
-                    const A ov = __shfl_xor(bv, o, G);
-                    const int oi = __shfl_xor(bi, o, G);
+                reduce<G>([&](auto o) {
+                    const A ov = across<o.value>(bv);
+                    const int oi = across<o.value>(bi);
                     if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
-                }
+                });
                 if (at >= 0 && mine == bi) used |= 1u << at;
                 if (lane == 0) {
                     const bool none = r.bad || bi == 0x7fffffff;
@@ -239,34 +301,6 @@ __device__ __forceinline__ void load_piece(const typename Ty::S* zr, int64_t e0,
     }
 }
 
-// ---- lanes ---------------------------------------------------------------------------------------------------------
-// a value of one lane (the lane's number is the same for the whole wave) for all, and a value of the lane before
-__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(lane_of(__float_as_int(v), lane)); }
-__device__ __forceinline__ double lane_of(double v, int lane) {
-    return __hiloint2double(lane_of(__double2hiint(v), lane), lane_of(__double2loint(v), lane));
-}
-template <int kCtrl>
-__device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, kCtrl, 0xf, 0xf, false); }
-template <int kCtrl>
-__device__ __forceinline__ float dpp(float old, float v) { return __int_as_float(dpp<kCtrl>(__float_as_int(old), __float_as_int(v))); }
-template <int kCtrl>
-__device__ __forceinline__ double dpp(double old, double v) {
-    return __hiloint2double(dpp<kCtrl>(__double2hiint(old), __double2hiint(v)), dpp<kCtrl>(__double2loint(old), __double2loint(v)));
-}
-constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143, kWaveShr1 = 0x138;
-// the largest of a wave's values, for all lanes
-template <class A>
-__device__ __forceinline__ A wave_max(A v) {
-    v = max_of(v, dpp<kShr1>(v, v));
-    v = max_of(v, dpp<kShr2>(v, v));
-    v = max_of(v, dpp<kShr4>(v, v));
-    v = max_of(v, dpp<kShr8>(v, v));
-    v = max_of(v, dpp<kBcast15>(v, v));
-    v = max_of(v, dpp<kBcast31>(v, v));
-    return lane_of(v, 63);
-}
-
 // a wave's list of its best outcomes, one a lane, best first (value, then lower index)
 template <class A>
 struct Best {
@@ -296,32 +330,60 @@ __device__ __forceinline__ void merge(Best<A>& b, const Best<A>& c, int top_k, i
     }
 }
 
-// B elements a lane into the wave's running state.  m is the wave's (the same in all lanes), s and t are the lane's.
-template <class Ty, int B, bool kTop>
+// A bound below the k-th best of a wave's first elements, from the lanes' own best mx: k lanes or more reach it.  It keeps
+// the first pieces from inserting each element that is better than those before it (about k log(elements / k) of them).
+template <class A>
+__device__ __forceinline__ A first_bound(A mx, int top_k) {
+    if (__popcll(__ballot(mx > neg_inf(A(0)))) < top_k) return neg_inf(A(0));
+    A hi = wave_max(mx), lo = -wave_max(mx > neg_inf(A(0)) ? -mx : neg_inf(A(0)));
+    for (int n = 0; n < 12; ++n) {
+        const A mid = A(0.5) * lo + A(0.5) * hi;
+        const int reach = __popcll(__ballot(mx >= mid));
+        if (reach >= top_k) lo = mid;
+        else hi = mid;
+        if (reach == top_k) break;
+    }
+    return lo;
+}
+
+// U pieces a lane into the wave's running state.  m is the wave's (the same in all lanes), s and t are the lane's.
+template <class Ty, int U, bool kTop>
 __device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Part<typename Ty::A>& p, Best<typename Ty::A>& best,
-                                     int top_k, typename Ty::A scale, int lane) {
+                                     int top_k, typename Ty::A k, int lane) {
     using A = typename Ty::A;
-    constexpr int N = Piece<Ty>::N;
-    A mx = v[0];
+    constexpr int N = Piece<Ty>::N, B = U * N;
+    A piece_max[U], mx = neg_inf(A(0));
 #pragma unroll
-    for (int j = 1; j < B; ++j) mx = max_of(mx, v[j]);
+    for (int u = 0; u < U; ++u) {
+        piece_max[u] = v[u * N];
+#pragma unroll
+        for (int j = 1; j < N; ++j) piece_max[u] = max_of(piece_max[u], v[u * N + j]);
+        mx = max_of(mx, piece_max[u]);
+    }
     if constexpr (kTop) {
         A kv = lane_of(best.v, top_k - 1);
         if (__ballot(mx >= kv && mx > neg_inf(A(0)))) {
             int ki = lane_of(best.i, top_k - 1);
+            A bound = kv;
+            if (kv == neg_inf(A(0))) bound = first_bound(mx, top_k);
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                uint64_t want = __ballot(v[j] >= kv && v[j] > neg_inf(A(0)));
-                while (want) {
-                    const int src = __builtin_ctzll(want);
-                    const A cv = lane_of(v[j], src);
-                    const int ci = lane_of(at[j / N], src) + j % N;
-                    want &= want - 1;
-                    if (before(cv, ci, kv, ki)) {
-                        insert(best, cv, ci, lane);
-                        kv = lane_of(best.v, top_k - 1);
-                        ki = lane_of(best.i, top_k - 1);
-                        want &= __ballot(v[j] >= kv);
+            for (int u = 0; u < U; ++u) {
+                if (!__ballot(piece_max[u] >= bound)) continue;
+#pragma unroll
+                for (int j = u * N; j < (u + 1) * N; ++j) {
+                    uint64_t want = __ballot(v[j] >= bound && v[j] > neg_inf(A(0)));
+                    while (want) {
+                        const int src = __builtin_ctzll(want);
+                        const A cv = lane_of(v[j], src);
+                        const int ci = lane_of(at[u], src) + j % N;
+                        want &= want - 1;
+                        if (before(cv, ci, kv, ki)) {
+                            insert(best, cv, ci, lane);
+                            kv = lane_of(best.v, top_k - 1);
+                            ki = lane_of(best.i, top_k - 1);
+                            bound = max_of(bound, kv);
+                            want &= __ballot(v[j] >= bound);
+                        }
                     }
                 }
             }
@@ -331,7 +393,7 @@ __device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Par
         const A m = wave_max(max_of(mx, p.m));
         const uint64_t holders = __ballot(mx == m);
         if (p.m > neg_inf(A(0))) {                // the old one's term comes in, in lane 0's sums
-            const A d = floor_of((p.m - m) * scale), f = exp_neg<Ty>(d), all = p.s + (lane == 0 ? A(1) : A(0));
+            const A d = floor_of((p.m - m) * k), f = raise<Ty>(d), all = p.s + (lane == 0 ? A(1) : A(0));
             p.s = f * all;
             p.t = f * (p.t + d * all);
         }
@@ -339,10 +401,10 @@ __device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Par
         bool left_out = lane != __builtin_ctzll(holders);     // one of the lanes that have it leaves its first one out
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            const A d = (v[j] - m) * scale;
+            const A d = (v[j] - m) * k;
             const bool out = !left_out && v[j] == m;
             left_out |= out;
-            const A e = out ? A(0) : exp_neg<Ty>(d);
+            const A e = out ? A(0) : raise<Ty>(d);
             p.s += e;
             p.t += e * floor_of(d);
         }
@@ -350,12 +412,41 @@ __device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Par
         const A m = p.m == neg_inf(A(0)) ? A(0) : p.m;
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            const A d = (v[j] - m) * scale;
-            const A e = exp_neg<Ty>(d);
+            const A d = (v[j] - m) * k;
+            const A e = raise<Ty>(d);
             p.s += e;
             p.t += e * floor_of(d);
         }
     }
+}
+
+// pieces p0 + first + lane, + step .. of a row by one wave; all lanes hold the result
+template <class Ty, bool kTop>
+__device__ __forceinline__ Part<typename Ty::A> read_pieces(const typename Ty::S* zr, int64_t width, const Piece<Ty>& pc, int64_t p0,
+                                                            int64_t p1, int step, typename Ty::A scale, int top_k, Best<typename Ty::A>& best) {
+    using A = typename Ty::A;
+    constexpr int N = Piece<Ty>::N, U = 4;
+    const int lane = threadIdx.x & 63;
+    Part<A> p = nothing<A>();
+    best = nobody<A>();
+    const A k = scale * unit<Ty>();
+    for (int64_t q = p0; q < p1; q += step * U) {    // the same count for a wave's lanes
+        A v[U * N];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t piece = q + u * step + lane, e0 = piece < p1 ? piece * N - pc.off : width;
+            at[u] = (int)e0;
+            load_piece<Ty>(zr, e0, width, v + u * N);
+        }
+        take<Ty, U, kTop>(v, at, p, best, top_k, k, lane);
+    }
+    reduce<64>([&](auto o) {
+        p.s += across<o.value>(p.s);
+        p.t += across<o.value>(p.t);
+    });
+    p.t *= A(1) / unit<Ty>();
+    return p;
 }
 
 // a part of a row by one workgroup; the result is complete in wave 0 (all lanes)
@@ -363,29 +454,10 @@ template <class Ty, bool kTop>
 __device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* zr, int64_t width, int split, int splits,
                                                           typename Ty::A scale, int top_k, Best<typename Ty::A>& best) {
     using A = typename Ty::A;
-    constexpr int N = Piece<Ty>::N, U = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Piece<Ty> pc(zr, width);
-    const int64_t per = (pc.pieces + splits - 1) / splits;
-    const int64_t p0 = split * per, p1 = min(pc.pieces, p0 + per);
-    Part<A> p = { neg_inf(A(0)), A(0), A(0) };
-    best = nobody<A>();
-    for (int64_t q = p0 + wave * 64; q < p1; q += kT * U) {    // the same count for a wave's lanes
-        A v[U * N];
-        int at[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t piece = q + u * kT + lane, e0 = piece < p1 ? piece * N - pc.off : width;
-            at[u] = (int)e0;
-            load_piece<Ty>(zr, e0, width, v + u * N);
-        }
-        take<Ty, U * N, kTop>(v, at, p, best, top_k, scale, lane);
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        p.s += __shfl_xor(p.s, o);
-        p.t += __shfl_xor(p.t, o);
-    }
+    const int64_t per = (pc.pieces + splits - 1) / splits, p0 = split * per, p1 = min(pc.pieces, p0 + per);
+    Part<A> p = read_pieces<Ty, kTop>(zr, width, pc, p0 + wave * 64, p1, kT, scale, top_k, best);
     __shared__ Part<A> sp[kWaves];
     __shared__ Best<A> sb[kWaves][64];
     if (lane == 0) sp[wave] = p;
@@ -455,10 +527,24 @@ __global__ __launch_bounds__(kT) void k_lp_parts(const typename Ty::S* __restric
     }
 }
 
+// one wave a row
+template <class Ty, bool kTop>
+__global__ __launch_bounds__(kT) void k_lp_wave(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                typename Ty::A scale, int top_k, Out<Ty> out) {
+    using A = typename Ty::A;
+    for (int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * kWaves) {
+        const typename Ty::S* zr = z + row * ld;
+        const Piece<Ty> pc(zr, width);
+        Best<A> best;
+        const Part<A> p = read_pieces<Ty, kTop>(zr, width, pc, 0, pc.pieces, 64, scale, top_k, best);
+        out.write(row, zr, width, p, best, scale, threadIdx.x & 63);
+    }
+}
+
 // a row's parts (at most 64), joined in a fixed tree by a wave
 template <class A>
 __device__ __forceinline__ Part<A> join_parts(const Part<A>* part, int splits, A scale, int lane) {
-    Part<A> p = { neg_inf(A(0)), A(0), A(0) };
+    Part<A> p = nothing<A>();
     if (lane < splits) p = part[lane];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) p = join(p, Part<A>{ __shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o) }, scale);
@@ -560,7 +646,7 @@ __global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restric
 
 // A row's loss with the row in the registers of one workgroup (NP pieces of 16 bytes a thread): read once, written once.
 template <class Ty, int T, int NP>
-__global__ __launch_bounds__(T) void k_lp_loss(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+__global__ __launch_bounds__(T, NP <= 8 && sizeof(typename Ty::A) == 4 ? 8 : 4) void k_lp_loss(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
                                                typename Ty::A scale, LossOut<Ty> out) {
     using A = typename Ty::A;
     using S = typename Ty::S;
@@ -610,6 +696,7 @@ __global__ __launch_bounds__(T) void k_lp_loss(const typename Ty::S* __restrict_
         const A base = m == neg_inf(A(0)) ? A(0) : m;
         // s: the terms below the maximum; the elements at the maximum are counted, and one of them is left out
         A s = A(0), t = A(0);
+        const A k = scale * unit<Ty>();
         int top = 0;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
@@ -617,26 +704,26 @@ __global__ __launch_bounds__(T) void k_lp_loss(const typename Ty::S* __restrict_
             piece(n, v);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const A d = (v[j] - base) * scale, e = exp_neg<Ty>(d);
-                const bool at = v[j] == m && m > neg_inf(A(0));
+                const A d = (v[j] - base) * k, e = raise<Ty>(d);
+                const bool at = v[j] == m;              // (everything masked: counted, and not used)
                 top += at;
                 s += at ? A(0) : e;
                 t += e * floor_of(d);
             }
         }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            s += __shfl_xor(s, o);
-            t += __shfl_xor(t, o);
-            top += __shfl_xor(top, o);
-        }
+        reduce<64>([&](auto o) {
+            s += across<o.value>(s);
+            t += across<o.value>(t);
+            top += across<o.value>(top);
+        });
         if (lane == 0) { ss[wave] = s; st[wave] = t; sc[wave] = top; }
         __syncthreads();
         s = A(0);
         t = A(0);
         top = -1;
         for (int w = 0; w < W; ++w) { s += ss[w]; t += st[w]; top += sc[w]; }
-        if (top > 0) s += (A)top;
+        if (m > neg_inf(A(0)) && top > 0) s += (A)top;
+        t *= A(1) / unit<Ty>();
         int tg;
         Grad<A> w;
         const Row<A> r = out.row(row, zr, width, Part<A>{ m, s, t }, scale, threadIdx.x == 0, tg, w);
@@ -688,6 +775,7 @@ __global__ __launch_bounds__(kT) void k_psr_chain_sum(const double* __restrict__
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 constexpr int kShortWidth = 1024;
+constexpr int kWaveRows = 512, kWaveWidth = 8192;
 constexpr int64_t kMaxGrid = 1 << 20;
 
 // Parts of a row: enough workgroups for the chip (about 4 a CU) while a part keeps 4096 elements, at most one a lane of
@@ -732,6 +820,13 @@ int score(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld
         const int splits = splits_of(rows, width);
         const Ws<A> w = splits > 1 ? ws_of<A>(ws, rows * splits) : Ws<A>{ nullptr, nullptr };
         const Out<Ty> out = { target, (A*)lp, (A*)ent, (A*)top_lp, top_ix, top_k };
+        if (rows >= kWaveRows && width <= kWaveWidth) {
+            const dim3 waves((unsigned)std::min<int64_t>(kMaxGrid, (rows + kWaves - 1) / kWaves));
+            if (top_k > 0) hipLaunchKernelGGL((k_lp_wave<Ty, true>), waves, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, out);
+            else hipLaunchKernelGGL((k_lp_wave<Ty, false>), waves, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, out);
+            VQA_HIP(hipGetLastError());
+            return VQA_OK;
+        }
         const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows * splits)), grid2((unsigned)std::min<int64_t>(kMaxGrid, rows));
         if (top_k > 0) hipLaunchKernelGGL((k_lp_parts<Ty, true>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
         else hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
@@ -758,8 +853,8 @@ int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld,
     const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows));
     // One workgroup a row needs rows enough for half of the CUs; fewer rows are split, and read a second time.
     if (rows >= 128 && pieces <= 16 * 1024) {
-        if (pieces <= 4 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 4>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
-        else if (pieces <= 4 * 1024) hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 4>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
+        if (pieces <= 8 * 64) hipLaunchKernelGGL((k_lp_loss<Ty, 64, 8>), grid, dim3(64), 0, st, zz, rows, width, ld, (A)scale, out);
+        else if (pieces <= 8 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 8>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
         else if (pieces <= 8 * 1024) hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 8>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
         else hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 16>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
     } else {
