@@ -16,6 +16,8 @@ namespace vqa {
 
 namespace {
 
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
 constexpr int kT = 256;
 constexpr int kWaves = kT / 64;
 
@@ -38,7 +40,14 @@ __device__ __forceinline__ float nan_of(float) { return __builtin_nanf(""); }
 __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double exp_of(double d) { return exp(d); }
-__device__ __forceinline__ float exp_of(float d) { return expf(d); }
+// exp(d), d <= 0, as 2^h (1 + l ln 2) with d log2 e = h + l: the hardware's 2^h (1 step off) with the rounding of the product
+// brought back, 7 instructions beside it; the library's expf takes about 15.  l is taken of a bounded d (-inf - -inf is NaN).
+__device__ __forceinline__ float exp_of(float d) {
+    constexpr float kLog2e = 1.442695041f, kRest = 1.925963033e-8f;     // log2 e = kLog2e + kRest
+    const float b = fmaxf(d, -16000.f), l = __builtin_fmaf(b, kRest, __builtin_fmaf(b, kLog2e, -(b * kLog2e)));
+    const float e = __builtin_amdgcn_exp2f(d * kLog2e);
+    return __builtin_fmaf(e, l * 0.693147181f, e);
+}
 __device__ __forceinline__ double log1p_of(double d) { return log1p(d); }
 __device__ __forceinline__ float log1p_of(float d) { return log1pf(d); }
 
@@ -592,6 +601,42 @@ __device__ __forceinline__ void store_piece(typename Ty::S* dr, int64_t e0, int6
     }
 }
 
+// The gradient of pieces first, + T .. below `past` of a row whose state is known.
+template <class Ty, int T>
+__device__ __forceinline__ void write_slopes(const typename Ty::S* zr, typename Ty::S* dr, int64_t width, const Piece<Ty>& pc, int64_t first,
+                                             int64_t past, const Row<typename Ty::A>& r, int tg, const Grad<typename Ty::A>& w,
+                                             typename Ty::A scale) {
+    using A = typename Ty::A;
+    constexpr int N = Piece<Ty>::N, U = 2;
+    const bool whole = (((uintptr_t)zr ^ (uintptr_t)dr) & 15) == 0, plain = !r.bad && !r.empty;
+    const A k = scale * unit<Ty>(), w0 = -scale * (w.g + w.h * r.entropy), w1 = -scale * w.h / unit<Ty>(), ls = r.ls * unit<Ty>();
+    for (int64_t q = first; q < past; q += T * U) {
+        A v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_piece<Ty>(zr, q + u * T < past ? (q + u * T) * N - pc.off : width, width, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (q + u * T >= past) break;
+            const int64_t e0 = (q + u * T) * N - pc.off;
+            if (plain) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const A lp = floor_of((v[u][j] - r.m) * k - ls);     // masked: p is 0, and 0 times a number
+                    v[u][j] = raise<Ty>(lp) * (lp * w1 + w0);
+                }
+                if (tg >= e0 && tg < e0 + N) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) v[u][j] += tg == e0 + j ? scale * w.g : A(0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[u][j] = r.bad ? nan_of(A(0)) : A(0);
+            }
+            store_piece<Ty>(dr, e0, width, whole, v[u]);
+        }
+    }
+}
+
 // the row's log probability and entropy beside its gradient, by one thread; returns the state for the gradient
 template <class Ty>
 struct LossOut {
@@ -631,23 +676,21 @@ __global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restric
         const Row<A> r = out.row(row, zr, width, join_parts(ws.part + row * splits, splits, scale, threadIdx.x & 63), scale,
                                  split == 0 && threadIdx.x == 0, tg, w);
         const Piece<Ty> pc(zr, width);
-        const bool whole = (((uintptr_t)zr ^ (uintptr_t)dr) & 15) == 0;
         const int64_t per = (pc.pieces + splits - 1) / splits, p1 = min(pc.pieces, (split + 1) * per);
-        for (int64_t q = split * per + threadIdx.x; q < p1; q += kT) {
-            A v[N];
-            const int64_t e0 = q * N - pc.off;
-            load_piece<Ty>(zr, e0, width, v);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = slope<Ty>(r, v[j], scale, e0 + j == tg, w);
-            store_piece<Ty>(dr, e0, width, whole, v);
-        }
+        write_slopes<Ty, kT>(zr, dr, width, pc, split * per + threadIdx.x, p1, r, tg, w, scale);
     }
 }
 
+// Waves a SIMD that the registers shall leave room for, where more would spill.
+constexpr int waves_a_simd(int T, int NP, size_t size) { return size == 8 ? (T >= 1024 ? 4 : 2) : NP <= 8 ? 5 : 4; }
+
 // A row's loss with the row in the registers of one workgroup (NP pieces of 16 bytes a thread): read once, written once.
+// Three passes over the registers: the maximum; the sums; the gradient p (w0 + w1 log p), w0 = -scale (g + h H), w1 = -scale h.
+// Bound by HBM as long as the passes' arithmetic (about 30 instruction slots an element of 32 bits, 22 of 16) hides under it.
 template <class Ty, int T, int NP>
-__global__ __launch_bounds__(T, NP <= 8 && sizeof(typename Ty::A) == 4 ? 8 : 4) void k_lp_loss(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
-                                               typename Ty::A scale, LossOut<Ty> out) {
+__global__ __launch_bounds__(T, waves_a_simd(T, NP, sizeof(typename Ty::S))) void k_lp_loss(const typename Ty::S* __restrict__ z, int64_t rows,
+                                                                                          int64_t width, int64_t ld, typename Ty::A scale,
+                                                                                          LossOut<Ty> out) {
     using A = typename Ty::A;
     using S = typename Ty::S;
     constexpr int N = Piece<Ty>::N, W = T / 64;
@@ -656,59 +699,96 @@ __global__ __launch_bounds__(T, NP <= 8 && sizeof(typename Ty::A) == 4 ? 8 : 4) 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const S* zr = z + row * ld;
-        const int off = (int)Piece<Ty>(zr, width).off;
-        uint4 raw[NP];
-        A m = neg_inf(A(0));
+        const int off = (int)Piece<Ty>(zr, width).off, end = (int)width + off;      // elements from the first piece on
+        const int first = (int)threadIdx.x * N;                                       // the thread's, of its piece 0
+        // pieces lo <= n < hi of the thread lie whole in the row, those from past on outside it
+        int lo = first < off ? 1 : 0, hi = end - N < first ? 0 : (end - N - first) / (T * N) + 1, past = end <= first ? 0 : (end - 1 - first) / (T * N) + 1;
+        // element j of a piece that does not lie whole in the row
+        auto inside = [&](int n, int j) { return first + n * (T * N) + j >= off && first + n * (T * N) + j < end; };
+        auto edge = [&](int n) {      // a piece that the row begins or ends in
+            alignas(16) S v[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = inside(n, j) ? zr[n * (T * N) + first - off + j] : Ty::down(neg_inf(A(0)));
+            return *reinterpret_cast<const uint4v*>(v);
+        };
+        alignas(16) S masked[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) masked[j] = Ty::down(neg_inf(A(0)));
+        uint4v raw[NP];
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            const int e0 = (n * T + (int)threadIdx.x) * N - off;
-            alignas(16) S v[N];
-            if (e0 >= 0 && e0 + N <= width) {
-                raw[n] = *reinterpret_cast<const uint4*>(zr + e0);
-            } else {
+            raw[n] = *reinterpret_cast<const uint4v*>(masked);
+            if (n >= lo && n < hi) raw[n] = *reinterpret_cast<const uint4v*>(zr - off + n * (T * N) + first);
+        }
+        if (lo > 0) raw[0] = edge(0);
+        if (__ballot(past > hi && past > lo)) {
+            const int last = past > hi && past > lo ? past - 1 : -1;
+            uint4v e = *reinterpret_cast<const uint4v*>(masked);
+            if (last >= 0) e = edge(last);
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = e0 + j >= 0 && e0 + j < width ? zr[e0 + j] : Ty::down(neg_inf(A(0)));
-                raw[n] = *reinterpret_cast<const uint4*>(v);
-            }
+            for (int n = 0; n < NP; ++n) raw[n] = n == last ? e : raw[n];
         }
         // the stored 16 bits are unpacked anew in each pass (twice the registers would not do), so the compiler may not
         // know that they are the same
+        auto anew = [&] {
+            if constexpr (sizeof(S) == 2) {
+#pragma unroll
+                for (int n = 0; n < NP; ++n) asm volatile("" : "+v"(raw[n]));
+            }
+        };
         auto piece = [&](int n, A* v) {
             alignas(16) S x[N];
-            asm volatile("" : "+v"(raw[n].x), "+v"(raw[n].y), "+v"(raw[n].z), "+v"(raw[n].w));
-            *reinterpret_cast<uint4*>(x) = raw[n];
+            __builtin_amdgcn_sched_barrier(0);     // a piece at a time: many at once take more registers than the row
+            *reinterpret_cast<uint4v*>(x) = raw[n];
 #pragma unroll
             for (int j = 0; j < N; ++j) v[j] = Ty::up(x[j]);
         };
+        A mine_max = neg_inf(A(0));
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             A v[N];
             piece(n, v);
 #pragma unroll
-            for (int j = 0; j < N; ++j) m = max_of(m, v[j]);
+            for (int j = 0; j < N; ++j) mine_max = max_of(mine_max, v[j]);
         }
-        m = wave_max(m);
-        if (lane == 0) sm[wave] = m;
-        __syncthreads();
-        m = sm[0];
+        A m = wave_max(mine_max);
+        if (W > 1) {
+            if (lane == 0) sm[wave] = m;
+            __syncthreads();
+            m = sm[0];
 #pragma unroll
-        for (int w = 1; w < W; ++w) m = max_of(m, sm[w]);
-        const A base = m == neg_inf(A(0)) ? A(0) : m;
+            for (int w = 1; w < W; ++w) m = max_of(m, sm[w]);
+        }
+        const A from = m == neg_inf(A(0)) ? A(0) : m, k = scale * unit<Ty>();
         // s: the terms below the maximum; the elements at the maximum are counted, and one of them is left out
         A s = A(0), t = A(0);
-        const A k = scale * unit<Ty>();
         int top = 0;
+        anew();
+        if (__ballot(mine_max == m)) {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            A v[N];
-            piece(n, v);
+            for (int n = 0; n < NP; ++n) {
+                A v[N];
+                piece(n, v);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const A d = (v[j] - base) * k, e = raise<Ty>(d);
-                const bool at = v[j] == m;              // (everything masked: counted, and not used)
-                top += at;
-                s += at ? A(0) : e;
-                t += e * floor_of(d);
+                for (int j = 0; j < N; ++j) {
+                    const A d = (v[j] - from) * k, e = raise<Ty>(d);
+                    const bool at = v[j] == m;              // (everything masked: counted, and not used)
+                    top += at;
+                    s += at ? A(0) : e;
+                    t += e * floor_of(d);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                A v[N];
+                piece(n, v);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const A d = (v[j] - from) * k, e = raise<Ty>(d);
+                    s += e;
+                    t += e * floor_of(d);
+                }
             }
         }
         reduce<64>([&](auto o) {
@@ -716,29 +796,82 @@ __global__ __launch_bounds__(T, NP <= 8 && sizeof(typename Ty::A) == 4 ? 8 : 4) 
             t += across<o.value>(t);
             top += across<o.value>(top);
         });
-        if (lane == 0) { ss[wave] = s; st[wave] = t; sc[wave] = top; }
-        __syncthreads();
-        s = A(0);
-        t = A(0);
-        top = -1;
-        for (int w = 0; w < W; ++w) { s += ss[w]; t += st[w]; top += sc[w]; }
-        if (m > neg_inf(A(0)) && top > 0) s += (A)top;
+        if (W > 1) {
+            if (lane == 0) { ss[wave] = s; st[wave] = t; sc[wave] = top; }
+            __syncthreads();
+            s = A(0);
+            t = A(0);
+            top = 0;
+            for (int w = 0; w < W; ++w) { s += ss[w]; t += st[w]; top += sc[w]; }
+        }
+        if (m > neg_inf(A(0)) && top > 1) s += (A)(top - 1);
         t *= A(1) / unit<Ty>();
         int tg;
         Grad<A> w;
         const Row<A> r = out.row(row, zr, width, Part<A>{ m, s, t }, scale, threadIdx.x == 0, tg, w);
         S* dr = out.dz + row * out.ld_dz;
-        const bool whole = (((uintptr_t)zr ^ (uintptr_t)dr) & 15) == 0;
+        if (((uintptr_t)zr ^ (uintptr_t)dr) & 15) hi = 0;      // pieces of the gradient are not aligned as the scores' are
+        const A w0 = -scale * (w.g + w.h * r.entropy), w1 = -scale * w.h / unit<Ty>(), ls = r.ls * unit<Ty>();
+        const bool plain = !r.bad && !r.empty;
+        const int hit = tg < 0 ? -1 : tg + off - first;          // the target, counted from the thread's piece 0
+        anew();
+        asm volatile("" : "+v"(lo), "+v"(hi), "+v"(past));       // (compared again, not kept as NP masks)
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            const int e0 = (n * T + (int)threadIdx.x) * N - off;
             A v[N];
             piece(n, v);
+            if (plain) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = slope<Ty>(r, v[j], scale, e0 + j == tg, w);
-            store_piece<Ty>(dr, e0, width, whole, v);
+                for (int j = 0; j < N; ++j) {
+                    const A lp = floor_of((v[j] - m) * k - ls);     // masked: p is 0, and 0 times a number
+                    v[j] = raise<Ty>(lp) * (lp * w1 + w0);
+                }
+                if ((unsigned)(hit - n * (T * N)) < (unsigned)N) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) v[j] += hit == n * (T * N) + j ? scale * w.g : A(0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = r.bad ? nan_of(A(0)) : A(0);
+            }
+            S* to = dr - off + n * (T * N) + first;
+            if (n >= lo && n < hi) {
+                alignas(16) S x[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[j] = Ty::down(v[j]);
+                // (a gradient of this size is not read again from the caches: written past them)
+                __builtin_nontemporal_store(*reinterpret_cast<const uint4v*>(x), reinterpret_cast<uint4v*>(to));
+            } else if (n < past) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (inside(n, j)) to[j] = Ty::down(v[j]);
+            }
         }
-        __syncthreads();   // the shared arrays are written again
+        if (W > 1) __syncthreads();   // the shared arrays are written again
+    }
+}
+
+// A row a workgroup, read a second time for its gradient: rows whose registers would leave one workgroup on a CU, which
+// cannot read the next row while it works on this one.  The second reading comes from the memory-side cache.
+template <class Ty, int T>
+__global__ __launch_bounds__(T) void k_lp_twice(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+                                                typename Ty::A scale, LossOut<Ty> out) {
+    using A = typename Ty::A;
+    constexpr int W = T / 64;
+    __shared__ Part<A> sp[W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const typename Ty::S* zr = z + row * ld;
+        const Piece<Ty> pc(zr, width);
+        Best<A> none;
+        const Part<A> p = read_pieces<Ty, false>(zr, width, pc, wave * 64, pc.pieces, T, scale, 0, none);
+        if (lane == 0) sp[wave] = p;
+        __syncthreads();
+        int tg;
+        Grad<A> w;
+        const Row<A> r = out.row(row, zr, width, join_parts(sp, W, scale, lane), scale, threadIdx.x == 0, tg, w);
+        write_slopes<Ty, T>(zr, out.dz + row * out.ld_dz, width, pc, threadIdx.x, pc.pieces, r, tg, w, scale);
+        __syncthreads();   // the shared array is written again
     }
 }
 
@@ -852,11 +985,12 @@ int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld,
     const int64_t pieces = (width + 2 * Piece<Ty>::N - 2) / Piece<Ty>::N;    // of a row that begins anywhere
     const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows));
     // One workgroup a row needs rows enough for half of the CUs; fewer rows are split, and read a second time.
-    if (rows >= 128 && pieces <= 16 * 1024) {
+    if (rows >= 128) {
         if (pieces <= 8 * 64) hipLaunchKernelGGL((k_lp_loss<Ty, 64, 8>), grid, dim3(64), 0, st, zz, rows, width, ld, (A)scale, out);
-        else if (pieces <= 8 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 8>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
-        else if (pieces <= 8 * 1024) hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 8>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
-        else hipLaunchKernelGGL((k_lp_loss<Ty, 1024, 16>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
+        else if (pieces <= 16 * 64) hipLaunchKernelGGL((k_lp_loss<Ty, 64, 16>), grid, dim3(64), 0, st, zz, rows, width, ld, (A)scale, out);
+        else if (pieces <= 16 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 16>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
+        else if (pieces <= 16 * 512) hipLaunchKernelGGL((k_lp_loss<Ty, 512, 16>), grid, dim3(512), 0, st, zz, rows, width, ld, (A)scale, out);
+        else hipLaunchKernelGGL((k_lp_twice<Ty, 1024>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
     } else {
         const int splits = splits_of(rows, width);
         const Ws<A> w = ws_of<A>(ws, rows * splits);
