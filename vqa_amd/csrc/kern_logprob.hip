@@ -681,8 +681,8 @@ __global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restric
     }
 }
 
-// Waves a SIMD that the registers shall leave room for, where more would spill.
-constexpr int waves_a_simd(int T, int NP, size_t size) { return size == 8 ? (T >= 1024 ? 4 : 2) : NP <= 8 ? 5 : 4; }
+// Waves a SIMD that the registers shall leave room for: as many as do without the compiler's moving parts of the row out.
+constexpr int waves_a_simd(int T, int NP, size_t size) { return size == 8 ? 2 : NP <= 8 || T > 256 ? 4 : 3; }
 
 // A row's loss with the row in the registers of one workgroup (NP pieces of 16 bytes a thread): read once, written once.
 // Three passes over the registers: the maximum; the sums; the gradient p (w0 + w1 log p), w0 = -scale (g + h H), w1 = -scale h.
@@ -990,7 +990,7 @@ int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld,
         else if (pieces <= 16 * 64) hipLaunchKernelGGL((k_lp_loss<Ty, 64, 16>), grid, dim3(64), 0, st, zz, rows, width, ld, (A)scale, out);
         else if (pieces <= 16 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 16>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
         else if (pieces <= 16 * 512) hipLaunchKernelGGL((k_lp_loss<Ty, 512, 16>), grid, dim3(512), 0, st, zz, rows, width, ld, (A)scale, out);
-        else hipLaunchKernelGGL((k_lp_twice<Ty, 1024>), grid, dim3(1024), 0, st, zz, rows, width, ld, (A)scale, out);
+        else hipLaunchKernelGGL((k_lp_twice<Ty, 512>), grid, dim3(512), 0, st, zz, rows, width, ld, (A)scale, out);
     } else {
         const int splits = splits_of(rows, width);
         const Ws<A> w = ws_of<A>(ws, rows * splits);
