@@ -16,6 +16,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vqa_core.h"
 
@@ -445,24 +446,29 @@ constexpr float kSX = 4096.f, kSA = 1024.f, kSB = 1024.f;
 // values of a padded matrix: 64-bit, or a 16-bit pair in two arrays
 struct Pair {
     _Float16 *hi, *lo;
-    __device__ __forceinline__ float get(size_t i, float scale) const { return ((float)hi[i] + (float)lo[i]) * (1.f / scale); }
-    __device__ __forceinline__ void put(size_t i, float v, float scale) const {
-        v *= scale;
-        const _Float16 h = (_Float16)v;
-        hi[i] = h;
-        lo[i] = (_Float16)(v - (float)h);
-    }
-    // N neighbours, the first at a multiple of N
+    // N neighbours, the first at a multiple of N; as they are stored (the load is under way), and their values
     template <int N>
-    __device__ __forceinline__ void get(size_t i, float scale, float* v) const {
-        constexpr int V = N < 8 ? N : 8;
+    struct Raw {
+        static constexpr int V = N < 8 ? N : 8;
         typedef _Float16 halves __attribute__((ext_vector_type(V)));
+        halves h[N / V], l[N / V];
+        __device__ __forceinline__ void values(float scale, float* v) const {
 #pragma unroll
-        for (int m = 0; m < N / V; ++m) {
-            const halves h = *(const halves*)(hi + i + m * V), l = *(const halves*)(lo + i + m * V);
+            for (int m = 0; m < N / V; ++m)
 #pragma unroll
-            for (int n = 0; n < V; ++n) v[m * V + n] = ((float)h[n] + (float)l[n]) * (1.f / scale);
+                for (int n = 0; n < V; ++n) v[m * V + n] = ((float)h[m][n] + (float)l[m][n]) * (1.f / scale);
         }
+    };
+    template <int N>
+    __device__ __forceinline__ Raw<N> get(size_t i) const {
+        using halves = typename Raw<N>::halves;
+        Raw<N> r;
+#pragma unroll
+        for (int m = 0; m < N / Raw<N>::V; ++m) {
+            r.h[m] = *(const halves*)(hi + i + m * Raw<N>::V);
+            r.l[m] = *(const halves*)(lo + i + m * Raw<N>::V);
+        }
+        return r;
     }
     template <int N>
     __device__ __forceinline__ void put(size_t i, const float* v, float scale) const {
@@ -485,16 +491,23 @@ struct Pair {
 };
 struct Wide {
     double* v;
-    __device__ __forceinline__ double get(size_t i, float) const { return v[i]; }
-    __device__ __forceinline__ void put(size_t i, double x, float) const { v[i] = x; }
     template <int N>
-    __device__ __forceinline__ void get(size_t i, float, double* x) const {
+    struct Raw {
+        double2 d[N / 2];
+        __device__ __forceinline__ void values(float, double* x) const {
 #pragma unroll
-        for (int n = 0; n < N / 2; ++n) {
-            const double2 d = *(const double2*)(v + i + 2 * n);
-            x[2 * n] = d.x;
-            x[2 * n + 1] = d.y;
+            for (int n = 0; n < N / 2; ++n) {
+                x[2 * n] = d[n].x;
+                x[2 * n + 1] = d[n].y;
+            }
         }
+    };
+    template <int N>
+    __device__ __forceinline__ Raw<N> get(size_t i) const {
+        Raw<N> r;
+#pragma unroll
+        for (int n = 0; n < N / 2; ++n) r.d[n] = *(const double2*)(v + i + 2 * n);
+        return r;
     }
     template <int N>
     __device__ __forceinline__ void put(size_t i, const double* x, float) const {
@@ -601,30 +614,42 @@ template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG =
 template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG = 1, BK = 32, S = 2; };
 template <> struct Shape<double, 64> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 16, S = 4; };
 
+// Which parts of the operands a product takes.  Results of 8 bits (bfloat16, without an optimizer state) take the high parts
+// of X alone, 11 bits: X X^T from hi hi, b A + c A A from all, B X from hi hi + lo hi.  Errors beside the result's own
+// rounding, 1.66e-3 of its norm: 0.9e-3 (512 x 512, low rank and noise) to 1.0e-3 (100 x 4000); with the high parts of B alone
+// they reach 1.8e-3, with those of A in A A 3.5e-3.
+template <class Ty, Kind kind, bool kFew>
+struct Parts {
+    static constexpr bool kWide = sizeof(typename Ty::C) == 8;
+    static constexpr int P = kWide ? 1 : kFew && kind != kPoly ? 1 : 2, Q = kWide ? 1 : kFew && kind == kGram ? 1 : 2;
+};
+
 template <class C> struct Frag;   // what a wave reads of one 32-row (16 for 64 bits) block at once, and its products
 template <> struct Frag<float> {
     using M = Pair;
     using Acc = float16v;
-    static constexpr int kArrays = 4, kSide = 32, kRegs = 16;
+    static constexpr int kSide = 32, kRegs = 16;
     static __device__ __forceinline__ int row(int lane, int q) { return 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3); }
 };
 template <> struct Frag<double> {
     using M = Wide;
     using Acc = double4v;
-    static constexpr int kArrays = 2, kSide = 16, kRegs = 4;
+    static constexpr int kSide = 16, kRegs = 4;
     static __device__ __forceinline__ int row(int lane, int q) { return Mma<double>::row(lane, q); }
 };
 
-template <class C, int T>
+// NP, NQ: parts of P and Q that are multiplied (16-bit pairs: 1 or 2)
+template <class C, int T, int NP, int NQ>
 struct Tile : Shape<C, T> {
     using Sh = Shape<C, T>;
     using Fr = Frag<C>;
     using M = typename Fr::M;
-    static constexpr int WI = Sh::WI, WJ = Sh::WJ, KG = Sh::KG, BK = Sh::BK, S = Sh::S;
+    static constexpr int WI = Sh::WI, WJ = Sh::WJ, KG = Sh::KG, BK = Sh::BK;
+    static constexpr int kArrays = NP + NQ, S = Sh::S * (sizeof(C) == 4 ? 4 : 2) / kArrays;   // fewer parts leave room for more stages
     static constexpr int kWv = WI * WJ * KG, kThreads = 64 * kWv;
     static constexpr int kSize = sizeof(C) == 8 ? 8 : 2;              // of a stored value
     static constexpr int Q = BK * kSize / 16;                         // pieces of a row
-    static constexpr int kArray = T * Q * 16, kStage = Fr::kArrays * kArray;   // bytes
+    static constexpr int kArray = T * Q * 16, kStage = kArrays * kArray;   // bytes
     static constexpr int kCopies = kStage / 1024 / kWv;               // a wave's copies (1 KB each) of a stage
     static constexpr int NI = T / WI / Fr::kSide, NJ = T / WJ / Fr::kSide;     // blocks of a wave
     static constexpr int BI = T / WI / 32, BJ = T / WJ / 32;          // its 32 x 32 blocks as they leave
@@ -645,7 +670,7 @@ struct Tile : Shape<C, T> {
     static __device__ __forceinline__ int wave_j() { return wave() % WJ * (T / WJ); }
 
     static __device__ __forceinline__ const char* base(const Pair& p, const Pair& q, int arr) {
-        return (const char*)(arr < 2 ? arr == 0 ? p.hi : p.lo : arr == 2 ? q.hi : q.lo);
+        return (const char*)(arr < NP ? arr == 0 ? p.hi : p.lo : arr == NP ? q.hi : q.lo);
     }
     static __device__ __forceinline__ const char* base(const Wide& p, const Wide& q, int arr) { return (const char*)(arr ? q.v : p.v); }
 
@@ -660,7 +685,7 @@ struct Tile : Shape<C, T> {
 #pragma unroll
         for (int n = 0; n < kCopies; ++n) {
             const int id = n * kWv + w, arr = id / kChunks, r0 = id % kChunks * kRows, row = r0 + lane / Q;
-            c.from[n] = base(p, q, arr) + ((arr >= Fr::kArrays / 2 ? j0 : i0) + row) * (size_t)ld * kSize + ((lane % Q) ^ swz(row)) * 16;
+            c.from[n] = base(p, q, arr) + ((arr >= NP ? j0 : i0) + row) * (size_t)ld * kSize + ((lane % Q) ^ swz(row)) * 16;
             c.to[n] = arr * kArray + r0 * Q * 16;
         }
     }
@@ -674,29 +699,28 @@ struct Tile : Shape<C, T> {
         const int lane = threadIdx.x & 63;
         if constexpr (sizeof(C) == 4) {
             const int piece = 2 * kk + (lane >> 5);
-            half8v ph[NI], pl[NI], qh[NJ], ql[NJ];
+            half8v pv[NI][NP], qv[NJ][NQ];
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int r = wave_j() + 32 * j + (lane & 31);
-                const char* at = st + (r * Q + (piece ^ swz(r))) * 16;
-                qh[j] = *(const half8v*)(at + 2 * kArray);
-                ql[j] = *(const half8v*)(at + 3 * kArray);
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) qv[j][x] = *(const half8v*)(st + (r * Q + (piece ^ swz(r))) * 16 + (NP + x) * kArray);
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int r = wave_i() + 32 * i + (lane & 31);
-                const char* at = st + (r * Q + (piece ^ swz(r))) * 16;
-                ph[i] = *(const half8v*)at;
-                pl[i] = *(const half8v*)(at + kArray);
+#pragma unroll
+                for (int x = 0; x < NP; ++x) pv[i][x] = *(const half8v*)(st + (r * Q + (piece ^ swz(r))) * 16 + x * kArray);
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
+                auto go = [&](int x, int y) {
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pv[i][x], qv[j][y], acc[i][j], 0, 0, 0);
+                };
+                if constexpr (NP == 2) go(1, 0);     // lo hi
+                if constexpr (NQ == 2) go(0, 1);     // hi lo
+                go(0, 0);                            // hi hi
             }
         } else {
             // a lane's piece holds two neighbours of the summed index; the first ones of the four pieces make one matrix
@@ -753,16 +777,25 @@ struct Tile : Shape<C, T> {
         __syncthreads();   // the stages are read: the shared memory takes the result
     }
 
-    // The result, a row of 32 x 32 blocks of each wave at a time, through shared memory:  first(y, x, v) gets N neighbours
-    // D[y][x ..] and may change them, second(y, x, v) then N neighbours D[y ..][x] of the changed result.
-    template <class F, class G>
-    __device__ __forceinline__ void leave(char* lds, F first, G second) {
+    // The result, a row of 32 x 32 blocks of each wave at a time, through shared memory:  first(y, x, raw, v) gets N
+    // neighbours D[y][x ..] and may change them, second(y, x, v) then N neighbours D[y ..][x] of the changed result.
+    // raw: what load(y, x) fetched for them while the blocks before were on their way.
+    template <class L, class F, class G>
+    __device__ __forceinline__ void leave(char* lds, L load, F first, G second) {
         const int lane = threadIdx.x & 63, w = wave() % (WI * WJ), at = group() * 64 + lane, line = at / (2 * KG), seg = at % (2 * KG) * N;
         auto blk = [&](int g, int j) { return (C(*)[33])lds + ((g * WI * WJ + w) * BJ + j) * 32; };
         auto meet = [] { if (KG > 1) __syncthreads(); else wave_fence(); };
         constexpr int kPer = 32 / Fr::kSide;
+        using Raw = decltype(load(0, 0));
+        Raw raw[BJ];
+#pragma unroll
+        for (int j = 0; j < BJ; ++j) raw[j] = load(wave_i() + line, wave_j() + 32 * j + seg);
 #pragma unroll
         for (int i = 0; i < BI; ++i) {
+            Raw next[BJ];
+#pragma unroll
+            for (int j = 0; j < BJ; ++j)
+                if (i + 1 < BI) next[j] = load(wave_i() + 32 * (i + 1) + line, wave_j() + 32 * j + seg);
 #pragma unroll
             for (int j = 0; j < BJ; ++j) {
                 auto mine = blk(group(), j);
@@ -784,7 +817,7 @@ struct Tile : Shape<C, T> {
 #pragma unroll
                     for (int g = 1; g < KG; ++g) v[n] += blk(g, j)[line][seg + n];
                 }
-                first(wave_i() + 32 * i + line, wave_j() + 32 * j + seg, v);
+                first(wave_i() + 32 * i + line, wave_j() + 32 * j + seg, raw[j], v);
 #pragma unroll
                 for (int n = 0; n < N; ++n) blk(0, j)[line][seg + n] = v[n];
             }
@@ -796,6 +829,9 @@ struct Tile : Shape<C, T> {
                 for (int n = 0; n < N; ++n) v[n] = blk(0, j)[seg + n][line];
                 second(wave_i() + 32 * i + seg, wave_j() + 32 * j + line, v);
             }
+#pragma unroll
+            for (int j = 0; j < BJ; ++j)
+                if (i + 1 < BI) raw[j] = next[j];
             meet();
         }
     }
@@ -803,8 +839,8 @@ struct Tile : Shape<C, T> {
 
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
-template <class Ty, Kind kind, int T>
-__global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
+template <class Ty, Kind kind, int T, bool kFew>
+__global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
     using C = typename Ty::C;
     constexpr bool kSym = kind == kGram || kind == kPoly;
     extern __shared__ __attribute__((aligned(16))) char product_lds[];
@@ -818,8 +854,9 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
     }
     const size_t i0 = ti * T, j0 = tj * T;
     const auto a = w.a.at(off), bm = w.b.at(off);
-    Tile<C, T> t;
-    constexpr int N = Tile<C, T>::N;
+    using Tl = Tile<C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>;
+    Tl t;
+    constexpr int N = Tl::N;
     if (kind == kGram || kind == kPoly) {
         const auto m = (kind == kGram ? w.x[from] : w.a).at(off), out = kind == kGram ? a : bm;
         const int ld = kind == kGram ? w.cp : w.rp;
@@ -827,11 +864,15 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
         const float so = kind == kGram ? kSA : kSB;
         const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA));
         t.leave(product_lds,
-            [&](int y, int x, C* v) {
+            [&](int y, int x) {
+                if constexpr (kind == kPoly) return a.template get<N>((i0 + y) * w.rp + j0 + x);
+                else return 0;
+            },
+            [&](int y, int x, const auto& raw, C* v) {
                 const size_t at = (i0 + y) * w.rp + j0 + x;
-                if (kind == kPoly) {
+                if constexpr (kind == kPoly) {
                     C av[N];
-                    a.template get<N>(at, kSA, av);
+                    raw.values(kSA, av);
 #pragma unroll
                     for (int n = 0; n < N; ++n) v[n] = j.kb * av[n] + j.kc * (f * v[n]);
                 } else {
@@ -848,10 +889,11 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
         t.run(xt, bm, i0, j0, w.rp, w.rp, product_lds);   // rows: columns of X; columns: rows of X
         const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB));
         t.leave(product_lds,
-            [&](int y, int x, C* v) {
+            [&](int y, int x) { return xt.template get<N>((i0 + y) * w.rp + j0 + x); },
+            [&](int y, int x, const auto& raw, C* v) {
                 const size_t at = (i0 + y) * w.rp + j0 + x;
                 C xv[N];
-                xt.template get<N>(at, kSX, xv);
+                raw.values(kSX, xv);
 #pragma unroll
                 for (int n = 0; n < N; ++n) v[n] = j.ka * xv[n] + f * v[n];
                 if (kind == kUpdate) nt.template put<N>(at, v, kSX);
@@ -956,25 +998,36 @@ int block(hipStream_t st, const Job<Ty>& j) {
     return VQA_OK;
 }
 
-template <class Ty, Kind kind, int T>
+template <class Ty, Kind kind, int T, bool kFew>
 int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
-    using Tl = Tile<typename Ty::C, T>;
-    if (int rc = allow_lds(k_ns_product<Ty, kind, T>, Tl::kBytes)) return rc;
-    hipLaunchKernelGGL((k_ns_product<Ty, kind, T>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
+    using Tl = Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>;
+    if (int rc = allow_lds(k_ns_product<Ty, kind, T, kFew>, Tl::kBytes)) return rc;
+    hipLaunchKernelGGL((k_ns_product<Ty, kind, T, kFew>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
     return VQA_OK;
 }
 
-template <class Ty, int T>
+template <class Ty, int T, bool kFew>
 int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w) {
     const unsigned tr = w.rp / T, tc = w.cp / T, sym = tr * (tr + 1) / 2, nb = (unsigned)j.batch;
     int rc = VQA_OK;
     for (int s = 0; s < j.steps && !rc; ++s) {
         const int from = s & 1;
-        rc = product<Ty, kGram, T>(st, dim3(sym, 1, nb), j, w, from);
-        if (!rc) rc = product<Ty, kPoly, T>(st, dim3(sym, 1, nb), j, w, from);
-        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate, T>(st, dim3(tr, tc, nb), j, w, from) : product<Ty, kLast, T>(st, dim3(tr, tc, nb), j, w, from);
+        rc = product<Ty, kGram, T, kFew>(st, dim3(sym, 1, nb), j, w, from);
+        if (!rc) rc = product<Ty, kPoly, T, kFew>(st, dim3(sym, 1, nb), j, w, from);
+        if (!rc)
+            rc = s + 1 < j.steps ? product<Ty, kUpdate, T, kFew>(st, dim3(tr, tc, nb), j, w, from)
+                                 : product<Ty, kLast, T, kFew>(st, dim3(tr, tc, nb), j, w, from);
     }
     return rc;
+}
+
+template <class Ty, bool kFew>
+int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int tile) {
+    if constexpr (sizeof(typename Ty::C) == 4) {
+        if (tile == 256) return steps<Ty, 256, kFew>(st, j, w);
+        if (tile == 128) return steps<Ty, 128, kFew>(st, j, w);
+    }
+    return steps<Ty, 64, false>(st, j, w);   // (bound by other things than its products)
 }
 
 template <class Ty>
@@ -1029,9 +1082,8 @@ int run(hipStream_t st, const OrthoCall& q) {
     hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride, pieces);
     hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(w.cp / kTile, w.rp / kTile, nb), dim3(kT), 0, st, j, w, parts);
     int rc;
-    if constexpr (sizeof(C) == 4) {
-        rc = tile == 256 ? steps<Ty, 256>(st, j, w) : tile == 128 ? steps<Ty, 128>(st, j, w) : steps<Ty, 64>(st, j, w);
-    } else rc = steps<Ty, 64>(st, j, w);
+    if constexpr (std::is_same_v<Ty, BF16>) rc = j.m ? steps<Ty, false>(st, j, w, tile) : steps<Ty, true>(st, j, w, tile);
+    else rc = steps<Ty, false>(st, j, w, tile);
     if (rc) return rc;
     VQA_HIP(hipGetLastError());
     return VQA_OK;
