@@ -97,6 +97,83 @@ def test_larger_matrices(t):
         check(o, g, t)
 
 
+@pytest.mark.parametrize("t", list(UNIT))
+@pytest.mark.parametrize("batch,rows,cols", [(1, 11, 300), (2, 16, 1500), (1, 1700, 15), (1, 16, 2048), (2, 3, 4000), (1, 16, 4096), (1, 16, 4099),
+                                             (3, 20, 100), (1, 32, 700), (2, 33, 50), (1, 48, 400), (1, 270, 47), (3, 49, 64), (1, 64, 300)])
+def test_forms_of_small_matrices(t, batch, rows, cols):
+    """strips of one, four, eight and sixteen a wave, and blocks of two to four tiles, at their ends"""
+    g = matrices(np.random.default_rng(rows + cols), batch, rows, cols, t)
+    check(vqa_amd.orthogonalize(g), g, t)
+
+
+@pytest.mark.parametrize("batch,rows,cols,t", [(1, 100, 4000, "float32"), (3, 200, 1111, "float32"), (2, 4100, 70, "bfloat16"), (1, 80, 3000, "float64"),
+                                               (1, 500, 4096, "float16"), (5, 66, 600, "float64"), (120, 65, 300, "float32")])
+def test_split_sums_are_repeatable(batch, rows, cols, t):
+    """the parts of a split sum are added in their order, whichever comes last, also in a replayed graph"""
+    import torch
+
+    g = matrices(np.random.default_rng(rows), batch, rows, cols, t)
+    a = vqa_amd.orthogonalize(g)
+    check(a, g, t)
+    out = torch.empty_like(a)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        vqa_amd.orthogonalize(g, out=out)
+    for n in range(4):
+        out.zero_()
+        graph.replay()
+        b = vqa_amd.orthogonalize(g)
+        torch.cuda.synchronize()
+        assert torch.equal(out, a) and torch.equal(b, a), n
+
+
+def check_large(got, g, t, extra=0.0):
+    """against the same products in 64 bits on the GPU, matrix by matrix; as check() without the singular values"""
+    import torch
+
+    r, c = sorted(g.shape[-2:])
+    want = plain(g, torch.float64)
+    norm = torch.linalg.vector_norm(want, dim=(1, 2))
+    off = torch.linalg.vector_norm(got.double() - want, dim=(1, 2))
+    poff = torch.linalg.vector_norm(plain(g, torch.float32).double() - want, dim=(1, 2))
+    half = 0.0 if t == "float32" else torch.finfo(getattr(torch, t)).eps / 2
+    tol = torch.minimum(torch.full_like(norm, bound(t, r, c)), 4 * poff + UNIT[t] * math.sqrt(c + 2 * r) * norm * 4) + half * norm + extra
+    assert torch.isfinite(got).all() and (off <= tol).all(), (off, tol)
+
+
+@pytest.mark.parametrize("batch,rows,cols,t", [(1, 2048, 2048, "float32"), (1, 2000, 2111, "bfloat16"), (1, 1024, 4096, "bfloat16"), (1, 1500, 3001, "float32"),
+                                               (2, 1300, 1290, "float32"), (40, 130, 150, "bfloat16"), (1, 2500, 1100, "float16"), (300, 65, 70, "float32"),
+                                               (1, 4096, 4096, "float32"), (1, 4096, 4000, "bfloat16"), (1, 3900, 4032, "float16")])
+def test_tiles_of_all_sizes(batch, rows, cols, t):
+    """matrices whose products take tiles of 128 and 256, and different ones for X X^T and the update"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    k = min(rows, cols) // 8
+    g = torch.stack([torch.randn(rows, k, generator=gen, device="cuda") @ torch.randn(k, cols, generator=gen, device="cuda") / math.sqrt(k)
+                     + 0.5 * torch.randn(rows, cols, generator=gen, device="cuda") for _ in range(batch)]).to(getattr(torch, t))
+    check_large(vqa_amd.orthogonalize(g), g, t)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 2048, 1500), (1, 4000, 4096), (1, 150, 3000), (20, 200, 130)])
+def test_optimizer_step_of_large_matrices(batch, rows, cols):
+    """bfloat16 gradients, weights and momentum of 32 bits: the update keeps 32 bits' accuracy"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    g = (1e-2 * torch.randn(batch, rows, cols, generator=gen, device="cuda")).bfloat16()
+    w, m = torch.randn(batch, rows, cols, generator=gen, device="cuda"), 1e-2 * torch.randn(batch, rows, cols, generator=gen, device="cuda")
+    w0, m64 = w.clone(), 0.9 * m.double() + g.double()
+    vqa_amd.muon_step(w, g, m, 0.5, 0.9, 0.0, True)
+    assert ((m.double() - m64).abs() <= 2.0 ** -24 * (3 * m64.abs() + 3 * g.double().abs() + 3 * (m64 - g.double()).abs())).all()
+    u = g.double() + 0.9 * m64
+    rate = 0.5 * math.sqrt(max(1.0, rows / cols))
+    # W's own rounding, and that of its difference here, half a step each of a value of W's size; the entering matrix is off
+    # by 3 roundings of its norm, which grow as those of a product of 9 terms do
+    half = 2.0 ** -24 * float(torch.linalg.vector_norm(w0.double())) * 2 / rate
+    check_large((w0.double() - w.double()) / rate, u, "float32", half + bound("float32", min(rows, cols), 9 - 2 * min(rows, cols)))
+
+
 @pytest.mark.parametrize("t", ["float64", "float32"])
 @pytest.mark.parametrize("rows,cols", [(11, 36), (150, 70)])
 @pytest.mark.parametrize("steps,coefs", [(1, COEFS), (2, COEFS), (3, (15 / 8, -10 / 8, 3 / 8)), (12, (1.5, -0.5, 0.0)), (5, (3.0, -3.2, 1.2))])

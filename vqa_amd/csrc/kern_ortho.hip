@@ -5,14 +5,15 @@
 // a s + b s^3 + c s^5 and the singular vectors stay, so the result is U p(S) V^T of G = U S V^T without an SVD.
 // r = min(rows, cols), c = max: X is taken r x c (the transpose of a matrix with more rows than columns).
 //
-// Two forms:
-// * r <= 64 and X fits the LDS of a CU: one workgroup carries a matrix through all steps (k_ns_small), in 64-bit or
-//   32-bit matrix instructions.
+// Three forms:
+// * r <= 16 (c <= 4096, 64 bits 2048): one workgroup carries a matrix through all steps, X in the registers of its waves in
+//   strips of 16 columns (k_ns_strip), in 64-bit or 32-bit matrix instructions.
+// * r <= 64 and X fits the LDS of a CU: the same with X in shared memory (k_ns_block).
 // * else: three tiled products a step (k_ns_product), X, X^T, A and b A + c A A in device memory, all row-major with the
-//   summed index contiguous, padded with zeros to whole tiles.  64-bit matrices use 64-bit matrix instructions; the
-//   others hold every value as a sum of two 16-bit floats hi + lo (22 bits and a sign, scaled so that neither part
-//   leaves its normal range) and take the three products hi hi + hi lo + lo hi with 32-bit sums: the left-out lo lo is
-//   2^-22 of a product, the size of the roundings that 32-bit products make along a sum, at 5 times their rate.
+//   summed index contiguous, padded to whole tiles.  64-bit matrices use 64-bit matrix instructions; the others hold every
+//   value as a sum of two 16-bit floats hi + lo (22 bits and a sign, scaled so that neither part leaves its normal range) and
+//   take the three products hi hi + hi lo + lo hi with 32-bit sums: the left-out lo lo is 2^-22 of a product, the size of
+//   the roundings that 32-bit products make along a sum, at 5 times their rate.
 #include <math.h>
 
 #include <algorithm>
@@ -438,6 +439,7 @@ __global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
 // ---- tiled products -------------------------------------------------------------------------------------------------
 constexpr int kTile = 64;
 constexpr int kNormParts = 256;
+constexpr int kMaxCount = 128;        // tiles of a product whose sum is split: at most half of the CUs
 
 // Scales of the 16-bit pairs (powers of two).  Entries of X are at most the largest singular value, below 4 by the
 // caller's check, and 1 / sqrt(r c) at the start; of A below 16; of b A + c A A below 32.
@@ -523,9 +525,14 @@ template <> struct StoreOf<double> { using T = Wide; };
 template <class M>
 struct Mats {
     M x[2], xt[2], a, b;
-    double* part;
+    double* part;     // of the norm
+    void* sum;        // X X^T in parts: [tile][part][64 x 64], in C
+    unsigned* count;  // parts of a tile that are there (0 between the kernels)
+    int splits;
     size_t stride;    // bytes to the next matrix of the batch
-    int rp, cp;
+    // rows of X (and its columns) as they are stored, and as the products sum over them (r and c to whole stages).  Rows from
+    // rk on, which the tiles of one product cover and those of another may not, hold anything: they are never summed over.
+    int rp, cp, rk, ck;
 };
 
 // Parts of the sum of squares (and the momentum): a workgroup takes whole rows in turn, or, of few long rows, pieces of them.
@@ -560,6 +567,7 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
     const size_t off = b * w.stride;
     const double* part = (const double*)((char*)w.part + off);
     const double norm = sqrt(block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh)) + j.eps;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kMaxCount) ((unsigned*)((char*)w.count + off))[threadIdx.x] = 0;
     // rows and columns of the caller's matrix
     const int64_t r0 = (int64_t)(j.turned ? blockIdx.x : blockIdx.y) * kTile, c0 = (int64_t)(j.turned ? blockIdx.y : blockIdx.x) * kTile;
     constexpr int U = kTile * kTile / kT;
@@ -679,13 +687,13 @@ struct Tile : Shape<C, T> {
         const char* from[kCopies];
         int to[kCopies];
     };
-    __device__ __forceinline__ void aim(const M& p, const M& q, size_t i0, size_t j0, int ld, Copies& c) {
+    __device__ __forceinline__ void aim(const M& p, const M& q, size_t i0, size_t j0, int ld, int k0, Copies& c) {
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(wave());
         constexpr int kRows = 64 / Q, kChunks = T / kRows;            // rows of a copy, copies of an array
 #pragma unroll
         for (int n = 0; n < kCopies; ++n) {
             const int id = n * kWv + w, arr = id / kChunks, r0 = id % kChunks * kRows, row = r0 + lane / Q;
-            c.from[n] = base(p, q, arr) + ((arr >= NP ? j0 : i0) + row) * (size_t)ld * kSize + ((lane % Q) ^ swz(row)) * 16;
+            c.from[n] = base(p, q, arr) + ((arr >= NP ? j0 : i0) + row) * (size_t)ld * kSize + (size_t)k0 * kSize + ((lane % Q) ^ swz(row)) * 16;
             c.to[n] = arr * kArray + r0 * Q * 16;
         }
     }
@@ -748,8 +756,8 @@ struct Tile : Shape<C, T> {
         }
     }
 
-    // K: a multiple of BK
-    __device__ __forceinline__ void run(const M& p, const M& q, size_t i0, size_t j0, int ld, int K, char* lds) {
+    // summed over k0 .. k0 + K, K a multiple of BK
+    __device__ __forceinline__ void run(const M& p, const M& q, size_t i0, size_t j0, int ld, int k0, int K, char* lds) {
         constexpr int kSteps = Q / (sizeof(C) == 4 ? 2 : 4);
         static_assert(kSteps % KG == 0);
 #pragma unroll
@@ -760,7 +768,7 @@ struct Tile : Shape<C, T> {
                 for (int r = 0; r < Fr::kRegs; ++r) acc[i][j][r] = 0;
         const int n = K / BK;
         Copies c;
-        aim(p, q, i0, j0, ld, c);
+        aim(p, q, i0, j0, ld, k0, c);
 #pragma unroll
         for (int t = 0; t < S - 1; ++t)
             if (t < n) fetch(c, t, lds + t * kStage);
@@ -837,6 +845,43 @@ struct Tile : Shape<C, T> {
     }
 };
 
+// Values that workgroups on other XCDs read while this kernel runs: the loads and stores go past the XCD's own L2.
+template <int N, class C>
+__device__ __forceinline__ void give(C* to, const C* v) {
+    static_assert(N * sizeof(C) % 8 == 0);
+#pragma unroll
+    for (int n = 0; n < (int)(N * sizeof(C) / 8); ++n) {
+        uint64_t u;
+        __builtin_memcpy(&u, (const char*)v + 8 * n, 8);
+        __hip_atomic_store((uint64_t*)to + n, u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+template <int N, class C>
+__device__ __forceinline__ void take(C* from, C* v) {
+    uint64_t u[N * sizeof(C) / 8];
+    C x[N];
+#pragma unroll
+    for (int n = 0; n < (int)(N * sizeof(C) / 8); ++n) u[n] = __hip_atomic_load((uint64_t*)from + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_memcpy(x, u, sizeof(x));
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += x[n];
+}
+// Whether this workgroup is the last of n to come here with what it gave.  Each wave waits for its stores to be where all XCDs
+// see them, so that the count needs no fence: a fence writes the whole L2 back, 30 us with 200 workgroups at it.
+__device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned* sh) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == (unsigned)n - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *sh = before;
+    }
+    __syncthreads();
+    const unsigned before = *sh;
+    __syncthreads();
+    return before == (unsigned)n - 1;
+}
+
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
 template <class Ty, Kind kind, int T, bool kFew>
@@ -846,11 +891,12 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
     extern __shared__ __attribute__((aligned(16))) char product_lds[];
     const size_t off = blockIdx.z * w.stride;
     size_t ti = blockIdx.y, tj = blockIdx.x;
+    const int splits = kind == kGram && T == 64 ? w.splits : 1, tile_id = blockIdx.x / splits, split = blockIdx.x - tile_id * splits;
     if (kSym) {
-        ti = (size_t)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > blockIdx.x) --ti;
-        while ((ti + 1) * (ti + 2) / 2 <= blockIdx.x) ++ti;
-        tj = blockIdx.x - ti * (ti + 1) / 2;
+        ti = (size_t)((sqrtf(8.f * tile_id + 1.f) - 1.f) * 0.5f);
+        while (ti * (ti + 1) / 2 > (size_t)tile_id) --ti;
+        while ((ti + 1) * (ti + 2) / 2 <= (size_t)tile_id) ++ti;
+        tj = tile_id - ti * (ti + 1) / 2;
     }
     const size_t i0 = ti * T, j0 = tj * T;
     const auto a = w.a.at(off), bm = w.b.at(off);
@@ -859,10 +905,39 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
     constexpr int N = Tl::N;
     if (kind == kGram || kind == kPoly) {
         const auto m = (kind == kGram ? w.x[from] : w.a).at(off), out = kind == kGram ? a : bm;
-        const int ld = kind == kGram ? w.cp : w.rp;
-        t.run(m, m, i0, j0, ld, ld, product_lds);
         const float so = kind == kGram ? kSA : kSB;
         const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA));
+        if constexpr (kind == kGram && T == 64) {
+            if (w.splits > 1) {
+                const int per = (w.ck / 64 + w.splits - 1) / w.splits * 64, k0 = split * per;
+                t.run(m, m, i0, j0, w.cp, k0, min(per, w.ck - k0), product_lds);
+                C* sum = (C*)((char*)w.sum + off) + (size_t)tile_id * w.splits * (T * T);
+                t.leave(product_lds, [](int, int) { return 0; },
+                    [&](int y, int x, int, C* v) { give<N>(sum + (size_t)split * (T * T) + y * T + x, v); },
+                    [](int, int, const C*) {});
+                if (!last_to_arrive((unsigned*)((char*)w.count + off) + tile_id, w.splits, (unsigned*)product_lds)) return;
+                // The last part to arrive adds all of them, in their order.  (No part waits for another.)
+                struct Sum { C v[N]; };
+                t.leave(product_lds,
+                    [&](int y, int x) {
+                        Sum all;
+#pragma unroll
+                        for (int n = 0; n < N; ++n) all.v[n] = C(0);
+                        for (int q = 0; q < w.splits; ++q) take<N>(sum + (size_t)q * (T * T) + y * T + x, all.v);
+                        return all;
+                    },
+                    [&](int y, int x, const Sum& all, C* v) {
+#pragma unroll
+                        for (int n = 0; n < N; ++n) v[n] = f * all.v[n];
+                        out.template put<N>((i0 + y) * w.rp + j0 + x, v, so);
+                    },
+                    [&](int y, int x, const C* v) {
+                        if (ti != tj) out.template put<N>((j0 + x) * w.rp + i0 + y, v, so);
+                    });
+                return;
+            }
+        }
+        t.run(m, m, i0, j0, kind == kGram ? w.cp : w.rp, 0, kind == kGram ? w.ck : w.rk, product_lds);
         t.leave(product_lds,
             [&](int y, int x) {
                 if constexpr (kind == kPoly) return a.template get<N>((i0 + y) * w.rp + j0 + x);
@@ -886,7 +961,7 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
             });
     } else {
         const auto xt = w.xt[from].at(off), nx = w.x[from ^ 1].at(off), nt = w.xt[from ^ 1].at(off);
-        t.run(xt, bm, i0, j0, w.rp, w.rp, product_lds);   // rows: columns of X; columns: rows of X
+        t.run(xt, bm, i0, j0, w.rp, 0, w.rk, product_lds);   // rows: columns of X; columns: rows of X
         const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB));
         t.leave(product_lds,
             [&](int y, int x) { return xt.template get<N>((i0 + y) * w.rp + j0 + x); },
@@ -926,26 +1001,65 @@ int form_of(int dtype, int r, int c) {
     if (r > 64 || c > 8192) return 0;
     return (r <= 32 ? Block<2>::bytes(c, size) : r <= 48 ? Block<3>::bytes(c, size) : Block<4>::bytes(c, size)) <= kLds ? 2 : 0;
 }
-// Side of a product's tile: the largest whose symmetric products still have a tile for half of the 256 CUs; below that the
-// chip stands still, above it larger tiles read less.  All five steps, 32 bits, us: 4096 x 4096  6443 (64), 5295 (128),
-// 4892 (256);  2048 x 2048  956, 823, 2265;  1024 x 1024  199, 424, 1236.
-int tile_of(int dtype, int batch, int r) {
-    if (dtype == VQA_DTYPE_F64) return 64;
-    for (int t = 256; t > 64; t /= 2) {
-        const int64_t n = (r + t - 1) / t;
-        if (n * (n + 1) / 2 * batch >= 128) return t;
+// How the products are cut: sides of the tiles of the symmetric ones (X X^T and b A + c A A) and of the update, and into how
+// many parts the sum of X X^T is split.
+struct Cut { int sym, up, splits; };
+struct Side { int side, splits; };
+
+// The tile and the parts whose rounds of 256 workgroups (one a CU) take least.  In us: what a round takes at its ends, and for
+// a summed index of 64 with the chip filled.  Measured for the tile so chosen | the next best, us a product of 32 bits:
+//   update      of 4096 x 4096  420 (256) | 504 (128)    of 2048 x 2048  62 (128) | 85 (64)    of 1024 x 4096  37 (128) | 46 (64)
+//   b A + c A A of 3000         148 (128) | 230 (256)    of 2048          53 (128) | 58 (64)    of 1024         12 (64) | 26 (128)
+// (Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer: with all
+// matrix units busy the clock falls, the more the more a product moves besides.)
+// A split sum (few tiles and a long sum: X X^T of a wide matrix) also takes the giving and taking of its parts, 3.5 us and 0.35
+// a part.  Whole operator, split | not:  100 x 4000  123 us (8 parts) | 218;  512 x 4096  231 (3) | 306.  Tiles of 128 lose what
+// splitting gains to that (1024 x 4096: 588 us with 5 parts, 449 with tiles of 64 unsplit).
+struct Round { int side; double ends, sum; };
+constexpr Round kRounds32[] = { { 256, 8, 4.6 }, { 128, 5, 1.5 }, { 64, 5, 0.45 } }, kRounds64[] = { { 64, 5, 3.8 } };
+template <int N>
+Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool split) {
+    const int stages = (sum + 63) / 64;
+    Side best = { 64, 1 };
+    double least = 1e30;
+    for (const Round& k : rounds) {
+        const int64_t a = (rows + k.side - 1) / k.side, b = (cols + k.side - 1) / k.side, n = (rows == cols ? a * (a + 1) / 2 : a * b) * batch;
+        const int most = split && k.side == 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
+        for (int p = 1; p <= std::max(1, most); ++p) {
+            const int per = (stages + p - 1) / p;
+            if ((stages + per - 1) / per != p) continue;   // (the last parts would be empty)
+            const double us = (double)((n * p + 255) / 256) * (k.ends + per * k.sum) + (p > 1 ? 3.5 + p * 0.35 : 0);
+            if (us < least) { least = us; best = { k.side, p }; }
+        }
     }
-    return 64;
+    return best;
 }
+template <int N>
+Cut cut_of(const Round (&rounds)[N], int batch, int r, int c) {
+    const Side gram = side_of(rounds, batch, r, r, c, true);
+    return { gram.side, side_of(rounds, batch, c, r, r, false).side, gram.splits };
+}
+Cut cut_of(int dtype, int batch, int r, int c) { return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, batch, r, c) : cut_of(kRounds32, batch, r, c); }
 int pad_to(int v, int t) { return (v + t - 1) / t * t; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
+size_t sum_bytes(int r, Cut t, size_t size) {
+    const size_t a = (r + t.sym - 1) / t.sym;
+    return a * (a + 1) / 2 * t.splits * t.sym * t.sym * size;
+}
 template <class M>
-size_t lay_out(char* base, int r, int c, int tile, Mats<M>* w);
+void extents(int r, int c, Cut t, Mats<M>* w) {
+    w->rk = pad_to(r, 64);
+    w->ck = pad_to(c, 64);
+    w->rp = std::max(pad_to(r, t.sym), pad_to(r, t.up));
+    w->cp = pad_to(c, t.up);
+}
+
+template <class M>
+size_t lay_out(char* base, int r, int c, Cut t, Mats<M>* w);
 template <>
-size_t lay_out<Pair>(char* base, int r, int c, int tile, Mats<Pair>* w) {
-    w->rp = pad_to(r, tile);
-    w->cp = pad_to(c, tile);
+size_t lay_out<Pair>(char* base, int r, int c, Cut t, Mats<Pair>* w) {
+    extents(r, c, t, w);
     const size_t x = up256((size_t)w->rp * w->cp * 2), a = up256((size_t)w->rp * w->rp * 2);
     char* p = base;
     auto next = [&](size_t n) { char* q = p; p += n; return (_Float16*)q; };
@@ -957,12 +1071,16 @@ size_t lay_out<Pair>(char* base, int r, int c, int tile, Mats<Pair>* w) {
     w->b.hi = next(a); w->b.lo = next(a);
     w->part = (double*)p;
     p += kNormParts * 8;
+    w->count = (unsigned*)p;
+    p += kMaxCount * 4;
+    w->sum = p;
+    w->splits = t.splits;
+    if (t.splits > 1) p += sum_bytes(r, t, 4);
     return w->stride = (size_t)(p - base);
 }
 template <>
-size_t lay_out<Wide>(char* base, int r, int c, int tile, Mats<Wide>* w) {
-    w->rp = pad_to(r, tile);
-    w->cp = pad_to(c, tile);
+size_t lay_out<Wide>(char* base, int r, int c, Cut t, Mats<Wide>* w) {
+    extents(r, c, t, w);
     const size_t x = up256((size_t)w->rp * w->cp * 8), a = up256((size_t)w->rp * w->rp * 8);
     char* p = base;
     auto next = [&](size_t n) { char* q = p; p += n; return (double*)q; };
@@ -974,6 +1092,11 @@ size_t lay_out<Wide>(char* base, int r, int c, int tile, Mats<Wide>* w) {
     w->b.v = next(a);
     w->part = (double*)p;
     p += kNormParts * 8;
+    w->count = (unsigned*)p;
+    p += kMaxCount * 4;
+    w->sum = p;
+    w->splits = t.splits;
+    if (t.splits > 1) p += sum_bytes(r, t, 8);
     return w->stride = (size_t)(p - base);
 }
 
@@ -1006,28 +1129,27 @@ int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename Sto
     return VQA_OK;
 }
 
-template <class Ty, int T, bool kFew>
-int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w) {
-    const unsigned tr = w.rp / T, tc = w.cp / T, sym = tr * (tr + 1) / 2, nb = (unsigned)j.batch;
-    int rc = VQA_OK;
-    for (int s = 0; s < j.steps && !rc; ++s) {
-        const int from = s & 1;
-        rc = product<Ty, kGram, T, kFew>(st, dim3(sym, 1, nb), j, w, from);
-        if (!rc) rc = product<Ty, kPoly, T, kFew>(st, dim3(sym, 1, nb), j, w, from);
-        if (!rc)
-            rc = s + 1 < j.steps ? product<Ty, kUpdate, T, kFew>(st, dim3(tr, tc, nb), j, w, from)
-                                 : product<Ty, kLast, T, kFew>(st, dim3(tr, tc, nb), j, w, from);
+template <class Ty, Kind kind, bool kFew>
+int product(hipStream_t st, int tile, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
+    const unsigned tr = (j.r + tile - 1) / tile, tc = (j.c + tile - 1) / tile;
+    const dim3 grid = kind == kGram || kind == kPoly ? dim3(tr * (tr + 1) / 2 * (kind == kGram ? w.splits : 1), 1, (unsigned)j.batch) : dim3(tr, tc, (unsigned)j.batch);
+    if constexpr (sizeof(typename Ty::C) == 4) {
+        if (tile == 256) return product<Ty, kind, 256, kFew>(st, grid, j, w, from);
+        if (tile == 128) return product<Ty, kind, 128, kFew>(st, grid, j, w, from);
     }
-    return rc;
+    return product<Ty, kind, 64, false>(st, grid, j, w, from);   // (64: bound by other things than its products)
 }
 
 template <class Ty, bool kFew>
-int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int tile) {
-    if constexpr (sizeof(typename Ty::C) == 4) {
-        if (tile == 256) return steps<Ty, 256, kFew>(st, j, w);
-        if (tile == 128) return steps<Ty, 128, kFew>(st, j, w);
+int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, Cut t) {
+    int rc = VQA_OK;
+    for (int s = 0; s < j.steps && !rc; ++s) {
+        const int from = s & 1;
+        rc = product<Ty, kGram, kFew>(st, t.sym, j, w, from);
+        if (!rc) rc = product<Ty, kPoly, kFew>(st, t.sym, j, w, from);
+        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate, kFew>(st, t.up, j, w, from) : product<Ty, kLast, kFew>(st, t.up, j, w, from);
     }
-    return steps<Ty, 64, false>(st, j, w);   // (bound by other things than its products)
+    return rc;
 }
 
 template <class Ty>
@@ -1074,16 +1196,16 @@ int run(hipStream_t st, const OrthoCall& q) {
         return VQA_OK;
     }
     Mats<typename StoreOf<C>::T> w;
-    const int tile = tile_of(q.dtype, q.batch, j.r);
-    lay_out((char*)q.workspace, j.r, j.c, tile, &w);
+    const Cut cut = cut_of(q.dtype, q.batch, j.r, j.c);
+    lay_out((char*)q.workspace, j.r, j.c, cut, &w);
     const unsigned nb = (unsigned)q.batch;
     const int pieces = std::max(1, std::min((j.cols + 4 * kT - 1) / (4 * kT), (2 * kNormParts + j.rows - 1) / j.rows));
     const int parts = std::min(kNormParts, j.rows * pieces);
     hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride, pieces);
     hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(w.cp / kTile, w.rp / kTile, nb), dim3(kT), 0, st, j, w, parts);
     int rc;
-    if constexpr (std::is_same_v<Ty, BF16>) rc = j.m ? steps<Ty, false>(st, j, w, tile) : steps<Ty, true>(st, j, w, tile);
-    else rc = steps<Ty, false>(st, j, w, tile);
+    if constexpr (std::is_same_v<Ty, BF16>) rc = j.m ? steps<Ty, false>(st, j, w, cut) : steps<Ty, true>(st, j, w, cut);
+    else rc = steps<Ty, false>(st, j, w, cut);
     if (rc) return rc;
     VQA_HIP(hipGetLastError());
     return VQA_OK;
@@ -1096,10 +1218,10 @@ size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
     if (form_of(dtype, r, c)) return 0;
     if (dtype == VQA_DTYPE_F64) {
         Mats<Wide> w;
-        return lay_out<Wide>(nullptr, r, c, tile_of(dtype, batch, r), &w) * (size_t)batch;
+        return lay_out<Wide>(nullptr, r, c, cut_of(dtype, batch, r, c), &w) * (size_t)batch;
     }
     Mats<Pair> w;
-    return lay_out<Pair>(nullptr, r, c, tile_of(dtype, batch, r), &w) * (size_t)batch;
+    return lay_out<Pair>(nullptr, r, c, cut_of(dtype, batch, r, c), &w) * (size_t)batch;
 }
 
 int ortho_launch(hipStream_t stream, const OrthoCall& q) {
