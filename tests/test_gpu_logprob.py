@@ -304,6 +304,27 @@ def test_top_outcomes_with_many_ties(t, V):
         assert np.array_equal(r.top_index.cpu().numpy(), ix), k
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("copies,V", [(1, 1100), (1, 9000), (1, 140000), (40, 3000), (2, 8192), (64, 5001)])
+@pytest.mark.parametrize("k", [1, 7, 33, 64])
+def test_top_outcomes_of_rows_in_any_order(t, copies, V, k):
+    """rows in order, in reverse, all alike, of two or a few values, with everything but a few masked, close together beside
+    one far away: the same outcomes as a stable sort, however many candidates there are at once"""
+    import torch
+
+    rng = np.random.default_rng(V + k)
+    up = np.arange(V) / 64.0
+    rows = [up, up[::-1], np.zeros(V), np.full(V, -3.0), (np.arange(V) % 2).astype(float), (np.arange(V) // 700).astype(float),
+            rng.integers(0, 3, V).astype(float), np.where(rng.random(V) < 20 / V, 1.0, -np.inf), np.full(V, -np.inf),
+            np.where(np.arange(V) == V // 2, 6e4, 1.0 + np.arange(V) * 2.0 ** -17), rng.standard_normal(V), np.sort(rng.standard_normal(V))]
+    z = torch.from_numpy(np.stack(rows)).to(getattr(torch, t)).cuda().repeat(copies, 1)
+    r = vqa_amd.log_probs(z, top_k=k)
+    first = z[:len(rows)].double().cpu().numpy()
+    want = np.argsort(-first, axis=1, kind="stable")[:, :k]
+    want = np.where(np.take_along_axis(first, want, 1) == -np.inf, -1, want)
+    assert np.array_equal(r.top_index.cpu().numpy(), np.tile(want, (copies, 1)))
+
+
 @pytest.mark.parametrize("t", ["float64", "bfloat16"])
 @pytest.mark.parametrize("V,stride,first", [(3, 7, 1), (100, 105, 3), (1500, 1507, 5), (9001, 9100, 7)])
 def test_strided_rows_and_unaligned_starts(t, V, stride, first):

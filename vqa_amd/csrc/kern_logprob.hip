@@ -151,7 +151,7 @@ __device__ __forceinline__ typename Ty::A slope(const Row<typename Ty::A>& r, ty
 }
 
 // ---- lanes ---------------------------------------------------------------------------------------------------------
-// a value of one lane (the lane's number is the same for the whole wave) for all, and a value of the lane before
+// a value of one lane (the lane's number is the same for the whole wave) for all
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(lane_of(__float_as_int(v), lane)); }
 __device__ __forceinline__ double lane_of(double v, int lane) {
@@ -165,7 +165,7 @@ template <int kCtrl>
 __device__ __forceinline__ double dpp(double old, double v) {
     return __hiloint2double(dpp<kCtrl>(__double2hiint(old), __double2hiint(v)), dpp<kCtrl>(__double2loint(old), __double2loint(v)));
 }
-constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143, kWaveShr1 = 0x138;
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143;
 // the largest of a wave's values, for all lanes
 template <class A>
 __device__ __forceinline__ A wave_max(A v) {
@@ -310,7 +310,8 @@ __device__ __forceinline__ void load_piece(const typename Ty::S* zr, int64_t e0,
     }
 }
 
-// a wave's list of its best outcomes, one a lane, best first (value, then lower index)
+__device__ __forceinline__ float lowest(float) { return -3.402823466e38f; }
+__device__ __forceinline__ double lowest(double) { return -1.7976931348623157e308; }
 template <class A>
 struct Best {
     A v;
@@ -318,25 +319,11 @@ struct Best {
 };
 template <class A>
 __device__ __forceinline__ Best<A> nobody() { return Best<A>{ neg_inf(A(0)), 0x7fffffff }; }
-// v and i: the same for the whole wave
-template <class A>
-__device__ __forceinline__ void insert(Best<A>& b, A v, int i, int lane) {
-    const int pos = __popcll(__ballot(before(b.v, b.i, v, i)));
-    const A uv = dpp<kWaveShr1>(b.v, b.v);
-    const int ui = dpp<kWaveShr1>(b.i, b.i);
-    b.v = lane < pos ? b.v : lane == pos ? v : uv;
-    b.i = lane < pos ? b.i : lane == pos ? i : ui;
-}
 
-// another list (best first, one a lane) into a wave's
-template <class A>
-__device__ __forceinline__ void merge(Best<A>& b, const Best<A>& c, int top_k, int lane) {
-    for (int k = 0; k < top_k; ++k) {
-        const A v = lane_of(c.v, k);
-        const int i = lane_of(c.i, k);
-        if (!(v > neg_inf(A(0))) || !before(v, i, lane_of(b.v, top_k - 1), lane_of(b.i, top_k - 1))) break;
-        insert(b, v, i, lane);
-    }
+// orders a wave's own writes to and reads of shared memory
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // A bound below the k-th best of a wave's first elements, from the lanes' own best mx: k lanes or more reach it.  It keeps
@@ -355,10 +342,158 @@ __device__ __forceinline__ A first_bound(A mx, int top_k) {
     return lo;
 }
 
+// A wave's candidates for its top_k best outcomes, in shared memory and in no order: all that it has seen above a bound which
+// top_k of them reach.  Candidates are only written down, which many lanes do at once; when there are too many the bound is
+// raised, and the order is found at the end by counting.  (Kept in order by inserting them one by one, each took 0.19 us of
+// its wave: a row of 131072, top 20, in 32 workgroups 15.8 us where the read-out without outcomes takes 5.5, and the joining
+// of the lists as long again.)
+constexpr int kPool = 128;
+template <class A>
+struct Store {
+    A v[kPool];
+    int i[kPool];
+};
+__device__ __forceinline__ float next_up(float v) {
+    const int b = __float_as_int(v);
+    return v == 0.f ? __int_as_float(1) : __int_as_float(b < 0 ? b - 1 : b + 1);
+}
+__device__ __forceinline__ double next_up(double v) {
+    const long long b = __double_as_longlong(v);
+    return v == 0.0 ? __longlong_as_double(1) : __longlong_as_double(b < 0 ? b - 1 : b + 1);
+}
+template <class A>
+struct Pool {
+    Store<A>* of;
+    int n, top_k;      // the same for the wave, as the rest:
+    A bound;           // top_k of what was seen reach it
+    A least;           // the least value that counts: the bound, or above it what reaches it was there before, at lower indices
+
+    __device__ __forceinline__ Pool(Store<A>* s, int k) : of(s), n(0), top_k(k), bound(neg_inf(A(0))), least(lowest(A(0))) {}
+    __device__ __forceinline__ void raise_to(A b) {
+        if (b > bound) bound = least = b;
+    }
+    // Values v[0 .. B) of each lane, id(j) the index of v[j]; possible(j): whether any lane's v[j ..] up to a multiple of N may
+    // count.  ordered: what is offered has lower indices than all that follows.
+    template <int B, int N, class F, class G>
+    __device__ __forceinline__ void offer(const A* v, F id, G possible, bool ordered, int lane) {
+        int from = 0;      // those before it are written down
+        for (;;) {
+            int stop = B;  // the first that there is no room for
+#pragma unroll
+            for (int j0 = 0; j0 < B; j0 += N) {
+                if (j0 + N <= from || stop < B || !possible(j0)) continue;
+#pragma unroll
+                for (int j = j0; j < j0 + N; ++j) {
+                    const uint64_t want = __ballot(v[j] >= least);
+                    if (!want || j < from || stop < B) continue;
+                    const int c = __popcll(want);
+                    if (n + c > kPool) {
+                        stop = j;
+                        continue;
+                    }
+                    if (want >> lane & 1) {
+                        const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(want >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)want, 0));
+                        of->v[at] = v[j];
+                        of->i[at] = id(j);
+                    }
+                    n += c;
+                }
+            }
+            wave_fence();
+            if (n > min(kPool / 2, max(8, 2 * top_k))) prune(lane);
+            if (stop == B) break;
+            from = stop;
+        }
+        if (ordered) least = next_up(bound);
+    }
+    // at most 64 of them, or top_k, with all that are among the best
+    __device__ __forceinline__ void prune(int lane) {
+        if (n <= top_k) return;
+        const A v0 = lane < n ? of->v[lane] : neg_inf(A(0)), v1 = 64 + lane < n ? of->v[64 + lane] : neg_inf(A(0));
+        const int i0 = of->i[lane], i1 = of->i[64 + lane];
+        wave_fence();
+        const A inf = -neg_inf(A(0));
+        A lo = -wave_max(max_of(lane < n ? -v0 : -inf, 64 + lane < n ? -v1 : -inf)), hi = wave_max(max_of(v0, v1));
+        int reach = n;
+        for (int s = 0; s < 14 && reach > top_k; ++s) {
+            const A mid = A(0.5) * lo + A(0.5) * hi;
+            const int r = __popcll(__ballot(v0 >= mid)) + __popcll(__ballot(v1 >= mid));
+            if (r >= top_k) {
+                lo = mid;
+                reach = r;
+            } else {
+                hi = mid;
+            }
+        }
+        if (reach > kPool / 2 || reach > top_k + 8) {     // close together or equal: by their ranks
+            rank(lane);
+            return;
+        }
+        const uint64_t w0 = __ballot(lane < n && v0 >= lo), w1 = __ballot(64 + lane < n && v1 >= lo);
+        const int n0 = __popcll(w0);
+        if (w0 >> lane & 1) {
+            const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(w0 >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)w0, 0));
+            of->v[at] = v0;
+            of->i[at] = i0;
+        }
+        if (w1 >> lane & 1) {
+            const int at = n0 + __builtin_amdgcn_mbcnt_hi((uint32_t)(w1 >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)w1, 0));
+            of->v[at] = v1;
+            of->i[at] = i1;
+        }
+        wave_fence();
+        n = reach;
+        raise_to(lo);
+    }
+    // the best top_k of them (or all), best first
+    __device__ __forceinline__ void rank(int lane) {
+        const bool two = n > 64;
+        const Best<A> a = lane < n ? Best<A>{ of->v[lane], of->i[lane] } : nobody<A>();
+        const Best<A> b = 64 + lane < n ? Best<A>{ of->v[64 + lane], of->i[64 + lane] } : nobody<A>();
+        int ra = 0, rb = 0;
+        if (two) {
+            for (int e = 0; e < n; ++e) {
+                ra += before(of->v[e], of->i[e], a.v, a.i);
+                rb += before(of->v[e], of->i[e], b.v, b.i);
+            }
+        } else {
+#pragma unroll 4
+            for (int e = 0; e < n; ++e) ra += before(of->v[e], of->i[e], a.v, a.i);
+        }
+        wave_fence();
+        if (lane < n && ra < top_k) {
+            of->v[ra] = a.v;
+            of->i[ra] = a.i;
+        }
+        if (64 + lane < n && rb < top_k) {
+            of->v[rb] = b.v;
+            of->i[rb] = b.i;
+        }
+        wave_fence();
+        if (n >= top_k) {
+            n = top_k;
+            raise_to(lane_of(of->v[top_k - 1], 0));
+        }
+    }
+    __device__ __forceinline__ void finish(int lane) {
+        if (n > top_k + 16) prune(lane);
+        rank(lane);
+    }
+    __device__ __forceinline__ Best<A> best(int lane) const { return lane < n ? Best<A>{ of->v[lane], of->i[lane] } : nobody<A>(); }
+    // how many of a finished pool's outcomes come before one of another pool
+    static __device__ __forceinline__ int ahead(const Store<A>& s, int n, const Best<A>& b) {
+        int at = 0;
+#pragma unroll
+        for (int step = 64; step; step >>= 1)
+            if (at + step <= n && before(s.v[at + step - 1], s.i[at + step - 1], b.v, b.i)) at += step;
+        return at;
+    }
+};
+
 // U pieces a lane into the wave's running state.  m is the wave's (the same in all lanes), s and t are the lane's.
 template <class Ty, int U, bool kTop>
-__device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Part<typename Ty::A>& p, Best<typename Ty::A>& best,
-                                     int top_k, typename Ty::A k, int lane) {
+__device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Part<typename Ty::A>& p, Pool<typename Ty::A>& pool,
+                                     typename Ty::A k, int lane) {
     using A = typename Ty::A;
     constexpr int N = Piece<Ty>::N, B = U * N;
     A piece_max[U], mx = neg_inf(A(0));
@@ -370,32 +505,15 @@ __device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Par
         mx = max_of(mx, piece_max[u]);
     }
     if constexpr (kTop) {
-        A kv = lane_of(best.v, top_k - 1);
-        if (__ballot(mx >= kv && mx > neg_inf(A(0)))) {
-            int ki = lane_of(best.i, top_k - 1);
-            A bound = kv;
-            if (kv == neg_inf(A(0))) bound = first_bound(mx, top_k);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (!__ballot(piece_max[u] >= bound)) continue;
-#pragma unroll
-                for (int j = u * N; j < (u + 1) * N; ++j) {
-                    uint64_t want = __ballot(v[j] >= bound && v[j] > neg_inf(A(0)));
-                    while (want) {
-                        const int src = __builtin_ctzll(want);
-                        const A cv = lane_of(v[j], src);
-                        const int ci = lane_of(at[u], src) + j % N;
-                        want &= want - 1;
-                        if (before(cv, ci, kv, ki)) {
-                            insert(best, cv, ci, lane);
-                            kv = lane_of(best.v, top_k - 1);
-                            ki = lane_of(best.i, top_k - 1);
-                            bound = max_of(bound, kv);
-                            want &= __ballot(v[j] >= bound);
-                        }
-                    }
-                }
-            }
+        if (__ballot(mx >= pool.least)) {
+            if (pool.bound == neg_inf(A(0))) pool.raise_to(first_bound(mx, pool.top_k));
+            const auto id = [&](int j) {
+                int i = at[j / N];
+                asm volatile("" : "+v"(i));   // (added where it is needed: B sums kept for the loop cost B registers)
+                return i + j % N;
+            };
+            pool.template offer<B, N>(v, id, [&](int j) { return __ballot(piece_max[j / N] >= pool.least) != 0; },
+                                      true, lane);
         }
     }
     if (__ballot(mx > p.m)) {                     // a new maximum (a NaN is not taken as one, it shows in s)
@@ -432,12 +550,11 @@ __device__ __forceinline__ void take(const typename Ty::A* v, const int* at, Par
 // pieces p0 + first + lane, + step .. of a row by one wave; all lanes hold the result
 template <class Ty, bool kTop>
 __device__ __forceinline__ Part<typename Ty::A> read_pieces(const typename Ty::S* zr, int64_t width, const Piece<Ty>& pc, int64_t p0,
-                                                            int64_t p1, int step, typename Ty::A scale, int top_k, Best<typename Ty::A>& best) {
+                                                            int64_t p1, int step, typename Ty::A scale, Pool<typename Ty::A>& pool) {
     using A = typename Ty::A;
-    constexpr int N = Piece<Ty>::N, U = 4;
+    constexpr int N = Piece<Ty>::N, U = 2;
     const int lane = threadIdx.x & 63;
     Part<A> p = nothing<A>();
-    best = nobody<A>();
     const A k = scale * unit<Ty>();
     for (int64_t q = p0; q < p1; q += step * U) {    // the same count for a wave's lanes
         A v[U * N];
@@ -448,13 +565,14 @@ __device__ __forceinline__ Part<typename Ty::A> read_pieces(const typename Ty::S
             at[u] = (int)e0;
             load_piece<Ty>(zr, e0, width, v + u * N);
         }
-        take<Ty, U, kTop>(v, at, p, best, top_k, k, lane);
+        take<Ty, U, kTop>(v, at, p, pool, k, lane);
     }
     reduce<64>([&](auto o) {
         p.s += across<o.value>(p.s);
         p.t += across<o.value>(p.t);
     });
     p.t *= A(1) / unit<Ty>();
+    if constexpr (kTop) pool.finish(lane);
     return p;
 }
 
@@ -466,18 +584,33 @@ __device__ __forceinline__ Part<typename Ty::A> read_part(const typename Ty::S* 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Piece<Ty> pc(zr, width);
     const int64_t per = (pc.pieces + splits - 1) / splits, p0 = split * per, p1 = min(pc.pieces, p0 + per);
-    Part<A> p = read_pieces<Ty, kTop>(zr, width, pc, p0 + wave * 64, p1, kT, scale, top_k, best);
     __shared__ Part<A> sp[kWaves];
-    __shared__ Best<A> sb[kWaves][64];
-    if (lane == 0) sp[wave] = p;
-    if constexpr (kTop) sb[wave][lane] = best;
+    __shared__ Store<A> store[kTop ? kWaves : 1];
+    __shared__ Best<A> sb[64];
+    __shared__ int sn[kWaves];
+    Pool<A> pool(&store[kTop ? wave : 0], top_k);
+    Part<A> p = read_pieces<Ty, kTop>(zr, width, pc, p0 + wave * 64, p1, kT, scale, pool);
+    if (lane == 0) {
+        sp[wave] = p;
+        sn[wave] = pool.n;
+    }
     __syncthreads();
+    if constexpr (kTop) {
+        // an outcome's place among all waves': those before it in its own pool and in the others
+        const Best<A> mine = pool.best(lane);
+        int at = lane, all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            all += sn[w];
+            if (w != wave) at += Pool<A>::ahead(store[w], sn[w], mine);
+        }
+        if (lane < pool.n && at < top_k) sb[at] = mine;
+        __syncthreads();
+        best = lane < min(all, top_k) ? sb[lane] : nobody<A>();
+    }
     if (wave == 0) {
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) p = join(p, sp[w], scale);
-        if constexpr (kTop) {
-            for (int w = 1; w < kWaves; ++w) merge(best, sb[w][lane], top_k, lane);
-        }
     }
     return p;
 }
@@ -513,9 +646,11 @@ struct Out {
     }
 };
 
-// splits = 1: the workgroup writes the row's results, else its part of them
+// splits = 1: the workgroup writes the row's results, else its part of them.
+// Eight waves a SIMD hide the way from memory (64 registers; two pieces of 16 bytes a lane at once): 2048 rows of 100003
+// bfloat16, top 8, 114 us = 3.6 TB/s, 151 with 5 waves and four pieces; without outcomes 96 us = 4.3 TB/s.
 template <class Ty, bool kTop>
-__global__ __launch_bounds__(kT) void k_lp_parts(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
+__global__ __launch_bounds__(kT, sizeof(typename Ty::A) == 4 ? 8 : 4) void k_lp_parts(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
                                                  typename Ty::A scale, int top_k, int splits, Ws<typename Ty::A> ws, Out<Ty> out) {
     using A = typename Ty::A;
     for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
@@ -541,11 +676,13 @@ template <class Ty, bool kTop>
 __global__ __launch_bounds__(kT) void k_lp_wave(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
                                                 typename Ty::A scale, int top_k, Out<Ty> out) {
     using A = typename Ty::A;
+    __shared__ Store<A> store[kTop ? kWaves : 1];
     for (int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * kWaves) {
         const typename Ty::S* zr = z + row * ld;
         const Piece<Ty> pc(zr, width);
-        Best<A> best;
-        const Part<A> p = read_pieces<Ty, kTop>(zr, width, pc, 0, pc.pieces, 64, scale, top_k, best);
+        Pool<A> pool(&store[kTop ? threadIdx.x >> 6 : 0], top_k);
+        const Part<A> p = read_pieces<Ty, kTop>(zr, width, pc, 0, pc.pieces, 64, scale, pool);
+        const Best<A> best = kTop ? pool.best(threadIdx.x & 63) : nobody<A>();
         out.write(row, zr, width, p, best, scale, threadIdx.x & 63);
     }
 }
@@ -566,21 +703,29 @@ __global__ __launch_bounds__(64) void k_lp_join(const typename Ty::S* __restrict
                                                 typename Ty::A scale, int top_k, int splits, Ws<typename Ty::A> ws, Out<Ty> out) {
     using A = typename Ty::A;
     const int lane = threadIdx.x;
+    __shared__ Store<A> store;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        Best<A> best = nobody<A>();
+        Pool<A> pool(&store, top_k);
         if (top_k > 0) {
-            constexpr int U = 8;
-            for (int s0 = 0; s0 < splits; s0 += U) {
-                Best<A> c[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) c[u] = s0 + u < splits && lane < top_k ? ws.best[(row * splits + s0 + u) * top_k + lane] : nobody<A>();
+            constexpr int U = 16;
+            const Best<A>* from = ws.best + row * splits * top_k;
+            const int all = splits * top_k;
+            for (int e0 = 0; e0 < all; e0 += 64 * U) {
+                A v[U], mx = neg_inf(A(0));
+                int ix[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (s0 + u == 0) best = c[u];
-                    else merge(best, c[u], top_k, lane);
+                    const Best<A> c = e0 + u * 64 + lane < all ? from[e0 + u * 64 + lane] : nobody<A>();
+                    v[u] = c.v;
+                    ix[u] = c.i;
+                    mx = max_of(mx, c.v);
                 }
+                if (pool.bound == neg_inf(A(0))) pool.raise_to(first_bound(mx, top_k));
+                pool.template offer<U, U>(v, [&](int j) { return ix[j]; }, [](int) { return true; }, false, lane);
             }
+            pool.finish(lane);
         }
+        const Best<A> best = pool.best(lane);
         out.write(row, z + row * ld, width, join_parts(ws.part + row * splits, splits, scale, lane), best, scale, lane);
     }
 }
@@ -863,8 +1008,8 @@ __global__ __launch_bounds__(T) void k_lp_twice(const typename Ty::S* __restrict
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const typename Ty::S* zr = z + row * ld;
         const Piece<Ty> pc(zr, width);
-        Best<A> none;
-        const Part<A> p = read_pieces<Ty, false>(zr, width, pc, wave * 64, pc.pieces, T, scale, 0, none);
+        Pool<A> none(nullptr, 0);
+        const Part<A> p = read_pieces<Ty, false>(zr, width, pc, wave * 64, pc.pieces, T, scale, none);
         if (lane == 0) sp[wave] = p;
         __syncthreads();
         int tg;
@@ -907,7 +1052,7 @@ __global__ __launch_bounds__(kT) void k_psr_chain_sum(const double* __restrict__
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
-constexpr int kShortWidth = 1024;
+constexpr int kLaneWidth = 64, kShortWidth = 1024;
 constexpr int kWaveRows = 512, kWaveWidth = 8192;
 constexpr int64_t kMaxGrid = 1 << 20;
 
@@ -932,7 +1077,7 @@ void launch_short(hipStream_t st, const typename Ty::S* z, int64_t rows, int wid
     else if (width <= 16) VQA_SHORT(4, 4);
     else if (width <= 64) VQA_SHORT(16, 4);
     else if (width <= 256) VQA_SHORT(64, 4);
-    else VQA_SHORT(64, 16);
+    else if constexpr (kGrad) VQA_SHORT(64, 16);
 #undef VQA_SHORT
 }
 
@@ -946,14 +1091,17 @@ int score(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld
           void* ws, void* lp, void* ent, void* top_lp, int32_t* top_ix) {
     using A = typename Ty::A;
     const auto* zz = (const typename Ty::S*)z;
-    if (width <= kShortWidth) {
+    // A row in a part of a wave or with four elements a lane: registers alone, the best outcomes one by one, 5 us each for
+    // 65536 rows;  else candidates are gathered.  65536 rows, us, so | the other way:  256 float32, top 4  57 | 51, none 30 | 35;
+    // top 20  64 | 165;  400 float32, top 4  55 | 98;  1024 bfloat16, none  41 | 87.
+    if (width <= kLaneWidth || (width <= 4 * kLaneWidth && top_k <= 4)) {
         launch_short<Ty, false>(st, zz, rows, (int)width, ld, scale, target, top_k, nullptr, nullptr, (A*)lp, (A*)ent, (A*)top_lp,
                                 top_ix, nullptr, 0);
     } else {
         const int splits = splits_of(rows, width);
         const Ws<A> w = splits > 1 ? ws_of<A>(ws, rows * splits) : Ws<A>{ nullptr, nullptr };
         const Out<Ty> out = { target, (A*)lp, (A*)ent, (A*)top_lp, top_ix, top_k };
-        if (rows >= kWaveRows && width <= kWaveWidth) {
+        if (width <= kShortWidth || (rows >= kWaveRows && width <= kWaveWidth)) {
             const dim3 waves((unsigned)std::min<int64_t>(kMaxGrid, (rows + kWaves - 1) / kWaves));
             if (top_k > 0) hipLaunchKernelGGL((k_lp_wave<Ty, true>), waves, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, out);
             else hipLaunchKernelGGL((k_lp_wave<Ty, false>), waves, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, out);
