@@ -99,11 +99,57 @@ def test_larger_matrices(t):
 
 @pytest.mark.parametrize("t", list(UNIT))
 @pytest.mark.parametrize("batch,rows,cols", [(1, 11, 300), (2, 16, 1500), (1, 1700, 15), (1, 16, 2048), (2, 3, 4000), (1, 16, 4096), (1, 16, 4099),
+                                             (2, 17, 2000), (1, 64, 5000), (5, 33, 777), (1, 1, 65536), (3, 1300, 64), (2, 48, 512), (1, 3000, 12), (300, 9, 530),
                                              (3, 20, 100), (1, 32, 700), (2, 33, 50), (1, 48, 400), (1, 270, 47), (3, 49, 64), (1, 64, 300)])
 def test_forms_of_small_matrices(t, batch, rows, cols):
-    """strips of one, four, eight and sixteen a wave, and blocks of two to four tiles, at their ends"""
+    """strips of one, four and eight a wave, blocks of two to four tiles, long rows in one part and several, at their ends"""
     g = matrices(np.random.default_rng(rows + cols), batch, rows, cols, t)
     check(vqa_amd.orthogonalize(g), g, t)
+
+
+@pytest.mark.parametrize("t", list(UNIT))
+@pytest.mark.parametrize("rows,cols", [(20, 600), (2100, 50), (9, 3000)])
+def test_long_rows(t, rows, cols):
+    """special matrices, in place, more steps than one round holds, momentum, replayed graphs"""
+    import torch
+
+    g = matrices(np.random.default_rng(30), 6, rows, cols, t)
+    g[1] = 0
+    g[2, 0, 0] = float("nan")
+    g[3, rows - 1, cols - 1] = float("inf")
+    g[4] = 0
+    g[4, 1, 2] = 3.0
+    o = vqa_amd.orthogonalize(g)
+    assert (o[1] == 0).all() and torch.isnan(o[2]).all() and torch.isnan(o[3]).all()
+    check(torch.stack([o[0], o[4], o[5]]), torch.stack([g[0], g[4], g[5]]), t)
+    assert torch.equal(vqa_amd.orthogonalize(g[5]), vqa_amd.orthogonalize(g[5:])[0])
+    h = g[[0, 5]].contiguous()
+    want = vqa_amd.orthogonalize(h.clone())
+    assert vqa_amd.orthogonalize(h, out=h).data_ptr() == h.data_ptr() and torch.equal(h, want)
+    g = g[[0, 5]].contiguous()
+    for steps in (1, 7, 8, 12):
+        check(vqa_amd.orthogonalize(g, steps=steps), g, t, steps=steps)
+    wide = torch.float64 if t == "float64" else torch.float32
+    w, m = torch.ones(2, rows, cols, dtype=wide).cuda(), 1e-2 * torch.ones(2, rows, cols, dtype=wide).cuda()
+    w0, m64 = w.double().clone(), 0.9 * m.double() + g.double()
+    ew, em = w.clone(), m.clone()
+    vqa_amd.muon_step(w, g, m, 0.1, 0.9, 0.2)
+    u = UNIT[t]
+    assert ((m.double() - m64).abs() <= u * (3 * m64.abs() + 3 * g.double().abs() + 3 * (m64 - g.double()).abs())).all()
+    rate = 0.1 * math.sqrt(max(1.0, rows / cols))
+    w64 = 0.98 * w0.cpu().numpy() - rate * defined((g.double() + 0.9 * m64).cpu().numpy())
+    off = np.sqrt(((w.double().cpu().numpy() - w64) ** 2).sum(axis=(1, 2)))
+    r, c = sorted((rows, cols))
+    assert (off <= rate * bound(t, r, c) * 2 + 4 * u * np.sqrt((w64 ** 2).sum(axis=(1, 2)))).all()
+    graph = torch.cuda.CUDAGraph()
+    cw, cm = ew.clone(), em.clone()
+    with torch.cuda.graph(graph):
+        vqa_amd.muon_step(cw, g, cm, 0.1, 0.9, 0.2)
+    for _ in range(4):
+        graph.replay()
+        vqa_amd.muon_step(ew, g, em, 0.1, 0.9, 0.2)
+        torch.cuda.synchronize()
+        assert torch.equal(cw, ew) and torch.equal(cm, em)
 
 
 @pytest.mark.parametrize("batch,rows,cols,t", [(1, 100, 4000, "float32"), (3, 200, 1111, "float32"), (2, 4100, 70, "bfloat16"), (1, 80, 3000, "float64"),

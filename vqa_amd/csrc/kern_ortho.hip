@@ -5,10 +5,11 @@
 // a s + b s^3 + c s^5 and the singular vectors stay, so the result is U p(S) V^T of G = U S V^T without an SVD.
 // r = min(rows, cols), c = max: X is taken r x c (the transpose of a matrix with more rows than columns).
 //
-// Three forms:
-// * r <= 16 (c <= 4096, 64 bits 2048): one workgroup carries a matrix through all steps, X in the registers of its waves in
-//   strips of 16 columns (k_ns_strip), in 64-bit or 32-bit matrix instructions.
-// * r <= 64 and X fits the LDS of a CU: the same with X in shared memory (k_ns_block).
+// Four forms:
+// * r <= 16, short rows: one workgroup carries a matrix through all steps, X in the registers of its waves in strips of 16
+//   columns (k_ns_strip), in 64-bit or 32-bit matrix instructions.
+// * r <= 64, short rows: the same with X in shared memory (k_ns_block).
+// * r <= 64, long rows: the steps on X X^T alone, between two passes over the matrix (k_ns_gram, k_ns_poly, k_ns_apply).
 // * else: three tiled products a step (k_ns_product), X, X^T, A and b A + c A A in device memory, all row-major with the
 //   summed index contiguous, padded to whole tiles.  64-bit matrices use 64-bit matrix instructions; the others hold every
 //   value as a sum of two 16-bit floats hi + lo (22 bits and a sign, scaled so that neither part leaves its normal range) and
@@ -433,6 +434,215 @@ __global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
             w.step();
         }
         j.template leave<8>(b, v, [&](int u, int& r, int& c) { r = row[u]; c = col[u]; return row[u] < j.rows; });
+    }
+}
+
+// ---- r <= 64 and long rows: the steps on X X^T -------------------------------------------------------------------------
+// What the steps make of X is P X with P a polynomial of A = X X^T: with Q = a I + b A + c A A a step takes P to Q P and A to
+// Q A Q, r x r all.  So a round of steps reads the matrix twice (A; P X), and the r x r products between are a workgroup's.
+// A has the squares of the singular values: an error u of it moves P X by up to |a|^(2 steps) u.  For matrices of 32 and 16
+// bits, with the products in 64 bits, a round is as many steps as keep |a|^steps <= 2^13 (u |a|^(2 steps) <= 2^-27), with the
+// usual coefficients all of them; 64-bit matrices take a round a step, and X lies in the workspace between rounds.
+// All r x r matrices are symmetric: a lower tile a wave, written to both sides of the diagonal.
+template <int NT>
+struct Long {
+    static constexpr int kRows = 16 * NT, kTiles = NT * (NT + 1) / 2, LD = kRows + 2;
+    static constexpr size_t kBytes = (size_t)4 * kRows * LD * 8 + 64;
+};
+constexpr int kMaxParts = 16;   // of the columns of a matrix
+struct LongWs {
+    double* part;      // A0 of a part of the columns: [part][lower tile][16 x 16]
+    double* poly;      // P (in the first round / (|G| + eps)), [16 NT][16 NT]
+    double* x;         // X^T between rounds, [c][16 NT]
+    size_t stride;     // bytes of a matrix
+    int parts;
+    template <class T> __device__ T* at(T* p, int b) const { return (T*)((char*)p + b * stride); }
+};
+
+template <class Ty, int NT, bool kEnter>
+__global__ __launch_bounds__(kT) void k_ns_gram(Job<Ty> j, LongWs w) {
+    using Lg = Long<NT>;
+    constexpr int V = 4;                                    // instructions' columns under way at once
+    __shared__ double sum[2][kWaves][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.y;
+    const int per = ((j.c + 15) / 16 + w.parts - 1) / w.parts * 16, c0 = blockIdx.x * per, c1 = min(j.c, c0 + per);
+    double4v acc[Lg::kTiles];
+#pragma unroll
+    for (int t = 0; t < Lg::kTiles; ++t) acc[t] = double4v{ 0, 0, 0, 0 };
+    for (int k0 = c0 + wave * 4 * V; k0 < c1; k0 += kWaves * 4 * V) {
+        std::conditional_t<kEnter, typename Ty::C, double> x[NT * V];
+        if constexpr (kEnter) {
+            j.template enter<true, NT * V>(b, x, [&](int u, int& row, int& col) {
+                const int i = u / V * 16 + (lane & 15), k = k0 + u % V * 4 + (lane >> 4);
+                row = j.turned ? k : i;
+                col = j.turned ? i : k;
+                return i < j.r && k < c1;
+            });
+        } else {
+            const double* xt = w.at(w.x, b);
+#pragma unroll
+            for (int u = 0; u < NT * V; ++u) {
+                const int k = k0 + u % V * 4 + (lane >> 4);
+                x[u] = k < c1 ? xt[(size_t)k * Lg::kRows + u / V * 16 + (lane & 15)] : 0.0;
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int t = 0; t < Lg::kTiles; ++t) {
+                int ti = 0, tj = 0;
+                lower(t, ti, tj);
+                acc[t] = Mma<double>::go((double)x[ti * V + v], (double)x[tj * V + v], acc[t]);
+            }
+    }
+    double* out = w.at(w.part, b) + (size_t)blockIdx.x * Lg::kTiles * 256;
+#pragma unroll
+    for (int t = 0; t < Lg::kTiles; ++t) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[t & 1][wave][Mma<double>::row(lane, q) * 16 + (lane & 15)] = acc[t][q];
+        __syncthreads();
+        double v = 0;
+#pragma unroll
+        for (int u = 0; u < kWaves; ++u) v += sum[t & 1][u][threadIdx.x];
+        out[t * 256 + threadIdx.x] = v;
+    }
+}
+
+template <int NT>
+__global__ __launch_bounds__(64 * Long<NT>::kTiles) void k_ns_poly(LongWs w, int r, int steps, double ka, double kb, double kc, double eps,
+                                                                      bool first) {
+    using Lg = Long<NT>;
+    constexpr int R = Lg::kRows, LD = Lg::LD, T = 64 * Lg::kTiles, N4 = R / 4;
+    extern __shared__ __attribute__((aligned(16))) char poly_lds[];
+    double* A = (double*)poly_lds;
+    double *Q = A + R * LD, *P = Q + R * LD, *W = P + R * LD, *inv = W + R * LD;
+    const int lane = threadIdx.x & 63, b = blockIdx.x;
+    int ti, tj;
+    lower(threadIdx.x >> 6, ti, tj);
+    const int row0 = ti * 16, col0 = tj * 16 + (lane & 15);
+    // operands of the wave's tile of a product of symmetric matrices, and its elements of the result
+    const int left = (row0 + (lane & 15)) * LD + (lane >> 4), right = col0 * LD + (lane >> 4);
+    auto put = [&](double* m, const double4v& v) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = row0 + Mma<double>::row(lane, q);
+            m[row * LD + col0] = v[q];
+            if (ti != tj) m[col0 * LD + row] = v[q];
+        }
+    };
+    auto get = [&](const double* m) {
+        double4v v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = m[(row0 + Mma<double>::row(lane, q)) * LD + col0];
+        return v;
+    };
+    {
+        double4v v = { 0, 0, 0, 0 };
+        const double* part = w.at(w.part, b) + (threadIdx.x >> 6) * 256 + (lane & 15);
+#pragma unroll 4
+        for (int p = 0; p < w.parts; ++p)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] += part[(size_t)p * Lg::kTiles * 256 + Mma<double>::row(lane, q) * 16];
+        put(A, v);
+    }
+    __syncthreads();
+    double scale = 1;
+    if (first) {
+        if (threadIdx.x < 64) {
+            double d = lane < r ? A[lane * LD + lane] : 0.0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) d += __shfl_xor(d, o);
+            if (lane == 0) *inv = 1.0 / (sqrt(d) + eps);
+        }
+        __syncthreads();
+        scale = *inv;
+        double4v v = get(A);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = v[q] * scale * scale;
+        __syncthreads();
+        put(A, v);
+        __syncthreads();
+    }
+    for (int s = 0; s < steps; ++s) {
+        double4v q = dot16<double>(A + left, A + right, N4);
+        const double4v a = get(A);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = kb * a[e] + kc * q[e] + (row0 + Mma<double>::row(lane, e) == col0 ? ka : 0.0);
+        put(Q, q);
+        if (s == 0) put(P, q);
+        __syncthreads();
+        double4v p, v;
+        if (s > 0) p = dot16<double>(Q + left, P + right, N4);
+        if (s + 1 < steps) {
+            v = dot16<double>(Q + left, A + right, N4);
+            put(W, v);
+        }
+        __syncthreads();
+        if (s > 0) put(P, p);
+        if (s + 1 < steps) {
+            v = dot16<double>(W + left, Q + right, N4);
+            put(A, v);
+        }
+        __syncthreads();
+    }
+    double* out = w.at(w.poly, b);
+    for (int e = threadIdx.x; e < R * R; e += T) out[e] = P[e / R * LD + e % R] * scale;
+}
+
+template <class Ty, int NT, bool kEnter, bool kLeave>
+__global__ __launch_bounds__(kT) void k_ns_apply(Job<Ty> j, LongWs w) {
+    using C = typename Ty::C;
+    using Lg = Long<NT>;
+    constexpr int R = Lg::kRows, LD = Lg::LD, N4 = R / 4;
+    __shared__ double P[R * LD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lk = lane >> 4, b = blockIdx.y;
+    const double* from = w.at(w.poly, b);
+    double* xt = w.at(w.x, b);
+    for (int e = threadIdx.x; e < R * R; e += kT) P[e / R * LD + e % R] = from[e];
+    __syncthreads();
+    // 16 columns of X a wave, read whole before they are written
+    for (int k0 = (blockIdx.x * kWaves + wave) * 16; k0 < j.c; k0 += gridDim.x * kWaves * 16) {
+        std::conditional_t<kEnter, C, double> x[N4];
+        if constexpr (kEnter) {
+            j.template enter<false, N4>(b, x, [&](int u, int& row, int& col) {
+                const int i = 4 * u + lk, k = k0 + lr;
+                row = j.turned ? k : i;
+                col = j.turned ? i : k;
+                return i < j.r && k < j.c;
+            });
+        } else {
+#pragma unroll
+            for (int u = 0; u < N4; ++u) x[u] = k0 + lr < j.c ? xt[(size_t)(k0 + lr) * R + 4 * u + lk] : 0.0;
+        }
+        // (P is symmetric: the same operands give the result's transpose when they change places)
+        const bool turned = !kLeave || j.turned;
+        double4v o[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            o[t] = double4v{ 0, 0, 0, 0 };
+#pragma unroll
+            for (int u = 0; u < N4; ++u) {
+                const double p = P[(t * 16 + lr) * LD + 4 * u + lk];
+                o[t] = turned ? Mma<double>::go((double)x[u], p, o[t]) : Mma<double>::go(p, (double)x[u], o[t]);
+            }
+        }
+        if constexpr (kLeave) {
+            C v[4 * NT];
+#pragma unroll
+            for (int u = 0; u < 4 * NT; ++u) v[u] = (C)o[u >> 2][u & 3];
+            j.template leave<4 * NT>(b, v, [&](int u, int& row, int& col) {
+                const int d = Mma<double>::row(lane, u & 3), t = u >> 2;
+                row = j.turned ? k0 + d : t * 16 + d;
+                col = j.turned ? t * 16 + lr : k0 + lr;
+                return row < j.rows && col < j.cols;
+            });
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4 * NT; ++u) {
+                const int k = k0 + Mma<double>::row(lane, u & 3);
+                if (k < j.c) xt[(size_t)k * R + (u >> 2) * 16 + lr] = o[u >> 2][u & 3];
+            }
+        }
     }
 }
 
@@ -994,12 +1204,28 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
 // ---- launches -------------------------------------------------------------------------------------------------------
 constexpr size_t kLds = 160 * 1024;
 
-// Which form carries a matrix: 0 tiled products, 1 strips in registers, 2 blocks in shared memory
-int form_of(int dtype, int r, int c) {
+// Which form carries a matrix.  Measured, us, long | strip or block (batch x r x c):  32 bits  1 x 11 x 512  17 | 18,  256 x 16 x
+// 512  23 | 21,  1 x 16 x 4096  18 | 73,  1 x 32 x 512  25 | 39,  1 x 64 x 256  61 | 57,  256 x 48 x 256  56 | 44;  64 bits, where
+// the long form takes three launches a step,  1 x 16 x 1024  51 | 35,  256 x 11 x 2048  189 | 79,  1 x 64 x 128  115 | 72.
+// Against the tiles of 64 x 64:  256 x 17 x 2048 of 32 bits  79 | 2710,  1 x 64 x 4096  66 | 110.
+enum Form { kTiled, kStrip, kBlock, kLong };
+Form form_of(int dtype, int r, int c) {
     const size_t size = dtype == VQA_DTYPE_F64 ? 8 : 4;
-    if (r <= 16) return c <= (size == 8 ? 2048 : 4096) ? 1 : 0;   // (the registers of 16 waves)
-    if (r > 64 || c > 8192) return 0;
-    return (r <= 32 ? Block<2>::bytes(c, size) : r <= 48 ? Block<3>::bytes(c, size) : Block<4>::bytes(c, size)) <= kLds ? 2 : 0;
+    if (r > 64) return kTiled;
+    if (size == 4 && c >= 512) return kLong;
+    if (r <= 16) return c <= 2048 ? kStrip : kLong;   // (the registers of 16 waves)
+    return (r <= 32 ? Block<2>::bytes(c, size) : r <= 48 ? Block<3>::bytes(c, size) : Block<4>::bytes(c, size)) <= kLds ? kBlock : kLong;
+}
+// Parts of the columns: enough workgroups for the chip, each with 256 columns or more
+LongWs long_ws(char* base, int batch, int r, int c) {
+    LongWs w;
+    const size_t nt = (r + 15) / 16, tile = 256;
+    w.parts = std::max(1, std::min({ kMaxParts, (c + 255) / 256, (1024 + batch - 1) / std::max(batch, 1) }));
+    w.part = (double*)base;
+    w.poly = w.part + w.parts * (nt * (nt + 1) / 2) * tile;
+    w.x = w.poly + nt * nt * tile;
+    w.stride = (w.parts * (nt * (nt + 1) / 2) * tile + nt * nt * tile + (size_t)c * nt * 16) * 8;
+    return w;
 }
 // How the products are cut: sides of the tiles of the symmetric ones (X X^T and b A + c A A) and of the update, and into how
 // many parts the sum of X X^T is split.
@@ -1114,6 +1340,28 @@ int allow_lds(F* fn, size_t bytes) {
 }
 
 template <class Ty, int NT>
+int long_rows(hipStream_t st, const Job<Ty>& j, const LongWs& w) {
+    if (int rc = allow_lds(k_ns_poly<NT>, Long<NT>::kBytes)) return rc;
+    int round = 1;
+    if (sizeof(typename Ty::C) == 4)
+        for (double a = fabs((double)j.ka), p = a * a; round < j.steps && p <= 8192.0; p *= a) ++round;
+    const dim3 parts(w.parts, (unsigned)j.batch), one((unsigned)j.batch), wide((unsigned)std::max(1, std::min((j.c + 63) / 64, 2048 / j.batch)), (unsigned)j.batch);
+    for (int s = 0; s < j.steps; s += round) {
+        const bool first = s == 0, last = s + round >= j.steps;
+        if (first) hipLaunchKernelGGL((k_ns_gram<Ty, NT, true>), parts, dim3(kT), 0, st, j, w);
+        else hipLaunchKernelGGL((k_ns_gram<Ty, NT, false>), parts, dim3(kT), 0, st, j, w);
+        hipLaunchKernelGGL((k_ns_poly<NT>), one, dim3(64 * Long<NT>::kTiles), Long<NT>::kBytes, st, w, j.r, std::min(round, j.steps - s),
+                           (double)j.ka, (double)j.kb, (double)j.kc, j.eps, first);
+        if (first && last) hipLaunchKernelGGL((k_ns_apply<Ty, NT, true, true>), wide, dim3(kT), 0, st, j, w);
+        else if (first) hipLaunchKernelGGL((k_ns_apply<Ty, NT, true, false>), wide, dim3(kT), 0, st, j, w);
+        else if (last) hipLaunchKernelGGL((k_ns_apply<Ty, NT, false, true>), wide, dim3(kT), 0, st, j, w);
+        else hipLaunchKernelGGL((k_ns_apply<Ty, NT, false, false>), wide, dim3(kT), 0, st, j, w);
+    }
+    VQA_HIP(hipGetLastError());
+    return VQA_OK;
+}
+
+template <class Ty, int NT>
 int block(hipStream_t st, const Job<Ty>& j) {
     const size_t lds = Block<NT>::bytes(j.c, sizeof(typename Ty::C));
     if (int rc = allow_lds(k_ns_block<Ty, NT>, lds)) return rc;
@@ -1177,19 +1425,22 @@ int run(hipStream_t st, const OrthoCall& q) {
     j.kb = (C)q.coefs[1];
     j.kc = (C)q.coefs[2];
     j.eps = q.eps;
-    const int form = form_of(q.dtype, j.r, j.c);
-    if (form == 1) {
+    const Form form = form_of(q.dtype, j.r, j.c);
+    if (form == kLong) {
+        const LongWs w = long_ws((char*)q.workspace, q.batch, j.r, j.c);
+        return j.r <= 16 ? long_rows<Ty, 1>(st, j, w) : j.r <= 32 ? long_rows<Ty, 2>(st, j, w) : j.r <= 48 ? long_rows<Ty, 3>(st, j, w) : long_rows<Ty, 4>(st, j, w);
+    }
+    if (form == kStrip) {
         const int strips = (j.c + 15) / 16;
         const dim3 grid((unsigned)q.batch);
         if (strips <= 4) hipLaunchKernelGGL((k_ns_strip<Ty, 4, 1>), grid, dim3(256), 0, st, j);
         else if (strips <= 16) hipLaunchKernelGGL((k_ns_strip<Ty, 4, 4>), grid, dim3(256), 0, st, j);
         else if (strips <= 64) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 4>), grid, dim3(1024), 0, st, j);
-        else if (strips <= 128) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 8>), grid, dim3(1024), 0, st, j);
-        else if constexpr (sizeof(C) == 4) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 16>), grid, dim3(1024), 0, st, j);
+        else if constexpr (sizeof(C) == 8) hipLaunchKernelGGL((k_ns_strip<Ty, 16, 8>), grid, dim3(1024), 0, st, j);
         VQA_HIP(hipGetLastError());
         return VQA_OK;
     }
-    if (form == 2) {
+    if (form == kBlock) {
         const int rc = j.r <= 32 ? block<Ty, 2>(st, j) : j.r <= 48 ? block<Ty, 3>(st, j) : block<Ty, 4>(st, j);
         if (rc) return rc;
         VQA_HIP(hipGetLastError());
@@ -1215,7 +1466,11 @@ int run(hipStream_t st, const OrthoCall& q) {
 
 size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
     const int r = std::min(rows, cols), c = std::max(rows, cols);
-    if (form_of(dtype, r, c)) return 0;
+    switch (form_of(dtype, r, c)) {
+        case kStrip: case kBlock: return 0;
+        case kLong: return long_ws(nullptr, batch, r, c).stride * (size_t)batch;
+        default: break;
+    }
     if (dtype == VQA_DTYPE_F64) {
         Mats<Wide> w;
         return lay_out<Wide>(nullptr, r, c, cut_of(dtype, batch, r, c), &w) * (size_t)batch;
