@@ -98,7 +98,7 @@ def test_larger_matrices(t):
 
 
 @pytest.mark.parametrize("t", list(UNIT))
-@pytest.mark.parametrize("batch,rows,cols", [(1, 11, 300), (2, 16, 1500), (1, 1700, 15), (1, 16, 2048), (2, 3, 4000), (1, 16, 4096), (1, 16, 4099),
+@pytest.mark.parametrize("batch,rows,cols", [(1, 11, 300), (2, 16, 1500), (1, 1700, 15), (1, 16, 2048), (33, 16, 2048), (40, 1500, 3), (2, 3, 4000), (1, 16, 4096), (1, 16, 4099),
                                              (2, 17, 2000), (1, 64, 5000), (5, 33, 777), (1, 1, 65536), (3, 1300, 64), (2, 48, 512), (1, 3000, 12), (300, 9, 530),
                                              (3, 20, 100), (1, 32, 700), (2, 33, 50), (1, 48, 400), (1, 270, 47), (3, 49, 64), (1, 64, 300)])
 def test_forms_of_small_matrices(t, batch, rows, cols):

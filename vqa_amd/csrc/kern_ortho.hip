@@ -830,7 +830,9 @@ template <class C, int T> struct Shape;
 template <> struct Shape<float, 64> { static constexpr int WI = 2, WJ = 2, KG = 4, BK = 64, S = 4; };
 template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 32, S = 4; };
 template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG = 1, BK = 32, S = 2; };
-template <> struct Shape<double, 64> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 16, S = 4; };
+// 64 bits: two workgroups a CU hide each other's barriers and ends (8 x 1024 x 1024 3620 us = 47 TFLOP/s, with four shorter
+// stages 3820; 1000 x 1000 823 | 996).
+template <> struct Shape<double, 64> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 32, S = 2; };
 
 // Which parts of the operands a product takes.  Results of 8 bits (bfloat16, without an optimizer state) take the high parts
 // of X alone, 11 bits: X X^T from hi hi, b A + c A A from all, B X from hi hi + lo hi.  Errors beside the result's own
@@ -875,12 +877,12 @@ struct Tile : Shape<C, T> {
     static constexpr size_t kOut = (size_t)kWv * BJ * kBlock * sizeof(C);
     static constexpr size_t kBytes = (size_t)S * kStage > kOut ? (size_t)S * kStage : kOut;
     static constexpr int N = 16 / KG;                                 // neighbours of a block's row that a lane takes
-    static_assert(kStage % (1024 * kWv) == 0 && (Q == 4 || Q == 8) && kBytes <= 160 * 1024);
+    static_assert(kStage % (1024 * kWv) == 0 && (Q == 4 || Q == 8 || Q == 16) && kBytes <= 160 * 1024);
 
     typename Fr::Acc acc[NI][NJ];
 
     static __device__ __forceinline__ int swz(int row) {
-        return Q == 4 ? (((row >> 1) ^ (row >> 3)) & 1) | ((row >> 2) & 1) << 1 : ((row ^ (row >> 3)) & 1) | (row & 6);
+        return Q == 16 ? row & 15 : Q == 4 ? (((row >> 1) ^ (row >> 3)) & 1) | ((row >> 2) & 1) << 1 : ((row ^ (row >> 3)) & 1) | (row & 6);
     }
     static __device__ __forceinline__ int wave() { return threadIdx.x >> 6; }
     static __device__ __forceinline__ int group() { return wave() / (WI * WJ); }
@@ -1206,14 +1208,15 @@ constexpr size_t kLds = 160 * 1024;
 
 // Which form carries a matrix.  Measured, us, long | strip or block (batch x r x c):  32 bits  1 x 11 x 512  17 | 18,  256 x 16 x
 // 512  23 | 21,  1 x 16 x 4096  18 | 73,  1 x 32 x 512  25 | 39,  1 x 64 x 256  61 | 57,  256 x 48 x 256  56 | 44;  64 bits, where
-// the long form takes three launches a step,  1 x 16 x 1024  51 | 35,  256 x 11 x 2048  189 | 79,  1 x 64 x 128  115 | 72.
+// the long form takes three launches a step,  1 x 16 x 1024  51 | 35,  1 x 11 x 2048  52 | 64,  256 x 11 x
+// 2048  189 | 79,  1 x 64 x 128  115 | 72.
 // Against the tiles of 64 x 64:  256 x 17 x 2048 of 32 bits  79 | 2710,  1 x 64 x 4096  66 | 110.
 enum Form { kTiled, kStrip, kBlock, kLong };
-Form form_of(int dtype, int r, int c) {
+Form form_of(int dtype, int batch, int r, int c) {
     const size_t size = dtype == VQA_DTYPE_F64 ? 8 : 4;
     if (r > 64) return kTiled;
     if (size == 4 && c >= 512) return kLong;
-    if (r <= 16) return c <= 2048 ? kStrip : kLong;   // (the registers of 16 waves)
+    if (r <= 16) return c <= (batch > 32 ? 2048 : 1024) ? kStrip : kLong;   // (2048: the registers of 16 waves)
     return (r <= 32 ? Block<2>::bytes(c, size) : r <= 48 ? Block<3>::bytes(c, size) : Block<4>::bytes(c, size)) <= kLds ? kBlock : kLong;
 }
 // Parts of the columns: enough workgroups for the chip, each with 256 columns or more
@@ -1425,7 +1428,7 @@ int run(hipStream_t st, const OrthoCall& q) {
     j.kb = (C)q.coefs[1];
     j.kc = (C)q.coefs[2];
     j.eps = q.eps;
-    const Form form = form_of(q.dtype, j.r, j.c);
+    const Form form = form_of(q.dtype, q.batch, j.r, j.c);
     if (form == kLong) {
         const LongWs w = long_ws((char*)q.workspace, q.batch, j.r, j.c);
         return j.r <= 16 ? long_rows<Ty, 1>(st, j, w) : j.r <= 32 ? long_rows<Ty, 2>(st, j, w) : j.r <= 48 ? long_rows<Ty, 3>(st, j, w) : long_rows<Ty, 4>(st, j, w);
@@ -1466,7 +1469,7 @@ int run(hipStream_t st, const OrthoCall& q) {
 
 size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
     const int r = std::min(rows, cols), c = std::max(rows, cols);
-    switch (form_of(dtype, r, c)) {
+    switch (form_of(dtype, batch, r, c)) {
         case kStrip: case kBlock: return 0;
         case kLong: return long_ws(nullptr, batch, r, c).stride * (size_t)batch;
         default: break;
