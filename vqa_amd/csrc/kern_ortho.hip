@@ -825,10 +825,11 @@ __device__ __forceinline__ void wait_and_meet() {
 // A stage holds BK values of T rows of each array; a row is Q pieces of 16 bytes, whose order in the row is turned by
 // swz(row), so that the 8 or 16 rows that a part of a wave reads at once lie in different banks.
 template <class C, int T> struct Shape;
-// Stages in flight: a stage's way from memory takes about 0.5 us, longer than small tiles compute on it, so two or three
-// are under way while one is read; 256 x 256 tiles compute longer than that on one stage, and have room for two.
+// Stages in flight: a stage's way from memory takes about 0.5 us, longer than tiles of 64 compute on it, so three are under
+// way while one is read (with two 1000 x 777 takes 213 us, with four 174);  larger tiles compute longer than that on one, and
+// do better with fewer, longer stages (2048 x 2048: 781 us with two of 64, 822 with four of 32).
 template <> struct Shape<float, 64> { static constexpr int WI = 2, WJ = 2, KG = 4, BK = 64, S = 4; };
-template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 32, S = 4; };
+template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 64, S = 2; };
 template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG = 1, BK = 32, S = 2; };
 // 64 bits: two workgroups a CU hide each other's barriers and ends (8 x 1024 x 1024 3620 us = 47 TFLOP/s, with four shorter
 // stages 3820; 1000 x 1000 823 | 996).
