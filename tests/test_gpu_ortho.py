@@ -270,6 +270,18 @@ def test_sizes_of_entries(size):
             assert o.abs().max() < 1e-18
 
 
+@pytest.mark.parametrize("rows,cols", [(6, 10), (40, 60), (5, 3000), (80, 70)])
+def test_squares_beyond_64_bits_give_nan(rows, cols):
+    """and a zero matrix stays zero with the smallest eps"""
+    import torch
+
+    g = matrices(np.random.default_rng(4), 2, rows, cols, "float64")
+    big = g * 1e180
+    assert torch.isnan(vqa_amd.orthogonalize(big)).all()
+    assert (vqa_amd.orthogonalize(torch.zeros_like(g), eps=1e-300) == 0).all()
+    check(vqa_amd.orthogonalize(g * 1e-100, eps=1e-300), g * 1e-100, "float64", eps=1e-300)
+
+
 @pytest.mark.parametrize("t", ["float64", "bfloat16"])
 def test_strides_out_and_in_place(t):
     import torch

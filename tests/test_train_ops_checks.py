@@ -72,7 +72,7 @@ def k3(*v):
     (dict(sb=31), _lib.EINVAL, "batch_stride"), (dict(steps=0), _lib.EINVAL, "steps"), (dict(steps=101), _lib.EINVAL, "steps"),
     (dict(k=None), _lib.EINVAL, "coefs"), (dict(k=k3(1, float("nan"), 0)), _lib.EINVAL, "finite"),
     (dict(k=k3(5.0, 0, 0)), _lib.EUNSUPPORTED, "singular value"), (dict(k=k3(1.5, 0, 0)), _lib.EUNSUPPORTED, "singular value"),
-    (dict(k=k3(0.0, 0.0, 40.0)), _lib.EUNSUPPORTED, "polynomial"), (dict(eps=0.0), _lib.EINVAL, "eps"),
+    (dict(k=k3(0.0, 0.0, 40.0)), _lib.EUNSUPPORTED, "polynomial"), (dict(eps=0.0), _lib.EINVAL, "eps"), (dict(eps=1e-301), _lib.EINVAL, "eps"),
     (dict(eps=float("inf")), _lib.EINVAL, "eps"), (dict(g=None), _lib.EINVAL, "g is NULL"), (dict(g=P + 2), _lib.EINVAL, "aligned"),
     (dict(out=None), _lib.EINVAL, "out"), (dict(out=P + 8), _lib.EINVAL, "overlap"), (dict(out=P, sr=9, sb=36), _lib.EINVAL, "overlap"),
     (dict(rows=100, cols=100, sr=100, sb=10000, batch=1, out=P + 80000), _lib.EINVAL, "workspace"),

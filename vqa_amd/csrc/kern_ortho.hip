@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "vqa_core.h"
@@ -152,6 +153,11 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
     return s;
 }
 
+// |G| + eps from the sum of squares; NaN where the squares leave 64 bits (a matrix divided by infinity would pass for zero)
+__device__ __forceinline__ double size_of_matrix(double squares, double eps) {
+    return squares < __builtin_inf() ? sqrt(squares) + eps : __builtin_nan("");
+}
+
 // What a wave's lanes wrote to shared memory before this is what its lanes read after it (and the other way round).  The
 // hardware runs a wave's shared memory accesses in order; this keeps the compiler from moving one lane's accesses past each
 // other that do not meet in that lane.
@@ -211,7 +217,7 @@ __global__ __launch_bounds__(NW * 64) void k_ns_strip(Job<Ty> j) {
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int q = 0; q < 4; ++q) ss += (double)x[s][q] * (double)x[s][q];
-    const double norm = sqrt(block_sum(ss, sh)) + j.eps;
+    const double norm = size_of_matrix(block_sum(ss, sh), j.eps);
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
             ss += (double)v[u] * (double)v[u];
         }
     }
-    const double norm = sqrt(block_sum(ss, sh)) + j.eps;
+    const double norm = size_of_matrix(block_sum(ss, sh), j.eps);
     for (int i = threadIdx.x; i < rp * ldx; i += kBlockThreads) X[i] = (C)((double)X[i] / norm);
     __syncthreads();
 
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(64 * Long<NT>::kTiles) void k_ns_poly(LongWs w, int
             double d = lane < r ? A[lane * LD + lane] : 0.0;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) d += __shfl_xor(d, o);
-            if (lane == 0) *inv = 1.0 / (sqrt(d) + eps);
+            if (lane == 0) *inv = 1.0 / size_of_matrix(d, eps);
         }
         __syncthreads();
         scale = *inv;
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
     const int b = blockIdx.z;
     const size_t off = b * w.stride;
     const double* part = (const double*)((char*)w.part + off);
-    const double norm = sqrt(block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh)) + j.eps;
+    const double norm = size_of_matrix(block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh), j.eps);
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kMaxCount) ((unsigned*)((char*)w.count + off))[threadIdx.x] = 0;
     // rows and columns of the caller's matrix
     const int64_t r0 = (int64_t)(j.turned ? blockIdx.x : blockIdx.y) * kTile, c0 = (int64_t)(j.turned ? blockIdx.y : blockIdx.x) * kTile;
@@ -1333,7 +1339,7 @@ size_t lay_out<Wide>(char* base, int r, int c, Cut t, Mats<Wide>* w) {
 // Dynamic shared memory beyond 64 KB is asked for once for each kernel and device
 template <class F>
 int allow_lds(F* fn, size_t bytes) {
-    static uint64_t done = 0;   // a bit a device; asking twice does no harm
+    static std::atomic<uint64_t> done{ 0 };   // a bit a device; asking twice does no harm
     int dev = 0;
     VQA_HIP(hipGetDevice(&dev));
     if (bytes > 65536 && !(done >> (dev & 63) & 1)) {

@@ -174,7 +174,7 @@ int check_matrices(OrthoCall& q, const double* coefs, size_t* g_bytes) {
     const int64_t one = (int64_t)(q.rows - 1) * q.g_row_stride + q.cols;
     if (q.batch > 1 && (q.g_batch_stride < one || q.g_batch_stride > ((int64_t)1 << 42)))
         VQA_FAIL(VQA_EINVAL, "batch_stride must be in [a matrix's extent, 2^42] (got %lld)", (long long)q.g_batch_stride);
-    if (!(q.eps > 0.0) || !isfinite(q.eps)) VQA_FAIL(VQA_EINVAL, "eps must be > 0");
+    if (!(q.eps >= 1e-300) || !isfinite(q.eps)) VQA_FAIL(VQA_EINVAL, "eps must be at least 1e-300 and finite");
     if ((rc = check_coefs(q.steps, coefs))) return rc;
     std::copy(coefs, coefs + 3, q.coefs);
     *g_bytes = q.batch ? ((size_t)(q.batch - 1) * q.g_batch_stride + one) * size_of(q.dtype) : 0;
