@@ -411,7 +411,8 @@ int vqa_class_stats_dev(int device, void* stream, const int64_t* d_counts, const
  * vqa_class_stats_dev reads class frequencies.  No counterpart in the reference.
  *
  * dtype is the scores' type; log probabilities, entropies and their weights are double for VQA_DTYPE_F64 and float for
- * the others, sums are held in that type.  Rows lie row_stride elements apart.  scale > 0, finite.
+ * the others, sums are held in that type.  Rows lie row_stride elements apart.  scale in
+ * [1e-30, 1e30].
  *   log_prob[r]  log p of outcome targets[r]; 0 for targets[r] < 0 (no outcome given)
  *   entropy[r]   -sum p log p
  *   top_index / top_log_prob [r, top_k]   the outcomes with the largest stored scores, largest first, equal ones by
