@@ -492,7 +492,7 @@ def test_large_offsets():
 # ---- the chain into circuit parameters, and the classifier's loss -------------------------------------------------
 
 
-@pytest.mark.parametrize("B,P,n_obs", [(1, 1, 1), (3, 5, 3), (64, 64, 2), (65, 65, 12), (1000, 37, 3), (0, 4, 2)])
+@pytest.mark.parametrize("B,P,n_obs", [(1, 1, 1), (3, 5, 3), (64, 64, 2), (65, 65, 12), (1000, 37, 3), (9000, 20, 3), (0, 4, 2)])
 def test_chain_matches_numpy(B, P, n_obs):
     import torch
 

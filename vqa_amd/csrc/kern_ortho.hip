@@ -185,7 +185,8 @@ template <> struct Mma<float> {
 // * for a symmetric matrix the first operand as well, so A A and B X take A and B as the products before left them.
 // Only X X^T needs X with the columns as summed index: each wave turns its own strip through shared memory and sums over its
 // own columns; the waves' parts of A are added in a fixed order (one barrier a step, two with 16 waves).
-// Bound by the chain of 12 dependent matrix instructions a step (64 cycles each in 64 bits).
+// Bound by the chain of 12 dependent matrix instructions a step (64 cycles each in 64 bits).  11 x 36 in 64 bits: 6.4 us, with
+// X in shared memory and a barrier between the products 14.5; 256 of 9 x 60 (one a CU) 7.7.
 template <class Ty, int NW, int S>
 __global__ __launch_bounds__(NW * 64) void k_ns_strip(Job<Ty> j) {
     using C = typename Ty::C;
@@ -319,6 +320,8 @@ __device__ __forceinline__ typename Mma<C>::Acc dot16(const C* xa, const C* xb, 
     return a0 + a1;
 }
 
+// Bound by the matrix instructions of one CU and the reading of their operands: 48 x 250 in 32 bits 38 us, 64 x 128 in 64 bits
+// 70 us = 0.12 TFLOP/s of the CU's 0.28.
 template <class Ty, int NT>
 __global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
     using C = typename Ty::C;
@@ -465,6 +468,8 @@ struct LongWs {
     template <class T> __device__ T* at(T* p, int b) const { return (T*)((char*)p + b * stride); }
 };
 
+// A of a part of the columns: each wave sums its own, operands straight from memory (a column's elements in 16 lanes).
+// 256 x 17 x 2048 in 32 bits, us: 27 here (36 MB), 12 for the polynomials, 41 for P X (71 MB); 64 x 4096: 17, 35 and 14.
 template <class Ty, int NT, bool kEnter>
 __global__ __launch_bounds__(kT) void k_ns_gram(Job<Ty> j, LongWs w) {
     using Lg = Long<NT>;
@@ -514,6 +519,8 @@ __global__ __launch_bounds__(kT) void k_ns_gram(Job<Ty> j, LongWs w) {
     }
 }
 
+// The steps of a round on A: three phases a step, each a barrier and N4 dependent matrix instructions (64 rows: 16 of them,
+// 2.3 us a phase with the reading of the operands).
 template <int NT>
 __global__ __launch_bounds__(64 * Long<NT>::kTiles) void k_ns_poly(LongWs w, int r, int steps, double ka, double kb, double kc, double eps,
                                                                       bool first) {
@@ -595,6 +602,7 @@ __global__ __launch_bounds__(64 * Long<NT>::kTiles) void k_ns_poly(LongWs w, int
     for (int e = threadIdx.x; e < R * R; e += T) out[e] = P[e / R * LD + e % R] * scale;
 }
 
+// P X, P in shared memory, 16 columns a wave at a time
 template <class Ty, int NT, bool kEnter, bool kLeave>
 __global__ __launch_bounds__(kT) void k_ns_apply(Job<Ty> j, LongWs w) {
     using C = typename Ty::C;
@@ -752,7 +760,7 @@ struct Mats {
 };
 
 // Parts of the sum of squares (and the momentum): a workgroup takes whole rows in turn, or, of few long rows, pieces of them.
-// 16 loads of a thread are under way at once.
+// 16 loads of a thread are under way at once.  4096 x 4096 bfloat16: 21 us = 1.6 TB/s (with 4 under way 127).
 template <class Ty>
 __global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t stride, int pieces) {
     using C = typename Ty::C;
@@ -773,7 +781,7 @@ __global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t 
     if (threadIdx.x == 0) ((double*)((char*)part + b * stride))[blockIdx.x] = ss;
 }
 
-// X0 and its transpose, a tile a workgroup
+// X0 and its transpose, a tile a workgroup.  4096 x 4096 bfloat16: 39 us = 4.3 TB/s of the reading and of the four arrays written.
 template <class Ty>
 __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int norm_parts) {
     using C = typename Ty::C;
@@ -1103,6 +1111,11 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned*
 
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
+// Time of X X^T | b A + c A A | update, us:  4096 x 4096 bfloat16  139 | 300 | 271, the three products of the second at 1.03
+// PFLOP/s with the clock down to 1.97 GHz from heat (the library's product of 16-bit floats of this size: 1.26);  2048 x 2048
+// float32  54 | 54 | 64;  1000 x 777  12 | 10 | 12: bound by the 5 us that a launch, the way of the first stage, the epilogue
+// and the last stores take;  1024 x 4096 float32  34 | 12 | 40: 136 tiles for 256 CUs, and an update that writes 34 MB in one
+// round, after its products.
 template <class Ty, Kind kind, int T, bool kFew>
 __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
     using C = typename Ty::C;
