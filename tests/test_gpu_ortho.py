@@ -270,6 +270,27 @@ def test_sizes_of_entries(size):
             assert o.abs().max() < 1e-18
 
 
+@pytest.mark.parametrize("t", list(UNIT))
+@pytest.mark.parametrize("rows,cols", [(11, 36), (40, 60), (20, 600), (96, 128), (128, 96), (97, 130), (2000, 2048)])
+def test_results_that_begin_anywhere(t, rows, cols):
+    """out, weight and momentum an element behind an aligned address: the same values, and nothing written around them"""
+    import torch
+
+    g = matrices(np.random.default_rng(8), 1, rows, cols, t)[0]
+    want = vqa_amd.orthogonalize(g)
+    wide = torch.float64 if t == "float64" else torch.float32
+    n = rows * cols
+    buf = torch.full((n + 2,), 7.0, dtype=g.dtype).cuda()
+    o = vqa_amd.orthogonalize(g, out=buf[1:n + 1].view(rows, cols))
+    assert torch.equal(o, want) and buf[0] == 7 and buf[n + 1] == 7
+    w, m = torch.ones(rows, cols, dtype=wide).cuda(), torch.ones(rows, cols, dtype=wide).cuda()
+    wb, mb = torch.ones(n + 2, dtype=wide).cuda(), torch.ones(n + 2, dtype=wide).cuda()
+    vqa_amd.muon_step(w, g, m, 0.1)
+    vqa_amd.muon_step(wb[1:n + 1].view(rows, cols), g, mb[1:n + 1].view(rows, cols), 0.1)
+    assert torch.equal(wb[1:n + 1].view(rows, cols), w) and torch.equal(mb[1:n + 1].view(rows, cols), m)
+    assert wb[0] == 1 and wb[n + 1] == 1 and mb[0] == 1 and mb[n + 1] == 1
+
+
 @pytest.mark.parametrize("rows,cols", [(6, 10), (40, 60), (5, 3000), (80, 70)])
 def test_squares_beyond_64_bits_give_nan(rows, cols):
     """and a zero matrix stays zero with the smallest eps"""

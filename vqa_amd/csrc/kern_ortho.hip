@@ -128,6 +128,42 @@ struct Job {
                 if (ok[u]) out[to[u]] = Ty::down(o[u]);
         }
     }
+    // N neighbours of a row of the result from (row, col) on; those outside the matrix are left out
+    template <int N>
+    __device__ __forceinline__ void leave_run(int b, const C* o, int row, int col) const {
+        const int64_t to = ((int64_t)b * rows + row) * cols + col;
+        if (row < rows && col + N <= cols) {
+            if (m ? aligned<C, N>(w + to) : aligned<S, N>(out + to)) {
+                if (m) {
+                    alignas(16) C v[N];
+                    move<C, N>(v, w + to);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) v[n] = decay * v[n] - rate * o[n];
+                    move<C, N>(w + to, v);
+                } else {
+                    alignas(16) S v[N];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) v[n] = Ty::down(o[n]);
+                    move<S, N>(out + to, v);
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {   // (a few at a time: their places take registers)
+            leave<4>(b, o + k, [&](int n, int& r, int& c) { r = row; c = col + k + n; return row < rows && col + k + n < cols; });
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    template <class E, int N> static constexpr int kPiece = N * sizeof(E) < 16 ? (int)(N * sizeof(E)) : 16;
+    template <class E, int N> static __device__ __forceinline__ bool aligned(const E* p) { return (uintptr_t)p % kPiece<E, N> == 0; }
+    template <class E, int N>
+    static __device__ __forceinline__ void move(E* to, const E* from) {   // (both aligned to a piece)
+        using V = std::conditional_t<kPiece<E, N> == 16, uint4, uint2>;
+        static_assert(N * sizeof(E) % sizeof(V) == 0);
+#pragma unroll
+        for (int n = 0; n < (int)(N * sizeof(E) / sizeof(V)); ++n) ((V*)to)[n] = ((const V*)from)[n];
+    }
 };
 
 // the elements of a rows x cols matrix in row-major order, T threads apart, U at a time: next(row, col) steps T elements on
@@ -1205,20 +1241,12 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
                 for (int n = 0; n < N; ++n) v[n] = j.ka * xv[n] + f * v[n];
                 if (kind == kUpdate) nt.template put<N>(at, v, kSX);
                 else if (j.turned)
-                    j.template leave<N>(blockIdx.z, v, [&](int n, int& row, int& col) {
-                        row = (int)i0 + y;
-                        col = (int)j0 + x + n;
-                        return row < j.rows && col < j.cols;
-                    });
+                    j.template leave_run<N>(blockIdx.z, v, (int)i0 + y, (int)j0 + x);
             },
             [&](int y, int x, const C* v) {
                 if (kind == kUpdate) nx.template put<N>((j0 + x) * w.cp + i0 + y, v, kSX);
                 else if (!j.turned)
-                    j.template leave<N>(blockIdx.z, v, [&](int n, int& row, int& col) {
-                        row = (int)j0 + x;
-                        col = (int)i0 + y + n;
-                        return row < j.rows && col < j.cols;
-                    });
+                    j.template leave_run<N>(blockIdx.z, v, (int)j0 + x, (int)i0 + y);
             });
     }
 }
