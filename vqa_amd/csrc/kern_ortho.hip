@@ -1378,13 +1378,13 @@ size_t lay_out<Wide>(char* base, int r, int c, Cut t, Mats<Wide>* w) {
 }
 
 // Dynamic shared memory beyond 64 KB is asked for once for each kernel and device
-template <class F>
-int allow_lds(F* fn, size_t bytes) {
+template <auto kKernel>
+int allow_lds(size_t bytes) {
     static std::atomic<uint64_t> done{ 0 };   // a bit a device; asking twice does no harm
     int dev = 0;
     VQA_HIP(hipGetDevice(&dev));
     if (bytes > 65536 && !(done >> (dev & 63) & 1)) {
-        VQA_HIP(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
+        VQA_HIP(hipFuncSetAttribute((const void*)kKernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
         done |= (uint64_t)1 << (dev & 63);
     }
     return VQA_OK;
@@ -1392,7 +1392,7 @@ int allow_lds(F* fn, size_t bytes) {
 
 template <class Ty, int NT>
 int long_rows(hipStream_t st, const Job<Ty>& j, const LongWs& w) {
-    if (int rc = allow_lds(k_ns_poly<NT>, Long<NT>::kBytes)) return rc;
+    if (int rc = allow_lds<k_ns_poly<NT>>(Long<NT>::kBytes)) return rc;
     int round = 1;
     if (sizeof(typename Ty::C) == 4)
         for (double a = fabs((double)j.ka), p = a * a; round < j.steps && p <= 8192.0; p *= a) ++round;
@@ -1415,7 +1415,7 @@ int long_rows(hipStream_t st, const Job<Ty>& j, const LongWs& w) {
 template <class Ty, int NT>
 int block(hipStream_t st, const Job<Ty>& j) {
     const size_t lds = Block<NT>::bytes(j.c, sizeof(typename Ty::C));
-    if (int rc = allow_lds(k_ns_block<Ty, NT>, lds)) return rc;
+    if (int rc = (allow_lds<k_ns_block<Ty, NT>>(lds))) return rc;
     hipLaunchKernelGGL((k_ns_block<Ty, NT>), dim3((unsigned)j.batch), dim3(kBlockThreads), lds, st, j);
     return VQA_OK;
 }
@@ -1423,7 +1423,7 @@ int block(hipStream_t st, const Job<Ty>& j) {
 template <class Ty, Kind kind, int T, bool kFew>
 int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
     using Tl = Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>;
-    if (int rc = allow_lds(k_ns_product<Ty, kind, T, kFew>, Tl::kBytes)) return rc;
+    if (int rc = allow_lds<k_ns_product<Ty, kind, T, kFew>>(Tl::kBytes)) return rc;
     hipLaunchKernelGGL((k_ns_product<Ty, kind, T, kFew>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
     return VQA_OK;
 }
