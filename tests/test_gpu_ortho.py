@@ -201,6 +201,19 @@ def test_tiles_of_all_sizes(batch, rows, cols, t):
     check_large(vqa_amd.orthogonalize(g), g, t)
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(8, 1024, 1024), (3, 981, 614), (29, 276, 160), (2, 97, 1001), (1, 1500, 1490)])
+def test_tiles_of_all_sizes_in_64_bits(batch, rows, cols):
+    """tiles of 32 and 64 and both in one matrix; against the same products by the library, each within the bound"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    g = torch.randn(batch, rows, cols, generator=gen, device="cuda", dtype=torch.float64)
+    want = plain(g, torch.float64)
+    off = torch.linalg.vector_norm(vqa_amd.orthogonalize(g) - want, dim=(1, 2))
+    r, c = sorted((rows, cols))
+    assert (off <= 2 * bound("float64", r, c)).all(), off
+
+
 @pytest.mark.parametrize("batch,rows,cols", [(1, 2048, 1500), (1, 4000, 4096), (1, 150, 3000), (20, 200, 130)])
 def test_optimizer_step_of_large_matrices(batch, rows, cols):
     """bfloat16 gradients, weights and momentum of 32 bits: the update keeps 32 bits' accuracy"""

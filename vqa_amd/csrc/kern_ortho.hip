@@ -786,7 +786,7 @@ template <class M>
 struct Mats {
     M x[2], xt[2], a, b;
     double* part;     // of the norm
-    void* sum;        // X X^T in parts: [tile][part][64 x 64], in C
+    void* sum;        // X X^T in parts: [tile][part][T x T], in C
     unsigned* count;  // parts of a tile that are there (0 between the kernels)
     int splits;
     size_t stride;    // bytes to the next matrix of the batch
@@ -881,9 +881,11 @@ template <class C, int T> struct Shape;
 template <> struct Shape<float, 64> { static constexpr int WI = 2, WJ = 2, KG = 4, BK = 64, S = 4; };
 template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 64, S = 2; };
 template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG = 1, BK = 32, S = 2; };
-// 64 bits: two workgroups a CU hide each other's barriers and ends (8 x 1024 x 1024 3620 us = 47 TFLOP/s, with four shorter
-// stages 3820; 1000 x 1000 823 | 996).
+// 64 bits: several workgroups a CU hide each other's barriers and ends (8 x 1024 x 1024 3620 us = 47 TFLOP/s, with four shorter
+// stages 3820; 1000 x 1000 823 | 996).  Tiles of 32 read twice as much for a product, but the last round is fuller and fewer
+// of its rows are padding (1000 x 1000 717 us; 29 x 276 x 160 270 | 370; 8 x 1024 x 1024 4070).
 template <> struct Shape<double, 64> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 32, S = 2; };
+template <> struct Shape<double, 32> { static constexpr int WI = 1, WJ = 1, KG = 4, BK = 32, S = 2; };
 
 // Which parts of the operands a product takes.  Results of 8 bits (bfloat16, without an optimizer state) take the high parts
 // of X alone, 11 bits: X X^T from hi hi, b A + c A A from all, B X from hi hi + lo hi.  Errors beside the result's own
@@ -1159,7 +1161,7 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
     extern __shared__ __attribute__((aligned(16))) char product_lds[];
     const size_t off = blockIdx.z * w.stride;
     size_t ti = blockIdx.y, tj = blockIdx.x;
-    const int splits = kind == kGram && T == 64 ? w.splits : 1, tile_id = blockIdx.x / splits, split = blockIdx.x - tile_id * splits;
+    const int splits = kind == kGram && T <= 64 ? w.splits : 1, tile_id = blockIdx.x / splits, split = blockIdx.x - tile_id * splits;
     if (kSym) {
         ti = (size_t)((sqrtf(8.f * tile_id + 1.f) - 1.f) * 0.5f);
         while (ti * (ti + 1) / 2 > (size_t)tile_id) --ti;
@@ -1175,9 +1177,9 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
         const auto m = (kind == kGram ? w.x[from] : w.a).at(off), out = kind == kGram ? a : bm;
         const float so = kind == kGram ? kSA : kSB;
         const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA));
-        if constexpr (kind == kGram && T == 64) {
+        if constexpr (kind == kGram && T <= 64) {
             if (w.splits > 1) {
-                const int per = (w.ck / 64 + w.splits - 1) / w.splits * 64, k0 = split * per;
+                const int per = ((w.ck + 63) / 64 + w.splits - 1) / w.splits * 64, k0 = split * per;
                 t.run(m, m, i0, j0, w.cp, k0, min(per, w.ck - k0), product_lds);
                 C* sum = (C*)((char*)w.sum + off) + (size_t)tile_id * w.splits * (T * T);
                 t.leave(product_lds, [](int, int) { return 0; },
@@ -1293,15 +1295,15 @@ struct Side { int side, splits; };
 // a part.  Whole operator, split | not:  100 x 4000  123 us (8 parts) | 218;  512 x 4096  231 (3) | 306.  Tiles of 128 lose what
 // splitting gains to that (1024 x 4096: 588 us with 5 parts, 449 with tiles of 64 unsplit).
 struct Round { int side; double ends, sum; };
-constexpr Round kRounds32[] = { { 256, 8, 4.6 }, { 128, 5, 1.5 }, { 64, 5, 0.45 } }, kRounds64[] = { { 64, 5, 3.8 } };
+constexpr Round kRounds32[] = { { 256, 8, 4.6 }, { 128, 5, 1.5 }, { 64, 5, 0.45 } }, kRounds64[] = { { 64, 5, 2.1 }, { 32, 1.5, 0.68 } };
 template <int N>
-Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool split) {
+Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool gram) {
     const int stages = (sum + 63) / 64;
     Side best = { 64, 1 };
     double least = 1e30;
     for (const Round& k : rounds) {
-        const int64_t a = (rows + k.side - 1) / k.side, b = (cols + k.side - 1) / k.side, n = (rows == cols ? a * (a + 1) / 2 : a * b) * batch;
-        const int most = split && k.side == 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
+        const int64_t a = (rows + k.side - 1) / k.side, b = (cols + k.side - 1) / k.side, n = (gram ? a * (a + 1) / 2 : a * b) * batch;
+        const int most = gram && k.side <= 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
         for (int p = 1; p <= std::max(1, most); ++p) {
             const int per = (stages + p - 1) / p;
             if ((stages + per - 1) / per != p) continue;   // (the last parts would be empty)
@@ -1326,10 +1328,11 @@ size_t sum_bytes(int r, Cut t, size_t size) {
 }
 template <class M>
 void extents(int r, int c, Cut t, Mats<M>* w) {
-    w->rk = pad_to(r, 64);
-    w->ck = pad_to(c, 64);
-    w->rp = std::max(pad_to(r, t.sym), pad_to(r, t.up));
-    w->cp = pad_to(c, t.up);
+    constexpr int kLeast = std::is_same_v<M, Wide> ? 32 : 64;   // the smallest tile; whole stages
+    w->rk = pad_to(r, kLeast);
+    w->ck = pad_to(c, kLeast);
+    w->rp = pad_to(std::max(pad_to(r, t.sym), pad_to(r, t.up)), kTile);
+    w->cp = pad_to(pad_to(c, t.up), kTile);
 }
 
 template <class M>
@@ -1435,7 +1438,10 @@ int product(hipStream_t st, int tile, const Job<Ty>& j, const Mats<typename Stor
     if constexpr (sizeof(typename Ty::C) == 4) {
         if (tile == 256) return product<Ty, kind, 256, kFew>(st, grid, j, w, from);
         if (tile == 128) return product<Ty, kind, 128, kFew>(st, grid, j, w, from);
+    } else {
+        if (tile == 32) return product<Ty, kind, 32, false>(st, grid, j, w, from);
     }
+    if (tile != 64) VQA_FAIL(VQA_EINVAL, "no tile of %d", tile);
     return product<Ty, kind, 64, false>(st, grid, j, w, from);   // (64: bound by other things than its products)
 }
 
