@@ -875,9 +875,10 @@ __device__ __forceinline__ void wait_and_meet() {
 // A stage holds BK values of T rows of each array; a row is Q pieces of 16 bytes, whose order in the row is turned by
 // swz(row), so that the 8 or 16 rows that a part of a wave reads at once lie in different banks.
 template <class C, int T> struct Shape;
-// Stages in flight: a stage's way from memory takes about 0.5 us, longer than tiles of 64 compute on it, so three are under
-// way while one is read (with two 1000 x 777 takes 213 us, with four 174);  larger tiles compute longer than that on one, and
-// do better with fewer, longer stages (2048 x 2048: 781 us with two of 64, 822 with four of 32).
+// Stages in flight: a stage's way from memory takes about 0.5 us, longer than tiles of 32 and 64 compute on it, so three are
+// under way while one is read (with two 1000 x 777 takes 213 us, with four 174);  larger tiles compute longer than that on one,
+// and do better with fewer, longer stages (2048 x 2048: 781 us with two of 64, 822 with four of 32).
+template <> struct Shape<float, 32> { static constexpr int WI = 1, WJ = 1, KG = 4, BK = 64, S = 4; };
 template <> struct Shape<float, 64> { static constexpr int WI = 2, WJ = 2, KG = 4, BK = 64, S = 4; };
 template <> struct Shape<float, 128> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 64, S = 2; };
 template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG = 1, BK = 32, S = 2; };
@@ -1286,51 +1287,63 @@ struct Cut { int sym, up, splits; };
 struct Side { int side, splits; };
 
 // The tile and the parts whose rounds of 256 workgroups (one a CU) take least.  In us: what a round takes at its ends, and for
-// a summed index of 64 with the chip filled.  Measured for the tile so chosen | the next best, us a product of 32 bits:
+// a summed index of 64 with the chip filled.  Of tiles of 32 a CU holds several workgroups, so the last round's share counts.
+// Measured for the tile so chosen | the next best, us a product of 32 bits:
 //   update      of 4096 x 4096  420 (256) | 504 (128)    of 2048 x 2048  62 (128) | 85 (64)    of 1024 x 4096  37 (128) | 46 (64)
 //   b A + c A A of 3000         148 (128) | 230 (256)    of 2048          53 (128) | 58 (64)    of 1024         12 (64) | 26 (128)
+// and the whole operator with tiles of 32 | 64:  512 x 512  92 | 133,  300 x 300  77 | 105,  1000 x 1000  233 | 196.
 // (Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer: with all
 // matrix units busy the clock falls, the more the more a product moves besides.)
 // A split sum (few tiles and a long sum: X X^T of a wide matrix) also takes the giving and taking of its parts, 3.5 us and 0.35
-// a part.  Whole operator, split | not:  100 x 4000  123 us (8 parts) | 218;  512 x 4096  231 (3) | 306.  Tiles of 128 lose what
-// splitting gains to that (1024 x 4096: 588 us with 5 parts, 449 with tiles of 64 unsplit).
+// a part.  Whole operator, split | not, tiles of 64:  100 x 4000  123 us (8 parts) | 218;  512 x 4096  231 (3) | 306.  Tiles of
+// 128 lose what splitting gains to that (1024 x 4096: 588 us with 5 parts, 449 with tiles of 64 unsplit).
 struct Round { int side; double ends, sum; };
-constexpr Round kRounds32[] = { { 256, 8, 4.6 }, { 128, 5, 1.5 }, { 64, 5, 0.45 } }, kRounds64[] = { { 64, 5, 2.1 }, { 32, 1.5, 0.68 } };
+constexpr Round kRounds32[] = { { 256, 8, 4.6 }, { 128, 5, 1.5 }, { 64, 5, 0.45 }, { 32, 3, 0.33 } }, kRounds64[] = { { 64, 5, 2.1 }, { 32, 1.5, 0.68 } };
 template <int N>
 Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool gram) {
-    const int stages = (sum + 63) / 64;
     Side best = { 64, 1 };
     double least = 1e30;
     for (const Round& k : rounds) {
         const int64_t a = (rows + k.side - 1) / k.side, b = (cols + k.side - 1) / k.side, n = (gram ? a * (a + 1) / 2 : a * b) * batch;
-        const int most = gram && k.side <= 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
+        auto time = [&](int64_t tiles, int stages) {
+            const double full = k.side == 32 ? std::max(1.0, (double)tiles / 256) : (double)((tiles + 255) / 256);
+            return full * (k.ends + stages * k.sum);
+        };
+        const int stages = (sum + 63) / 64, most = gram && k.side <= 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
+        const double also = gram ? time(n, (rows + 63) / 64) : 0;      // b A + c A A
         for (int p = 1; p <= std::max(1, most); ++p) {
             const int per = (stages + p - 1) / p;
             if ((stages + per - 1) / per != p) continue;   // (the last parts would be empty)
-            const double us = (double)((n * p + 255) / 256) * (k.ends + per * k.sum) + (p > 1 ? 3.5 + p * 0.35 : 0);
+            const double us = time(n * p, per) + (p > 1 ? 3.5 + p * 0.35 : 0) + also;
             if (us < least) { least = us; best = { k.side, p }; }
         }
     }
     return best;
 }
+int pad_to(int v, int t) { return (v + t - 1) / t * t; }
 template <int N>
 Cut cut_of(const Round (&rounds)[N], int batch, int r, int c) {
     const Side gram = side_of(rounds, batch, r, r, c, true);
     return { gram.side, side_of(rounds, batch, c, r, r, false).side, gram.splits };
 }
-Cut cut_of(int dtype, int batch, int r, int c) { return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, batch, r, c) : cut_of(kRounds32, batch, r, c); }
-int pad_to(int v, int t) { return (v + t - 1) / t * t; }
+// whole stages, of which a tile's summed index is made up: what is summed over, and what tiles cover at the least
+int least_pad(int dtype) { return dtype == VQA_DTYPE_F64 ? 32 : 64; }
+Cut cut_of(int dtype, int batch, int r, int c) {
+    r = pad_to(r, least_pad(dtype));
+    c = pad_to(c, least_pad(dtype));
+    return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, batch, r, c) : cut_of(kRounds32, batch, r, c);
+}
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-size_t sum_bytes(int r, Cut t, size_t size) {
-    const size_t a = (r + t.sym - 1) / t.sym;
+size_t sum_bytes(int rk, Cut t, size_t size) {
+    const size_t a = (rk + t.sym - 1) / t.sym;
     return a * (a + 1) / 2 * t.splits * t.sym * t.sym * size;
 }
 template <class M>
 void extents(int r, int c, Cut t, Mats<M>* w) {
-    constexpr int kLeast = std::is_same_v<M, Wide> ? 32 : 64;   // the smallest tile; whole stages
-    w->rk = pad_to(r, kLeast);
-    w->ck = pad_to(c, kLeast);
+    const int least = least_pad(std::is_same_v<M, Wide> ? VQA_DTYPE_F64 : VQA_DTYPE_F32);
+    w->rk = pad_to(r, least);
+    w->ck = pad_to(c, least);
     w->rp = pad_to(std::max(pad_to(r, t.sym), pad_to(r, t.up)), kTile);
     w->cp = pad_to(pad_to(c, t.up), kTile);
 }
@@ -1355,7 +1368,7 @@ size_t lay_out<Pair>(char* base, int r, int c, Cut t, Mats<Pair>* w) {
     p += kMaxCount * 4;
     w->sum = p;
     w->splits = t.splits;
-    if (t.splits > 1) p += sum_bytes(r, t, 4);
+    if (t.splits > 1) p += sum_bytes(w->rk, t, 4);
     return w->stride = (size_t)(p - base);
 }
 template <>
@@ -1376,7 +1389,7 @@ size_t lay_out<Wide>(char* base, int r, int c, Cut t, Mats<Wide>* w) {
     p += kMaxCount * 4;
     w->sum = p;
     w->splits = t.splits;
-    if (t.splits > 1) p += sum_bytes(r, t, 8);
+    if (t.splits > 1) p += sum_bytes(w->rk, t, 8);
     return w->stride = (size_t)(p - base);
 }
 
@@ -1433,16 +1446,15 @@ int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename Sto
 
 template <class Ty, Kind kind, bool kFew>
 int product(hipStream_t st, int tile, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
-    const unsigned tr = (j.r + tile - 1) / tile, tc = (j.c + tile - 1) / tile;
+    const unsigned tr = (w.rk + tile - 1) / tile, tc = (w.ck + tile - 1) / tile;   // (all that is summed over is written)
     const dim3 grid = kind == kGram || kind == kPoly ? dim3(tr * (tr + 1) / 2 * (kind == kGram ? w.splits : 1), 1, (unsigned)j.batch) : dim3(tr, tc, (unsigned)j.batch);
     if constexpr (sizeof(typename Ty::C) == 4) {
         if (tile == 256) return product<Ty, kind, 256, kFew>(st, grid, j, w, from);
         if (tile == 128) return product<Ty, kind, 128, kFew>(st, grid, j, w, from);
-    } else {
-        if (tile == 32) return product<Ty, kind, 32, false>(st, grid, j, w, from);
     }
+    if (tile == 32) return product<Ty, kind, 32, false>(st, grid, j, w, from);
     if (tile != 64) VQA_FAIL(VQA_EINVAL, "no tile of %d", tile);
-    return product<Ty, kind, 64, false>(st, grid, j, w, from);   // (64: bound by other things than its products)
+    return product<Ty, kind, 64, false>(st, grid, j, w, from);   // (32 and 64: bound by other things than their products)
 }
 
 template <class Ty, bool kFew>
