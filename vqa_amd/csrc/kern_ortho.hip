@@ -1152,8 +1152,8 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned*
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
 // Time of X X^T | b A + c A A | update, us:  4096 x 4096 bfloat16  139 | 300 | 271, the three products of the second at 1.03
 // PFLOP/s with the clock down to 1.97 GHz from heat (the library's product of 16-bit floats of this size: 1.26);  2048 x 2048
-// float32  54 | 54 | 64;  1000 x 777  12 | 10 | 12: bound by the 5 us that a launch, the way of the first stage, the epilogue
-// and the last stores take;  1024 x 4096 float32  34 | 12 | 40: 136 tiles for 256 CUs, and an update that writes 34 MB in one
+// float32  54 | 54 | 64;  1000 x 777  10 | 8 | 12 (with tiles of 64 12 | 10 | 12): bound by the 3 to 5 us that a launch, the way
+// of the first stage, the epilogue and the last stores take;  1024 x 4096 float32  34 | 12 | 40: 136 tiles for 256 CUs, and an update that writes 34 MB in one
 // round, after its products.
 template <class Ty, Kind kind, int T, bool kFew>
 __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
