@@ -421,6 +421,27 @@ def test_the_same_call_gives_the_same_bits_on_any_stream():
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and all(torch.equal(x, y) for x, y in zip(a2, b2))
 
 
+@pytest.mark.parametrize("R,V", [(1, 131072), (7, 40000), (600, 3000)])
+def test_calls_at_the_same_time(R, V):
+    """queued on three streams without waiting, each call's workspace is its own"""
+    import torch
+
+    zs = [scores(np.random.default_rng(k), R, V, "float32") for k in range(3)]
+    tg = torch.zeros(R, dtype=torch.int32).cuda()
+    want = [(vqa_amd.log_probs(z, tg, top_k=20), vqa_amd.log_probs_grad(z, tg, -1.0, 0.1)) for z in zs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in zs]
+    got = [[], [], []]
+    for _ in range(8):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append((vqa_amd.log_probs(zs[k], tg, top_k=20), vqa_amd.log_probs_grad(zs[k], tg, -1.0, 0.1)))
+    torch.cuda.synchronize()
+    for k in range(3):
+        for a, b in got[k]:
+            assert all(torch.equal(x, y) for x, y in zip(a, want[k][0])) and all(torch.equal(x, y) for x, y in zip(b, want[k][1]))
+
+
 @pytest.mark.parametrize("V", [12, 40000])
 def test_captured_calls_replay_with_new_scores(V):
     """two graphs of the same call, each with its own memory, replayed in turn with eager work between"""

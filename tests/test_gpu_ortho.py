@@ -409,6 +409,25 @@ def test_streams_and_captured_steps(rows, cols):
         assert torch.equal(w, ew) and torch.equal(m, em), n
 
 
+@pytest.mark.parametrize("rows,cols,t", [(100, 4000, "float32"), (20, 3000, "float32"), (300, 300, "float64"), (700, 800, "bfloat16"), (30, 80, "float64")])
+def test_calls_at_the_same_time(rows, cols, t):
+    """queued on three streams without waiting, each call's workspace is its own"""
+    import torch
+
+    gs = [matrices(np.random.default_rng(k), 1, rows, cols, t)[0] for k in range(3)]
+    want = [vqa_amd.orthogonalize(g) for g in gs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in gs]
+    got = [[], [], []]
+    for _ in range(8):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(vqa_amd.orthogonalize(gs[k]))
+    torch.cuda.synchronize()
+    for k in range(3):
+        assert all(torch.equal(o, want[k]) for o in got[k])
+
+
 def test_refusals_on_the_gpu():
     import torch
 
