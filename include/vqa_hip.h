@@ -443,7 +443,8 @@ int vqa_log_probs(int device, int dtype, const void* scores, int64_t rows, int64
  *   d_dscores[r, c] = scale * (dlog_prob (delta_{c, target} - p_c) - dentropy p_c (log p_c + entropy))
  * in the scores' type, rows dscores_row_stride elements apart, columns behind `width` left as they were.  A row without
  * a target takes dlog_prob as 0; a row with every outcome masked has gradient 0, a row with NaN outputs has NaN.
- * d_targets is needed for d_dlog_prob.  d_dscores must not overlap the scores.  Workspace: vqa_log_probs_workspace with
+ * d_targets is needed for d_dlog_prob.  d_dscores must not overlap the scores (columns
+ * of one array with the same row stride may be scores and gradient).  Workspace: vqa_log_probs_workspace with
  * top_k 0.  The chain into circuit parameters is vqa_psr_chain_dev.
  */
 int vqa_log_probs_grad_dev(int device, void* stream, int dtype, const void* d_scores, int64_t rows, int64_t width,

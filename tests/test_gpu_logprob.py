@@ -354,6 +354,24 @@ def test_strided_rows_and_unaligned_starts(t, V, stride, first):
         assert torch.equal(r.top_index, s.top_index)
 
 
+@pytest.mark.parametrize("t", ["float64", "float16"])
+@pytest.mark.parametrize("R,V", [(5, 7), (130, 1500), (3, 5000)])
+def test_scores_and_gradient_in_one_array(t, R, V):
+    """columns of one array hold the scores, others take the gradient; the columns between stay"""
+    import torch
+
+    big = torch.full((R, 2 * V + 5), 3.0, dtype=getattr(torch, t)).cuda()
+    big[:, 1:V + 1] = scores(np.random.default_rng(V), R, V, t)
+    z, out = big[:, 1:V + 1], big[:, V + 3:2 * V + 3]
+    tg = torch.zeros(R, dtype=torch.int32).cuda()
+    want = vqa_amd.log_probs_grad(z, tg, -1.0, 0.2)     # (the same addresses: where a row begins decides which lane adds what)
+    got = vqa_amd.log_probs_grad(z, tg, -1.0, 0.2, out=out)
+    assert torch.equal(got.d_logits, want.d_logits) and torch.equal(got.log_prob, want.log_prob)
+    assert (big[:, 0] == 3).all() and (big[:, V + 1:V + 3] == 3).all() and (big[:, 2 * V + 3:] == 3).all()
+    with pytest.raises(_lib.VqaError):
+        vqa_amd.log_probs_grad(z, tg, -1.0, 0.2, out=big[:, 2:V + 2])
+
+
 def test_expanded_rows_and_one_number_weights():
     import torch
 

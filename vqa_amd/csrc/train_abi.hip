@@ -120,6 +120,13 @@ struct Loss {
     int64_t dz_stride;
     size_t bytes, dz_bytes;
 
+    // rows of one array, the scores in some of its columns and their gradient in others
+    bool side_by_side() const {
+        if (stride != dz_stride) return false;
+        const int64_t d = ((int64_t)((intptr_t)dz - (intptr_t)z) / (int64_t)size_of(dtype) % stride + stride) % stride;
+        return d >= width && stride - d >= width;
+    }
+
     int check() {
         int rc = check_dtype(dtype);
         if (rc) return rc;
@@ -128,7 +135,7 @@ struct Loss {
         if ((rc = check_scale(scale))) return rc;
         if (rows == 0) return VQA_OK;
         if ((log_prob || dlog_prob) && !targets) VQA_FAIL(VQA_EINVAL, "log_prob and dlog_prob need the targets");
-        if (overlap(z, bytes, dz, dz_bytes)) VQA_FAIL(VQA_EINVAL, "dscores must not overlap the scores");
+        if (overlap(z, bytes, dz, dz_bytes) && !side_by_side()) VQA_FAIL(VQA_EINVAL, "dscores must not overlap the scores");
         return VQA_OK;
     }
 };
