@@ -411,8 +411,7 @@ int vqa_class_stats_dev(int device, void* stream, const int64_t* d_counts, const
  * vqa_class_stats_dev reads class frequencies.  No counterpart in the reference.
  *
  * dtype is the scores' type; log probabilities, entropies and their weights are double for VQA_DTYPE_F64 and float for
- * the others, sums are held in that type.  Rows lie row_stride elements apart.  scale in
- * [1e-30, 1e30].
+ * the others, sums are held in that type.  Rows lie row_stride elements apart.  scale in [1e-30, 1e30].
  *   log_prob[r]  log p of outcome targets[r]; 0 for targets[r] < 0 (no outcome given)
  *   entropy[r]   -sum p log p
  *   top_index / top_log_prob [r, top_k]   the outcomes with the largest stored scores, largest first, equal ones by
@@ -420,7 +419,8 @@ int vqa_class_stats_dev(int device, void* stream, const int64_t* d_counts, const
  * A score of -inf masks its outcome (p = 0, never among the top ones; places that find no outcome hold -1 and -inf).
  * A row with every outcome masked: log_prob -inf, entropy 0.  A row that holds a NaN or +inf, or a targets[r] >= width:
  * NaN in the row's outputs, -1 in its top_index.  log_prob (with targets) and entropy may each be NULL.
- * Deterministic; columns behind `width` are not read.
+ * Deterministic (the order of a row's additions depends on the sizes and on where it begins in its 16 bytes); columns
+ * behind `width` are not read.
  * _dev: device pointers, queued on `stream`, not waited for, nothing allocated: workspace is
  * vqa_log_probs_workspace(...) bytes of the caller's device memory (0: may be NULL), not shared with work that may run
  * at the same time.  The calling thread's current device is kept.
