@@ -1281,9 +1281,9 @@ LongWs long_ws(char* base, int batch, int r, int c) {
     w.stride = (w.parts * (nt * (nt + 1) / 2) * tile + nt * nt * tile + (size_t)c * nt * 16) * 8;
     return w;
 }
-// How the products are cut: sides of the tiles of the symmetric ones (X X^T and b A + c A A) and of the update, and into how
-// many parts the sum of X X^T is split.
-struct Cut { int sym, up, splits; };
+// How the products are cut: sides of the tiles of X X^T, of b A + c A A and of the update, and into how many parts the sum of
+// X X^T is split.
+struct Cut { int gram, poly, up, splits; };
 struct Side { int side, splits; };
 
 // The tile and the parts whose rounds of 256 workgroups (one a CU) take least.  In us: what a round takes at its ends, and for
@@ -1292,59 +1292,57 @@ struct Side { int side, splits; };
 //   update      of 4096 x 4096  420 (256) | 504 (128)    of 2048 x 2048  62 (128) | 85 (64)    of 1024 x 4096  37 (128) | 46 (64)
 //   b A + c A A of 3000         148 (128) | 230 (256)    of 2048          53 (128) | 58 (64)    of 1024         12 (64) | 26 (128)
 // and the whole operator with tiles of 32 | 64:  512 x 512  92 | 133,  300 x 300  77 | 105,  1000 x 1000  233 | 196.
-// (Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer: with all
+// (4096 x 4096 bfloat16 with b A + c A A in tiles of 128, as chosen, | 256: 3330 | 3440.  Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer: with all
 // matrix units busy the clock falls, the more the more a product moves besides.)
-// A split sum (few tiles and a long sum: X X^T of a wide matrix) also takes the giving and taking of its parts, 3.5 us and 0.35
+// A split sum (few tiles and a long sum: X X^T of a wide matrix) also takes the giving and taking of its parts, 4.5 us and 0.35
 // a part.  Whole operator, split | not, tiles of 64:  100 x 4000  123 us (8 parts) | 218;  512 x 4096  231 (3) | 306.  Tiles of
 // 128 lose what splitting gains to that (1024 x 4096: 588 us with 5 parts, 449 with tiles of 64 unsplit).
 struct Round { int side; double ends, sum; };
-constexpr Round kRounds32[] = { { 256, 8, 4.6 }, { 128, 5, 1.5 }, { 64, 5, 0.45 }, { 32, 3, 0.33 } }, kRounds64[] = { { 64, 5, 2.1 }, { 32, 1.5, 0.68 } };
+constexpr Round kRounds32[] = { { 256, 8, 4.62 }, { 128, 5, 1.5 }, { 64, 5, 0.45 }, { 32, 3, 0.33 } }, kRounds64[] = { { 64, 5, 2.1 }, { 32, 1.5, 0.68 } };
+constexpr Round kRoundsFew[] = { { 256, 8, 2.05 }, { 128, 5, 0.77 }, { 64, 5, 0.45 }, { 32, 3, 0.33 } };   // X X^T of the high parts alone
 template <int N>
-Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool gram) {
+Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool symmetric, bool split) {
     Side best = { 64, 1 };
     double least = 1e30;
     for (const Round& k : rounds) {
-        const int64_t a = (rows + k.side - 1) / k.side, b = (cols + k.side - 1) / k.side, n = (gram ? a * (a + 1) / 2 : a * b) * batch;
-        auto time = [&](int64_t tiles, int stages) {
-            const double full = k.side == 32 ? std::max(1.0, (double)tiles / 256) : (double)((tiles + 255) / 256);
-            return full * (k.ends + stages * k.sum);
-        };
-        const int stages = (sum + 63) / 64, most = gram && k.side <= 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
-        const double also = gram ? time(n, (rows + 63) / 64) : 0;      // b A + c A A
+        const int64_t a = (rows + k.side - 1) / k.side, b = (cols + k.side - 1) / k.side, n = (symmetric ? a * (a + 1) / 2 : a * b) * batch;
+        const int stages = (sum + 63) / 64, most = split && k.side <= 64 ? (int)std::min<int64_t>(256 / n, stages / 4) : 1;
         for (int p = 1; p <= std::max(1, most); ++p) {
             const int per = (stages + p - 1) / p;
             if ((stages + per - 1) / per != p) continue;   // (the last parts would be empty)
-            const double us = time(n * p, per) + (p > 1 ? 3.5 + p * 0.35 : 0) + also;
+            const double full = k.side == 32 ? std::max(1.0, (double)(n * p) / 256) : (double)((n * p + 255) / 256);
+            const double us = full * (k.ends + per * k.sum) + (p > 1 ? 4.5 + p * 0.35 : 0);
             if (us < least) { least = us; best = { k.side, p }; }
         }
     }
     return best;
 }
 int pad_to(int v, int t) { return (v + t - 1) / t * t; }
-template <int N>
-Cut cut_of(const Round (&rounds)[N], int batch, int r, int c) {
-    const Side gram = side_of(rounds, batch, r, r, c, true);
-    return { gram.side, side_of(rounds, batch, c, r, r, false).side, gram.splits };
+template <int N, int M>
+Cut cut_of(const Round (&gram)[N], const Round (&others)[M], int batch, int r, int c) {
+    const Side x = side_of(gram, batch, r, r, c, true, true);
+    return { x.side, side_of(others, batch, r, r, r, true, false).side, side_of(others, batch, c, r, r, false, false).side, x.splits };
 }
 // whole stages, of which a tile's summed index is made up: what is summed over, and what tiles cover at the least
 int least_pad(int dtype) { return dtype == VQA_DTYPE_F64 ? 32 : 64; }
 Cut cut_of(int dtype, int batch, int r, int c) {
     r = pad_to(r, least_pad(dtype));
     c = pad_to(c, least_pad(dtype));
-    return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, batch, r, c) : cut_of(kRounds32, batch, r, c);
+    return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, kRounds64, batch, r, c) : dtype == VQA_DTYPE_BF16 ? cut_of(kRoundsFew, kRounds32, batch, r, c)
+                                                                             : cut_of(kRounds32, kRounds32, batch, r, c);
 }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 size_t sum_bytes(int rk, Cut t, size_t size) {
-    const size_t a = (rk + t.sym - 1) / t.sym;
-    return a * (a + 1) / 2 * t.splits * t.sym * t.sym * size;
+    const size_t a = (rk + t.gram - 1) / t.gram;
+    return a * (a + 1) / 2 * t.splits * t.gram * t.gram * size;
 }
 template <class M>
 void extents(int r, int c, Cut t, Mats<M>* w) {
     const int least = least_pad(std::is_same_v<M, Wide> ? VQA_DTYPE_F64 : VQA_DTYPE_F32);
     w->rk = pad_to(r, least);
     w->ck = pad_to(c, least);
-    w->rp = pad_to(std::max(pad_to(r, t.sym), pad_to(r, t.up)), kTile);
+    w->rp = pad_to(std::max({ pad_to(r, t.gram), pad_to(r, t.poly), pad_to(r, t.up) }), kTile);
     w->cp = pad_to(pad_to(c, t.up), kTile);
 }
 
@@ -1462,8 +1460,8 @@ int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename
     int rc = VQA_OK;
     for (int s = 0; s < j.steps && !rc; ++s) {
         const int from = s & 1;
-        rc = product<Ty, kGram, kFew>(st, t.sym, j, w, from);
-        if (!rc) rc = product<Ty, kPoly, kFew>(st, t.sym, j, w, from);
+        rc = product<Ty, kGram, kFew>(st, t.gram, j, w, from);
+        if (!rc) rc = product<Ty, kPoly, kFew>(st, t.poly, j, w, from);
         if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate, kFew>(st, t.up, j, w, from) : product<Ty, kLast, kFew>(st, t.up, j, w, from);
     }
     return rc;
