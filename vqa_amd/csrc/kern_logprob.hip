@@ -329,7 +329,7 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // A bound below the k-th best of a wave's first elements, from the lanes' own best mx: k lanes or more reach it.  It keeps
-// the first pieces from inserting each element that is better than those before it (about k log(elements / k) of them).
+// the first pieces from offering each element that is better than those before it (about k log(elements / k) of them).
 template <class A>
 __device__ __forceinline__ A first_bound(A mx, int top_k) {
     if (__popcll(__ballot(mx > neg_inf(A(0)))) < top_k) return neg_inf(A(0));
