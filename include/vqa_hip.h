@@ -473,8 +473,7 @@ int vqa_psr_chain_dev(int device, void* stream, const double* d_expect, int64_t 
  *   A = X X^T,  X <- coefs[0] X + (coefs[1] A + coefs[2] A A) X
  * (on the transpose when rows > cols), which keeps G's singular vectors and carries its singular values towards 1.
  * No counterpart in the reference.  dtype as above; state and sums are double for VQA_DTYPE_F64, else 32 bits or more,
- * or pairs of 16-bit floats that hold as much (for bfloat16 results of more than 64 rows and columns two of the three
- * products of a step take the high parts of X, 11 bits: an error of 1e-3, below the results' own rounding).  Matrix b's element (i, j) is d_g[b * batch_stride + i * row_stride + j];
+ * or pairs of 16-bit floats that hold as much.  Matrix b's element (i, j) is d_g[b * batch_stride + i * row_stride + j];
  * d_out is contiguous and may be d_g where that is contiguous too, but not overlap it otherwise.
  * rows, cols in [1, 65536], batch in [0, 65535], steps in [1, 100], eps >= 1e-300.  coefs that let a singular value
  * exceed 4 within `steps` steps, or the polynomial of A 32, are refused (VQA_EUNSUPPORTED).

@@ -468,3 +468,41 @@ def test_muon_optimizer_trains_the_regressor():
     want = p - 0.02 * np.concatenate([o.reshape(-1), g[24:]])
     want = map_to_pi_range(want, q.optimizer.periodic_para_inds)
     assert np.max(np.abs(path[1] - want)) < 1e-9
+
+
+def before_rounding(got, want):
+    """The Frobenius norm of the least error that takes `want` into what rounds to `got` (16 bits): a result is off by its
+    rounding and by what it was off before, and only the second counts here."""
+    import torch
+
+    bits = got.contiguous().view(torch.int16)
+    mag = bits & 0x7fff
+    value = lambda m: m.view(got.dtype).double()
+    x, up, down = value(mag), value(mag + 1), value((mag - 1).clamp(min=0))
+    w = torch.where(bits < 0, -want, want)
+    high = (x + up) / 2
+    low = torch.where(mag == 0, -high, (x + down) / 2)
+    return torch.linalg.vector_norm(torch.maximum(w - high, low - w).clamp(min=0), dim=(-2, -1))
+
+
+@pytest.mark.parametrize("t", ["bfloat16", "float16"])
+@pytest.mark.parametrize("batch,rows,cols", [(2, 11, 36), (2, 40, 60), (2, 20, 600), (3, 80, 70), (1, 300, 300), (1, 100, 4000), (1, 1024, 4096), (1, 2048, 1500),
+                                             (1, 2000, 2111), (1, 4096, 4096)])
+def test_results_of_16_bits_are_rounded_once(t, batch, rows, cols):
+    """what a 16-bit result is off before its rounding is held to what a 32-bit result may be off, whatever its size and tiles"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows + cols)
+    k = max(1, min(rows, cols) // 8)
+    g = (torch.randn(batch, rows, k, generator=gen, device="cuda") @ torch.randn(batch, k, cols, generator=gen, device="cuda") / math.sqrt(k)
+         + 0.5 * torch.randn(batch, rows, cols, generator=gen, device="cuda")).to(getattr(torch, t))
+    o = vqa_amd.orthogonalize(g)
+    want = plain(g, torch.float64)
+    r, c = sorted((rows, cols))
+    norm = torch.linalg.vector_norm(want, dim=(1, 2))
+    poff = torch.linalg.vector_norm(plain(g, torch.float32).double() - want, dim=(1, 2))
+    tol = torch.minimum(torch.full_like(norm, bound(t, r, c)), 4 * poff + UNIT[t] * math.sqrt(c + 2 * r) * norm * 4)
+    off = before_rounding(o, want)
+    assert torch.isfinite(o).all() and (off <= tol).all(), (off / norm, tol / norm)
+    for _ in range(3):
+        assert torch.equal(vqa_amd.orthogonalize(g), o)

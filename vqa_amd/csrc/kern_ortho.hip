@@ -888,16 +888,6 @@ template <> struct Shape<float, 256> { static constexpr int WI = 2, WJ = 4, KG =
 template <> struct Shape<double, 64> { static constexpr int WI = 2, WJ = 2, KG = 2, BK = 32, S = 2; };
 template <> struct Shape<double, 32> { static constexpr int WI = 1, WJ = 1, KG = 4, BK = 32, S = 2; };
 
-// Which parts of the operands a product takes.  Results of 8 bits (bfloat16, without an optimizer state) take the high parts
-// of X alone, 11 bits: X X^T from hi hi, b A + c A A from all, B X from hi hi + lo hi.  Errors beside the result's own
-// rounding, 1.66e-3 of its norm: 0.9e-3 (512 x 512, low rank and noise) to 1.0e-3 (100 x 4000); with the high parts of B alone
-// they reach 1.8e-3, with those of A in A A 3.5e-3.
-template <class Ty, Kind kind, bool kFew>
-struct Parts {
-    static constexpr bool kWide = sizeof(typename Ty::C) == 8;
-    static constexpr int P = kWide ? 1 : kFew && kind != kPoly ? 1 : 2, Q = kWide ? 1 : kFew && kind == kGram ? 1 : 2;
-};
-
 template <class C> struct Frag;   // what a wave reads of one 32-row (16 for 64 bits) block at once, and its products
 template <> struct Frag<float> {
     using M = Pair;
@@ -912,14 +902,16 @@ template <> struct Frag<double> {
     static __device__ __forceinline__ int row(int lane, int q) { return Mma<double>::row(lane, q); }
 };
 
-// NP, NQ: parts of P and Q that are multiplied (16-bit pairs: 1 or 2)
-template <class C, int T, int NP, int NQ>
+// All parts of a value are multiplied, also where the result has 16 bits: without the low parts of X (11 bits) a bfloat16 result
+// of 4096 x 4096 is off by 1.0e-3 of its norm before it is rounded, with them by 1e-6.
+template <class C, int T>
 struct Tile : Shape<C, T> {
     using Sh = Shape<C, T>;
     using Fr = Frag<C>;
     using M = typename Fr::M;
     static constexpr int WI = Sh::WI, WJ = Sh::WJ, KG = Sh::KG, BK = Sh::BK;
-    static constexpr int kArrays = NP + NQ, S = Sh::S * (sizeof(C) == 4 ? 4 : 2) / kArrays;   // fewer parts leave room for more stages
+    static constexpr int NP = sizeof(C) == 4 ? 2 : 1, NQ = NP;         // parts of a value (16-bit pairs: 2)
+    static constexpr int kArrays = NP + NQ, S = Sh::S;
     static constexpr int kWv = WI * WJ * KG, kThreads = 64 * kWv;
     static constexpr int kSize = sizeof(C) == 8 ? 8 : 2;              // of a stored value
     static constexpr int Q = BK * kSize / 16;                         // pieces of a row
@@ -992,9 +984,9 @@ struct Tile : Shape<C, T> {
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pv[i][x], qv[j][y], acc[i][j], 0, 0, 0);
                 };
-                if constexpr (NP == 2) go(1, 0);     // lo hi
-                if constexpr (NQ == 2) go(0, 1);     // hi lo
-                go(0, 0);                            // hi hi
+                go(1, 0);     // lo hi
+                go(0, 1);     // hi lo
+                go(0, 0);     // hi hi
             }
         } else {
             // a lane's piece holds two neighbours of the summed index; the first ones of the four pieces make one matrix
@@ -1150,13 +1142,12 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned*
 
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
-// Time of X X^T | b A + c A A | update, us:  4096 x 4096 bfloat16  139 | 300 | 271, the three products of the second at 1.03
-// PFLOP/s with the clock down to 1.97 GHz from heat (the library's product of 16-bit floats of this size: 1.26);  2048 x 2048
+// Time of X X^T | b A + c A A | update, us:  2048 x 2048
 // float32  54 | 54 | 64;  1000 x 777  10 | 8 | 12 (with tiles of 64 12 | 10 | 12): bound by the 3 to 5 us that a launch, the way
 // of the first stage, the epilogue and the last stores take;  1024 x 4096 float32  34 | 12 | 40: 136 tiles for 256 CUs, and an update that writes 34 MB in one
 // round, after its products.
-template <class Ty, Kind kind, int T, bool kFew>
-__global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
+template <class Ty, Kind kind, int T>
+__global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
     using C = typename Ty::C;
     constexpr bool kSym = kind == kGram || kind == kPoly;
     extern __shared__ __attribute__((aligned(16))) char product_lds[];
@@ -1171,7 +1162,7 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, 
     }
     const size_t i0 = ti * T, j0 = tj * T;
     const auto a = w.a.at(off), bm = w.b.at(off);
-    using Tl = Tile<C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>;
+    using Tl = Tile<C, T>;
     Tl t;
     constexpr int N = Tl::N;
     if (kind == kGram || kind == kPoly) {
@@ -1292,14 +1283,12 @@ struct Side { int side, splits; };
 //   update      of 4096 x 4096  420 (256) | 504 (128)    of 2048 x 2048  62 (128) | 85 (64)    of 1024 x 4096  37 (128) | 46 (64)
 //   b A + c A A of 3000         148 (128) | 230 (256)    of 2048          53 (128) | 58 (64)    of 1024         12 (64) | 26 (128)
 // and the whole operator with tiles of 32 | 64:  512 x 512  92 | 133,  300 x 300  77 | 105,  1000 x 1000  233 | 196.
-// (4096 x 4096 bfloat16 with b A + c A A in tiles of 128, as chosen, | 256: 3330 | 3440.  Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer: with all
-// matrix units busy the clock falls, the more the more a product moves besides.)
+// (Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer.)
 // A split sum (few tiles and a long sum: X X^T of a wide matrix) also takes the giving and taking of its parts, 4.5 us and 0.35
 // a part.  Whole operator, split | not, tiles of 64:  100 x 4000  123 us (8 parts) | 218;  512 x 4096  231 (3) | 306.  Tiles of
 // 128 lose what splitting gains to that (1024 x 4096: 588 us with 5 parts, 449 with tiles of 64 unsplit).
 struct Round { int side; double ends, sum; };
 constexpr Round kRounds32[] = { { 256, 8, 4.62 }, { 128, 5, 1.5 }, { 64, 5, 0.45 }, { 32, 3, 0.33 } }, kRounds64[] = { { 64, 5, 2.1 }, { 32, 1.5, 0.68 } };
-constexpr Round kRoundsFew[] = { { 256, 8, 2.05 }, { 128, 5, 0.77 }, { 64, 5, 0.45 }, { 32, 3, 0.33 } };   // X X^T of the high parts alone
 template <int N>
 Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int sum, bool symmetric, bool split) {
     Side best = { 64, 1 };
@@ -1318,18 +1307,17 @@ Side side_of(const Round (&rounds)[N], int64_t batch, int rows, int cols, int su
     return best;
 }
 int pad_to(int v, int t) { return (v + t - 1) / t * t; }
-template <int N, int M>
-Cut cut_of(const Round (&gram)[N], const Round (&others)[M], int batch, int r, int c) {
-    const Side x = side_of(gram, batch, r, r, c, true, true);
-    return { x.side, side_of(others, batch, r, r, r, true, false).side, side_of(others, batch, c, r, r, false, false).side, x.splits };
+template <int N>
+Cut cut_of(const Round (&rounds)[N], int batch, int r, int c) {
+    const Side x = side_of(rounds, batch, r, r, c, true, true);
+    return { x.side, side_of(rounds, batch, r, r, r, true, false).side, side_of(rounds, batch, c, r, r, false, false).side, x.splits };
 }
 // whole stages, of which a tile's summed index is made up: what is summed over, and what tiles cover at the least
 int least_pad(int dtype) { return dtype == VQA_DTYPE_F64 ? 32 : 64; }
 Cut cut_of(int dtype, int batch, int r, int c) {
     r = pad_to(r, least_pad(dtype));
     c = pad_to(c, least_pad(dtype));
-    return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, kRounds64, batch, r, c) : dtype == VQA_DTYPE_BF16 ? cut_of(kRoundsFew, kRounds32, batch, r, c)
-                                                                             : cut_of(kRounds32, kRounds32, batch, r, c);
+    return dtype == VQA_DTYPE_F64 ? cut_of(kRounds64, batch, r, c) : cut_of(kRounds32, batch, r, c);
 }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -1434,35 +1422,35 @@ int block(hipStream_t st, const Job<Ty>& j) {
     return VQA_OK;
 }
 
-template <class Ty, Kind kind, int T, bool kFew>
+template <class Ty, Kind kind, int T>
 int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
-    using Tl = Tile<typename Ty::C, T, Parts<Ty, kind, kFew>::P, Parts<Ty, kind, kFew>::Q>;
-    if (int rc = allow_lds<k_ns_product<Ty, kind, T, kFew>>(Tl::kBytes)) return rc;
-    hipLaunchKernelGGL((k_ns_product<Ty, kind, T, kFew>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
+    using Tl = Tile<typename Ty::C, T>;
+    if (int rc = allow_lds<k_ns_product<Ty, kind, T>>(Tl::kBytes)) return rc;
+    hipLaunchKernelGGL((k_ns_product<Ty, kind, T>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
     return VQA_OK;
 }
 
-template <class Ty, Kind kind, bool kFew>
+template <class Ty, Kind kind>
 int product(hipStream_t st, int tile, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
     const unsigned tr = (w.rk + tile - 1) / tile, tc = (w.ck + tile - 1) / tile;   // (all that is summed over is written)
     const dim3 grid = kind == kGram || kind == kPoly ? dim3(tr * (tr + 1) / 2 * (kind == kGram ? w.splits : 1), 1, (unsigned)j.batch) : dim3(tr, tc, (unsigned)j.batch);
     if constexpr (sizeof(typename Ty::C) == 4) {
-        if (tile == 256) return product<Ty, kind, 256, kFew>(st, grid, j, w, from);
-        if (tile == 128) return product<Ty, kind, 128, kFew>(st, grid, j, w, from);
+        if (tile == 256) return product<Ty, kind, 256>(st, grid, j, w, from);
+        if (tile == 128) return product<Ty, kind, 128>(st, grid, j, w, from);
     }
-    if (tile == 32) return product<Ty, kind, 32, false>(st, grid, j, w, from);
+    if (tile == 32) return product<Ty, kind, 32>(st, grid, j, w, from);
     if (tile != 64) VQA_FAIL(VQA_EINVAL, "no tile of %d", tile);
-    return product<Ty, kind, 64, false>(st, grid, j, w, from);   // (32 and 64: bound by other things than their products)
+    return product<Ty, kind, 64>(st, grid, j, w, from);
 }
 
-template <class Ty, bool kFew>
+template <class Ty>
 int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, Cut t) {
     int rc = VQA_OK;
     for (int s = 0; s < j.steps && !rc; ++s) {
         const int from = s & 1;
-        rc = product<Ty, kGram, kFew>(st, t.gram, j, w, from);
-        if (!rc) rc = product<Ty, kPoly, kFew>(st, t.poly, j, w, from);
-        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate, kFew>(st, t.up, j, w, from) : product<Ty, kLast, kFew>(st, t.up, j, w, from);
+        rc = product<Ty, kGram>(st, t.gram, j, w, from);
+        if (!rc) rc = product<Ty, kPoly>(st, t.poly, j, w, from);
+        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate>(st, t.up, j, w, from) : product<Ty, kLast>(st, t.up, j, w, from);
     }
     return rc;
 }
@@ -1521,10 +1509,7 @@ int run(hipStream_t st, const OrthoCall& q) {
     const int parts = std::min(kNormParts, j.rows * pieces);
     hipLaunchKernelGGL((k_ns_norm<Ty>), dim3(parts, nb), dim3(kT), 0, st, j, w.part, w.stride, pieces);
     hipLaunchKernelGGL((k_ns_enter<Ty>), dim3(w.cp / kTile, w.rp / kTile, nb), dim3(kT), 0, st, j, w, parts);
-    int rc;
-    if constexpr (std::is_same_v<Ty, BF16>) rc = j.m ? steps<Ty, false>(st, j, w, cut) : steps<Ty, true>(st, j, w, cut);
-    else rc = steps<Ty, false>(st, j, w, cut);
-    if (rc) return rc;
+    if (const int rc = steps(st, j, w, cut)) return rc;
     VQA_HIP(hipGetLastError());
     return VQA_OK;
 }
