@@ -506,3 +506,57 @@ def test_results_of_16_bits_are_rounded_once(t, batch, rows, cols):
     assert torch.isfinite(o).all() and (off <= tol).all(), (off / norm, tol / norm)
     for _ in range(3):
         assert torch.equal(vqa_amd.orthogonalize(g), o)
+
+
+def of_norm(gen, batch, rows, cols, norm):
+    import torch
+
+    k = max(1, min(rows, cols) // 8)
+    g = (torch.randn(batch, rows, k, generator=gen, device="cuda", dtype=torch.float64) @ torch.randn(batch, k, cols, generator=gen, device="cuda", dtype=torch.float64)
+         / math.sqrt(k) + 0.5 * torch.randn(batch, rows, cols, generator=gen, device="cuda", dtype=torch.float64))
+    return g / torch.linalg.vector_norm(g, dim=(1, 2), keepdim=True) * norm
+
+
+@pytest.mark.parametrize("rows,cols", [(11, 36), (40, 60), (20, 600), (80, 70), (300, 300), (100, 4000), (2000, 1500)])
+@pytest.mark.parametrize("steps", [1, 5, 16])
+def test_norms_far_below_eps(rows, cols, steps):
+    """X = G / (|G| + eps) is then small itself, and stays so for many steps: relative to the result's own norm it is as exact as
+    32-bit products are (a batch of all sizes of norm, each matrix for itself)"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows + cols + steps)
+    norms = [1.0, 3e-7, 1e-7, 1e-9, 1e-11, 1e-13, 1e-16, 1e-22, 1e-27]
+    g64 = of_norm(gen, len(norms), rows, cols, torch.tensor(norms, device="cuda", dtype=torch.float64)[:, None, None])
+    for t in ("float32", "bfloat16"):
+        g = g64.to(getattr(torch, t))
+        o = vqa_amd.orthogonalize(g, steps=steps)
+        want, p = plain(g, torch.float64, steps), plain(g, torch.float32, steps)
+        r, c = sorted((rows, cols))
+        norm = torch.linalg.vector_norm(want, dim=(1, 2))
+        off = torch.linalg.vector_norm(o.double() - want, dim=(1, 2)) if t == "float32" else before_rounding(o, want)
+        tol = 4 * torch.linalg.vector_norm(p.double() - want, dim=(1, 2)) + UNIT[t] * math.sqrt(c + 2 * r) * norm * 4
+        assert torch.isfinite(o).all() and (off <= tol).all(), (t, off / norm, tol / norm)
+        for b in range(len(norms)):
+            assert (off[b] <= tol[b]) and norm[b] > 0
+
+
+@pytest.mark.parametrize("rows,cols,eps", [(80, 70, 1.0), (80, 70, 1e4), (300, 200, 1e9), (1100, 1000, 1e30)])
+def test_eps_far_above_the_norm(rows, cols, eps):
+    """the same by way of eps, with float16 as well; weights that take the step, and a matrix of zeros"""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    g64 = of_norm(gen, 3, rows, cols, 1.0)
+    g64[1] = 0
+    r, c = sorted((rows, cols))
+    for t in ("float32", "float16"):
+        g = g64.to(getattr(torch, t))
+        m, w = torch.zeros(3, rows, cols, device="cuda"), torch.zeros(3, rows, cols, device="cuda")
+        vqa_amd.muon_step(w, g, m, 1.0, 0.0, eps=eps)        # momentum and update are g itself, w becomes -rate * result
+        want, p = plain(g, torch.float64, eps=eps), plain(g, torch.float32, eps=eps)
+        rate = math.sqrt(max(1.0, rows / cols))
+        off = torch.linalg.vector_norm(-w.double() / rate - want, dim=(1, 2))
+        norm = torch.linalg.vector_norm(want, dim=(1, 2))
+        # (the rate is rounded and multiplied: a step of each value)
+        tol = 4 * torch.linalg.vector_norm(p.double() - want, dim=(1, 2)) + UNIT[t] * (math.sqrt(c + 2 * r) * 4 + 2) * norm
+        assert (w[1] == 0).all() and (off <= tol).all(), (t, off / norm, tol / norm)

@@ -12,7 +12,7 @@
 // * r <= 64, long rows: the steps on X X^T alone, between two passes over the matrix (k_ns_gram, k_ns_poly, k_ns_apply).
 // * else: three tiled products a step (k_ns_product), X, X^T, A and b A + c A A in device memory, all row-major with the
 //   summed index contiguous, padded to whole tiles.  64-bit matrices use 64-bit matrix instructions; the others hold every
-//   value as a sum of two 16-bit floats hi + lo (22 bits and a sign, scaled so that neither part leaves its normal range) and
+//   value as a sum of two 16-bit floats hi + lo (22 bits and a sign, scaled by powers of two that follow X's size) and
 //   take the three products hi hi + hi lo + lo hi with 32-bit sums: the left-out lo lo is 2^-22 of a product, the size of
 //   the roundings that 32-bit products make along a sum, at 5 times their rate.
 #include <math.h>
@@ -703,7 +703,12 @@ constexpr int kMaxCount = 128;        // tiles of a product whose sum is split: 
 
 // Scales of the 16-bit pairs (powers of two).  Entries of X are at most the largest singular value, below 4 by the
 // caller's check, and 1 / sqrt(r c) at the start; of A below 16; of b A + c A A below 32.
+// Where |G| is far below eps, X starts small and grows by about |a| a step: it is held as 2^k X, and A and b A + c A A as
+// 4^k times themselves, k of each matrix and step such that 2^k |X| <= 1 (b + c, so 4^k |b A + c A A|, at most 32 by the
+// caller's check).  k = 0 from |X| = 1 / 2 on, which is where a matrix far above eps starts.
 constexpr float kSX = 4096.f, kSA = 1024.f, kSB = 1024.f;
+constexpr int kMostSteps = 100, kMostLift = 110;      // (2^-110 is left in the last product: its values stay normal numbers)
+__device__ __forceinline__ int lift_of(float size) { return min(kMostLift, max(0, -1 - ilogbf(fmaxf(size, 1e-36f)))); }
 
 // values of a padded matrix: 64-bit, or a 16-bit pair in two arrays
 struct Pair {
@@ -788,6 +793,7 @@ struct Mats {
     double* part;     // of the norm
     void* sum;        // X X^T in parts: [tile][part][T x T], in C
     unsigned* count;  // parts of a tile that are there (0 between the kernels)
+    int* lift;        // of 16-bit pairs: k of each step's X, and 0 for the result
     int splits;
     size_t stride;    // bytes to the next matrix of the batch
     // rows of X (and its columns) as they are stored, and as the products sum over them (r and c to whole stages).  Rows from
@@ -817,7 +823,7 @@ __global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t 
     if (threadIdx.x == 0) ((double*)((char*)part + b * stride))[blockIdx.x] = ss;
 }
 
-// X0 and its transpose, a tile a workgroup.  4096 x 4096 bfloat16: 39 us = 4.3 TB/s of the reading and of the four arrays written.
+// X0 and its transpose, a tile a workgroup, and the scales of the steps.  4096 x 4096 bfloat16: 39 us = 4.3 TB/s of the reading and of the four arrays written.
 template <class Ty>
 __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int norm_parts) {
     using C = typename Ty::C;
@@ -826,8 +832,24 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
     const int b = blockIdx.z;
     const size_t off = b * w.stride;
     const double* part = (const double*)((char*)w.part + off);
-    const double norm = size_of_matrix(block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh), j.eps);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kMaxCount) ((unsigned*)((char*)w.count + off))[threadIdx.x] = 0;
+    const double squares = block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh), norm = size_of_matrix(squares, j.eps);
+    const bool one = blockIdx.x == 0 && blockIdx.y == 0;      // of the matrix's workgroups
+    if (one && threadIdx.x < kMaxCount) ((unsigned*)((char*)w.count + off))[threadIdx.x] = 0;
+    double scale = 1.0;
+    if constexpr (sizeof(C) == 4) {
+        float size = (float)(sqrt(squares) / norm);           // |X|, NaN with the norm
+        const int first = lift_of(size);
+        scale = ldexp(1.0, first);
+        if (one && threadIdx.x == 0) {
+            int* lift = (int*)((char*)w.lift + off);
+            lift[0] = first;
+            for (int s = 1; s <= j.steps; ++s) {              // (a singular value grows by |a + b y + c y^2| at most, and to 4)
+                const float y = size * size;
+                size = fminf(4.f, 1.01f * size * (fabsf(j.ka) + y * (fabsf(j.kb) + y * fabsf(j.kc))));
+                lift[s] = s < j.steps ? lift_of(size) : 0;
+            }
+        }
+    }
     // rows and columns of the caller's matrix
     const int64_t r0 = (int64_t)(j.turned ? blockIdx.x : blockIdx.y) * kTile, c0 = (int64_t)(j.turned ? blockIdx.y : blockIdx.x) * kTile;
     constexpr int U = kTile * kTile / kT;
@@ -839,7 +861,7 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
         return row < j.rows && col < j.cols;
     });
 #pragma unroll
-    for (int u = 0; u < U; ++u) tile[(threadIdx.x + u * kT) / kTile][threadIdx.x % kTile] = (C)((double)v[u] / norm);
+    for (int u = 0; u < U; ++u) tile[(threadIdx.x + u * kT) / kTile][threadIdx.x % kTile] = (C)((double)v[u] / norm * scale);
     __syncthreads();
     const auto xm = w.x[0].at(off), xt = w.xt[0].at(off);
     const size_t x0 = (size_t)blockIdx.y * kTile, y0 = (size_t)blockIdx.x * kTile;   // row and column of X
@@ -1147,8 +1169,9 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned*
 // of the first stage, the epilogue and the last stores take;  1024 x 4096 float32  34 | 12 | 40: 136 tiles for 256 CUs, and an update that writes 34 MB in one
 // round, after its products.
 template <class Ty, Kind kind, int T>
-__global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int from) {
+__global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int step) {
     using C = typename Ty::C;
+    const int from = step & 1;
     constexpr bool kSym = kind == kGram || kind == kPoly;
     extern __shared__ __attribute__((aligned(16))) char product_lds[];
     const size_t off = blockIdx.z * w.stride;
@@ -1165,10 +1188,17 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
     using Tl = Tile<C, T>;
     Tl t;
     constexpr int N = Tl::N;
+    int lift = 0, next = 0;
+    if constexpr (sizeof(C) == 4 && kind != kGram) {
+        const int* of = (const int*)((const char*)w.lift + off) + step;
+        lift = of[0];
+        next = of[1];
+    }
+    const C square = sizeof(C) == 4 ? (C)ldexpf(1.f, -2 * lift) : C(1);     // (0 where b A + c A A is nothing beside a)
     if (kind == kGram || kind == kPoly) {
         const auto m = (kind == kGram ? w.x[from] : w.a).at(off), out = kind == kGram ? a : bm;
         const float so = kind == kGram ? kSA : kSB;
-        const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA));
+        const C f = sizeof(C) == 8 ? C(1) : kind == kGram ? C(1.f / (kSX * kSX)) : C(1.f / (kSA * kSA)) * square;
         if constexpr (kind == kGram && T <= 64) {
             if (w.splits > 1) {
                 const int per = ((w.ck + 63) / 64 + w.splits - 1) / w.splits * 64, k0 = split * per;
@@ -1224,7 +1254,7 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
     } else {
         const auto xt = w.xt[from].at(off), nx = w.x[from ^ 1].at(off), nt = w.xt[from ^ 1].at(off);
         t.run(xt, bm, i0, j0, w.rp, 0, w.rk, product_lds);   // rows: columns of X; columns: rows of X
-        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB));
+        const C f = sizeof(C) == 8 ? C(1) : C(1.f / (kSX * kSB)) * square, grow = sizeof(C) == 4 ? (C)ldexpf(1.f, next - lift) : C(1);
         t.leave(product_lds,
             [&](int y, int x) { return xt.template get<N>((i0 + y) * w.rp + j0 + x); },
             [&](int y, int x, const auto& raw, C* v) {
@@ -1232,7 +1262,7 @@ __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_prod
                 C xv[N];
                 raw.values(kSX, xv);
 #pragma unroll
-                for (int n = 0; n < N; ++n) v[n] = j.ka * xv[n] + f * v[n];
+                for (int n = 0; n < N; ++n) v[n] = (j.ka * xv[n] + f * v[n]) * grow;
                 if (kind == kUpdate) nt.template put<N>(at, v, kSX);
                 else if (j.turned)
                     j.template leave_run<N>(blockIdx.z, v, (int)i0 + y, (int)j0 + x);
@@ -1352,6 +1382,8 @@ size_t lay_out<Pair>(char* base, int r, int c, Cut t, Mats<Pair>* w) {
     p += kNormParts * 8;
     w->count = (unsigned*)p;
     p += kMaxCount * 4;
+    w->lift = (int*)p;
+    p += up256((kMostSteps + 1) * 4);
     w->sum = p;
     w->splits = t.splits;
     if (t.splits > 1) p += sum_bytes(w->rk, t, 4);
@@ -1373,6 +1405,7 @@ size_t lay_out<Wide>(char* base, int r, int c, Cut t, Mats<Wide>* w) {
     p += kNormParts * 8;
     w->count = (unsigned*)p;
     p += kMaxCount * 4;
+    w->lift = nullptr;
     w->sum = p;
     w->splits = t.splits;
     if (t.splits > 1) p += sum_bytes(w->rk, t, 8);
@@ -1423,34 +1456,33 @@ int block(hipStream_t st, const Job<Ty>& j) {
 }
 
 template <class Ty, Kind kind, int T>
-int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
+int product(hipStream_t st, dim3 grid, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int step) {
     using Tl = Tile<typename Ty::C, T>;
     if (int rc = allow_lds<k_ns_product<Ty, kind, T>>(Tl::kBytes)) return rc;
-    hipLaunchKernelGGL((k_ns_product<Ty, kind, T>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, from);
+    hipLaunchKernelGGL((k_ns_product<Ty, kind, T>), grid, dim3(Tl::kThreads), Tl::kBytes, st, j, w, step);
     return VQA_OK;
 }
 
 template <class Ty, Kind kind>
-int product(hipStream_t st, int tile, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int from) {
+int product(hipStream_t st, int tile, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, int step) {
     const unsigned tr = (w.rk + tile - 1) / tile, tc = (w.ck + tile - 1) / tile;   // (all that is summed over is written)
     const dim3 grid = kind == kGram || kind == kPoly ? dim3(tr * (tr + 1) / 2 * (kind == kGram ? w.splits : 1), 1, (unsigned)j.batch) : dim3(tr, tc, (unsigned)j.batch);
     if constexpr (sizeof(typename Ty::C) == 4) {
-        if (tile == 256) return product<Ty, kind, 256>(st, grid, j, w, from);
-        if (tile == 128) return product<Ty, kind, 128>(st, grid, j, w, from);
+        if (tile == 256) return product<Ty, kind, 256>(st, grid, j, w, step);
+        if (tile == 128) return product<Ty, kind, 128>(st, grid, j, w, step);
     }
-    if (tile == 32) return product<Ty, kind, 32>(st, grid, j, w, from);
+    if (tile == 32) return product<Ty, kind, 32>(st, grid, j, w, step);
     if (tile != 64) VQA_FAIL(VQA_EINVAL, "no tile of %d", tile);
-    return product<Ty, kind, 64>(st, grid, j, w, from);
+    return product<Ty, kind, 64>(st, grid, j, w, step);
 }
 
 template <class Ty>
 int steps(hipStream_t st, const Job<Ty>& j, const Mats<typename StoreOf<typename Ty::C>::T>& w, Cut t) {
     int rc = VQA_OK;
     for (int s = 0; s < j.steps && !rc; ++s) {
-        const int from = s & 1;
-        rc = product<Ty, kGram>(st, t.gram, j, w, from);
-        if (!rc) rc = product<Ty, kPoly>(st, t.poly, j, w, from);
-        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate>(st, t.up, j, w, from) : product<Ty, kLast>(st, t.up, j, w, from);
+        rc = product<Ty, kGram>(st, t.gram, j, w, s);
+        if (!rc) rc = product<Ty, kPoly>(st, t.poly, j, w, s);
+        if (!rc) rc = s + 1 < j.steps ? product<Ty, kUpdate>(st, t.up, j, w, s) : product<Ty, kLast>(st, t.up, j, w, s);
     }
     return rc;
 }
@@ -1501,6 +1533,7 @@ int run(hipStream_t st, const OrthoCall& q) {
         VQA_HIP(hipGetLastError());
         return VQA_OK;
     }
+    if (q.steps > kMostSteps) VQA_FAIL(VQA_EINVAL, "more than %d steps", kMostSteps);
     Mats<typename StoreOf<C>::T> w;
     const Cut cut = cut_of(q.dtype, q.batch, j.r, j.c);
     lay_out((char*)q.workspace, j.r, j.c, cut, &w);
