@@ -613,3 +613,27 @@ def test_strided_scores_of_a_sweep_are_read_in_place():
     a = vqa_amd.log_probs_grad(E[:, 0], torch.zeros(10, dtype=torch.int32).cuda(), 1.0)
     b = vqa_amd.log_probs_grad(E[:, 0].contiguous(), torch.zeros(10, dtype=torch.int32).cuda(), 1.0)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dt", ["uint8", "int8", "int16", "int64", "uint16", "uint32", "uint64"])
+@pytest.mark.parametrize("V", [3, 100, 200, 1000, 40000])
+def test_targets_of_every_integer_type(dt, V):
+    """narrow types that hold neither -1 nor the width give what int32 targets give, on the GPU and from the host"""
+    import torch
+
+    z = scores(np.random.default_rng(V), 40, V, "float32", masked=0.0)
+    most = min(V, np.iinfo(dt).max + 1)
+    tg = np.arange(40) * (most - 1) // 39
+    if dt[0] == "i":
+        tg[::7] = -1
+    want = vqa_amd.log_probs(z, torch.from_numpy(tg.astype(np.int32)).cuda(), top_k=2)
+    assert torch.isfinite(want.log_prob).all()
+    t = torch.from_numpy(tg.astype(dt)).cuda()
+    got, host = vqa_amd.log_probs(z, t, top_k=2), vqa_amd.log_probs(z.cpu().numpy(), tg.astype(dt), top_k=2)
+    assert all(torch.equal(a, b) and np.array_equal(a.cpu().numpy(), c) for a, b, c in zip(want, got, host))
+    a, b = vqa_amd.log_probs_grad(z, torch.from_numpy(tg.astype(np.int32)).cuda(), -1.0), vqa_amd.log_probs_grad(z, t, -1.0)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    if dt == "uint64":
+        tg = np.full(40, 2 ** 63 + 5, np.uint64)
+        far = vqa_amd.log_probs(z, torch.from_numpy(tg).cuda())
+        assert torch.isnan(far.log_prob).all() and np.isnan(vqa_amd.log_probs(z.cpu().numpy(), tg).log_prob).all()

@@ -93,7 +93,10 @@ def _targets(targets, z):
     if t.device != z.device:
         raise ValueError("targets must be on the scores' device")
     if t.dtype != torch.int32:
-        t = t.clamp(-1, width).to(torch.int32)
+        wide = t.to(torch.int64)                  # (their own type may hold neither -1 nor the width)
+        if t.dtype == torch.uint64:
+            wide = torch.where(wide < 0, width, wide)                 # from 2^63 on
+        t = wide.clamp(-1, width).to(torch.int32)
     return t.contiguous()
 
 
