@@ -166,3 +166,56 @@ def test_muon_needs_a_matrix():
     Target.n_c_params = 24
     o = vqa_amd.optimizers.get_optimizer_class("Muon")({}, dict(target_obj=Target(), init_params=np.zeros(25)))
     assert o._shape() == (2, 12)
+
+
+@pytest.mark.parametrize("builder,angles", [("create_jerbi_ansatz", 3), ("create_ibm_HEA_ansatz", 3), ("create_ry_rz_cz_ansatz", 2), ("create_ry_cz_ansatz", 1)])
+@pytest.mark.parametrize("n_qubits", [2, 3, 4])
+def test_the_default_matrix_has_a_row_a_layer(builder, angles, n_qubits):
+    """for every shipped builder and depth, also where the number of angles would go into layers of three a qubit"""
+    from vqa_amd import qml_utils
+
+    class Target:
+        shots_counter = call_counter = circuit_counter = epoch_counter = [0]
+        methods_for_optimization = {}
+
+    for depth in range(9):
+        Target.n_qubits, Target.circuit = n_qubits, getattr(qml_utils, builder)(n_qubits, depth)
+        Target.n_c_params = Target.circuit.n_theta
+        for more in (0, 1):                      # the regressor's scale stands behind them
+            o = vqa_amd.optimizers.Muon({}, dict(target_obj=Target(), init_params=np.zeros(Target.n_c_params + more)))
+            assert o._shape() == (depth + 1, angles * n_qubits), depth
+
+
+def test_a_circuit_without_layers_needs_matrix_shape():
+    """gates that repeat nothing form no matrix, whatever their number; a shared angle counts where it first turns"""
+    from vqa_amd.circuit import GateList
+
+    class Target:
+        n_qubits = 2
+        shots_counter = call_counter = circuit_counter = epoch_counter = [0]
+        methods_for_optimization = {}
+
+    def made(gates, shared=()):
+        c = GateList(2)
+        for kind, q in gates:
+            getattr(c, f"add_parametric_R{kind}_gate")(q, 0.1)
+        for p in shared:
+            c.add_parametric_RX_gate(0, 0.0, share_with=p)
+        Target.circuit, Target.n_c_params = c, c.n_theta
+        return vqa_amd.optimizers.Muon({}, dict(target_obj=Target(), init_params=np.zeros(c.n_theta)))._shape()
+
+    with pytest.raises(ValueError, match="matrix_shape"):
+        made([("X", 0), ("Y", 0), ("Z", 0), ("X", 1), ("Y", 0), ("Z", 0)])       # 6 angles on 2 qubits
+    with pytest.raises(ValueError, match="matrix_shape"):
+        made([("X", 0)] * 6)                                                     # one qubit of two
+    assert made([("X", 0), ("X", 1)] * 3) == (3, 2)
+    assert made([("X", 0), ("X", 1)] * 3, shared=[0, 2]) == (3, 2)
+    assert made([(k, q) for q in (0, 1) for k in "YZY"]) == (1, 6)               # one layer, every qubit turned as often
+    assert made([(k, q) for q in (0, 1) for k in "YZY"] * 2) == (2, 6)
+
+    class Other:                                                                 # a circuit whose gates cannot be read
+        pass
+
+    Target.circuit, Target.n_c_params = Other(), 6
+    with pytest.raises(ValueError, match="matrix_shape"):
+        vqa_amd.optimizers.Muon({}, dict(target_obj=Target(), init_params=np.zeros(6)))

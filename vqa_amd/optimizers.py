@@ -238,13 +238,36 @@ class SGDM(MiniBatchOptimizer):
         return params - self.LR_t * self.m_t
 
 
+def _layer_of(circuit, n_params):
+    """How many angles a layer of the circuit has: the fewest after which its trainable gates (kind and qubit, where an angle
+    turns first) repeat, each qubit among them.  None: they form no layers, or the gates cannot be read."""
+    if not hasattr(circuit, "op_table"):
+        return None
+    from .circuit import SRC_THETA
+
+    first = {}
+    for op in circuit.op_table():
+        if op["src"] == SRC_THETA:
+            first.setdefault(int(op["idx"]), (int(op["kind"]), int(op["q0"])))
+    if n_params < 1 or sorted(first) != list(range(n_params)):
+        return None
+    gates = [first[i] for i in range(n_params)]
+    for cols in range(1, n_params + 1):
+        if n_params % cols == 0 and gates == gates[:cols] * (n_params // cols):
+            turned = np.bincount([q for _, q in gates[:cols]], minlength=circuit.n_qubit)
+            return cols if turned.min() > 0 and (cols < n_params or turned.min() == turned.max()) else None
+
+
 class Muon(MiniBatchOptimizer):
     """SGDM whose update is orthogonalised (vqa_amd.orthogonal.muon_step, on the GPU): the circuit parameters are taken as a
     matrix, one row a layer, and the momentum's singular values are carried towards 1 before it is applied.  Parameters
     behind the matrix (the regressor's scale) take SGDM's step.  Rules evaluated as in SGDM.
 
-    hpara: mu, nesterov, weight_decay, ns_steps, and matrix_shape = (layers, angles of a layer); by default the layers of
-    the shipped ansatz builders, three angles a qubit (vqa/QNN/QML_utils.py:76-98, 143-163).  Not in the reference."""
+    hpara: mu, nesterov, weight_decay, ns_steps, and matrix_shape = (layers, angles of a layer).  By default a layer is what
+    the circuit's trainable gates repeat (kind and qubit, in the order of their angles), as in the shipped ansatz builders
+    (vqa/QNN/QML_utils.py:76-98, 143-163: three angles a qubit; ``create_ry_rz_cz_ansatz`` two, ``create_ry_cz_ansatz`` one);
+    a circuit that repeats nothing has one layer if every qubit is turned as often, else matrix_shape is needed.  Not in the
+    reference."""
 
     optimizer_name = "Muon"
     default_hpara = dict(mu=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, matrix_shape=None)
@@ -256,9 +279,14 @@ class Muon(MiniBatchOptimizer):
                 raise ValueError(f"matrix_shape {self.matrix_shape} does not fit {self.n_params} parameters")
             return rows, cols
         n_c, n_q = getattr(self.target_obj, "n_c_params", self.n_params), getattr(self.target_obj, "n_qubits", None)
-        if not n_q or n_c < 1 or n_c % (3 * n_q):
-            raise ValueError("the circuit parameters do not form layers of three angles a qubit: give matrix_shape")
-        return n_c // (3 * n_q), 3 * n_q
+        circuit = getattr(self.target_obj, "circuit", None)
+        if circuit is not None:
+            cols = _layer_of(circuit, n_c)
+        else:                                      # a target object without a circuit: layers of three angles a qubit
+            cols = 3 * n_q if n_q and n_c >= 1 and n_c % (3 * n_q) == 0 else None
+        if not cols:
+            raise ValueError("the circuit parameters do not form layers of the same gates: give matrix_shape")
+        return n_c // cols, cols
 
     def _reset_state(self):
         self.m_t = np.zeros(self.n_params)
