@@ -637,3 +637,24 @@ def test_targets_of_every_integer_type(dt, V):
         tg = np.full(40, 2 ** 63 + 5, np.uint64)
         far = vqa_amd.log_probs(z, torch.from_numpy(tg).cuda())
         assert torch.isnan(far.log_prob).all() and np.isnan(vqa_amd.log_probs(z.cpu().numpy(), tg).log_prob).all()
+
+
+def test_softmax_loss_takes_the_penalty():
+    """L2_reg_lmd, which cross_entropy beside it applies, reaches loss and gradient, also through fit()"""
+    q, p = classifier()
+    n, lmd = len(q.x_train), 0.3
+    g0, g1 = q.softmax_CE_grad_eval(p, mini_batch_size=n), q.softmax_CE_grad_eval(p, mini_batch_size=n, L2_reg_lmd=lmd)
+    # the two batches hold the samples in different orders: 72 terms of the sum in another one, together below 3 (24 samples of
+    # weight 1 / 24, three class values whose differences are at most 1), each addition 2^-53 of what it gives
+    assert np.abs(g1 - (lmd * p + g0)).max() <= 2.0 ** -53 * 2 * (72 + 8) * (3 + lmd * 4)
+    loss = lambda w: q.softmax_CE_loss_eval(w, mini_batch_size=n, L2_reg_lmd=lmd)
+    assert abs(loss(p) - q._softmax_CE(p, "train") - 0.15 * np.sum(p * p)) < 1e-13
+    for i in (0, 7, len(p) - 1):
+        e = np.zeros_like(p)
+        e[i] = 1e-4
+        assert abs((loss(p + e) - loss(p - e)) / 2e-4 - g1[i]) < 2e-7          # third derivative of the penalty: 0
+    q.compile(optimizer="SGD", loss="softmax_cross_entropy", hpara=dict(LR_rule=0.05, batch_size_rule=n, s_list_rule=1), init_params=p)
+    path = np.array(q.fit(options=dict(max_iter=1), auto_save=False, L2_reg_lmd=lmd)["para_evol"])
+    from vqa_amd.optimizers import map_to_pi_range
+
+    assert np.max(np.abs(path[1] - map_to_pi_range(p - 0.05 * g1, np.arange(len(p))))) < 1e-12

@@ -219,3 +219,14 @@ def test_a_circuit_without_layers_needs_matrix_shape():
     Target.circuit, Target.n_c_params = Other(), 6
     with pytest.raises(ValueError, match="matrix_shape"):
         vqa_amd.optimizers.Muon({}, dict(target_obj=Target(), init_params=np.zeros(6)))
+
+
+def test_softmax_loss_refuses_what_it_does_not_know():
+    """a keyword that would change nothing without saying so"""
+    from vqa_amd.qnn_classifier import myQNN_classifier as Q
+
+    q = Q.__new__(Q)
+    for f in (Q.softmax_CE_grad_eval, Q.softmax_CE_loss_eval):
+        for kw in (dict(partial_MSE=True), dict(L2_reg=0.1)):
+            with pytest.raises(TypeError, match=next(iter(kw))):
+                f(q, np.zeros(3), **kw)

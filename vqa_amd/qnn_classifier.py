@@ -643,17 +643,21 @@ class myQNN_classifier(myQNN_base):
         entropy_weight times the mean entropy."""
         return {"test": self._softmax_CE(params, "test"), "train": self._softmax_CE(params, "train")}
 
-    def softmax_CE_loss_eval(self, params, n_shots=None, mini_batch_size=None, option_weight=None, **unused):
+    def softmax_CE_loss_eval(self, params, n_shots=None, mini_batch_size=None, option_weight=None, option_min_approx=None, L2_reg_lmd=0.0):
+        """The mini-batch loss whose gradient softmax_CE_grad_eval is (its arguments too)."""
         _, eval_ind, _, _ = self._setup(mini_batch_size, option_weight)
         self.circuit_counter[0] += len(eval_ind)
         self.call_counter[0] += len(eval_ind)
-        return self._softmax_CE(params, "train", idx=eval_ind)
+        return self._softmax_CE(params, "train", idx=eval_ind) + 0.5 * L2_reg_lmd * float(np.sum(np.square(params)))
 
-    def softmax_CE_grad_eval(self, params, n_shots_list=None, mini_batch_size=None, option_weight=None, **unused):
-        """Gradient of the mini-batch loss  mean(-log p_label) - entropy_weight * mean(entropy)  of the softmax read-out, from
-        exact class values (no shots are drawn or counted): the parameter-shift sweep of the class observables, the loss's
-        gradient by the unshifted values, and their chain, all on the GPU.  With a process group the batch is split over the
-        ranks and the sums are added with one all-reduce, as in the other oracles."""
+    def softmax_CE_grad_eval(self, params, n_shots_list=None, mini_batch_size=None, option_weight=None, option_min_approx=None,
+                             L2_reg_lmd=0.0, second_order=False, Max_n_shots0=True):
+        """Gradient of the mini-batch loss  mean(-log p_label) - entropy_weight * mean(entropy) + L2_reg_lmd / 2 |params|^2  of
+        the softmax read-out, from exact class values (no shots are drawn or counted): the parameter-shift sweep of the class
+        observables, the loss's gradient by the unshifted values, and their chain, all on the GPU.  With a process group the
+        batch is split over the ranks and the sums are added with one all-reduce, as in the other oracles.  The keywords of
+        CE_grad_eval; those that say how shots are dealt and counted change nothing here (n_shots_list, option_weight,
+        option_min_approx, second_order, Max_n_shots0)."""
         import torch
 
         from .softmax import log_probs_grad, psr_chain
@@ -672,8 +676,8 @@ class myQNN_classifier(myQNN_base):
         sums = psr_chain(E, r.d_logits)
         self.circuit_counter[0] += B * E.shape[1]
         self.call_counter[0] += B * E.shape[1]
-        out = np.zeros_like(params, dtype=float)
-        out[:self.n_c_params] = sums.cpu().numpy() if sh is None else sh.reduce(sums)[0]
+        out = L2_reg_lmd * np.asarray(params, dtype=float)
+        out[:self.n_c_params] += sums.cpu().numpy() if sh is None else sh.reduce(sums)[0]
         return out
 
     # MSE_loss_eval: inherited from the regressor as in the reference (myQNNs_base.py:1397-1419 through
