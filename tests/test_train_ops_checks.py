@@ -230,3 +230,36 @@ def test_softmax_loss_refuses_what_it_does_not_know():
         for kw in (dict(partial_MSE=True), dict(L2_reg=0.1)):
             with pytest.raises(TypeError, match=next(iter(kw))):
                 f(q, np.zeros(3), **kw)
+
+
+def test_softmax_gradient_runs_on_the_circuits_gpu(monkeypatch):
+    """a sweep that comes back as numpy goes to the GPU that the circuit names, not to the current one"""
+    import torch
+
+    from vqa_amd import qnn_classifier, softmax
+
+    went = []
+
+    class Circuit:
+        device = 3
+
+        def psr_full(self, theta, handle, sel, **kw):
+            return np.zeros((len(sel), 2 * len(theta) + 1, 3)), None
+
+    q = qnn_classifier.myQNN_classifier.__new__(qnn_classifier.myQNN_classifier)
+    q.circuit, q.n_c_params = Circuit(), 4
+    q.circuit_counter, q.call_counter = [0], [0]
+    q._setup = lambda *a: (None, np.arange(5), np.zeros(5, int), None)
+    q._shard = lambda n: None
+    q._handle = lambda which: None
+    q.class_observables = lambda: []
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda t, *a, **k: went.append(("current", a)) or t)
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *a, **k: went.append(a[0] if a else k) or t)
+    monkeypatch.setattr(softmax, "log_probs_grad", lambda z, *a, **k: softmax.LogProbsGrad(None, None, z))
+    monkeypatch.setattr(softmax, "psr_chain", lambda E, d: torch.zeros(4, dtype=torch.float64))
+    assert np.array_equal(q.softmax_CE_grad_eval(np.ones(4)), np.zeros(4))
+    assert went == ["cuda:3"]
+    del Circuit.device                       # a circuit that names none: the first, as its other calls take it
+    went.clear()
+    q.softmax_CE_grad_eval(np.ones(4))
+    assert went == ["cuda:0"]

@@ -670,7 +670,7 @@ class myQNN_classifier(myQNN_base):
         E, _ = self.circuit.psr_full(theta, self._handle("train"), sel=np.asarray(eval_ind[rows], np.int32),
                                      obs_list=self.class_observables(), n_marg_bits=0)
         if not hasattr(E, "is_cuda"):
-            E = torch.from_numpy(np.ascontiguousarray(E)).cuda()
+            E = torch.from_numpy(np.ascontiguousarray(E)).to(f"cuda:{getattr(self.circuit, 'device', None) or 0}")
         r = log_probs_grad(E[:, 0], np.asarray(y_eval)[rows].astype(np.int32), -1.0 / B, -self.entropy_weight / B if self.entropy_weight else None,
                            scale=self.softmax_scale)
         sums = psr_chain(E, r.d_logits)
