@@ -263,3 +263,21 @@ def test_softmax_gradient_runs_on_the_circuits_gpu(monkeypatch):
     went.clear()
     q.softmax_CE_grad_eval(np.ones(4))
     assert went == ["cuda:0"]
+
+
+def read_only(a):
+    a = a.copy()
+    a.flags.writeable = False
+    return a
+
+
+@pytest.mark.parametrize("out", [read_only(np.zeros((3, 4))), np.frombuffer(bytes(96)).reshape(3, 4)])
+def test_results_do_not_go_to_read_only_arrays(out):
+    z = np.zeros((3, 4))
+    with pytest.raises(ValueError, match="writable"):
+        vqa_amd.orthogonalize(z, out=out)
+    with pytest.raises(ValueError, match="writable"):
+        vqa_amd.log_probs_grad(z, np.zeros(3, int), 1.0, out=out)
+    with pytest.raises(ValueError, match="writable"):
+        vqa_amd.muon_step(out, z, np.zeros((3, 4)), 0.1)
+    assert not out.any()

@@ -76,8 +76,9 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
         batch, rows, cols = (1,) * (3 - g.ndim) + g.shape
         if out is None:
             out = np.empty_like(g)
-        elif not (isinstance(out, np.ndarray) and out.shape == g.shape and out.dtype == g.dtype and out.flags.c_contiguous):
-            raise ValueError("out must be a C-contiguous array of G's shape and type")
+        elif not (isinstance(out, np.ndarray) and out.shape == g.shape and out.dtype == g.dtype and out.flags.c_contiguous
+                  and out.flags.writeable):
+            raise ValueError("out must be a writable C-contiguous array of G's shape and type")
         _lib.check(L.vqa_orthogonalize(device, _NP_CODE[g.dtype.name], _lib.nptr(g), batch, rows, cols, cols, rows * cols, int(steps),
                                        k, float(eps), _lib.nptr(out)))
         return out

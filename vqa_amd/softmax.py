@@ -188,8 +188,9 @@ def log_probs_grad(logits, targets, d_log_prob=None, d_entropy=None, scale: floa
         g, h = vec(d_log_prob), vec(d_entropy)
         if out is None:
             out = np.empty_like(z)
-        elif not (isinstance(out, np.ndarray) and out.shape == z.shape and out.dtype == z.dtype and out.flags.c_contiguous):
-            raise ValueError("out must be a C-contiguous array of the scores' shape and type")
+        elif not (isinstance(out, np.ndarray) and out.shape == z.shape and out.dtype == z.dtype and out.flags.c_contiguous
+                  and out.flags.writeable):
+            raise ValueError("out must be a writable C-contiguous array of the scores' shape and type")
         lp = None if t is None else np.empty(rows, wide)
         ent = np.empty(rows, wide)
         _lib.check(L.vqa_log_probs_grad(device, _NP_CODE[z.dtype.name], _lib.nptr(z), rows, width, width, scale, _lib.nptr(t),
