@@ -281,3 +281,30 @@ def test_results_do_not_go_to_read_only_arrays(out):
     with pytest.raises(ValueError, match="writable"):
         vqa_amd.muon_step(out, z, np.zeros((3, 4)), 0.1)
     assert not out.any()
+
+
+def test_arrays_in_the_other_byte_order_and_complex_ones():
+    """numpy arrays reach the library in the machine's byte order; an imaginary part is not dropped"""
+    from vqa_amd import orthogonal, softmax
+
+    a = np.arange(12.0).reshape(3, 4) - 5
+    for kind in ("f8", "f4", "f2"):
+        for take in (softmax._np_rows, orthogonal._np_matrices):
+            got = take(a.astype(">" + kind), "it")
+            assert got.dtype.isnative and got.dtype == np.dtype(kind) and np.array_equal(got, a)
+    for take in (softmax._np_rows, orthogonal._np_matrices):
+        assert take(a.astype(">i4"), "it").dtype == np.float64
+        with pytest.raises(ValueError, match="real"):
+            take(a + 1j, "it")
+    assert softmax._np_targets(np.array([2, 0, 1], ">i8"), 3, 4).tolist() == [2, 0, 1]
+    with pytest.raises(ValueError):
+        vqa_amd.orthogonalize(a, out=np.empty((3, 4), ">f8"))
+    w = np.zeros((3, 4))
+    with pytest.raises(ValueError):
+        vqa_amd.muon_step(w.astype(">f8"), w, w.copy(), 0.1)
+    for bad in (a + 1j, "abcd"):
+        with pytest.raises(ValueError):
+            vqa_amd.muon_step(w, bad, w.copy(), 0.1)
+    for kw in (dict(d_log_prob=1j), dict(d_entropy=np.full(3, 1j))):
+        with pytest.raises(ValueError):
+            vqa_amd.log_probs_grad(a, np.zeros(3, int), **kw)

@@ -11,7 +11,7 @@ from typing import Sequence
 import numpy as np
 
 from . import _lib
-from .softmax import _NP_CODE, _is_numpy, _torch_codes
+from .softmax import _NP_CODE, _is_numpy, _np_real, _torch_codes
 
 # steepens small singular values fast; what lies in (0, 1] ends in about [0.7, 1.2] after five steps
 COEFS = (3.4445, -4.7750, 2.0315)
@@ -53,9 +53,7 @@ def _matrices(g, what):
 
 
 def _np_matrices(g, what):
-    g = np.asarray(g)
-    if g.dtype.name not in _NP_CODE:
-        g = g.astype(np.float64)
+    g = _np_real(g, what)
     if g.ndim not in (2, 3):
         raise ValueError(f"{what} must be [rows, cols] or [batch, rows, cols]")
     return np.ascontiguousarray(g)
@@ -114,7 +112,7 @@ def muon_step(weight, grad, momentum, lr: float, mu: float = 0.95, weight_decay:
             if not (isinstance(a, np.ndarray) and a.dtype in (np.float64, np.float32) and a.flags.c_contiguous and a.flags.writeable
                     and a.ndim in (2, 3)):
                 raise ValueError(f"{what} must be a writable C-contiguous float64 or float32 array [rows, cols] or [batch, rows, cols]")
-        g = np.ascontiguousarray(np.asarray(grad, dtype=weight.dtype))
+        g = np.ascontiguousarray(_np_real(grad, "grad", weight.dtype))
         if momentum.shape != weight.shape or momentum.dtype != weight.dtype or g.shape != weight.shape:
             raise ValueError("weight, grad and momentum must have one shape, weight and momentum one type")
         batch, rows, cols = (1,) * (3 - g.ndim) + g.shape

@@ -51,10 +51,19 @@ class LogProbsGrad(NamedTuple):
     d_logits: Any
 
 
-def _np_rows(a, what):
+def _np_real(a, what, dtype=None):
+    """An array that the library can read: of ``dtype`` (None: its own type, float64 where that is not a float that the library
+    takes), in the machine's byte order."""
     a = np.asarray(a)
-    if a.dtype.name not in _NP_CODE:
-        a = a.astype(np.float64)
+    if a.dtype.kind not in "fiubO":
+        raise ValueError(f"{what} must be real numbers (got {a.dtype})")
+    if dtype is None:
+        dtype = a.dtype.newbyteorder("=") if a.dtype.name in _NP_CODE else np.float64
+    return a.astype(dtype, copy=False)
+
+
+def _np_rows(a, what):
+    a = _np_real(a, what)
     if a.ndim != 2:
         raise ValueError(f"{what} must be [R, V]")
     return np.ascontiguousarray(a)
@@ -108,13 +117,15 @@ def _weights(w, z, wide, what):
     if w is None:
         return None
     if not isinstance(w, torch.Tensor):
-        w = torch.as_tensor(np.asarray(w, dtype=np.float64)).to(z.device, wide)
+        w = torch.as_tensor(_np_real(w, what, np.float64)).to(z.device, wide)
     if w.dim() == 0:
         w = w.expand(rows)
     if tuple(w.shape) != (rows,):
         raise ValueError(f"{what} must have shape [R]")
     if w.device != z.device:
         raise ValueError(f"{what} must be on the scores' device")
+    if w.is_complex():
+        raise ValueError(f"{what} must be real numbers (got {w.dtype})")
     return w.to(wide).contiguous()
 
 
@@ -184,8 +195,8 @@ def log_probs_grad(logits, targets, d_log_prob=None, d_entropy=None, scale: floa
         rows, width = z.shape
         wide = np.float64 if z.dtype == np.float64 else np.float32
         t = None if targets is None else _np_targets(targets, rows, width)
-        vec = lambda w: None if w is None else np.ascontiguousarray(np.broadcast_to(np.asarray(w, wide), (rows,)))
-        g, h = vec(d_log_prob), vec(d_entropy)
+        vec = lambda w, what: None if w is None else np.ascontiguousarray(np.broadcast_to(_np_real(w, what, wide), (rows,)))
+        g, h = vec(d_log_prob, "d_log_prob"), vec(d_entropy, "d_entropy")
         if out is None:
             out = np.empty_like(z)
         elif not (isinstance(out, np.ndarray) and out.shape == z.shape and out.dtype == z.dtype and out.flags.c_contiguous
