@@ -658,3 +658,29 @@ def test_softmax_loss_takes_the_penalty():
     from vqa_amd.optimizers import map_to_pi_range
 
     assert np.max(np.abs(path[1] - map_to_pi_range(p - 0.05 * g1, np.arange(len(p))))) < 1e-12
+
+
+def test_tensors_that_torch_holds_negated():
+    """a view whose sign is not yet applied in memory (of a conjugate's imaginary part) is read as what it stands for, and is
+    no place for results; complex weights are refused"""
+    import torch
+
+    z, g = torch.randn(6, 40, device="cuda"), torch.randn(6, device="cuda")
+    neg = lambda t: torch._neg_view(-t)
+    tg = torch.arange(6, device="cuda")
+    assert neg(z).is_neg() and torch.equal(neg(z), z)
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))
+    assert same(vqa_amd.log_probs(neg(z), tg, top_k=3), vqa_amd.log_probs(z, tg, top_k=3))
+    assert same(vqa_amd.log_probs_grad(neg(z), tg, neg(g), neg(g)), vqa_amd.log_probs_grad(z, tg, g, g))
+    E, d = torch.randn(4, 5, 2, dtype=torch.float64, device="cuda"), torch.randn(4, 2, dtype=torch.float64, device="cuda")
+    assert torch.equal(vqa_amd.psr_chain(neg(E), neg(d)), vqa_amd.psr_chain(E, d))
+    assert torch.equal(vqa_amd.orthogonalize(neg(z)), vqa_amd.orthogonalize(z))
+    w, m = torch.ones_like(z), torch.zeros_like(z)
+    vqa_amd.muon_step(w, neg(z), m, 0.1)
+    v, n = torch.ones_like(z), torch.zeros_like(z)
+    vqa_amd.muon_step(v, z, n, 0.1)
+    assert torch.equal(w, v) and torch.equal(m, n)
+    for call in (lambda: vqa_amd.orthogonalize(z, out=neg(w)), lambda: vqa_amd.muon_step(neg(w), z, m, 0.1), lambda: vqa_amd.muon_step(w, z, neg(m), 0.1),
+                 lambda: vqa_amd.log_probs_grad(z, tg, g, out=neg(w)), lambda: vqa_amd.log_probs_grad(z, tg, g.to(torch.complex64))):
+        with pytest.raises(ValueError):
+            call()

@@ -40,6 +40,7 @@ def _matrices(g, what):
         raise ValueError(f"{what} must be float64, float32, bfloat16 or float16 (got {g.dtype})")
     if not g.is_cuda:
         raise ValueError(f"{what} must be a numpy array or a cuda tensor")
+    g = g.resolve_neg()                     # (a view that torch holds negated: its memory has the other sign)
     batch = g.shape[0] if g.dim() == 3 else 1
     rows, cols = g.shape[-2:]
     sb, sr, sc = (g.stride() if g.dim() == 3 else (0,) + tuple(g.stride()))
@@ -87,8 +88,8 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
     dev = g.device
     if out is None:
         out = torch.empty(G.shape, dtype=g.dtype, device=dev)
-    elif out.shape != G.shape or out.dtype != g.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of G's shape, type and device")
+    elif out.shape != G.shape or out.dtype != g.dtype or out.device != dev or not out.is_contiguous() or out.is_neg():
+        raise ValueError("out must be contiguous, of G's shape, type and device, and not a negated view")
     n = L.vqa_orthogonalize_workspace(code, batch, rows, cols)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _lib.check(L.vqa_orthogonalize_dev(dev.index, _lib.current_stream(dev.index), code, g.data_ptr(), batch, rows, cols,
@@ -126,8 +127,8 @@ def muon_step(weight, grad, momentum, lr: float, mu: float = 0.95, weight_decay:
     code, wide = _torch_codes()[g.dtype]
     dev = g.device
     for a, what in ((weight, "weight"), (momentum, "momentum")):
-        if a.shape != grad.shape or a.dtype != wide or a.device != dev or not a.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous {wide} tensor of grad's shape on its device")
+        if a.shape != grad.shape or a.dtype != wide or a.device != dev or not a.is_contiguous() or a.is_neg():
+            raise ValueError(f"{what} must be a contiguous {wide} tensor of grad's shape on its device, and not a negated view")
     n = L.vqa_orthogonalize_workspace(code, batch, rows, cols)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _lib.check(L.vqa_muon_step_dev(dev.index, _lib.current_stream(dev.index), code, weight.data_ptr(), g.data_ptr(),

@@ -89,6 +89,7 @@ def _rows(z, what):
         raise ValueError(f"{what} must have at least one column")
     if width > 1 and z.stride(1) != 1 or rows > 1 and z.stride(0) < width:
         z = z.contiguous()
+    z = z.resolve_neg()                     # (a view that torch holds negated: its memory has the other sign)
     return z, (z.stride(0) if rows > 1 else width)
 
 
@@ -106,7 +107,7 @@ def _targets(targets, z):
         if t.dtype == torch.uint64:
             wide = torch.where(wide < 0, width, wide)                 # from 2^63 on
         t = wide.clamp(-1, width).to(torch.int32)
-    return t.contiguous()
+    return t.contiguous().resolve_neg()
 
 
 def _weights(w, z, wide, what):
@@ -126,7 +127,7 @@ def _weights(w, z, wide, what):
         raise ValueError(f"{what} must be on the scores' device")
     if w.is_complex():
         raise ValueError(f"{what} must be real numbers (got {w.dtype})")
-    return w.to(wide).contiguous()
+    return w.to(wide).contiguous().resolve_neg()
 
 
 def _ptr(t):
@@ -218,8 +219,8 @@ def log_probs_grad(logits, targets, d_log_prob=None, d_entropy=None, scale: floa
     if out is None:
         out = torch.empty((rows, width), dtype=z.dtype, device=dev)
     elif (tuple(out.shape) != (rows, width) or out.dtype != z.dtype or out.device != dev or width > 1 and out.stride(1) != 1
-          or rows > 1 and out.stride(0) < width):
-        raise ValueError("out must have the scores' shape, type and device, with contiguous rows")
+          or rows > 1 and out.stride(0) < width or out.is_neg()):
+        raise ValueError("out must have the scores' shape, type and device, with contiguous rows, and not be a negated view")
     lp = None if t is None else torch.empty(rows, dtype=wide, device=dev)
     ent = torch.empty(rows, dtype=wide, device=dev)
     n = L.vqa_log_probs_workspace(code, rows, width, 0)
@@ -239,12 +240,12 @@ def psr_chain(E, d_expect, factor: float = 0.5):
 
     if E.dim() != 3 or E.dtype != torch.float64 or not E.is_cuda or E.shape[1] % 2 != 1:
         raise ValueError("E must be a float64 cuda tensor [B, 2P+1, n_obs]")
-    E = E.contiguous()
+    E = E.contiguous().resolve_neg()
     B, K, n_obs = E.shape
     P = (K - 1) // 2
-    if tuple(d_expect.shape) != (B, n_obs) or d_expect.device != E.device:
-        raise ValueError("d_expect must be [B, n_obs] on E's device")
-    d = d_expect.to(torch.float64).contiguous()
+    if tuple(d_expect.shape) != (B, n_obs) or d_expect.device != E.device or d_expect.is_complex():
+        raise ValueError("d_expect must be real numbers [B, n_obs] on E's device")
+    d = d_expect.to(torch.float64).contiguous().resolve_neg()
     out = torch.empty(P, dtype=torch.float64, device=E.device)
     L = _lib.lib()
     ws = torch.empty(max(int(L.vqa_psr_chain_workspace(B, max(P, 1))) // 8, 1), dtype=torch.float64, device=E.device)
