@@ -560,3 +560,36 @@ def test_eps_far_above_the_norm(rows, cols, eps):
         # (the rate is rounded and multiplied: a step of each value)
         tol = 4 * torch.linalg.vector_norm(p.double() - want, dim=(1, 2)) + UNIT[t] * (math.sqrt(c + 2 * r) * 4 + 2) * norm
         assert (w[1] == 0).all() and (off <= tol).all(), (t, off / norm, tol / norm)
+
+
+def test_autograd_sees_what_was_overwritten():
+    """weight, momentum and out= move torch's version counters: a backward pass that saved them raises, as after torch's own
+    in-place operations, and does not take the new values for the old; tensors of inference mode have no counters"""
+    import torch
+
+    for rows, cols in ((4, 6), (80, 70)):
+        g = torch.randn(rows, cols, device="cuda")
+        w, m, out = torch.ones_like(g), torch.zeros_like(g), torch.empty_like(g)
+        a = torch.ones_like(g, requires_grad=True)
+        for write, written in ((lambda: vqa_amd.muon_step(w, g, m, 0.1), (w, m)), (lambda: vqa_amd.orthogonalize(g, out=out), (out,)),
+                               (lambda: vqa_amd.log_probs_grad(g, torch.zeros(rows, dtype=torch.int32, device="cuda"), 1.0, out=out), (out,))):
+            read = g._version
+            losses = [(a * t).sum() for t in written]
+            before = [t._version for t in written]
+            write()
+            assert all(t._version > v for t, v in zip(written, before)) and g._version == read
+            for y in losses:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    y.backward()
+        y = (a * g).sum()
+        vqa_amd.orthogonalize(g)                     # a result of its own: nothing that was there has changed
+        y.backward()
+        y = (a * g).sum()
+        vqa_amd.orthogonalize(g, out=g)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with torch.inference_mode():
+            w, m = torch.ones(rows, cols, device="cuda"), torch.zeros(rows, cols, device="cuda")
+            vqa_amd.muon_step(w, torch.ones_like(w), m, 0.1)
+            vqa_amd.orthogonalize(w, out=w)
+            assert torch.isfinite(w).all() and (m == 1).all()

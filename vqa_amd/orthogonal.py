@@ -11,7 +11,7 @@ from typing import Sequence
 import numpy as np
 
 from . import _lib
-from .softmax import _NP_CODE, _is_numpy, _np_real, _torch_codes
+from .softmax import _NP_CODE, _is_numpy, _np_real, _torch_codes, _written
 
 # steepens small singular values fast; what lies in (0, 1] ends in about [0.7, 1.2] after five steps
 COEFS = (3.4445, -4.7750, 2.0315)
@@ -67,7 +67,7 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
     A zero matrix gives zero; one with a NaN or inf, or whose sum of squares leaves 64 bits, gives NaN.
 
     numpy: host-pointer path on GPU ``device``.  torch cuda tensors (rows may be strided): queued on the current torch
-    stream; ``out`` may be G itself."""
+    stream; ``out`` may be G itself.  Nothing is recorded for autograd; a backward pass that saved ``out`` raises."""
     L = _lib.lib()
     k = _coefs(coefs)
     if _is_numpy(G):
@@ -86,6 +86,7 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
     g, batch, rows, cols, sr, sb = _matrices(G, "G")
     code = _torch_codes()[g.dtype][0]
     dev = g.device
+    given = out is not None
     if out is None:
         out = torch.empty(G.shape, dtype=g.dtype, device=dev)
     elif out.shape != G.shape or out.dtype != g.dtype or out.device != dev or not out.is_contiguous() or out.is_neg():
@@ -94,6 +95,8 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _lib.check(L.vqa_orthogonalize_dev(dev.index, _lib.current_stream(dev.index), code, g.data_ptr(), batch, rows, cols,
                                        sr, sb, int(steps), k, float(eps), None if ws is None else ws.data_ptr(), out.data_ptr()))
+    if given:
+        _written(out)
     return out
 
 
@@ -105,7 +108,8 @@ def muon_step(weight, grad, momentum, lr: float, mu: float = 0.95, weight_decay:
         weight   <- (1 - lr * weight_decay) * weight - lr * sqrt(max(1, rows / cols)) * orthogonalize(u)
 
     weight and momentum are contiguous: float64 with float64 gradients, float32 with float32, bfloat16 and float16 ones.
-    Returns weight.  Paths as in ``orthogonalize`` (numpy: weight and momentum are overwritten, grad is taken in their type)."""
+    Returns weight.  Nothing is recorded for autograd; a backward pass that saved what is overwritten raises.  Paths as in
+    ``orthogonalize`` (numpy: weight and momentum are overwritten, grad is taken in their type)."""
     L = _lib.lib()
     k = _coefs(coefs)
     if _is_numpy(weight):
@@ -134,4 +138,5 @@ def muon_step(weight, grad, momentum, lr: float, mu: float = 0.95, weight_decay:
     _lib.check(L.vqa_muon_step_dev(dev.index, _lib.current_stream(dev.index), code, weight.data_ptr(), g.data_ptr(),
                                    momentum.data_ptr(), batch, rows, cols, sr, sb, float(lr), float(mu), float(weight_decay),
                                    int(bool(nesterov)), int(steps), k, float(eps), None if ws is None else ws.data_ptr()))
+    _written(weight, momentum)
     return weight

@@ -130,6 +130,18 @@ def _weights(w, z, wide, what):
     return w.to(wide).contiguous().resolve_neg()
 
 
+_bump = None
+
+
+def _written(*tensors):
+    """What the library overwrote, for torch's version counters: a backward pass that saved it raises instead of taking the new
+    values.  (Tensors of inference mode have no counter.)"""
+    global _bump
+    if _bump is None:
+        from torch.autograd.graph import increment_version as _bump
+    _bump([t for t in tensors if not t.is_inference()])
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -216,6 +228,7 @@ def log_probs_grad(logits, targets, d_log_prob=None, d_entropy=None, scale: floa
     dev = z.device
     t = None if targets is None else _targets(targets, z)
     g, h = _weights(d_log_prob, z, wide, "d_log_prob"), _weights(d_entropy, z, wide, "d_entropy")
+    given = out is not None
     if out is None:
         out = torch.empty((rows, width), dtype=z.dtype, device=dev)
     elif (tuple(out.shape) != (rows, width) or out.dtype != z.dtype or out.device != dev or width > 1 and out.stride(1) != 1
@@ -228,6 +241,8 @@ def log_probs_grad(logits, targets, d_log_prob=None, d_entropy=None, scale: floa
     _lib.check(L.vqa_log_probs_grad_dev(dev.index, _lib.current_stream(dev.index), code, z.data_ptr(), rows, width,
                                         stride, scale, _ptr(t), _ptr(g), _ptr(h), _ptr(ws), _ptr(lp), ent.data_ptr(),
                                         out.data_ptr(), out.stride(0) if rows > 1 else width))
+    if given:
+        _written(out)
     return LogProbsGrad(lp, ent, out)
 
 
