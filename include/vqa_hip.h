@@ -422,8 +422,9 @@ int vqa_class_stats_dev(int device, void* stream, const int64_t* d_counts, const
  * Deterministic (the order of a row's additions depends on the sizes and on where it begins in its 16 bytes); columns
  * behind `width` are not read.
  * _dev: device pointers, queued on `stream`, not waited for, nothing allocated: workspace is
- * vqa_log_probs_workspace(...) bytes of the caller's device memory (0: may be NULL), not shared with work that may run
- * at the same time.  The calling thread's current device is kept.
+ * vqa_log_probs_workspace(...) bytes of the caller's device memory (0: may be NULL), at a multiple of 16 bytes, not shared
+ * with work that may run at the same time.  Other pointers are aligned to their types, at least.  The calling thread's
+ * current device is kept.
  */
 #define VQA_DTYPE_F64  0
 #define VQA_DTYPE_F32  1

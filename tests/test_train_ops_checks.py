@@ -308,3 +308,47 @@ def test_arrays_in_the_other_byte_order_and_complex_ones():
     for kw in (dict(d_log_prob=1j), dict(d_entropy=np.full(3, 1j))):
         with pytest.raises(ValueError):
             vqa_amd.log_probs_grad(a, np.zeros(3, int), **kw)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(t=P + 4098), dict(lp=P + 8196), dict(ent=P + 12292), dict(tl=P + 16388), dict(ti=P + 20482), dict(dtype=1, lp=P + 8194),
+    dict(rows=1, width=5000, stride=5000, ws=P + 131080)])
+def test_score_pointers_are_aligned(kw):
+    refused(score(**kw), _lib.EINVAL, "aligned")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(t=P + 4097), dict(g=P + 4100), dict(h=P + 4100), dict(lp=P + 8196), dict(ent=P + 8196), dict(dz=P + 16388), dict(dtype=2, g=P + 4098),
+    dict(rows=1, width=3000, stride=3000, dz_stride=3000, dz=P + 32768, ws=P + 131080)])
+def test_loss_pointers_are_aligned(kw):
+    refused(loss(**kw), _lib.EINVAL, "aligned")
+
+
+def test_matrix_and_chain_pointers_are_aligned():
+    refused(ortho(out=P + 8196), _lib.EINVAL, "aligned")
+    refused(ortho(dtype=2, out=P + 8193), _lib.EINVAL, "aligned")
+    refused(ortho(dtype=1, rows=100, cols=100, sr=100, sb=10000, batch=1, out=P + 80000, ws=P + 131080), _lib.EINVAL, "aligned")
+    refused(step(w=P + 4), _lib.EINVAL, "aligned")
+    refused(step(m=P + 16388), _lib.EINVAL, "aligned")
+    refused(step(dtype=3, w=P + 2), _lib.EINVAL, "aligned")
+    L = _lib.lib()
+    ok = dict(e=P, d=P + 1024, ws=P + 2048, out=P + 4096)
+    for k in ok:
+        a = dict(ok)
+        a[k] += 4
+        refused(L.vqa_psr_chain_dev(0, None, a["e"], 2, 3, 1, 0.5, a["d"], a["ws"], a["out"]), _lib.EINVAL, "aligned")
+
+
+def test_refused_pointers_were_the_only_fault():
+    """the calls of the alignment tests with their ordinary pointers reach the device (or find none here)"""
+    if _lib.lib().vqa_device_count() > 0:
+        pytest.skip("the pointers are host memory")
+    for rc in (score(), loss(), ortho(), step(), _lib.lib().vqa_psr_chain_dev(0, None, P, 2, 3, 1, 0.5, P, P, P),
+               score(rows=1, width=5000, stride=5000, ws=P + 131072), ortho(dtype=1, rows=100, cols=100, sr=100, sb=10000, batch=1, out=P + 80000, ws=P + 131072)):
+        assert rc == _lib.ENODEVICE
+    # the host-pointer forms copy: their outputs may lie anywhere
+    L = _lib.lib()
+    for rc in (L.vqa_muon_step(0, 0, P + 4, P + 8192, P + 16388, 2, 4, 8, 8, 32, 0.1, 0.9, 0.0, 1, 5, K, 1e-7),
+               L.vqa_orthogonalize(0, 0, P, 2, 4, 8, 8, 32, 5, K, 1e-7, P + 8196),
+               L.vqa_log_probs(0, 0, P, 4, 8, 8, 1.0, P + 4097, 2, P + 8196, P + 12292, P + 16388, P + 20482)):
+        assert rc == _lib.ENODEVICE

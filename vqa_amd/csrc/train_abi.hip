@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <new>
 
 #include "vqa_core.h"
@@ -60,6 +61,19 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     return na && nb && x < y + nb && y < x + na;
 }
 
+// kernels read and write whole values, and 16 bytes at once of a workspace
+struct Aligned {
+    const void* p;
+    size_t to;
+    const char* what;
+};
+int check_aligned(std::initializer_list<Aligned> all) {
+    for (const Aligned& a : all)
+        if ((uintptr_t)a.p % a.to) VQA_FAIL(VQA_EINVAL, "%s is not aligned to %zu bytes", a.what, a.to);
+    return VQA_OK;
+}
+constexpr size_t kWorkspaceAlign = 16;
+
 int check_dtype(int dtype) {
     if (dtype < 0 || dtype > 3) VQA_FAIL(VQA_EINVAL, "dtype must be one of VQA_DTYPE_* (got %d)", dtype);
     return VQA_OK;
@@ -107,6 +121,11 @@ struct Score {
         if (log_prob && !targets) VQA_FAIL(VQA_EINVAL, "log_prob needs the targets");
         return VQA_OK;
     }
+    int check_aligned_to_types() const {     // device pointers
+        const size_t w = wide_of(dtype);
+        return check_aligned({ { targets, 4, "targets" }, { log_prob, w, "log_prob" }, { entropy, w, "entropy" },
+                               { top_k ? top_log_prob : nullptr, w, "top_log_prob" }, { top_k ? top_index : nullptr, 4, "top_index" } });
+    }
 };
 
 struct Loss {
@@ -137,6 +156,11 @@ struct Loss {
         if ((log_prob || dlog_prob) && !targets) VQA_FAIL(VQA_EINVAL, "log_prob and dlog_prob need the targets");
         if (overlap(z, bytes, dz, dz_bytes) && !side_by_side()) VQA_FAIL(VQA_EINVAL, "dscores must not overlap the scores");
         return VQA_OK;
+    }
+    int check_aligned_to_types() const {     // device pointers
+        const size_t w = wide_of(dtype);
+        return check_aligned({ { targets, 4, "targets" }, { dlog_prob, w, "dlog_prob" }, { dentropy, w, "dentropy" },
+                               { log_prob, w, "log_prob" }, { entropy, w, "entropy" } });
     }
 };
 
@@ -214,9 +238,11 @@ int check_step(const OrthoCall& q, size_t g_bytes) {
 int queue_ortho(int device, void* stream, OrthoCall& q) {
     if (!q.batch) return VQA_OK;
     if (!q.workspace && ortho_workspace_bytes(q.dtype, q.batch, q.rows, q.cols)) VQA_FAIL(VQA_EINVAL, "workspace is NULL");
-    DeviceScope scope;
-    int rc = scope.enter(device);
+    int rc = check_aligned({ { q.out, size_of(q.dtype), "out" }, { q.weight, wide_of(q.dtype), "weight" }, { q.momentum, wide_of(q.dtype), "momentum" },
+                             { q.workspace, kWorkspaceAlign, "workspace" } });
     if (rc) return rc;
+    DeviceScope scope;
+    if ((rc = scope.enter(device))) return rc;
     return ortho_launch((hipStream_t)stream, q);
 }
 
@@ -242,7 +268,9 @@ int vqa_log_probs_dev(int device, void* stream, int dtype, const void* d_scores,
     Score q = { dtype, d_scores, rows, width, row_stride, scale, d_targets, top_k, d_log_prob, d_entropy, d_top_log_prob, d_top_index, 0 };
     int rc = q.check();
     if (rc || rows == 0) return rc;
+    if ((rc = q.check_aligned_to_types())) return rc;
     if (!d_workspace && log_probs_workspace_bytes(dtype, rows, width, top_k)) VQA_FAIL(VQA_EINVAL, "workspace is NULL");
+    if ((rc = check_aligned({ { d_workspace, kWorkspaceAlign, "workspace" } }))) return rc;
     DeviceScope scope;
     if ((rc = scope.enter(device))) return rc;
     return log_probs_launch((hipStream_t)stream, dtype, d_scores, rows, width, row_stride, scale, d_targets, top_k, d_workspace,
@@ -286,7 +314,9 @@ int vqa_log_probs_grad_dev(int device, void* stream, int dtype, const void* d_sc
                d_dscores, dscores_row_stride, 0, 0 };
     int rc = q.check();
     if (rc || rows == 0) return rc;
+    if ((rc = q.check_aligned_to_types())) return rc;
     if (!d_workspace && log_probs_workspace_bytes(dtype, rows, width, 0)) VQA_FAIL(VQA_EINVAL, "workspace is NULL");
+    if ((rc = check_aligned({ { d_workspace, kWorkspaceAlign, "workspace" } }))) return rc;
     DeviceScope scope;
     if ((rc = scope.enter(device))) return rc;
     return log_probs_grad_launch((hipStream_t)stream, dtype, d_scores, rows, width, row_stride, scale, d_targets, d_dlog_prob,
@@ -337,9 +367,10 @@ int vqa_psr_chain_dev(int device, void* stream, const double* d_expect, int64_t 
     if (n_params == 0) return VQA_OK;
     if (!d_out) VQA_FAIL(VQA_EINVAL, "out is NULL");
     if (n_samples > 0 && (!d_expect || !d_dexpect || !d_workspace)) VQA_FAIL(VQA_EINVAL, "expect, dexpect and workspace must not be NULL");
-    DeviceScope scope;
-    int rc = scope.enter(device);
+    int rc = check_aligned({ { d_expect, 8, "expect" }, { d_dexpect, 8, "dexpect" }, { d_workspace, 8, "workspace" }, { d_out, 8, "out" } });
     if (rc) return rc;
+    DeviceScope scope;
+    if ((rc = scope.enter(device))) return rc;
     return psr_chain_launch((hipStream_t)stream, d_expect, n_samples, n_params, n_obs, factor, d_dexpect, d_workspace, d_out);
     VQA_EXIT
 }
