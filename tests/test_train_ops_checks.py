@@ -352,3 +352,22 @@ def test_refused_pointers_were_the_only_fault():
                L.vqa_orthogonalize(0, 0, P, 2, 4, 8, 8, 32, 5, K, 1e-7, P + 8196),
                L.vqa_log_probs(0, 0, P, 4, 8, 8, 1.0, P + 4097, 2, P + 8196, P + 12292, P + 16388, P + 20482)):
         assert rc == _lib.ENODEVICE
+
+
+def test_a_workspace_is_asked_for_where_it_is_used():
+    """its size and the launches go by one rule: without one a call is refused or needs none; one sized for outcomes does for a
+    gradient too"""
+    L = _lib.lib()
+    if L.vqa_device_count() > 0:
+        pytest.skip("the pointers are host memory")
+    for rows in (1, 2, 100, 127, 128, 200, 511, 512, 1023, 1024, 5000):
+        for width in (3, 64, 256, 257, 1024, 1025, 4095, 8191, 8192, 8193, 20000, 500000):
+            for k in (0, 3):
+                n = L.vqa_log_probs_workspace(1, rows, width, k)
+                rc = score(dtype=1, rows=rows, width=width, stride=width, k=k)
+                assert (rc == _lib.EINVAL) if n else (rc == _lib.ENODEVICE), (rows, width, k)
+                assert n >= L.vqa_log_probs_workspace(1, rows, width, 0)
+            rc = loss(dtype=1, rows=rows, width=width, stride=2 * width, dz_stride=2 * width, dz=P + 4 * width)
+            assert (rc == _lib.EINVAL) if L.vqa_log_probs_workspace(1, rows, width, 0) else (rc == _lib.ENODEVICE), (rows, width)
+    assert L.vqa_log_probs_workspace(1, 5000, 2000, 8) == 0       # a wave a row: nothing is kept between kernels
+    assert L.vqa_log_probs_workspace(1, 4, 10 ** 6, 8) > L.vqa_log_probs_workspace(1, 4, 10 ** 6, 0) > 0

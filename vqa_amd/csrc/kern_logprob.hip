@@ -1075,6 +1075,8 @@ __global__ __launch_bounds__(kSumRows * kSumParts) void k_psr_chain_sum(const do
 // ---- launches -----------------------------------------------------------------------------------------------------
 constexpr int kLaneWidth = 64, kShortWidth = 1024;
 constexpr int kWaveRows = 512, kWaveWidth = 8192;
+// One workgroup a row needs rows enough for half of the CUs; of fewer rows the gradient is split, and reads them a second time.
+constexpr int kWholeRows = 128;
 constexpr int64_t kMaxGrid = 1 << 20;
 
 // Parts of a row: enough workgroups for the chip (about 4 a CU) while a part keeps 4096 elements, at most one a lane of
@@ -1084,6 +1086,15 @@ int splits_of(int64_t rows, int64_t width) {
     const int64_t most = width / 4096;
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+}
+
+bool wave_a_row(int64_t rows, int64_t width) { return width <= kShortWidth || (rows >= kWaveRows && width <= kWaveWidth); }
+// Parts of a row whose states lie in the workspace, in the outputs alone and in the gradient; 0: the workspace is not touched.
+// Both the size of the workspace and the launches go by this.
+struct Dealt { int score, loss; };
+Dealt dealt(int64_t rows, int64_t width) {
+    const int splits = rows > 0 ? splits_of(rows, width) : 0;
+    return { splits > 1 && !wave_a_row(rows, width) ? splits : 0, rows < kWholeRows && width > kShortWidth ? splits : 0 };
 }
 
 template <class Ty, bool kGrad>
@@ -1119,16 +1130,17 @@ int score(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld
         launch_short<Ty, false>(st, zz, rows, (int)width, ld, scale, target, top_k, nullptr, nullptr, (A*)lp, (A*)ent, (A*)top_lp,
                                 top_ix, nullptr, 0);
     } else {
-        const int splits = splits_of(rows, width);
-        const Ws<A> w = splits > 1 ? ws_of<A>(ws, rows * splits) : Ws<A>{ nullptr, nullptr };
         const Out<Ty> out = { target, (A*)lp, (A*)ent, (A*)top_lp, top_ix, top_k };
-        if (width <= kShortWidth || (rows >= kWaveRows && width <= kWaveWidth)) {
+        if (wave_a_row(rows, width)) {
             const dim3 waves((unsigned)std::min<int64_t>(kMaxGrid, (rows + kWaves - 1) / kWaves));
             if (top_k > 0) hipLaunchKernelGGL((k_lp_wave<Ty, true>), waves, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, out);
             else hipLaunchKernelGGL((k_lp_wave<Ty, false>), waves, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, out);
             VQA_HIP(hipGetLastError());
             return VQA_OK;
         }
+        const int splits = std::max(1, dealt(rows, width).score);
+        if (splits > 1 && !ws) VQA_FAIL(VQA_EINVAL, "workspace is NULL");
+        const Ws<A> w = splits > 1 ? ws_of<A>(ws, rows * splits) : Ws<A>{ nullptr, nullptr };
         const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows * splits)), grid2((unsigned)std::min<int64_t>(kMaxGrid, rows));
         if (top_k > 0) hipLaunchKernelGGL((k_lp_parts<Ty, true>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
         else hipLaunchKernelGGL((k_lp_parts<Ty, false>), grid, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, top_k, splits, w, out);
@@ -1153,15 +1165,15 @@ int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld,
     const LossOut<Ty> out = { target, (const A*)dg, (const A*)dh, (A*)lp, (A*)ent, (S*)dz, ld_dz };
     const int64_t pieces = (width + 2 * Piece<Ty>::N - 2) / Piece<Ty>::N;    // of a row that begins anywhere
     const dim3 grid((unsigned)std::min<int64_t>(kMaxGrid, rows));
-    // One workgroup a row needs rows enough for half of the CUs; fewer rows are split, and read a second time.
-    if (rows >= 128) {
+    const int splits = dealt(rows, width).loss;
+    if (!splits) {
         if (pieces <= 8 * 64) hipLaunchKernelGGL((k_lp_loss<Ty, 64, 8>), grid, dim3(64), 0, st, zz, rows, width, ld, (A)scale, out);
         else if (pieces <= 16 * 64) hipLaunchKernelGGL((k_lp_loss<Ty, 64, 16>), grid, dim3(64), 0, st, zz, rows, width, ld, (A)scale, out);
         else if (pieces <= 16 * 256) hipLaunchKernelGGL((k_lp_loss<Ty, 256, 16>), grid, dim3(256), 0, st, zz, rows, width, ld, (A)scale, out);
         else if (pieces <= 16 * 512) hipLaunchKernelGGL((k_lp_loss<Ty, 512, 16>), grid, dim3(512), 0, st, zz, rows, width, ld, (A)scale, out);
         else hipLaunchKernelGGL((k_lp_twice<Ty, 512>), grid, dim3(512), 0, st, zz, rows, width, ld, (A)scale, out);
     } else {
-        const int splits = splits_of(rows, width);
+        if (!ws) VQA_FAIL(VQA_EINVAL, "workspace is NULL");
         const Ws<A> w = ws_of<A>(ws, rows * splits);
         const dim3 all((unsigned)std::min<int64_t>(kMaxGrid, rows * splits));
         hipLaunchKernelGGL((k_lp_parts<Ty, false>), all, dim3(kT), 0, st, zz, rows, width, ld, (A)scale, 0, splits, w, Out<Ty>{});
@@ -1174,11 +1186,11 @@ int loss(hipStream_t st, const void* z, int64_t rows, int64_t width, int64_t ld,
 }  // namespace
 
 size_t log_probs_workspace_bytes(int dtype, int64_t rows, int64_t width, int top_k) {
-    if (width <= kShortWidth || rows <= 0) return 0;
-    const size_t parts = (size_t)rows * splits_of(rows, width);
+    const Dealt d = dealt(rows, width);
+    const size_t parts = (size_t)std::max<int64_t>(rows, 0) * std::max(d.score, d.loss);
     const bool wide = dtype == VQA_DTYPE_F64;
     return (parts * (wide ? sizeof(Part<double>) : sizeof(Part<float>)) + 15) / 16 * 16 +
-           parts * top_k * (wide ? sizeof(Best<double>) : sizeof(Best<float>));
+           (size_t)std::max<int64_t>(rows, 0) * d.score * top_k * (wide ? sizeof(Best<double>) : sizeof(Best<float>));
 }
 
 int log_probs_launch(hipStream_t st, int dtype, const void* z, int64_t rows, int64_t width, int64_t ld, double scale,
