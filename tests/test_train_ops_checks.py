@@ -371,3 +371,26 @@ def test_a_workspace_is_asked_for_where_it_is_used():
             assert (rc == _lib.EINVAL) if L.vqa_log_probs_workspace(1, rows, width, 0) else (rc == _lib.ENODEVICE), (rows, width)
     assert L.vqa_log_probs_workspace(1, 5000, 2000, 8) == 0       # a wave a row: nothing is kept between kernels
     assert L.vqa_log_probs_workspace(1, 4, 10 ** 6, 8) > L.vqa_log_probs_workspace(1, 4, 10 ** 6, 0) > 0
+
+
+def test_the_build_refuses_cut_literals(tmp_path):
+    """every object of the library is made by the rule that searches its assembly, and the rule stops at a wide literal"""
+    import os
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.abspath(vqa_amd.__file__)), "csrc")
+    make = open(os.path.join(csrc, "Makefile")).read()
+    body = make[make.index("define compile"):make.index("endef")]
+    pattern = make[make.index("WIDE_MOVE :="):].splitlines()[0].split(":= ")[1]
+    for rule in ("%.o:", "kern_hbm.o:", "kern_hbm_t11.o:"):
+        assert make[make.index("\n" + rule):].split("\n")[2].startswith("\t$(call compile,")
+    # a compiler that writes the assembly at hand in place of its own
+    for move, fine in (("s_mov_b64 s[90:91], 0xfff0000000000000", False), ("s_mov_b64 s[0:1], 0x1000", True), ("s_mov_b64 s[0:1], 1.0", True),
+                       ("s_mov_b64 s[0:1], -1 ; 0xfff0000000000000", True)):
+        (tmp_path / "x.hip").write_text(move)
+        (tmp_path / "cc").write_text('#!/bin/sh\nfor o; do :; done\ncp x.hip $(dirname $o)/x-gfx950.s && touch $o\n')
+        (tmp_path / "cc").chmod(0o755)
+        (tmp_path / "Makefile").write_text(f"HIPCC := ./cc\nARCH := gfx950\nWIDE_MOVE := {pattern}\n{body}endef\n\nx.o: x.hip\n\t$(call compile,)\n")
+        run = subprocess.run(["make", "-B", "x.o"], cwd=tmp_path, capture_output=True, text=True)
+        assert (run.returncode == 0) == fine and (tmp_path / "x.o").exists() == fine, run.stdout + run.stderr
+        (tmp_path / "x.o").unlink(missing_ok=True)

@@ -79,7 +79,8 @@ struct Part {
 };
 
 // Nothing read yet.  m goes through a register that the compiler cannot see into: where it knew this m to be the same for a
-// wave and -infinity in 64 bits, it moved it with one scalar instruction whose constant holds 32 bits, and it became 0.
+// wave and -infinity in 64 bits, it moved it with one scalar instruction whose constant holds 32 bits, and it became 0.  (The
+// build searches the assembly of every object for such moves and fails where it finds one: other constants may meet it too.)
 template <class A>
 __device__ __forceinline__ Part<A> nothing() {
     A m = neg_inf(A(0));
@@ -815,7 +816,6 @@ template <class Ty>
 __global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
                                                  typename Ty::A scale, int splits, Ws<typename Ty::A> ws, LossOut<Ty> out) {
     using A = typename Ty::A;
-    constexpr int N = Piece<Ty>::N;
     for (int64_t it = blockIdx.x; it < rows * splits; it += gridDim.x) {
         const int64_t row = it / splits;
         const int split = (int)(it - row * splits);
