@@ -684,3 +684,25 @@ def test_tensors_that_torch_holds_negated():
                  lambda: vqa_amd.log_probs_grad(z, tg, g, out=neg(w)), lambda: vqa_amd.log_probs_grad(z, tg, g.to(torch.complex64))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("V", [12, 3000, 60000])
+def test_numbers_as_weights_in_a_captured_call(V):
+    """one number for all rows needs no copy from the host, so the call can be captured; the same as a tensor of it"""
+    import torch
+
+    data = [scores(np.random.default_rng(k), 7, V, "float32") for k in range(2)]
+    z, tg = data[0].clone(), torch.arange(7, device="cuda")
+    full = lambda v: torch.full((7,), v, device="cuda")
+    a, b = vqa_amd.log_probs_grad(z, tg, -1.0 / 7, 0.3), vqa_amd.log_probs_grad(z, tg, full(-1.0 / 7), full(0.3))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = vqa_amd.log_probs_grad(z, tg, -1.0 / 7, np.float32(0.3))
+    for n in range(4):
+        z.copy_(data[n % 2])
+        graph.replay()
+        want = vqa_amd.log_probs_grad(data[n % 2], tg, full(-1.0 / 7), full(0.3))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), n

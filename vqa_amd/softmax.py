@@ -118,7 +118,10 @@ def _weights(w, z, wide, what):
     if w is None:
         return None
     if not isinstance(w, torch.Tensor):
-        w = torch.as_tensor(_np_real(w, what, np.float64)).to(z.device, wide)
+        w = _np_real(w, what, np.float64)
+        if w.ndim == 0:                       # filled on the stream: nothing is copied from the host, also in a captured call
+            return torch.full((rows,), float(w), dtype=wide, device=z.device)
+        w = torch.as_tensor(w).to(z.device, wide)
     if w.dim() == 0:
         w = w.expand(rows)
     if tuple(w.shape) != (rows,):
