@@ -477,7 +477,9 @@ int vqa_psr_chain_dev(int device, void* stream, const double* d_expect, int64_t 
  * or pairs of 16-bit floats that hold as much.  Matrix b's element (i, j) is d_g[b * batch_stride + i * row_stride + j];
  * d_out is contiguous and may be d_g where that is contiguous too, but not overlap it otherwise.
  * rows, cols in [1, 65536], batch in [0, 65535], steps in [1, 100], eps >= 1e-300.  coefs that let a singular value
- * exceed 4 within `steps` steps, or the polynomial of A 32, are refused (VQA_EUNSUPPORTED).
+ * exceed 4 within `steps` steps, or the polynomial of A 32, are refused (VQA_EUNSUPPORTED), and so are coefs with
+ * |coefs[0]| < 1, which shrink small singular values, for matrices of 32 and 16 bits of more than 64 rows and columns (their
+ * 16-bit pairs would lose the result's last bits).
  * A zero matrix gives zero; NaN or inf in a matrix, or a sum of squares that leaves 64 bits, gives NaN in that matrix.
  * Workspace as for vqa_log_probs_dev.
  */

@@ -593,3 +593,31 @@ def test_autograd_sees_what_was_overwritten():
             vqa_amd.muon_step(w, torch.ones_like(w), m, 0.1)
             vqa_amd.orthogonalize(w, out=w)
             assert torch.isfinite(w).all() and (m == 1).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(11, 36), (40, 60), (60, 200), (20, 600), (64, 5000), (3000, 12), (150, 70), (300, 290)])
+@pytest.mark.parametrize("steps,coefs", [(3, (15 / 8, -10 / 8, 3 / 8)), (20, (15 / 8, -10 / 8, 3 / 8)), (12, (1.5, -0.5, 0.0)), (30, (1.5, -0.5, 0.0)),
+                                         (5, (3.0, -3.2, 1.2)), (9, (3.0, -3.2, 1.2)), (6, (2.0, -1.5, 0.5)), (4, (0.5, 3.0, -2.9)), (7, (-1.2, 0.9, -0.4)),
+                                         (5, (0.7, 0.0, 0.0)), (3, (0.0, 1.5, -0.9)), (12, (1.0, -0.9, 0.0)), (40, (1.0, -0.3, 0.0)), (10, (-1.0, 2.5, -1.6)),
+                                         (3, (1.0, 0.0, 0.0))])
+def test_other_coefficients_in_every_form(rows, cols, steps, coefs):
+    """strips, blocks, the steps on X X^T (several rounds of them, for small and large first coefficients) and tiles: as exact as
+    four runs of the products in the type's own precision, with the size of one product's roundings beside"""
+    import torch
+
+    for t in UNIT:
+        g = matrices(np.random.default_rng(rows + steps), 2, rows, cols, t)
+        if t != "float64" and min(rows, cols) > 64 and abs(coefs[0]) < 1:
+            from vqa_amd import _lib
+
+            with pytest.raises(_lib.VqaError, match="shrink"):
+                vqa_amd.orthogonalize(g, steps=steps, coefs=coefs)
+            continue
+        want = torch.from_numpy(defined(g.double().cpu().numpy(), steps, coefs)).cuda()
+        p = plain(g.double(), torch.float64 if t == "float64" else torch.float32, steps, coefs)
+        r, c = sorted((rows, cols))
+        norm = torch.linalg.vector_norm(want, dim=(1, 2))
+        o = vqa_amd.orthogonalize(g, steps=steps, coefs=coefs)
+        off = before_rounding(o, want) if t in ("bfloat16", "float16") else torch.linalg.vector_norm(o.double() - want, dim=(1, 2))
+        tol = 4 * torch.linalg.vector_norm(p.double() - want, dim=(1, 2)) + UNIT[t] * math.sqrt(c + 2 * r) * norm * 4
+        assert torch.isfinite(o).all() and (off <= tol).all(), (t, off / norm, tol / norm)

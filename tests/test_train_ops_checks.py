@@ -394,3 +394,13 @@ def test_the_build_refuses_cut_literals(tmp_path):
         run = subprocess.run(["make", "-B", "x.o"], cwd=tmp_path, capture_output=True, text=True)
         assert (run.returncode == 0) == fine and (tmp_path / "x.o").exists() == fine, run.stdout + run.stderr
         (tmp_path / "x.o").unlink(missing_ok=True)
+
+
+def test_coefficients_that_shrink_small_singular_values():
+    """refused where values are held as pairs of 16-bit floats, before anything else happens; not in the other forms"""
+    call = lambda dtype, n, a: ortho(dtype=dtype, rows=n, cols=n + 9, sr=n + 9, sb=n * (n + 9), batch=0, g=None, out=None, k=k3(a, 0.5, -0.3))
+    for dtype in (1, 2, 3):
+        refused(call(dtype, 65, 0.99), _lib.EUNSUPPORTED, "shrink")
+        refused(call(dtype, 65, -0.5), _lib.EUNSUPPORTED, "shrink")
+        assert call(dtype, 65, 1.0) == 0 and call(dtype, 65, -1.1) == 0 and call(dtype, 64, 0.5) == 0
+    assert call(0, 65, 0.5) == 0

@@ -705,7 +705,9 @@ constexpr int kMaxCount = 128;        // tiles of a product whose sum is split: 
 // caller's check, and 1 / sqrt(r c) at the start; of A below 16; of b A + c A A below 32.
 // Where |G| is far below eps, X starts small and grows by about |a| a step: it is held as 2^k X, and A and b A + c A A as
 // 4^k times themselves, k of each matrix and step such that 2^k |X| <= 1 (b + c, so 4^k |b A + c A A|, at most 32 by the
-// caller's check).  k = 0 from |X| = 1 / 2 on, which is where a matrix far above eps starts.
+// caller's check).  k = 0 from |X| = 1 / 2 on, which is where a matrix far above eps starts; with |a| >= 1, which the entry
+// points ask for, X then stays of that size but for what cancels (a smaller |a| shrinks small singular values without bound,
+// and only the size of X itself, not its bound, could be followed: 150 x 70 with (0, 1.5, -0.9), three steps, was 2e-4 off).
 constexpr float kSX = 4096.f, kSA = 1024.f, kSB = 1024.f;
 constexpr int kMostSteps = 100, kMostLift = 110;      // (2^-110 is left in the last product: its values stay normal numbers)
 __device__ __forceinline__ int lift_of(float size) { return min(kMostLift, max(0, -1 - ilogbf(fmaxf(size, 1e-36f)))); }
@@ -1548,6 +1550,8 @@ int run(hipStream_t st, const OrthoCall& q) {
 }
 
 }  // namespace
+
+bool ortho_in_pairs(int dtype, int rows, int cols) { return dtype != VQA_DTYPE_F64 && std::min(rows, cols) > 64; }
 
 size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols) {
     const int r = std::min(rows, cols), c = std::max(rows, cols);

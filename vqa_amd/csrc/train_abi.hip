@@ -207,6 +207,8 @@ int check_matrices(OrthoCall& q, const double* coefs, size_t* g_bytes) {
         VQA_FAIL(VQA_EINVAL, "batch_stride must be in [a matrix's extent, 2^42] (got %lld)", (long long)q.g_batch_stride);
     if (!(q.eps >= 1e-300) || !isfinite(q.eps)) VQA_FAIL(VQA_EINVAL, "eps must be at least 1e-300 and finite");
     if ((rc = check_coefs(q.steps, coefs))) return rc;
+    if (ortho_in_pairs(q.dtype, q.rows, q.cols) && fabs(coefs[0]) < 1.0)
+        VQA_FAIL(VQA_EUNSUPPORTED, "coefs (%g, %g, %g) shrink small singular values: of 32 and 16 bits, only matrices of up to 64 rows or columns take them", coefs[0], coefs[1], coefs[2]);
     std::copy(coefs, coefs + 3, q.coefs);
     *g_bytes = q.batch ? ((size_t)(q.batch - 1) * q.g_batch_stride + one) * size_of(q.dtype) : 0;
     if (q.batch && !q.g) VQA_FAIL(VQA_EINVAL, "g is NULL");

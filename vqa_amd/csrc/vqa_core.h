@@ -276,6 +276,7 @@ struct OrthoCall {
 };
 size_t ortho_workspace_bytes(int dtype, int batch, int rows, int cols);
 int ortho_launch(hipStream_t stream, const OrthoCall& call);
+bool ortho_in_pairs(int dtype, int rows, int cols);   // whether values are held as pairs of 16-bit floats: coefs[0] is 1 or more in size
 
 // the library's own stream of a device (host-pointer entry points)
 int library_stream(int device, hipStream_t* stream);

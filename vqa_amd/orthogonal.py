@@ -64,7 +64,8 @@ def orthogonalize(G, steps: int = 5, coefs: Sequence[float] = COEFS, eps: float 
     """Newton-Schulz products on [rows, cols] or [batch, rows, cols]: X = G / (|G|_F + eps), then ``steps`` times
     X <- coefs[0] X + (coefs[1] A + coefs[2] A A) X with A = X X^T (on the transpose of a matrix with more rows than columns).
     The singular vectors stay, the singular values go towards 1.  Result in G's type (sums in 64 bits for float64, else 32).
-    A zero matrix gives zero; one with a NaN or inf, or whose sum of squares leaves 64 bits, gives NaN.
+    |coefs[0]| >= 1 for matrices of more than 64 rows and columns that are not float64.  A zero matrix gives zero; one with a
+    NaN or inf, or whose sum of squares leaves 64 bits, gives NaN.
 
     numpy: host-pointer path on GPU ``device``.  torch cuda tensors (rows may be strided): queued on the current torch
     stream; ``out`` may be G itself.  Nothing is recorded for autograd; a backward pass that saved ``out`` raises."""
