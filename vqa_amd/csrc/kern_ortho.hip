@@ -837,11 +837,11 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
     const double squares = block_sum((int)threadIdx.x < norm_parts ? part[threadIdx.x] : 0.0, sh), norm = size_of_matrix(squares, j.eps);
     const bool one = blockIdx.x == 0 && blockIdx.y == 0;      // of the matrix's workgroups
     if (one && threadIdx.x < kMaxCount) ((unsigned*)((char*)w.count + off))[threadIdx.x] = 0;
-    double scale = 1.0;
+    double by = norm;
     if constexpr (sizeof(C) == 4) {
         float size = (float)(sqrt(squares) / norm);           // |X|, NaN with the norm
         const int first = lift_of(size);
-        scale = ldexp(1.0, first);
+        by = ldexp(norm, -first);
         if (one && threadIdx.x == 0) {
             int* lift = (int*)((char*)w.lift + off);
             lift[0] = first;
@@ -863,7 +863,7 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
         return row < j.rows && col < j.cols;
     });
 #pragma unroll
-    for (int u = 0; u < U; ++u) tile[(threadIdx.x + u * kT) / kTile][threadIdx.x % kTile] = (C)((double)v[u] / norm * scale);
+    for (int u = 0; u < U; ++u) tile[(threadIdx.x + u * kT) / kTile][threadIdx.x % kTile] = (C)((double)v[u] / by);
     __syncthreads();
     const auto xm = w.x[0].at(off), xt = w.xt[0].at(off);
     const size_t x0 = (size_t)blockIdx.y * kTile, y0 = (size_t)blockIdx.x * kTile;   // row and column of X
