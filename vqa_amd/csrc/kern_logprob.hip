@@ -51,8 +51,10 @@ __device__ __forceinline__ float exp_of(float d) {
 __device__ __forceinline__ double log1p_of(double d) { return log1p(d); }
 __device__ __forceinline__ float log1p_of(float d) { return log1pf(d); }
 
-// exp(d) for d <= 0.  Scores of 16 bits: the hardware's exp2 of the rounded product, off by |d| 2^-24 of a term exp(d),
-// which adds at most 2^-25 to a sum and is far below a 16-bit gradient's own rounding.
+// exp(d) for d <= 0.  Scores of 16 bits: the hardware's exp2 of the rounded product.  scale * log2 e and the product are each
+// rounded, so a term is off by up to |d| 2^-23 of itself, and terms at one distance in one direction: a sum by the mean of
+// |d| under p, which is the entropy less log S and so at most log V, times 2^-23, and log p and the entropy with it.  For a
+// 16-bit gradient that is far below its own rounding.
 template <class Ty>
 __device__ __forceinline__ typename Ty::A exp_neg(typename Ty::A d) {
     if constexpr (Ty::kFast) return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
@@ -650,7 +652,8 @@ struct Out {
 };
 
 // splits = 1: the workgroup writes the row's results, else its part of them.
-// Eight waves a SIMD hide the way from memory (64 registers; two pieces of 16 bytes a lane at once): 2048 rows of 100003
+// Eight waves a SIMD hide the way from memory (64 registers, with outcomes of 16 bits 4 more in scratch; two pieces of 16 bytes a
+// lane at once): 2048 rows of 100003
 // bfloat16, top 8, 114 us = 3.6 TB/s, 151 with 5 waves and four pieces; without outcomes 96 us = 4.3 TB/s.
 template <class Ty, bool kTop>
 __global__ __launch_bounds__(kT, sizeof(typename Ty::A) == 4 ? 8 : 4) void k_lp_parts(const typename Ty::S* __restrict__ z, int64_t rows, int64_t width, int64_t ld,
@@ -831,7 +834,8 @@ __global__ __launch_bounds__(kT) void k_lp_slope(const typename Ty::S* __restric
     }
 }
 
-// Waves a SIMD that the registers shall leave room for: as many as do without the compiler's moving parts of the row out.
+// Waves a SIMD that the registers shall leave room for: as many as do without the compiler's moving parts of the row out, but for
+// 16-bit rows of 512 threads, of whose 16 pieces 18 (bfloat16) and 27 registers (float16) lie in scratch.
 constexpr int waves_a_simd(int T, int NP, size_t size) { return size == 8 ? 2 : NP <= 8 || T > 256 ? 4 : 3; }
 
 // A row's loss with the row in the registers of one workgroup (NP pieces of 16 bytes a thread): read once, written once.

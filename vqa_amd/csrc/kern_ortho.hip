@@ -7,7 +7,8 @@
 //
 // Four forms:
 // * r <= 16, short rows: one workgroup carries a matrix through all steps, X in the registers of its waves in strips of 16
-//   columns (k_ns_strip), in 64-bit or 32-bit matrix instructions.
+//   columns (k_ns_strip), in 64-bit or 32-bit matrix instructions.  (64-bit rows beyond 1024, eight strips a wave: 64 of the
+//   registers lie in scratch.)
 // * r <= 64, short rows: the same with X in shared memory (k_ns_block).
 // * r <= 64, long rows: the steps on X X^T alone, between two passes over the matrix (k_ns_gram, k_ns_poly, k_ns_apply).
 // * else: three tiled products a step (k_ns_product), X, X^T, A and b A + c A A in device memory, all row-major with the
@@ -357,7 +358,7 @@ __device__ __forceinline__ typename Mma<C>::Acc dot16(const C* xa, const C* xb, 
 }
 
 // Bound by the matrix instructions of one CU and the reading of their operands: 48 x 250 in 32 bits 38 us, 64 x 128 in 64 bits
-// 70 us = 0.12 TFLOP/s of the CU's 0.28.
+// 70 us = 0.12 TFLOP/s of the CU's 0.28 (20 registers of a thread lie in scratch there).
 template <class Ty, int NT>
 __global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
     using C = typename Ty::C;
@@ -488,6 +489,9 @@ __global__ __launch_bounds__(kBlockThreads) void k_ns_block(Job<Ty> j) {
 // A has the squares of the singular values: an error u of it moves P X by up to |a|^(2 steps) u.  For matrices of 32 and 16
 // bits, with the products in 64 bits, a round is as many steps as keep |a|^steps <= 2^13 (u |a|^(2 steps) <= 2^-27), with the
 // usual coefficients all of them; 64-bit matrices take a round a step, and X lies in the workspace between rounds.
+// (For any coefficients: with s' = p(s) a step takes an error of s^2 times (s' / s) p'(s), a round times (s_n / s_0) prod p', so
+// s_n is off by u prod p' / (2 s_0) where steps on s itself in 32 bits are off by 2^-24 prod p': less from s_0 = 2^-30 on, and
+// a smaller s_0 stays where p(s) is a s, as |a|^steps <= 2^13 does not carry it out of there.)
 // All r x r matrices are symmetric: a lower tile a wave, written to both sides of the diagonal.
 template <int NT>
 struct Long {
@@ -1149,7 +1153,10 @@ __device__ __forceinline__ void take(C* from, C* v) {
     for (int n = 0; n < N; ++n) v[n] += x[n];
 }
 // Whether this workgroup is the last of n to come here with what it gave.  Each wave waits for its stores to be where all XCDs
-// see them, so that the count needs no fence: a fence writes the whole L2 back, 30 us with 200 workgroups at it.
+// see them, so that the count needs no fence: a fence writes the whole L2 back, 30 us with 200 workgroups at it.  The language's
+// memory model orders relaxed atomics of different addresses in no way; that the wait does is this hardware's: stores of agent
+// scope go past the L2 and are counted until they are there, loads of agent scope read past it, and both stay in program order
+// around the wait and the barriers (volatile assembly with a memory clobber, __syncthreads).
 __device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned* sh) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -1166,10 +1173,11 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* count, int n, unsigned*
 
 // One product of a step.  kGram: A = X X^T;  kPoly: B = b A + c A A  (lower tiles, written to both sides of the
 // diagonal);  kUpdate: X <- a X + B X as its transpose X^T B, both layouts written;  kLast: the same to the caller.
-// Time of X X^T | b A + c A A | update, us:  2048 x 2048
-// float32  54 | 54 | 64;  1000 x 777  10 | 8 | 12 (with tiles of 64 12 | 10 | 12): bound by the 3 to 5 us that a launch, the way
-// of the first stage, the epilogue and the last stores take;  1024 x 4096 float32  34 | 12 | 40: 136 tiles for 256 CUs, and an update that writes 34 MB in one
-// round, after its products.
+// Time of X X^T | b A + c A A | update, us:  4096 x 4096 280 | 287 | 390 (of 16- and 32-bit matrices alike; the last update of 16
+// bits keeps 8 registers of a thread in scratch): the symmetric products are 528 tiles of 128 in 3 rounds of 256, the third nearly
+// empty;  2048 x 2048 float32  54 | 57 | 65;  1000 x 777  10 | 8 | 12 (with tiles of 64 12 | 10 | 12): bound by the 3 to 5 us that a
+// launch, the way of the first stage, the epilogue and the last stores take;  1024 x 4096  31 | 11 | 40: 136 tiles for 256
+// CUs, and an update that writes 34 MB in one round, after its products.
 template <class Ty, Kind kind, int T>
 __global__ __launch_bounds__((Tile<typename Ty::C, T>::kThreads)) void k_ns_product(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int step) {
     using C = typename Ty::C;
@@ -1314,6 +1322,8 @@ struct Side { int side, splits; };
 // Measured for the tile so chosen | the next best, us a product of 32 bits:
 //   update      of 4096 x 4096  420 (256) | 504 (128)    of 2048 x 2048  62 (128) | 85 (64)    of 1024 x 4096  37 (128) | 46 (64)
 //   b A + c A A of 3000         148 (128) | 230 (256)    of 2048          53 (128) | 58 (64)    of 1024         12 (64) | 26 (128)
+// (Of 4096 the symmetric products' 528 tiles of 128, paid as 3 rounds, and 136 of 256 come out alike here, 303.0 and 303.7; measured,
+// the whole operator takes 4780 | 4950, so the choice that the sums make by little is the right one.)
 // and the whole operator with tiles of 32 | 64:  512 x 512  92 | 133,  300 x 300  77 | 105,  1000 x 1000  233 | 196.
 // (Tiles of 192 take 288 us for A A of 4096 by itself, those of 256 331, but the whole operator then takes 3% longer.)
 // A split sum (few tiles and a long sum: X X^T of a wide matrix) also takes the giving and taking of its parts, 4.5 us and 0.35
