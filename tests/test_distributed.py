@@ -212,3 +212,79 @@ def test_two_rank_target_object_equals_single_process():
             assert np.max(np.abs(out[k] - want_out[k])) < 1e-13 * max(1.0, np.max(np.abs(want_out[k]))), k
         assert counters == want_counters
         assert np.max(np.abs(pred - want_pred)) < 1e-13
+
+
+def softmax_problem():
+    """A classifier on the CPU oracle; the read-out's GPU kernels are replaced by their formulas."""
+    from vqa_amd import softmax
+    from vqa_amd.qnn_classifier import myQNN_classifier
+
+    class Circuit(OracleCircuit):
+        def psr_full(self, *a, **k):
+            e, m = super().psr_full(*a, **k)
+            return torch.from_numpy(np.ascontiguousarray(e)), m
+
+    def grad(z, t, g, h=None, scale=1.0):
+        x = scale * z
+        lp = x - torch.logsumexp(x, 1, keepdim=True)
+        p = lp.exp()
+        hot = torch.zeros_like(p)
+        hot[torch.arange(len(t)), torch.as_tensor(t, dtype=torch.int64)] = 1
+        d = g * (hot - p)
+        if h is not None:
+            d = d - h * p * (lp - (p * lp).sum(1, keepdim=True))
+        return softmax.LogProbsGrad(None, None, scale * d)
+
+    softmax.log_probs_grad = grad
+    softmax.psr_chain = lambda E, d, factor=0.5: factor * (d[:, None, :] * (E[:, 1::2] - E[:, 2::2])).sum((0, 2))
+    rng = np.random.default_rng(3)
+    c = create_ibm_HEA_ansatz(3, 1, seed=1, circuit_cls=Circuit)
+    x, y = rng.uniform(0, 1, (9, 3)), rng.integers(0, 3, 9)
+    q = myQNN_classifier(3, c, x, y, x, y)
+    q.softmax_scale, q.entropy_weight = 2.5, 0.1
+    return q, rng.uniform(-3, 3, q.n_params)
+
+
+def softmax_worker(rank, world, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    np.random.seed(rank)                     # the ranks draw different batches; rank 0's is taken
+    t, p = softmax_problem()
+    t.group = dist.group.WORLD
+    out = []
+    for B in (9, 4, 1):                      # one sample: the second rank has none
+        picked = []
+        setup = type(t)._setup
+        t._setup = lambda *a: picked.append(setup(t, *a)) or picked[-1]
+        out.append((t.softmax_CE_grad_eval(p, mini_batch_size=B, L2_reg_lmd=0.2), picked[0][1]))
+    q.put((rank, out, t.circuit_counter[0]))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_two_rank_softmax_gradient_equals_single_process():
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=softmax_worker, args=(r, 2, port, q)) for r in range(2)]
+    for pr in procs:
+        pr.start()
+    got = {r: (out, n) for r, out, n in (q.get(timeout=120) for _ in procs)}
+    for pr in procs:
+        pr.join(timeout=60)
+        assert pr.exitcode == 0
+    from vqa_amd import softmax
+
+    kept = softmax.log_probs_grad, softmax.psr_chain
+    try:
+        t, p = softmax_problem()
+        for k in range(3):
+            (g0, ind), (g1, other) = got[0][0][k], got[1][0][k]
+            assert np.array_equal(ind, other) and np.array_equal(g0, g1)
+            t._setup = lambda *a: (None, ind, t.y_train[ind], None)
+            assert np.max(np.abs(g0 - t.softmax_CE_grad_eval(p, mini_batch_size=len(ind), L2_reg_lmd=0.2))) < 1e-13
+        assert got[0][1] == got[1][1] == 14 * (2 * len(p) + 1)
+    finally:
+        softmax.log_probs_grad, softmax.psr_chain = kept

@@ -706,3 +706,20 @@ def test_numbers_as_weights_in_a_captured_call(V):
         want = vqa_amd.log_probs_grad(data[n % 2], tg, full(-1.0 / 7), full(0.3))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want)), n
+
+
+def test_a_rank_without_samples():
+    """a batch of fewer samples than ranks: the rank that gets none adds zeros"""
+    q, p = classifier()
+
+    class Shard:
+        lo = hi = 0
+
+        def reduce(self, sums, per_item=None):
+            return sums.cpu().numpy(), None
+
+        def bcast_ints(self, ind):
+            return ind
+
+    q._shard = lambda n: Shard()
+    assert np.array_equal(q.softmax_CE_grad_eval(p, mini_batch_size=1), np.zeros(len(p)))

@@ -331,6 +331,10 @@ class LearningCircuit(GateList):
         B = 0 if inputs is None else int(inputs.shape[0])
         if n_sel is None:
             n_sel = len(sel) if sel is not None else max(B, 1)
+        if n_sel == 0 and (isinstance(inputs, torch.Tensor) or isinstance(theta, torch.Tensor)):
+            # no samples (a rank of a batch of fewer samples than ranks): tensors without storage, which the C ABI takes for none
+            none = lambda given, n: given if given is not None else torch.empty((0, K, n), dtype=torch.float64, device=f"cuda:{self.device}")
+            return none(out_expect, n_obs), none(out_marginal, M) if n_marg_bits > 0 or out_marginal is not None else None
         if params is not None:
             host = not isinstance(inputs, torch.Tensor) and not isinstance(theta, torch.Tensor)
             mask = np.zeros(max(self.n_theta, 1), np.uint8)
