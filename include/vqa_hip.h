@@ -481,6 +481,7 @@ int vqa_psr_chain_dev(int device, void* stream, const double* d_expect, int64_t 
  * |coefs[0]| < 1, which shrink small singular values, for matrices of 32 and 16 bits of more than 64 rows and columns (their
  * 16-bit pairs would lose the result's last bits).
  * A zero matrix gives zero; NaN or inf in a matrix, or a sum of squares that leaves 64 bits, gives NaN in that matrix.
+ * (|G|_F is the root of that sum: an element below 1e-154 counts less than it is, or not, which an eps above 1e-138 hides.)
  * Workspace as for vqa_log_probs_dev.
  */
 int64_t vqa_orthogonalize_workspace(int dtype, int batch, int rows, int cols);

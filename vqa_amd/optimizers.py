@@ -281,7 +281,9 @@ class Muon(MiniBatchOptimizer):
         n_c, n_q = getattr(self.target_obj, "n_c_params", self.n_params), getattr(self.target_obj, "n_qubits", None)
         circuit = getattr(self.target_obj, "circuit", None)
         if circuit is not None:
-            cols = _layer_of(circuit, n_c)
+            if self._layer is None:                # (read once for a target object)
+                self._layer = _layer_of(circuit, n_c)
+            cols = self._layer
         else:                                      # a target object without a circuit: layers of three angles a qubit
             cols = 3 * n_q if n_q and n_c >= 1 and n_c % (3 * n_q) == 0 else None
         if not cols:
@@ -290,6 +292,7 @@ class Muon(MiniBatchOptimizer):
 
     def _reset_state(self):
         self.m_t = np.zeros(self.n_params)
+        self._layer = None
         self._shape()
 
     def optimizer_step(self, params, **kwargs):
