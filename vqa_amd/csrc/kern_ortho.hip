@@ -829,7 +829,8 @@ __global__ __launch_bounds__(kT) void k_ns_norm(Job<Ty> j, double* part, size_t 
     if (threadIdx.x == 0) ((double*)((char*)part + b * stride))[blockIdx.x] = ss;
 }
 
-// X0 and its transpose, a tile a workgroup, and the scales of the steps.  4096 x 4096 bfloat16: 39 us = 4.3 TB/s of the reading and of the four arrays written.
+// X0 and its transpose, a tile a workgroup, and the scales of the steps.  4096 x 4096 bfloat16: 43 to 46 us = 3.7 to 3.9 TB/s of the
+// reading and of the four arrays written.
 template <class Ty>
 __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreOf<typename Ty::C>::T> w, int norm_parts) {
     using C = typename Ty::C;
@@ -843,10 +844,14 @@ __global__ __launch_bounds__(kT) void k_ns_enter(Job<Ty> j, Mats<typename StoreO
     if (one && threadIdx.x < kMaxCount) ((unsigned*)((char*)w.count + off))[threadIdx.x] = 0;
     double by = norm;
     if constexpr (sizeof(C) == 4) {
-        float size = (float)(sqrt(squares) / norm);           // |X|, NaN with the norm
-        const int first = lift_of(size);
-        by = ldexp(norm, -first);
+        const double root = sqrt(squares);
+        int first = 0;
+        if (root < j.eps) {                                   // (else |X| is 1 / 2 or more)
+            first = lift_of((float)(root / norm));
+            by = ldexp(norm, -first);
+        }
         if (one && threadIdx.x == 0) {
+            float size = (float)(root / norm);                // |X|, NaN with the norm
             int* lift = (int*)((char*)w.lift + off);
             lift[0] = first;
             for (int s = 1; s <= j.steps; ++s) {              // (a singular value grows by |a + b y + c y^2| at most, and to 4)
